@@ -390,6 +390,143 @@ int latent_route_workspace_size(const latent_route_args* args, size_t* bytes);
  */
 int latent_route(const latent_route_args* args, latent_stream_t stream);
 
+/* ---- attention over a paged key-value cache ------------------------------ */
+/*
+ * The attention half of a decoder layer, beside the expert FFN: append a
+ * step's keys and values to a paged cache, attend to the cache with one new
+ * token a sequence, attend with whole prompts.  No counterpart in the reference,
+ * whose graph builder leaves attention to llama.cpp (README.md:111-113).
+ *
+ * Query head h reads key/value head h / (n_head / n_kv_head).  q, k, v and the
+ * cache share one element type (LATENT_F16 | LATENT_BF16); scores, softmax
+ * statistics and sums are fp32.  head_dim is a multiple of 8 up to 256 whose
+ * elements are adjacent; all other strides are free, in elements, multiples of 8,
+ * and every base is 16-byte aligned.
+ */
+/*
+ * A paged cache: position p of sequence b is row p % page_size of page
+ * pages[b][p / page_size], for k and v alike.  A page id outside [0, n_pages)
+ * names no page: nothing is stored there, and its positions are masked.
+ */
+typedef struct latent_kv_cache {
+  void* k;
+  void* v;
+  const int32_t* pages;  /* [n_seq] rows of max_pages ids, pages_stride apart */
+  int64_t n_pages;
+  int64_t page_size;     /* >= 1 */
+  int64_t n_seq;
+  int64_t max_pages;
+  int64_t pages_stride;
+  int64_t k_page_stride, k_row_stride, k_head_stride;
+  int64_t v_page_stride, v_row_stride, v_head_stride;
+} latent_kv_cache;
+
+/* Rotation of a head's leading rot_dim dimensions: which two form pair i. */
+#define LATENT_ROPE_HALF 0        /* i and i + rot_dim / 2 */
+#define LATENT_ROPE_INTERLEAVED 1 /* 2i and 2i + 1 */
+
+/*
+ * One append: token t of sequence seqs[t] (t itself when seqs is NULL) at
+ * position positions[t].  Its keys are rotated, rounded once and stored in the
+ * cache with its values; its queries, when given, are rotated into q_out (which
+ * may be q).  The pair (a, b) becomes (a c - b s, b c + a s) with
+ * c = rope[p][0][i], s = rope[p][1][i].  rope NULL: nothing is rotated.
+ * A token whose position is negative or not in the table is left out (no
+ * cache row, no q_out row); one whose sequence or page does not exist
+ * stores no cache row.  Tokens of a call address different cache rows; of
+ * tokens that name the same row, what that row then holds is unspecified.
+ */
+typedef struct latent_kv_append_args {
+  latent_kv_cache cache;
+  const void* q; /* [T][n_head][D] or NULL */
+  void* q_out;   /* [T][n_head][D] when q is given */
+  const void* k; /* [T][n_kv_head][D] */
+  const void* v; /* [T][n_kv_head][D] */
+  int64_t q_token_stride, q_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int32_t* positions; /* [T] */
+  const int32_t* seqs;      /* [T] or NULL */
+  const float* rope;        /* [rope_rows][2][rot_dim / 2], 16-byte aligned, or NULL */
+  int64_t rope_rows;
+  int64_t rot_dim;          /* even, <= head_dim */
+  int64_t n_tokens;
+  int64_t n_head;           /* 0 when q is NULL */
+  int64_t n_kv_head;
+  int64_t head_dim;
+  int32_t dtype;
+  int32_t rope_kind; /* LATENT_ROPE_* */
+} latent_kv_append_args;
+
+/* Stream ordered; allocates nothing. */
+int latent_kv_append(const latent_kv_append_args* args, latent_stream_t stream);
+
+/*
+ * One new token a sequence: out[b][h] = sum_j softmax_j(scale q[b][h] . k[j]) v[j]
+ * over the positions j < lengths[b] of the cache (lengths outside
+ * [0, max_pages * page_size] are clamped to it).  A row without a key gives
+ * zeros and lse -inf.  Sums are taken in a fixed order that depends on the
+ * lengths: equal calls give equal bits.
+ */
+typedef struct latent_attn_decode_args {
+  latent_kv_cache cache;
+  const void* q;          /* [n_seq][n_head][D] */
+  void* out;              /* [n_seq][n_head][D] */
+  float* lse;             /* [n_seq][n_head] log of the sum of exp(scale q . k), or NULL */
+  const int32_t* lengths; /* [n_seq] */
+  int64_t q_token_stride, q_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t n_head;
+  int64_t n_kv_head;
+  int64_t head_dim;
+  int32_t dtype;
+  float scale;            /* > 0 */
+  void* workspace;        /* device scratch, >= latent_attn_decode_workspace_size(), 16-byte aligned */
+  size_t workspace_bytes;
+} latent_attn_decode_args;
+
+int latent_attn_decode_workspace_size(const latent_attn_decode_args* args, size_t* bytes);
+
+/* Stream ordered; allocates nothing; calls that may overlap need workspaces of their own. */
+int latent_attn_decode(const latent_attn_decode_args* args, latent_stream_t stream);
+
+/*
+ * Whole prompts, packed: sequence b's queries are rows starts[b] ..
+ * starts[b + 1] - 1 of q (starts ascends from >= 0; what passes n_tokens is cut
+ * off), its keys either rows k_starts[b] .. k_starts[b + 1] - 1 of k and v, or
+ * (k NULL) positions 0 .. lengths[b] - 1 of the cache.  With n queries and m
+ * keys, query i sees keys j <= i + m - n when causal (the last query sees all),
+ * every key otherwise.  A row that sees none gives zeros and lse -inf.  Rows of
+ * out and lse that belong to no sequence are left as they are.
+ */
+typedef struct latent_attn_prompt_args {
+  latent_kv_cache cache; /* pages and below: used when k is NULL; n_seq always */
+  const void* q;         /* [n_tokens][n_head][D] */
+  void* out;             /* [n_tokens][n_head][D] */
+  float* lse;            /* [n_tokens][n_head] or NULL */
+  const void* k;         /* [n_keys][n_kv_head][D] or NULL */
+  const void* v;
+  const int32_t* starts;   /* [n_seq + 1] */
+  const int32_t* k_starts; /* [n_seq + 1], with k */
+  const int32_t* lengths;  /* [n_seq], with the cache */
+  int64_t q_token_stride, q_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t n_tokens;
+  int64_t n_keys;
+  int64_t n_head;
+  int64_t n_kv_head;
+  int64_t head_dim;
+  int32_t dtype;
+  int32_t causal;
+  float scale; /* > 0 */
+} latent_attn_prompt_args;
+
+/* Stream ordered; allocates nothing and needs no workspace. */
+int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,6 +3,7 @@
     from latent_amd import StackedLayer, moe_forward        # MoE layer (ggml op)
     from latent_amd.runtime import load_pair, swiglu_expert # loader/latent_runtime.py
     from latent_amd import route, Router, DecodeStack        # GPU routing, stacked decode
+    from latent_amd import kv_append, attend_decode, attend_prompt  # attention over a paged cache
 
 The compute runs in `liblatent_hip.so` (hand-written HIP for gfx950, C ABI in
 include/latent_ffn.h); torch provides device memory and streams.  Importing
@@ -17,6 +18,14 @@ from ._lib import (  # noqa: F401
     LATENT_OUT_REDUCED,
     LatentError,
     lib,
+)
+from .attention import (  # noqa: F401
+    attend_decode,
+    attend_decode_workspace_size,
+    attend_prompt,
+    attend_prompt_paged,
+    kv_append,
+    rope_table,
 )
 from .moe import (  # noqa: F401
     DeviceFactor,

@@ -55,6 +55,10 @@ EXPORTED = (
     "latent_expert_forward",
     "latent_tiles_supported",
     "latent_tiles_repack",
+    "latent_kv_append",
+    "latent_attn_decode_workspace_size",
+    "latent_attn_decode",
+    "latent_attn_prompt",
 )
 
 LATENT_NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -159,6 +163,63 @@ class LatentExpertArgs(ctypes.Structure):
     ]
 
 
+LATENT_ROPE_HALF = 0
+LATENT_ROPE_INTERLEAVED = 1
+
+
+class LatentKvCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("pages", ctypes.c_void_p),
+        *[(n, ctypes.c_int64) for n in (
+            "n_pages", "page_size", "n_seq", "max_pages", "pages_stride", "k_page_stride", "k_row_stride",
+            "k_head_stride", "v_page_stride", "v_row_stride", "v_head_stride")],
+    ]
+
+
+class LatentKvAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", LatentKvCache),
+        *[(n, ctypes.c_void_p) for n in ("q", "q_out", "k", "v")],
+        *[(n, ctypes.c_int64) for n in (
+            "q_token_stride", "q_head_stride", "q_out_token_stride", "q_out_head_stride", "k_token_stride",
+            "k_head_stride", "v_token_stride", "v_head_stride")],
+        *[(n, ctypes.c_void_p) for n in ("positions", "seqs", "rope")],
+        *[(n, ctypes.c_int64) for n in ("rope_rows", "rot_dim", "n_tokens", "n_head", "n_kv_head", "head_dim")],
+        ("dtype", ctypes.c_int32),
+        ("rope_kind", ctypes.c_int32),
+    ]
+
+
+class LatentAttnDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", LatentKvCache),
+        *[(n, ctypes.c_void_p) for n in ("q", "out", "lse", "lengths")],
+        *[(n, ctypes.c_int64) for n in (
+            "q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride", "n_head", "n_kv_head",
+            "head_dim")],
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LatentAttnPromptArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", LatentKvCache),
+        *[(n, ctypes.c_void_p) for n in ("q", "out", "lse", "k", "v", "starts", "k_starts", "lengths")],
+        *[(n, ctypes.c_int64) for n in (
+            "q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride", "k_token_stride",
+            "k_head_stride", "v_token_stride", "v_head_stride", "n_tokens", "n_keys", "n_head", "n_kv_head",
+            "head_dim")],
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 class LatentError(RuntimeError):
     def __init__(self, status: int, what: str):
         super().__init__(f"{what}: {status_string(status)} ({status})")
@@ -211,6 +272,16 @@ def _load() -> ctypes.CDLL:
         ctypes.c_int32, ctypes.POINTER(LatentFactor), ctypes.POINTER(LatentFactor), ctypes.c_int64, ctypes.c_int32,
         ctypes.c_void_p,
     ]
+    lib.latent_kv_append.restype = ctypes.c_int
+    lib.latent_kv_append.argtypes = [ctypes.POINTER(LatentKvAppendArgs), ctypes.c_void_p]
+    lib.latent_attn_decode_workspace_size.restype = ctypes.c_int
+    lib.latent_attn_decode_workspace_size.argtypes = [
+        ctypes.POINTER(LatentAttnDecodeArgs), ctypes.POINTER(ctypes.c_size_t),
+    ]
+    lib.latent_attn_decode.restype = ctypes.c_int
+    lib.latent_attn_decode.argtypes = [ctypes.POINTER(LatentAttnDecodeArgs), ctypes.c_void_p]
+    lib.latent_attn_prompt.restype = ctypes.c_int
+    lib.latent_attn_prompt.argtypes = [ctypes.POINTER(LatentAttnPromptArgs), ctypes.c_void_p]
     return lib
 
 

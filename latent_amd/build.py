@@ -21,7 +21,8 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
-SOURCES = ["chain32.hip", "codec.hip", "expert.hip", "moe.hip", "noalloc.hip", "prefill.hip", "route.hip", "rows.hip", "stream.hip"]
+SOURCES = ["chain32.hip", "codec.hip", "decode.hip", "expert.hip", "kvcache.hip", "moe.hip", "noalloc.hip", "prefill.hip",
+           "prompt.hip", "route.hip", "rows.hip", "stream.hip"]
 LIB = PKG / "liblatent_hip.so"
 ARCH = os.environ.get("LATENT_OFFLOAD_ARCH", "gfx950")
 

@@ -1,0 +1,124 @@
+// What the attention kernels share: element types and their matrix products,
+// the paged cache's addressing, the pairing of rows that turns loaded value rows
+// into matrix operands, and the host's checks.
+#pragma once
+
+#include "common.hpp"
+
+namespace latent {
+namespace attend {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxDim = 256;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// The two element types: conversions and the fp32-accumulating products.  Eight
+// elements of an operand travel as four dwords.
+struct F16 {
+  typedef _Float16 T;
+  typedef _Float16 T2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 T8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  }
+};
+struct BF16 {
+  typedef __bf16 T;
+  typedef __bf16 T2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 T8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  }
+};
+
+// Two fp32 values rounded to nearest even, the first in the low half.
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), typename E::T2));
+}
+template <typename E>
+__device__ __forceinline__ float unpack_lo(uint32_t w) {
+  if constexpr (sizeof(E) && __is_same(E, F16)) return half_bits_to_float(static_cast<uint16_t>(w));
+  return __uint_as_float(w << 16);
+}
+template <typename E>
+__device__ __forceinline__ float unpack_hi(uint32_t w) {
+  if constexpr (sizeof(E) && __is_same(E, F16)) return half_bits_to_float(static_cast<uint16_t>(w >> 16));
+  return __uint_as_float(w & 0xFFFF0000u);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A running maximum of -inf (nothing seen yet) would make -inf - -inf: its
+// exponentials are taken against 0 instead, where they are 0 too.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// What a masked key reads: 0 * p stays 0 whatever the cache's unused rows hold.
+__device__ const u32x4 kZeroRow[kMaxDim * 2 / 16] = {};
+
+// The cache as the kernels address it (byte strides).
+struct Cache {
+  const char* k;
+  const char* v;
+  const int32_t* pages;
+  int64_t pages_stride;
+  int64_t k_page, k_row, k_head;
+  int64_t v_page, v_row, v_head;
+  uint32_t n_pages, page_size, max_len;  // max_len: positions a page table row has room for
+};
+
+// ---- host ---------------------------------------------------------------------
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0; }
+
+// Sizes every call shares.
+inline int check_heads(int64_t n_head, int64_t n_kv_head, int64_t head_dim, int32_t dtype) {
+  if (n_kv_head <= 0 || n_head < 0 || head_dim <= 0) return LATENT_E_INVALID;
+  if (n_head % n_kv_head) return LATENT_E_INVALID;
+  if (dtype != LATENT_F16 && dtype != LATENT_BF16) return LATENT_E_INVALID;
+  if (head_dim % 8 || head_dim > kMaxDim || n_head > 1024 || n_kv_head > 1024) return LATENT_E_UNSUPPORTED;
+  return LATENT_OK;
+}
+
+inline int check_cache(const latent_kv_cache& c) {
+  if (c.n_pages < 0 || c.page_size <= 0 || c.max_pages < 0 || c.n_seq < 0) return LATENT_E_INVALID;
+  if (c.n_pages > INT32_MAX || c.page_size > INT32_MAX || c.n_seq > (1 << 20)) return LATENT_E_UNSUPPORTED;
+  if (c.max_pages > INT32_MAX || c.max_pages * c.page_size > INT32_MAX - 1024) return LATENT_E_UNSUPPORTED;
+  if (c.n_seq > 1 && c.pages_stride < c.max_pages) return LATENT_E_INVALID;
+  for (int64_t s : {c.k_page_stride, c.k_row_stride, c.k_head_stride, c.v_page_stride, c.v_row_stride, c.v_head_stride})
+    if (!stride_ok(s)) return LATENT_E_UNSUPPORTED;
+  if (!aligned16(c.k) || !aligned16(c.v)) return LATENT_E_UNSUPPORTED;
+  return LATENT_OK;
+}
+
+inline Cache device_cache(const latent_kv_cache& c) {
+  Cache d{};
+  d.k = static_cast<const char*>(c.k);
+  d.v = static_cast<const char*>(c.v);
+  d.pages = c.pages;
+  d.pages_stride = c.pages_stride;
+  d.k_page = c.k_page_stride * 2;
+  d.k_row = c.k_row_stride * 2;
+  d.k_head = c.k_head_stride * 2;
+  d.v_page = c.v_page_stride * 2;
+  d.v_row = c.v_row_stride * 2;
+  d.v_head = c.v_head_stride * 2;
+  d.n_pages = static_cast<uint32_t>(c.n_pages);
+  d.page_size = static_cast<uint32_t>(c.page_size);
+  d.max_len = static_cast<uint32_t>(c.max_pages * c.page_size);
+  return d;
+}
+
+}  // namespace attend
+}  // namespace latent

@@ -1,0 +1,590 @@
+// Attention of one new token a sequence over the paged cache.
+//
+//   out[b][h] = sum_j p_j v[j] / sum_j p_j,  p_j = exp(scale q[b][h] . k[j] - max)
+//
+// Bound by the cache's bytes: each key and value is read once, for all query
+// heads of its head (16 of them fill a matrix instruction's columns; fewer leave
+// columns idle, which costs nothing here).
+//
+// Work: a unit is one sequence, key/value head and chunk of its query heads; it
+// is cut into tiles of 128 keys.  The launch's workgroups take equal contiguous
+// spans of the list of all tiles, so one long sequence, or a batch of very
+// different lengths, loads every CU alike.  Each workgroup finds its span from
+// the lengths on the device.  A unit inside one span is finished there; others
+// leave a part (maximum, sum, unnormalised row) per workgroup, joined by a second
+// launch in workgroup order.
+//
+// Inside a workgroup each wave streams 32-key steps of its own, from the cache
+// straight to registers, no LDS and no barrier: scores^T = K Q^T puts a query
+// head in every lane column and keys in the rows, and the lane that holds
+// query n and keys 8 (lane / 16) .. + 7 of the probabilities is the one whose value
+// operand covers those keys.  A value row arrives as VEC = D / 16 neighbours a lane
+// for eight keys; eight rows are paired into operand dwords by byte permutes.
+#include "attend.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace latent {
+namespace attend {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kStep = 32;               // keys of a wave's step
+constexpr int kTile = kStep * kWaves;   // keys of a work item
+constexpr int kMaxGroups = 512;         // workgroups of a launch: two on every CU
+
+struct DecodeParams {
+  Cache cache;
+  const char* q;
+  char* out;
+  float* lse;
+  const int32_t* lengths;
+  int64_t q_token, q_head, o_token, o_head;  // bytes
+  uint32_t B, Hq, G, D;
+  uint32_t chunks;     // chunks of a head's query heads
+  uint32_t rows;       // query heads of a chunk (the last may have fewer)
+  uint32_t U;          // units of a sequence: n_kv_head * chunks
+  float scale_log2;
+  // Workspace: parts [groups][2][rows] (max, sum), [groups][2][rows][D] rows, and for each unit its first workgroup and number of parts.
+  float* part_ml;
+  float* part_acc;
+  int2* unit_parts;
+};
+
+__device__ __forceinline__ uint32_t length_of(const DecodeParams& p, uint32_t b) {
+  const int32_t n = p.lengths[b];
+  return n < 0 ? 0u : min(static_cast<uint32_t>(n), p.cache.max_len);
+}
+
+// The workgroup's span of tiles and the sequence it starts in.
+struct Span {
+  uint32_t begin, end;  // of all tiles
+  uint32_t per;         // tiles of a workgroup
+  uint32_t b;           // first sequence
+  uint32_t base;        // tiles (of one unit each) of the sequences before it
+};
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const uint32_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+__device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
+
+__device__ __forceinline__ Span find_span(const DecodeParams& p, int lane) {
+  uint32_t total = 0;
+  for (uint32_t b0 = 0; b0 < p.B; b0 += kWave) {
+    const uint32_t b = b0 + lane;
+    total += b < p.B ? tiles_of(length_of(p, b)) : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) total += __shfl_xor(total, d);
+  total *= p.U;
+  Span s;
+  s.per = max(1u, (total + gridDim.x - 1) / gridDim.x);
+  s.begin = min(total, s.per * blockIdx.x);
+  s.end = min(total, s.begin + s.per);
+  s.b = 0;
+  s.base = 0;
+  if (s.begin == s.end) return s;
+  const uint32_t at = s.begin / p.U;  // the sequence's tiles cover [base U, (base + its tiles) U)
+  for (uint32_t b0 = 0; b0 < p.B; b0 += kWave) {
+    const uint32_t b = b0 + lane, n = b < p.B ? tiles_of(length_of(p, b)) : 0;
+    const uint32_t upto = s.base + wave_scan(n, lane);
+    const uint64_t past = __ballot(upto > at);
+    if (past) {
+      const int first = __builtin_ctzll(past);
+      s.b = b0 + first;
+      s.base = __shfl(upto - n, first);
+      break;
+    }
+    s.base = __shfl(upto, kWave - 1);
+  }
+  return s;
+}
+
+template <int kMT, int kVec>
+struct Rows {  // a wave's running softmax: lane (query lane & 15, dims 4 kVec (lane >> 4) ..)
+  float m[kMT], l[kMT];  // l: this lane's keys
+  f32x4 acc[kMT][kVec];
+};
+
+// Pairs eight loaded value rows into the operand of product i: dword a holds keys 2a, 2a + 1 at element i.
+template <int kVec>
+__device__ __forceinline__ u32x4 pair_rows(const uint32_t (&v)[8][kVec / 2], int i) {
+  u32x4 r;
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+    r[a] = __builtin_amdgcn_perm(v[2 * a + 1][i / 2], v[2 * a][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
+  return r;
+}
+
+template <typename E, int kDP, bool kExact, int kMT, bool kPage8>
+struct Stream {
+  static constexpr int kVec = kDP / 16, kK = kDP / 32;
+
+  const DecodeParams& p;
+  int lane, kq;
+  uint32_t len;
+  const int32_t* pages;
+  const char* kbase;
+  const char* vbase;
+
+  // Where a step's keys lie: a page and the row in it.  Eight neighbours from a
+  // multiple of eight share a page where pages hold multiples of eight rows.
+  struct Place {
+    int32_t page;  // outside [0, n_pages): masked
+    uint32_t row;
+  };
+  struct Places {
+    Place k[kPage8 ? 1 : 2], v[kPage8 ? 1 : 8];
+  };
+  __device__ __forceinline__ Place place_of(uint32_t key) const {
+    const uint32_t slot = key / p.cache.page_size;
+    return {key < len ? pages[slot] : -1, key - slot * p.cache.page_size};
+  }
+  // Row m of score block blk is key 8 (m / 4) + 4 blk + m % 4 of the step: lane (query, kq) then holds keys 8 kq .. + 7.
+  __device__ __forceinline__ uint32_t k_key(uint32_t kb, int blk) const { return kb + 8 * ((lane & 15) >> 2) + 4 * blk + (lane & 3); }
+  __device__ __forceinline__ Places places(uint32_t kb) const {
+    Places r;
+    if constexpr (kPage8) {
+      r.k[0] = place_of(kb + 8 * ((lane & 15) >> 2));
+      r.v[0] = place_of(kb + 8 * kq);
+    } else {
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) r.k[blk] = place_of(k_key(kb, blk));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r.v[j] = place_of(kb + 8 * kq + j);
+    }
+    return r;
+  }
+  __device__ __forceinline__ bool valid(uint32_t key, int32_t page) const {
+    return key < len && static_cast<uint32_t>(page) < p.cache.n_pages;
+  }
+
+  __device__ __forceinline__ void load_k(uint32_t kb, const Places& at, u32x4 (&k)[2][kK]) const {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const Place pl = at.k[kPage8 ? 0 : blk];
+      const uint32_t row_in = kPage8 ? pl.row + 4 * blk + (lane & 3) : pl.row;
+      const char* row = valid(k_key(kb, blk), pl.page) ? kbase + pl.page * p.cache.k_page + row_in * p.cache.k_row
+                                                       : reinterpret_cast<const char*>(kZeroRow);
+#pragma unroll
+      for (int s = 0; s < kK; ++s) {
+        const int d = 32 * s + 8 * kq;
+        if constexpr (kExact) {
+          k[blk][s] = *reinterpret_cast<const u32x4*>(row + 2 * d);
+        } else {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(row + 2 * min(d, static_cast<int>(p.D) - 8));
+          k[blk][s] = d < static_cast<int>(p.D) ? x : u32x4{0, 0, 0, 0};
+        }
+      }
+    }
+  }
+  // Returns the mask of this lane's eight keys.
+  __device__ __forceinline__ uint32_t load_v(uint32_t kb, const Places& at, uint32_t (&v)[8][kVec / 2]) const {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const Place pl = at.v[kPage8 ? 0 : j];
+      const uint32_t row_in = kPage8 ? pl.row + j : pl.row;
+      const bool ok = valid(kb + 8 * kq + j, pl.page);
+      mask |= static_cast<uint32_t>(ok) << j;
+      const char* row = ok ? vbase + pl.page * p.cache.v_page + row_in * p.cache.v_row : reinterpret_cast<const char*>(kZeroRow);
+      const int d0 = kVec * (lane & 15);
+      if constexpr (kVec == 4) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(row + 2 * (kExact ? d0 : min(d0, static_cast<int>(p.D) - 4)));
+        const bool in = kExact || d0 < static_cast<int>(p.D);
+        v[j][0] = in ? x[0] : 0;
+        v[j][1] = in ? x[1] : 0;
+      } else {
+#pragma unroll
+        for (int w = 0; w < kVec / 8; ++w) {
+          const int d = d0 + 8 * w;
+          const u32x4 x = *reinterpret_cast<const u32x4*>(row + 2 * (kExact ? d : min(d, static_cast<int>(p.D) - 8)));
+          const bool in = kExact || d < static_cast<int>(p.D);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][4 * w + e] = in ? x[e] : 0;
+        }
+      }
+    }
+    return mask;
+  }
+
+  __device__ __forceinline__ void run(uint32_t first, uint32_t last, const u32x4 (&q)[kMT][kK], Rows<kMT, kVec>& r) const {
+    // Steps first, first + kTile, ... below last (a wave's share of the segment).
+    if (first >= last) return;
+    u32x4 k[2][kK];
+    uint32_t v[8][kVec / 2];
+    Places at = places(first);
+    load_k(first, at, k);
+    uint32_t mask = load_v(first, at, v);
+    uint32_t next = first + kTile;
+    if (next < last) at = places(next);
+    for (uint32_t kb = first; kb < last; kb = next, next += kTile) {
+      f32x4 s[kMT][2];
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          s[mt][blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < kK; ++st) s[mt][blk] = E::mfma16(k[blk][st], q[mt][st], s[mt][blk]);
+        }
+      if (next < last) load_k(next, at, k);
+      u32x4 prob[kMT];
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+        float x[8], top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = (mask >> j) & 1 ? s[mt][j >> 2][j & 3] * p.scale_log2 : -INFINITY;
+          top = fmaxf(top, x[j]);
+        }
+        top = fmaxf(r.m[mt], op_over(top, 16, 64, OpMax{}));
+        const float mm = finite_max(top), f = exp2_fast(r.m[mt] - mm);
+        r.m[mt] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = exp2_fast(x[j] - mm);
+          sum += x[j];
+        }
+        r.l[mt] = r.l[mt] * f + sum;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) r.acc[mt][i] *= f;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) prob[mt][a] = pack2<E>(x[2 * a], x[2 * a + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const u32x4 vt = pair_rows<kVec>(v, i);
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt) r.acc[mt][i] = E::mfma16(vt, prob[mt], r.acc[mt][i]);
+      }
+      if (next < last) {
+        mask = load_v(next, at, v);
+        if (next + kTile < last) at = places(next + kTile);
+      }
+    }
+  }
+};
+
+template <typename E, int kDP, bool kExact, int kMT, bool kPage8>
+__global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(DecodeParams p) {
+  constexpr int kVec = kDP / 16, kK = kDP / 32, kPad = kDP + 4;
+  __shared__ float ml[kWaves][kMT * 16][2];
+  __shared__ float rows[kWaves][16][kPad];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int n16 = lane & 15, kq = lane >> 4;
+
+  // Sequences without keys: a unit of no parts, a row of zeros.
+  for (uint32_t b = blockIdx.x; b < p.B; b += gridDim.x) {
+    if (length_of(p, b) != 0) continue;
+    for (uint32_t i = threadIdx.x; i < p.Hq * (p.D / 8); i += kThreads) {
+      const uint32_t h = i / (p.D / 8), c = i % (p.D / 8);
+      *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = u32x4{0, 0, 0, 0};
+      if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = -INFINITY;
+    }
+    for (uint32_t u = threadIdx.x; u < p.U; u += kThreads) p.unit_parts[b * p.U + u] = int2{0, 0};
+  }
+
+  const Span span = find_span(p, lane);
+  uint32_t cur = span.begin, b = span.b;
+  if (cur == span.end) return;
+  uint32_t len = length_of(p, b), nt = tiles_of(len);
+  uint32_t u = (cur - span.base * p.U) / nt, tile = (cur - span.base * p.U) % nt;
+  while (cur < span.end) {
+    const uint32_t n = min(nt - tile, span.end - cur);
+    const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
+    Stream<E, kDP, kExact, kMT, kPage8> st{p, lane, kq, len, p.cache.pages + b * p.cache.pages_stride,
+                                           p.cache.k + hk * p.cache.k_head, p.cache.v + hk * p.cache.v_head};
+    u32x4 q[kMT][kK];
+    Rows<kMT, kVec> r;
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      const uint32_t row = mt * 16 + n16;
+      const char* src = p.q + b * p.q_token + (hk * p.G + r0 + min(row, nr - 1)) * p.q_head;
+#pragma unroll
+      for (int s = 0; s < kK; ++s) {
+        const int d = 32 * s + 8 * kq;
+        const bool in = row < nr && (kExact || d < static_cast<int>(p.D));
+        const u32x4 x = *reinterpret_cast<const u32x4*>(src + 2 * (kExact ? d : min(d, static_cast<int>(p.D) - 8)));
+        q[mt][s] = in ? x : u32x4{0, 0, 0, 0};
+      }
+      r.m[mt] = -INFINITY;
+      r.l[mt] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) r.acc[mt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    st.run(tile * kTile + wave * kStep, min(len, (tile + n) * kTile), q, r);
+
+    // The four waves' rows under one maximum.
+    const bool whole = tile == 0 && n == nt;
+    const uint32_t slot = tile == 0 ? 1 : 0;  // a workgroup's last unit may begin here, its first may end here
+    const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + slot) * p.rows;
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      r.l[mt] = op_over(r.l[mt], 16, 64, OpAdd{});
+      if (kq == 0) {
+        ml[wave][mt * 16 + n16][0] = r.m[mt];
+        ml[wave][mt * 16 + n16][1] = r.l[mt];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[w][mt * 16 + n16][0]);
+      const float f = exp2_fast(r.m[mt] - finite_max(top));
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) rows[wave][n16][4 * kVec * kq + kVec * rr + i] = r.acc[mt][i][rr] * f;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < 16 * (p.D / 8); i += kThreads) {
+        const uint32_t row = mt * 16 + i / (p.D / 8), c = i % (p.D / 8);
+        if (row >= nr) continue;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[w][row][0]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) l += ml[w][row][1] * exp2_fast(ml[w][row][0] - finite_max(m));
+        f32x4 x[2] = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          x[0] += *reinterpret_cast<const f32x4*>(&rows[w][row & 15][8 * c]);
+          x[1] += *reinterpret_cast<const f32x4*>(&rows[w][row & 15][8 * c + 4]);
+        }
+        if (whole) {
+          const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+          const uint32_t h = hk * p.G + r0 + row;
+          u32x4 y;
+#pragma unroll
+          for (int a = 0; a < 4; ++a) y[a] = pack2<E>(x[a >> 1][2 * (a & 1)] * inv, x[a >> 1][2 * (a & 1) + 1] * inv);
+          *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = y;
+          if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+        } else {
+          f32x4* dst = reinterpret_cast<f32x4*>(p.part_acc + (part + row) * p.D + 8 * c);
+          dst[0] = x[0];
+          dst[1] = x[1];
+          if (c == 0) {
+            p.part_ml[2 * (part + row)] = m;
+            p.part_ml[2 * (part + row) + 1] = l;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (tile == 0 && threadIdx.x == 0)
+      p.unit_parts[b * p.U + u] = int2{static_cast<int>(blockIdx.x), static_cast<int>((cur + nt - 1) / span.per - blockIdx.x + 1)};
+    cur += n;
+    tile = 0;
+    if (++u == p.U && cur < span.end) {
+      u = 0;
+      do len = length_of(p, ++b);
+      while (len == 0 && b + 1 < p.B);
+      nt = tiles_of(len);
+    }
+  }
+}
+
+// Joins the parts of one unit, a query head a workgroup pass.
+template <typename E>
+__global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
+  __shared__ float red[kWaves];
+  __shared__ float weight[kMaxGroups];
+  __shared__ float rows[kThreads / 16][kMaxDim];
+  const uint32_t unit = blockIdx.x, b = unit / p.U, u = unit % p.U;
+  const int2 parts = p.unit_parts[unit];
+  if (parts.y < 2) return;
+  const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const uint32_t lanes = p.D / 8, sets = kThreads / 32;  // a part's row in at most 32 lanes of 8 elements
+  for (uint32_t row = blockIdx.y; row < nr; row += gridDim.y) {
+    auto at = [&](int i) { return (static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row; };
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < parts.y; i += kThreads) m = fmaxf(m, p.part_ml[2 * at(i)]);
+    m = op_over(m, 1, 64, OpMax{});
+    if (lane == 0) red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    float l = 0.f;
+    for (int i = threadIdx.x; i < parts.y; i += kThreads) {
+      const float f = exp2_fast(p.part_ml[2 * at(i)] - finite_max(m));
+      weight[i] = f;
+      l += f * p.part_ml[2 * at(i) + 1];
+    }
+    l = op_over(l, 1, 64, OpAdd{});
+    if (lane == 0) red[wave] = l;
+    __syncthreads();
+    l = red[0] + red[1] + red[2] + red[3];
+    const uint32_t set = threadIdx.x / 32, c = threadIdx.x % 32;
+    f32x4 x[2] = {};
+    if (c < lanes) {
+#pragma unroll 4
+      for (uint32_t i = set; i < static_cast<uint32_t>(parts.y); i += sets) {
+        const f32x4* src = reinterpret_cast<const f32x4*>(p.part_acc + at(i) * p.D + 8 * c);
+        x[0] += src[0] * weight[i];
+        x[1] += src[1] * weight[i];
+      }
+      *reinterpret_cast<f32x4*>(&rows[set][8 * c]) = x[0];
+      *reinterpret_cast<f32x4*>(&rows[set][8 * c + 4]) = x[1];
+    }
+    __syncthreads();
+    if (threadIdx.x < p.D / 2) {
+      float y[2] = {};
+      for (uint32_t s = 0; s < sets; ++s) {
+        y[0] += rows[s][2 * threadIdx.x];
+        y[1] += rows[s][2 * threadIdx.x + 1];
+      }
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+      const uint32_t h = hk * p.G + r0 + row;
+      *reinterpret_cast<uint32_t*>(p.out + b * p.o_token + h * p.o_head + 4 * threadIdx.x) = pack2<E>(y[0] * inv, y[1] * inv);
+      if (p.lse && threadIdx.x == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    }
+    __syncthreads();
+  }
+}
+
+struct Plan {
+  int mt;
+  uint32_t chunks, rows, U, groups;
+  size_t ml_bytes, acc_bytes, unit_bytes;
+  bool split;  // some unit may be split
+};
+
+Plan plan_for(const latent_attn_decode_args& a) {
+  Plan pl{};
+  const uint32_t G = static_cast<uint32_t>(a.n_head / a.n_kv_head);
+  pl.mt = G > 16 ? 2 : 1;
+  pl.chunks = (G + 16 * pl.mt - 1) / (16 * pl.mt);
+  pl.rows = std::min<uint32_t>(G, 16 * pl.mt);
+  pl.U = static_cast<uint32_t>(a.n_kv_head) * pl.chunks;
+  const int64_t tiles = (a.cache.max_pages * a.cache.page_size + kTile - 1) / kTile;
+  const int64_t items = a.cache.n_seq * pl.U * tiles;
+  pl.groups = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(items, kMaxGroups)));
+  pl.split = tiles > 1;
+  const size_t parts = static_cast<size_t>(pl.groups) * 2 * pl.rows;
+  auto up = [](size_t n) { return (n + 15) & ~size_t{15}; };
+  pl.ml_bytes = up(parts * 2 * sizeof(float));
+  pl.acc_bytes = up(parts * a.head_dim * sizeof(float));
+  pl.unit_bytes = up(static_cast<size_t>(a.cache.n_seq) * pl.U * sizeof(int2));
+  return pl;
+}
+
+int validate(const latent_attn_decode_args& a) {
+  const int st = check_heads(a.n_head, a.n_kv_head, a.head_dim, a.dtype);
+  if (st != LATENT_OK) return st;
+  if (a.n_head == 0 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return LATENT_E_INVALID;
+  const int sc = check_cache(a.cache);
+  if (sc != LATENT_OK) return sc;
+  // Tiles and output rows are counted in 32 bits.
+  const Plan pl = plan_for(a);
+  const int64_t tiles = (a.cache.max_pages * a.cache.page_size + kTile - 1) / kTile;
+  if (a.cache.n_seq * pl.U > INT32_MAX / std::max<int64_t>(1, tiles) - kMaxGroups) return LATENT_E_UNSUPPORTED;
+  return LATENT_OK;
+}
+
+}  // namespace
+}  // namespace attend
+}  // namespace latent
+
+using namespace latent;
+using namespace latent::attend;
+
+extern "C" int latent_attn_decode_workspace_size(const latent_attn_decode_args* args, size_t* bytes) {
+  if (!args || !bytes) return LATENT_E_INVALID;
+  const int st = validate(*args);
+  if (st != LATENT_OK) return st;
+  const Plan pl = plan_for(*args);
+  *bytes = pl.ml_bytes + pl.acc_bytes + pl.unit_bytes;
+  return LATENT_OK;
+}
+
+extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_stream_t stream) {
+  if (!args) return LATENT_E_INVALID;
+  const latent_attn_decode_args& a = *args;
+  const int st = validate(a);
+  if (st != LATENT_OK) return st;
+  if (a.cache.n_seq == 0) return LATENT_OK;
+  if (!a.q || !a.out || !a.lengths) return LATENT_E_INVALID;
+  const bool keys = a.cache.max_pages > 0 && a.cache.n_pages > 0;
+  if (keys && (!a.cache.k || !a.cache.v || !a.cache.pages)) return LATENT_E_INVALID;
+  if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.workspace)) return LATENT_E_UNSUPPORTED;
+  for (int64_t s : {a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride})
+    if (!stride_ok(s)) return LATENT_E_UNSUPPORTED;
+  if ((a.n_head > 1 && !a.out_head_stride) || (a.cache.n_seq > 1 && !a.out_token_stride)) return LATENT_E_INVALID;
+  const Plan pl = plan_for(a);
+  if (!a.workspace || a.workspace_bytes < pl.ml_bytes + pl.acc_bytes + pl.unit_bytes) return LATENT_E_WORKSPACE;
+  DecodeParams p{};
+  p.cache = device_cache(a.cache);
+  if (!keys) p.cache.max_len = 0;
+  p.q = static_cast<const char*>(a.q);
+  p.out = static_cast<char*>(a.out);
+  p.lse = a.lse;
+  p.lengths = a.lengths;
+  p.q_token = a.q_token_stride * 2, p.q_head = a.q_head_stride * 2;
+  p.o_token = a.out_token_stride * 2, p.o_head = a.out_head_stride * 2;
+  p.B = static_cast<uint32_t>(a.cache.n_seq);
+  p.Hq = static_cast<uint32_t>(a.n_head);
+  p.G = static_cast<uint32_t>(a.n_head / a.n_kv_head);
+  p.D = static_cast<uint32_t>(a.head_dim);
+  p.chunks = pl.chunks;
+  p.rows = pl.rows;
+  p.U = pl.U;
+  p.scale_log2 = a.scale * kLog2e;
+  char* ws = static_cast<char*>(a.workspace);
+  p.part_ml = reinterpret_cast<float*>(ws);
+  p.part_acc = reinterpret_cast<float*>(ws + pl.ml_bytes);
+  p.unit_parts = reinterpret_cast<int2*>(ws + pl.ml_bytes + pl.acc_bytes);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  auto launch = [&](auto e, auto dp, auto exact, auto mt, auto page8) {
+    hipLaunchKernelGGL((decode_kernel<decltype(e), decltype(dp)::value, decltype(exact)::value, decltype(mt)::value, decltype(page8)::value>),
+                       dim3(pl.groups), dim3(kThreads), 0, s, p);
+  };
+  using std::integral_constant;
+  auto with_dim = [&](auto e, auto dp) {
+    const bool exact = p.D == static_cast<uint32_t>(decltype(dp)::value);
+    auto with_mt = [&](auto mt) {
+      if (a.cache.page_size % 8)
+        launch(e, dp, std::false_type{}, mt, std::false_type{});
+      else if (exact)
+        launch(e, dp, std::true_type{}, mt, std::true_type{});
+      else
+        launch(e, dp, std::false_type{}, mt, std::true_type{});
+    };
+    pl.mt == 1 ? with_mt(integral_constant<int, 1>{}) : with_mt(integral_constant<int, 2>{});
+  };
+  auto with_type = [&](auto e) {
+    if (p.D <= 64)
+      with_dim(e, integral_constant<int, 64>{});
+    else if (p.D <= 128)
+      with_dim(e, integral_constant<int, 128>{});
+    else
+      with_dim(e, integral_constant<int, 256>{});
+  };
+  const bool f16 = a.dtype == LATENT_F16;
+  f16 ? with_type(F16{}) : with_type(BF16{});
+  if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
+  if (pl.split) {
+    // Units that were split have no more than kMaxGroups workgroups between them; where units are few, rows are spread.
+    const uint32_t units = p.B * p.U;
+    const dim3 grid(units, std::max(1u, std::min(p.rows, 2048 / units)));
+    if (f16)
+      hipLaunchKernelGGL(join_kernel<F16>, grid, dim3(kThreads), 0, s, p);
+    else
+      hipLaunchKernelGGL(join_kernel<BF16>, grid, dim3(kThreads), 0, s, p);
+    if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
+  }
+  return LATENT_OK;
+}

@@ -1,0 +1,475 @@
+"""kv_append, attend_decode, attend_prompt and attend_prompt_paged against plain
+attention in 64 bits (tests/_attention.py, where the tolerances are derived)."""
+
+import math
+
+import pytest
+
+from tests._attention import W, assert_attention, half_step, paged, visible
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": "float16", "bf16": "bfloat16"}
+
+
+def _dt(name):
+    import torch
+
+    return getattr(torch, DT[name])
+
+
+def _gen(seed):
+    import torch
+
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, *shape, dt, by=1.0):
+    import torch
+
+    return (torch.randn(shape, generator=gen, device="cuda") * by).to(dt)
+
+
+def _ints(v):
+    import torch
+
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# ---- append -------------------------------------------------------------------
+def _turn64(x, rope, pos, inter):
+    """x [T, H, D] rotated in 64 bits, and the tolerance of a rounded fp32 rotation."""
+    import torch
+
+    y, tol = x.double().clone(), torch.zeros_like(x, dtype=torch.float64)
+    if rope is not None:
+        half = rope.shape[2]
+        i = torch.arange(half, device=x.device)
+        a, b = (2 * i, 2 * i + 1) if inter else (i, i + half)
+        c, s = rope[pos.long(), 0].double()[:, None], rope[pos.long(), 1].double()[:, None]
+        xa, xb = x.double()[..., a], x.double()[..., b]
+        y[..., a], y[..., b] = xa * c - xb * s, xb * c + xa * s
+        tol[..., a] = 2 * W * ((xa * c).abs() + (xb * s).abs())
+        tol[..., b] = 2 * W * ((xb * c).abs() + (xa * s).abs())
+        tol = tol + half_step(x.dtype) * (y.abs() + tol) + torch.finfo(x.dtype).smallest_normal * half_step(x.dtype) * (tol > 0)
+    return y, tol
+
+
+@pytest.mark.parametrize("T,B,Hq,Hkv,D,rot,inter,page,dtype,order", [
+    (1, 1, 32, 8, 128, 128, False, 16, "bf16", "rows"),
+    (5, 3, 4, 2, 64, 32, True, 1, "f16", "heads"),
+    (7, 2, 3, 1, 24, 20, False, 3, "bf16", "rows"),     # one pair a thread
+    (6, 2, 2, 2, 40, 6, True, 5, "f16", "heads"),
+    (9, 4, 5, 5, 256, 256, True, 7, "bf16", "rows"),
+    (33, 2, 0, 3, 96, 48, False, 8, "f16", "rows"),     # keys and values only
+    (4, 4, 2, 1, 16, 0, False, 4, "bf16", "rows"),      # no rotation
+    (700, 3, 28, 4, 128, 64, False, 48, "bf16", "rows"),  # four heads a thread, 36 head rows
+    (900, 3, 21, 3, 80, 80, True, 16, "f16", "heads"),    # 27 head rows: the last thread has three
+])
+def test_append_stores_rotated_rows(gpu, T, B, Hq, Hkv, D, rot, inter, page, dtype, order):
+    import torch
+
+    dt, gen = _dt(dtype), _gen(T)
+    far = max(2 * T // B + 2, 20)
+    kc, vc, pages, _ = paged(gen, [far] * B, page, Hkv, D, dt, order=order)
+    qkv = _randn(gen, T, Hq + 2 * Hkv, D, dt=dt)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]
+    seqs = _ints([t % B for t in range(T)])
+    pos = _ints([(t // B) * 2 + t % 2 for t in range(T)])
+    rope = gpu.rope_table(far, rot) if rot else None
+    want_k, want_v = kc.clone(), vc.clone()
+    got = gpu.kv_append(k, v, kc, vc, pages, pos, seqs=seqs, q=q if Hq else None, rope=rope, interleaved=inter)
+    rows = pages[seqs.long(), pos.long() // page].long()
+    k64, tol = _turn64(k, rope, pos, inter)
+    stored = kc[rows, pos.long() % page]
+    assert float(((stored.double() - k64).abs() - tol).max()) <= 0
+    assert torch.equal(vc[rows, pos.long() % page], v)
+    want_k[rows, pos.long() % page], want_v[rows, pos.long() % page] = stored, v
+    assert torch.equal(kc.contiguous().view(torch.int16), want_k.contiguous().view(torch.int16))  # NaN rows elsewhere, untouched
+    assert torch.equal(vc.contiguous().view(torch.int16), want_v.contiguous().view(torch.int16))
+    if Hq:
+        q64, tol = _turn64(q, rope, pos, inter)
+        assert got.shape == q.shape and float(((got.double() - q64).abs() - tol).max()) <= 0
+        again = q.clone()  # in place
+        assert gpu.kv_append(k, v, kc, vc, pages, pos, seqs=seqs, q=again, rope=rope, interleaved=inter, q_out=again) is again
+        assert torch.equal(again, got)
+    else:
+        assert got is None
+
+
+@pytest.mark.parametrize("D", [32, 24])
+def test_append_leaves_out_what_has_no_place(gpu, D):
+    """Negative and far positions, sequences and pages that do not exist, table rows that end."""
+    import torch
+
+    gen, dt, page = _gen(1), torch.bfloat16, 4
+    kc, vc, pages, _ = paged(gen, [12, 8], page, 1, D, dt, width=3)
+    pages[0, 1], pages[1, 0] = -7, kc.shape[0]
+    before = kc.clone(), vc.clone()
+    #       stored, no page, stored, bad page, seq -1, seq 2, pos -1, beyond pages, beyond the table
+    seqs = [0, 0, 0, 1, -1, 2, 0, 0, 0]
+    pos = [0, 5, 11, 2, 3, 3, -1, 12, 15]
+    T = len(seqs)
+    k, v, q = (_randn(gen, T, 1, D, dt=dt) for _ in range(3))
+    rope = gpu.rope_table(14, 8)
+    out = torch.full_like(q, 7.0)
+    gpu.kv_append(k, v, kc, vc, pages, _ints(pos), seqs=_ints(seqs), q=q, rope=rope, q_out=out)
+    for t in (0, 2):
+        at = int(pages[0, pos[t] // page]), pos[t] % page
+        k64, tol = _turn64(k[t:t + 1], rope, _ints(pos[t:t + 1]), False)
+        assert float(((kc[at].double() - k64[0]).abs() - tol[0]).max()) <= 0 and torch.equal(vc[at], v[t])
+        kc[at], vc[at] = before[0][at], before[1][at]
+    assert torch.equal(kc.view(torch.int16), before[0].view(torch.int16))
+    assert torch.equal(vc.view(torch.int16), before[1].view(torch.int16))
+    fine = torch.tensor([0 <= p < 14 for p in pos], device="cuda")
+    assert bool((out[~fine] == 7.0).all())
+    q64, tol = _turn64(q[fine], rope, _ints(pos)[fine], False)
+    assert float(((out[fine].double() - q64).abs() - tol).max()) <= 0
+
+
+def test_append_without_tokens_or_sequences(gpu):
+    import torch
+
+    gen, dt = _gen(2), torch.float16
+    kc, vc, pages, _ = paged(gen, [4], 4, 1, 16, dt)
+    none = torch.empty((0, 1, 16), dtype=dt, device="cuda")
+    assert gpu.kv_append(none, none, kc, vc, pages, _ints([])) is None
+    k = _randn(gen, 1, 1, 16, dt=dt)
+    before = kc.clone()
+    gpu.kv_append(k, k, kc, vc, pages[:0], _ints([0]), seqs=_ints([0]))
+    assert torch.equal(kc.view(torch.int16), before.view(torch.int16))
+
+
+# ---- decode -------------------------------------------------------------------
+def _decode_check(gpu, q, kc, vc, pages, lengths, seqs, lens, scale=None, **kw):
+    import torch
+
+    lse = torch.full(q.shape[:2], 5.0, device="cuda")
+    out = gpu.attend_decode(q, kc, vc, pages, lengths, scale=scale, lse=lse, **kw)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    for b, n in enumerate(lens):
+        k, v = seqs[b]
+        assert_attention(out[b:b + 1], lse[b:b + 1], q[b:b + 1], k[:n], v[:n], visible(1, n, True, "cuda"), scale)
+    return out
+
+
+@pytest.mark.parametrize("lens", [(1,), (0,), (31, 32, 33), (127, 128, 129, 0, 1), (0, 0, 700, 5, 0, 2049, 1, 0)])
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [
+    (8, 2, 128, 16, "bf16"), (5, 5, 64, 8, "f16"), (16, 1, 256, 32, "bf16"), (21, 3, 96, 24, "f16"), (20, 1, 72, 1, "bf16"),
+    (3, 1, 8, 3, "f16"), (40, 1, 128, 64, "f16"), (66, 2, 200, 7, "bf16"), (34, 2, 64, 16, "bf16"), (25, 1, 256, 40, "f16"),
+])
+def test_decode_matches_plain_attention(gpu, lens, Hq, Hkv, D, page, dtype):
+    import torch
+
+    dt, gen = _dt(dtype), _gen(sum(lens) + D)
+    kc, vc, pages, seqs = paged(gen, lens, page, Hkv, D, dt)  # unused rows hold NaN
+    q = _randn(gen, len(lens), Hq, D, dt=dt, by=2.0)
+    out = _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+    assert torch.equal(out, gpu.attend_decode(q, kc, vc, pages, _ints(lens)))  # equal calls, equal bits
+
+
+@pytest.mark.parametrize("B,L,Hq,Hkv,D", [(1, 40001, 8, 1, 128), (3, 9000, 4, 4, 64), (300, 150, 4, 2, 64), (1100, 40, 2, 1, 32)])
+def test_decode_split_over_the_chip(gpu, B, L, Hq, Hkv, D):
+    """Spans that cut sequences, many sequences in a span, more sequences than workgroups."""
+    import torch
+
+    gen = _gen(B)
+    lens = [max(0, L - (b * 37) % (L + 3)) for b in range(B)]
+    kc, vc, pages, seqs = paged(gen, lens, 16, Hkv, D, torch.bfloat16)
+    q = _randn(gen, B, Hq, D, dt=torch.bfloat16, by=3.0)
+    out = gpu.attend_decode(q, kc, vc, pages, _ints(lens))
+    for b in (range(B) if B < 10 else (0, 1, B // 2, B - 2, B - 1)):
+        n = lens[b]
+        assert_attention(out[b:b + 1], None, q[b:b + 1], *(x[:n] for x in seqs[b]), visible(1, n, True, "cuda"), D ** -0.5)
+
+
+def test_decode_masks_pages_that_do_not_exist(gpu):
+    import torch
+
+    gen, dt, page, D = _gen(4), torch.bfloat16, 16, 64
+    for order in ("rows", "heads"):
+        kc, vc, pages, seqs = paged(gen, [200, 64, 16], page, 2, D, dt, order=order)
+        q = _randn(gen, 3, 6, D, dt=dt)
+        pages[0, 3], pages[0, 7], pages[2, 0] = -1, kc.shape[0] + 5, 1 << 30
+        lse = torch.empty((3, 6), device="cuda")
+        out = gpu.attend_decode(q, kc, vc, pages, _ints([200, 64, 16]), lse=lse, scale=0.25)
+        seen = torch.ones((1, 200), dtype=torch.bool, device="cuda")
+        seen[0, 48:64] = seen[0, 112:128] = False
+        assert_attention(out[:1], lse[:1], q[:1], *seqs[0], seen, 0.25)
+        assert_attention(out[1:2], lse[1:2], q[1:2], *seqs[1], visible(1, 64, True, "cuda"), 0.25)
+        assert bool((out[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+
+
+def test_decode_clamps_lengths(gpu):
+    import torch
+
+    gen, dt = _gen(5), torch.float16
+    kc, vc, pages, seqs = paged(gen, [64, 64], 16, 1, 64, dt)
+    q = _randn(gen, 2, 4, 64, dt=dt)
+    got = gpu.attend_decode(q, kc, vc, pages, _ints([1 << 30, -5]))
+    assert torch.equal(got[0], gpu.attend_decode(q, kc, vc, pages, _ints([64, 0]))[0]) and bool((got[1] == 0).all())
+
+
+def test_decode_infinite_and_nan_keys_reach_their_own_rows_only(gpu):
+    import torch
+
+    gen, dt = _gen(6), torch.bfloat16
+    lens = [100, 100]
+    kc, vc, pages, seqs = paged(gen, lens, 16, 1, 64, dt)
+    q = _randn(gen, 2, 4, 64, dt=dt)
+    clean = gpu.attend_decode(q, kc, vc, pages, _ints(lens))
+    kc[pages[0, 2].long(), 3, 0, 5] = math.nan
+    got = gpu.attend_decode(q, kc, vc, pages, _ints(lens))
+    assert torch.isnan(got[0]).all() and torch.equal(got[1], clean[1])
+    # A row whose scores are all -inf has nothing to weigh: zeros.
+    q0 = torch.ones((1, 4, 64), dtype=dt, device="cuda")
+    kc2, vc2, pages2, _ = paged(gen, [40], 16, 1, 64, dt)
+    kc2[pages2[0, :3].long()] = -math.inf
+    lse = torch.empty((1, 4), device="cuda")
+    assert bool((gpu.attend_decode(q0, kc2, vc2, pages2, _ints([40]), lse=lse) == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_decode_cache_beyond_32_bit_offsets(gpu):
+    """Rows whose byte offsets pass 2^32."""
+    import torch
+
+    gen, dt, page, Hkv, D = _gen(7), torch.bfloat16, 64, 8, 128
+    n = (5 << 30) // (page * Hkv * D * 2)
+    kc, vc = (torch.empty((n, page, Hkv, D), dtype=dt, device="cuda") for _ in range(2))
+    lens = [300]
+    pages = _ints([[n - 1 - 2 * i for i in range(5)]])
+    k, v = (_randn(gen, 300, Hkv, D, dt=dt) for _ in range(2))
+    assert gpu.kv_append(k, v, kc, vc, pages, _ints(list(range(300))), seqs=_ints([0] * 300)) is None
+    q = _randn(gen, 1, 16, D, dt=dt)
+    _decode_check(gpu, q, kc, vc, pages, _ints(lens), [(k, v)], lens)
+    out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints(lens), _ints([0, 1]))
+    assert_attention(out, None, q, k, v, visible(1, 300, True, "cuda"), D ** -0.5)
+
+
+def test_decode_strided_operands_and_given_buffers(gpu):
+    import torch
+
+    gen, dt = _gen(8), torch.bfloat16
+    lens = [300, 17]
+    kc, vc, pages, seqs = paged(gen, lens, 16, 2, 64, dt, order="heads")
+    wide = torch.full((2, 30), -1, dtype=torch.int32, device="cuda")
+    wide[:, :pages.shape[1]] = pages
+    q = _randn(gen, 2, 9, 3, 64, dt=dt)[:, ::2, 1][:, :4]  # heads 384 apart
+    room = torch.full((2, 6, 64), 3.0, dtype=dt, device="cuda")
+    ws = torch.empty(gpu.attend_decode_workspace_size(2, 4, 2, 64, pages.shape[1], 16), dtype=torch.uint8, device="cuda")
+    got = _decode_check(gpu, q, kc, vc, wide[:, :pages.shape[1]], _ints(lens), seqs, lens, out=room[:, 1:5], workspace=ws)
+    assert got.data_ptr() == room[:, 1:5].data_ptr() and bool((room[:, 0] == 3).all()) and bool((room[:, 5] == 3).all())
+    # Not 16-byte aligned: copied.
+    odd = torch.empty(2 * 4 * 64 + 1, dtype=dt, device="cuda")[1:].view(2, 4, 64)
+    odd.copy_(q)
+    assert torch.equal(gpu.attend_decode(odd, kc, vc, pages, _ints(lens)), got)
+
+
+# ---- prompt -------------------------------------------------------------------
+def _prompt_check(gpu, gen, new, keys, Hq, Hkv, D, dt, causal, page=0, pad=0, by=2.0):
+    import torch
+
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    T = starts[-1] + pad
+    q = _randn(gen, T, Hq, D, dt=dt, by=by)
+    out = torch.full((T, Hq, D), 9.0, dtype=dt, device="cuda")
+    lse = torch.full((T, Hq), 9.0, device="cuda")
+    if page:
+        kc, vc, pages, seqs = paged(gen, keys, page, Hkv, D, dt)
+        gpu.attend_prompt_paged(q, kc, vc, pages, _ints(keys), _ints(starts), causal=causal, out=out, lse=lse)
+    else:
+        k_starts = [0]
+        for m in keys:
+            k_starts.append(k_starts[-1] + m)
+        k, v = (_randn(gen, k_starts[-1] + pad, Hkv, D, dt=dt) for _ in range(2))
+        seqs = [(k[a:b], v[a:b]) for a, b in zip(k_starts, k_starts[1:])]
+        gpu.attend_prompt(q, k, v, _ints(starts), k_starts=_ints(k_starts), causal=causal, out=out, lse=lse)
+    for b, (n, m) in enumerate(zip(new, keys)):
+        r = slice(starts[b], starts[b + 1])
+        assert_attention(out[r], lse[r], q[r], *seqs[b], visible(n, m, causal, "cuda"), D ** -0.5)
+    assert bool((out[starts[-1]:] == 9).all()) and bool((lse[starts[-1]:] == 9).all())  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [
+    (4, 1, 128, "bf16"), (2, 2, 64, "f16"), (3, 1, 256, "bf16"), (10, 2, 96, "f16"), (7, 1, 8, "bf16"), (33, 1, 40, "f16"),
+    (2, 1, 168, "bf16"),
+])
+@pytest.mark.parametrize("new,keys", [
+    ((1,), (1,)), ((0, 5, 0, 64, 1), (0, 5, 0, 64, 1)), ((130, 31, 257), (130, 31, 257)),
+    ((3, 40, 1), (200, 41, 129)),       # keys in front of the new tokens
+    ((70, 9, 4), (5, 0, 3)),            # fewer keys than queries: the first rows see none
+])
+@pytest.mark.parametrize("causal,page", [(True, 0), (False, 0), (True, 16), (True, 3), (False, 40)])
+def test_prompt_matches_plain_attention(gpu, Hq, Hkv, D, dtype, new, keys, causal, page):
+    _prompt_check(gpu, _gen(sum(new) + D), list(new), list(keys), Hq, Hkv, D, _dt(dtype), causal, page, pad=3)
+
+
+@pytest.mark.parametrize("new,ahead,Hq,Hkv,D,page", [
+    ((1500, 3, 700), 0, 8, 2, 128, 0), ((2000,), 0, 3, 3, 64, 0), ((600, 100), 3000, 8, 1, 128, 32), ((900,), 0, 2, 2, 256, 0),
+])
+def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
+    import torch
+
+    _prompt_check(gpu, _gen(D), list(new), [n + ahead for n in new], Hq, Hkv, D, torch.bfloat16, True, page, by=4.0)
+
+
+def test_prompt_many_sequences(gpu):
+    """More sequences than one look of a wave over `starts`."""
+    import torch
+
+    new = [(7 * i) % 5 for i in range(150)]
+    _prompt_check(gpu, _gen(9), new, new, 4, 2, 64, torch.float16, True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_nan_and_infinity_do_not_reach_rows_that_do_not_see_them(gpu, D):
+    import torch
+
+    gen, dt, n = _gen(10), torch.bfloat16, 150
+    q, k, v = (_randn(gen, n, 2, D, dt=dt) for _ in range(3))
+    v[70, 0, 5], v[149, 1, 3], v[100, 0, 7] = math.nan, math.inf, -math.inf
+    starts = _ints([0, n])
+    out = gpu.attend_prompt(q, k, v, starts)
+    assert_attention(out, None, q, k, v, visible(n, n, True, "cuda"), D ** -0.5)
+    k[80, 1, 0] = math.nan  # a NaN score: the rows that see it are NaN, the others as they were
+    got = gpu.attend_prompt(q, k, v, starts)
+    assert torch.equal(got[:70], out[:70]) and torch.equal(got[70:80, 1], out[70:80, 1])
+    assert torch.isnan(got[80:, 1]).all()
+
+
+def test_prompt_masks_pages_that_do_not_exist(gpu):
+    import torch
+
+    gen, dt, page, D = _gen(11), torch.bfloat16, 16, 128
+    kc, vc, pages, seqs = paged(gen, [200], page, 1, D, dt)
+    pages[0, 4], pages[0, 0] = -2, kc.shape[0]
+    q = _randn(gen, 90, 2, D, dt=dt)
+    lse = torch.empty((90, 2), device="cuda")
+    out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints([200]), _ints([0, 90]), lse=lse)
+    seen = visible(90, 200, True, "cuda").clone()
+    seen[:, 64:80] = seen[:, :16] = False
+    assert_attention(out, lse, q, *seqs[0], seen, D ** -0.5)
+
+
+def test_prompt_fused_projection_views_and_bad_starts(gpu):
+    import torch
+
+    gen, dt, T, D = _gen(12), torch.float16, 200, 64
+    qkv = _randn(gen, T, 8, D, dt=dt)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    out = gpu.attend_prompt(q, k, v, _ints([0, 60, 200]))
+    for a, b in ((0, 60), (60, 200)):
+        assert_attention(out[a:b], None, q[a:b], k[a:b], v[a:b], visible(b - a, b - a, True, "cuda"), D ** -0.5)
+    # What passes the rows is cut off, what descends is empty (rows 40 .. 59 then belong to the third sequence too).
+    room = torch.full_like(out, 9.0)
+    gpu.attend_prompt(q, k, v, _ints([-3, 60, 40, 1000]), out=room)
+    assert torch.equal(room[:40], out[:40])
+
+
+# ---- streams, graphs ------------------------------------------------------------
+def test_calls_on_another_stream(gpu):
+    import torch
+
+    gen, dt = _gen(13), torch.bfloat16
+    lens = [500, 900]
+    kc, vc, pages, _ = paged(gen, lens, 16, 2, 128, dt)
+    q, L = _randn(gen, 2, 8, 128, dt=dt), _ints(lens)
+    want = gpu.attend_decode(q, kc, vc, pages, L)
+    wide = _randn(gen, 40, 8, 128, dt=dt)
+    want_p = gpu.attend_prompt_paged(wide, kc, vc, pages, L, _ints([0, 10, 40]))
+    starts = _ints([0, 10, 40])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = gpu.attend_decode(q, kc, vc, pages, L, stream=side)
+    got_p = gpu.attend_prompt_paged(wide, kc, vc, pages, L, starts, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got_p, want_p)
+
+
+def test_captured_step_replays(gpu):
+    """Append, attend and count in one graph, replayed with the host's own work between; two graphs in turn."""
+    import torch
+
+    gen, dt, B, Hq, Hkv, D, page = _gen(14), torch.bfloat16, 3, 8, 2, 64, 16
+    rope = gpu.rope_table(200, D)
+    first = [5, 90, 0]
+
+    def make():
+        g = _gen(15)
+        kc, vc, pages, _ = paged(g, [160] * B, page, Hkv, D, dt)
+        return dict(kc=kc, vc=vc, pages=pages, pos=_ints(first), x=_randn(g, B, Hq + 2 * Hkv, D, dt=dt),
+                    out=torch.empty((B, Hq, D), dtype=dt, device="cuda"))
+
+    def step(s):
+        q, k, v = s["x"][:, :Hq], s["x"][:, Hq:Hq + Hkv], s["x"][:, Hq + Hkv:]
+        r = gpu.kv_append(k, v, s["kc"], s["vc"], s["pages"], s["pos"], q=q, rope=rope)
+        gpu.attend_decode(r, s["kc"], s["vc"], s["pages"], s["pos"] + 1, out=s["out"])
+        s["pos"].add_(1)
+
+    eager, a, b = make(), make(), make()
+    for s in (eager, a, b):
+        s["kc"].zero_(), s["vc"].zero_()
+    graphs = []
+    for s in (a, b):
+        step(s)  # warm
+        s["pos"].copy_(_ints(first))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(s)
+        graphs.append(g)
+    for i in range(6):
+        x = _randn(gen, B, Hq + 2 * Hkv, D, dt=dt)
+        for s in (eager, a, b):
+            s["x"].copy_(x)
+        step(eager)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a["out"], eager["out"]) and torch.equal(b["out"], eager["out"]), i
+        assert torch.equal(a["pos"], eager["pos"])
+        torch.randn((1000, 1000), device="cuda") @ torch.randn((1000, 1000), device="cuda")
+
+
+# ---- a run of them together -----------------------------------------------------
+def test_prompt_then_tokens_equal_one_prompt(gpu):
+    """Prompts appended in chunks and continued token by token see what one packed causal pass sees."""
+    import torch
+
+    gen, dt, Hq, Hkv, D, page = _gen(16), torch.bfloat16, 8, 2, 64, 16
+    lens, B = [133, 37, 64], 3
+    rope = gpu.rope_table(200, D)
+    kc, vc, pages, _ = paged(gen, lens, page, Hkv, D, dt)
+    q, k, v = ([_randn(gen, n, h, D, dt=dt) for n in lens] for h in (Hq, Hkv, Hkv))
+    turned = []
+    # The oracle's rows: rotated operands as the kernel rounds them.
+    out = [torch.empty((n, Hq, D), dtype=dt, device="cuda") for n in lens]
+    done = [0] * B
+    rot_q = [[] for _ in range(B)]
+    for chunk in ([60, 10, 1], [70, 25, 62], [1, 1, 0], [1, 1, 1], [1, 0, 0]):
+        T = sum(chunk)
+        take = [slice(done[b], done[b] + chunk[b]) for b in range(B)]
+        qq, kk, vv = (torch.cat([x[b][take[b]] for b in range(B)]) for x in (q, k, v))
+        seqs = _ints([b for b in range(B) for _ in range(chunk[b])])
+        pos = _ints([p for b in range(B) for p in range(done[b], done[b] + chunk[b])])
+        r = gpu.kv_append(kk, vv, kc, vc, pages, pos, seqs=seqs, q=qq, rope=rope)
+        done = [d + c for d, c in zip(done, chunk)]
+        starts = [0]
+        for c in chunk:
+            starts.append(starts[-1] + c)
+        if max(chunk) == 1:  # the single-token form, sequences without a new token padded
+            wide = torch.zeros((B, Hq, D), dtype=dt, device="cuda")
+            wide[seqs.long()] = r
+            got = gpu.attend_decode(wide, kc, vc, pages, _ints([d if c else 0 for d, c in zip(done, chunk)]))[seqs.long()]
+        else:
+            got = gpu.attend_prompt_paged(r, kc, vc, pages, _ints(done), _ints(starts))
+        for b in range(B):
+            out[b][take[b]] = got[starts[b]:starts[b + 1]]
+            rot_q[b].append(r[starts[b]:starts[b + 1]])
+    for b, n in enumerate(lens):
+        p = torch.arange(n, device="cuda")
+        rows = pages[b].long()[p // page]
+        turned.append(kc[rows, p % page])
+        assert done[b] == n
+        assert_attention(out[b], None, torch.cat(rot_q[b]), turned[b], v[b], visible(n, n, True, "cuda"), D ** -0.5)
