@@ -28,6 +28,10 @@ struct F16 {
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
   }
+  // c plus the dword's two elements.
+  static __device__ __forceinline__ float add2(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(T2, w), __builtin_bit_cast(T2, 0x3C003C00u), c, false);
+  }
 };
 struct BF16 {
   typedef __bf16 T;
@@ -38,6 +42,9 @@ struct BF16 {
   }
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(T2, w), __builtin_bit_cast(T2, 0x3F803F80u), c, false);
   }
 };
 
@@ -66,6 +73,48 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 // What a masked key reads: 0 * p stays 0 whatever the cache's unused rows hold.
 __device__ const u32x4 kZeroRow[kMaxDim * 2 / 16] = {};
+
+// Direct global -> LDS loads: lane l's 16 bytes land at LDS byte address lds + 16 l; lds is wave-uniform.  Inline
+// assembly, so that the compiler does not make every later LDS read wait for them; whoever issues them waits
+// (pipeline_barrier).  The second form takes a wave-uniform base and a 32-bit lane offset.
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "m0");
+}
+__device__ __forceinline__ void dma16s(const void* base, uint32_t off, uint32_t lds) {
+  const uint64_t v = reinterpret_cast<uintptr_t>(base);
+  const uint64_t u = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32 |
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(u),
+               "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "m0");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t lds_addr(T& obj) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(&obj)));
+}
+template <typename T>
+__device__ __forceinline__ T lds_ld(uint32_t addr) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) T*>(static_cast<uintptr_t>(addr));
+}
+template <typename T>
+__device__ __forceinline__ void lds_st(uint32_t addr, T v) {
+  *reinterpret_cast<__attribute__((address_space(3))) T*>(static_cast<uintptr_t>(addr)) = v;
+}
+
+// Workgroup barriers: every wave's direct loads have landed and its LDS accesses are done; or the latter alone.
+__device__ __forceinline__ void pipeline_barrier() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+__device__ __forceinline__ void lds_barrier() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
 
 // The cache as the kernels address it (byte strides).
 struct Cache {

@@ -28,6 +28,10 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kRowsWave = 32;
 constexpr int kRowsTile = kRowsWave * kWaves;
 constexpr int kKeys = 64;  // keys of a tile
+// The exponentials' reference follows the running maximum only when it is passed by more than this (log2): the sums are
+// rescaled a few times a row instead of with almost every tile.  Probabilities then reach 2^8 before the
+// division by their sum, which costs no precision (f16 holds up to 2^15).
+constexpr float kSlack = 8.f;
 
 struct PromptParams {
   Cache cache;  // packed keys: k, v, k_row, k_head, v_row, v_head alone
@@ -77,32 +81,29 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int x, int lane
   return false;
 }
 
+// A tile in LDS: rows of kC 16-byte pieces, permuted so that the lanes of a read spread over all banks: a key row's
+// pieces for neighbouring keys; 64 bytes of four neighbouring value rows.  Piece c of row `key` lies at place c ^ *_turn(key).
 template <int kDP>
 struct Shared {
-  static constexpr int kChunks = kDP / 8;  // 16-byte pieces of a row
-  u32x4 k[2][kKeys * kChunks];
-  u32x4 v[2][kKeys * kChunks];
+  static constexpr int kC = kDP / 8;
+  static constexpr uint32_t kTile = kKeys * kDP * 2;
+  u32x4 k[2][kKeys * kC];
+  u32x4 v[2][kKeys * kC];
   // Infinities and NaN among values must not reach the rows that do not see their keys: 0 times them is NaN.  Tiles
   // that some rows see in part hold 0 in their place; the keys they belong to are noted here, and added to
   // the rows that do see them.
-  unsigned long long bad[3];
-  // Where a row's piece lies: pieces are permuted so that the lanes of a read spread over all banks (a key row's pieces
-  // for 8 or 16 neighbouring keys; 64 bytes of four neighbouring value rows).
-  static __device__ __forceinline__ int k_at(int key, int c) {
-    return key * kChunks + (c ^ (kChunks >= 16 ? key & 15 : (key >> 1) & 7));
-  }
-  static __device__ __forceinline__ int v_at(int key, int c) {
-    return key * kChunks + (c ^ (kChunks >= 16 ? 4 * (key & 3) : 4 * ((key >> 1) & 1)));
-  }
+  unsigned long long bad[2];
+  static __device__ __forceinline__ int k_turn(int key) { return kC >= 16 ? key & 15 : (key >> 1) & 7; }
+  static __device__ __forceinline__ int v_turn(int key) { return kC >= 16 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Four 16-bit rows of 16 columns, read by 16 lanes: lane i's address is row i / 4, columns 4 (i % 4) .. + 3; it gets
 // column i of the four rows.
-__device__ __forceinline__ u32x2 read_transposed(const char* at) {
+__device__ __forceinline__ u32x2 read_transposed(uint32_t at) {
   typedef __attribute__((address_space(3))) s16x4* Lds;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds) static_cast<uintptr_t>(at)));
 }
 
 // 0xFFFF in the places of a dword's infinities and NaN.
@@ -112,12 +113,14 @@ __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
   return ((w & kExp) == kExp ? 0xFFFFu : 0u) | ((w >> 16 & kExp) == kExp ? 0xFFFF0000u : 0u);
 }
 
-template <typename E, int kDP, bool kPaged>
+template <typename E, int kDP, bool kPaged, bool kLse>
 __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(PromptParams p) {
   typedef Shared<kDP> S;
-  constexpr int kC = S::kChunks, kPassRows = kThreads / kC, kPasses = kKeys / kPassRows, kSteps = kDP / 16, kBlocks = kDP / 32;
+  constexpr int kC = S::kC, kSteps = kDP / 16, kBlocks = kDP / 32;
+  constexpr int kRowsLoad = kWave / kC, kLoads = kKeys / kWaves / kRowsLoad;  // rows of a direct load; loads of a wave and tile
+  constexpr uint32_t kRow = kDP * 2;
   __shared__ S sm;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, l32 = lane & 31, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
   const int hk = blockIdx.x % p.Hkv;
   int b, tile;
   if (!find_tile(p, blockIdx.x / p.Hkv, lane, &b, &tile)) return;
@@ -132,8 +135,8 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     m = ks.y;
   }
   const int32_t* pages = kPaged ? p.cache.pages + b * p.cache.pages_stride : nullptr;
-  const char* kbase = p.cache.k + hk * p.cache.k_head;
-  const char* vbase = p.cache.v + hk * p.cache.v_head;
+  const char* kbase = p.cache.k + hk * p.cache.k_head + k0 * p.cache.k_row;
+  const char* vbase = p.cache.v + hk * p.cache.v_head + k0 * p.cache.v_row;
 
   // This lane's row, and how many keys it sees.
   const int64_t all = static_cast<int64_t>(n) * p.G, row0 = static_cast<int64_t>(tile) * kRowsTile;
@@ -141,13 +144,13 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   const bool live = row < all;
   const int64_t rc = live ? row : all - 1;
   const int tok = static_cast<int>(rc / p.G), head = hk * p.G + static_cast<int>(rc % p.G);
-  auto sees = [&](int64_t r) { return p.causal ? max(0, min(m, static_cast<int>(r / p.G) + m - n + 1)) : m; };
+  auto sees = [&](int64_t r) { return p.causal ? max(0, min(m, static_cast<int>(min(r, all - 1) / p.G) + m - n + 1)) : m; };
   const int vis = sees(rc);
-  const int64_t w0 = row0 + wave * kRowsWave, w1 = w0 + kRowsWave - 1;
-  const int all_see = sees(row0);                        // keys that every row of the workgroup sees
-  const int wave_all = sees(w0 < all ? w0 : all - 1);   // keys that every row of the wave sees
-  const int wave_any = w0 < all ? sees(w1 < all ? w1 : all - 1) : 0;
-  const int end = sees(row0 + kRowsTile - 1 < all ? row0 + kRowsTile - 1 : all - 1);  // of the workgroup
+  const int64_t w0 = row0 + wave * kRowsWave;
+  const int all_see = __builtin_amdgcn_readfirstlane(sees(row0));                 // keys that every row of the workgroup sees
+  const int wave_all = __builtin_amdgcn_readfirstlane(sees(w0));                  // of the wave
+  const int wave_any = __builtin_amdgcn_readfirstlane(w0 < all ? sees(w0 + kRowsWave - 1) : 0);
+  const int end = __builtin_amdgcn_readfirstlane(sees(row0 + kRowsTile - 1));     // keys that some row sees
 
   u32x4 q[kSteps];
   {
@@ -160,78 +163,106 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
   }
 
-  // The tile's rows on their way: piece c of rows pr, pr + kPassRows, ...
-  const int c = tid % kC, pr = tid / kC;
-  const int cb = 16 * min(c, p.D / 8 - 1);
-  const bool cin = 8 * c < p.D;
-  u32x4 kr[kPasses], vr[kPasses];
-  auto fetch = [&](int kt) {
+  // Loading: load i of a wave covers kRowsLoad rows from 16 wave + i kRowsLoad; lane l takes the piece that belongs at place
+  // l % kC of row l / kC.  Offsets within a tile for packed rows; the pieces of a row for any.
+  const int lrow = 16 * wave + lane / kC, lpos = lane % kC;
+  uint32_t koff[kPaged ? 1 : kLoads], voff[kPaged ? 1 : kLoads];
+  if constexpr (!kPaged) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int key = kt + pr + i * kPassRows;
-      bool ok = key < end;
-      int64_t ko, vo;
-      if constexpr (kPaged) {
-        const uint32_t slot = static_cast<uint32_t>(key) / p.cache.page_size, off = static_cast<uint32_t>(key) - slot * p.cache.page_size;
-        const uint32_t page = ok ? static_cast<uint32_t>(pages[slot]) : 0xFFFFFFFFu;
-        ok = page < p.cache.n_pages;
-        ko = page * p.cache.k_page + off * p.cache.k_row;
-        vo = page * p.cache.v_page + off * p.cache.v_row;
-      } else {
-        ko = (k0 + key) * p.cache.k_row;
-        vo = (k0 + key) * p.cache.v_row;
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = lrow + i * kRowsLoad;
+      koff[i] = key * static_cast<uint32_t>(p.cache.k_row) + 16 * (lpos ^ S::k_turn(key));
+      voff[i] = key * static_cast<uint32_t>(p.cache.v_row) + 16 * (lpos ^ S::v_turn(key));
+    }
+  }
+  const uint32_t lds_k = lds_addr(sm.k[0][0]) + wave * (S::kTile / kWaves), lds_v = lds_addr(sm.v[0][0]) + wave * (S::kTile / kWaves);
+  const bool exact = p.D == kDP;
+  // K or V rows kt .. kt + 63 into buffer buf.
+  auto load = [&](bool values, int kt, int buf) {
+    const uint32_t to = (values ? lds_v : lds_k) + buf * S::kTile;
+    if constexpr (!kPaged) {
+      if (kt + kKeys <= end && exact) {
+        const char* from = values ? vbase + kt * p.cache.v_row : kbase + kt * p.cache.k_row;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) dma16s(from, values ? voff[i] : koff[i], to + i * (kWave * 16));
+        return;
       }
-      const char* zero = reinterpret_cast<const char*>(kZeroRow);
-      kr[i] = *reinterpret_cast<const u32x4*>((ok ? kbase + ko : zero) + cb);
-      vr[i] = *reinterpret_cast<const u32x4*>((ok ? vbase + vo : zero) + cb);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row_in = lrow + i * kRowsLoad, key = kt + row_in, c = lpos ^ (values ? S::v_turn(row_in) : S::k_turn(row_in));
+      bool ok = key < end;
+      const char* from;
+      if constexpr (kPaged) {
+        const uint32_t pg = static_cast<uint32_t>(key) / p.cache.page_size, off = static_cast<uint32_t>(key) - pg * p.cache.page_size;
+        const uint32_t page = ok ? static_cast<uint32_t>(pages[pg]) : 0xFFFFFFFFu;
+        ok = page < p.cache.n_pages;
+        from = values ? vbase + page * p.cache.v_page + off * p.cache.v_row : kbase + page * p.cache.k_page + off * p.cache.k_row;
+      } else {
+        from = values ? vbase + key * p.cache.v_row : kbase + key * p.cache.k_row;
+      }
+      from = ok && 8 * c < p.D ? from + 16 * c : reinterpret_cast<const char*>(kZeroRow);
+      dma16(from, to + i * (kWave * 16));
     }
   };
+
+  // Lane parts of the operands' LDS addresses.
+  uint32_t kat[kSteps], vat[kBlocks];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) kat[s] = lds_addr(sm.k[0][0]) + l32 * kRow + 16 * ((2 * s + h) ^ S::k_turn(l32));
+  {
+    const int i16 = lane & 15, row_in = 4 * h + (i16 >> 2);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+      vat[i] = lds_addr(sm.v[0][0]) + row_in * kRow + 16 * ((4 * i + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ S::v_turn(row_in)) + 8 * (i16 & 1);
+  }
 
   f32x16 acc[kBlocks];
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) acc[i] = f32x16{};
-  float top = -INFINITY, sum = 0.f;
+  // top: what the exponentials are taken against, within kSlack of the maximum.  The row is divided by the sum of the rounded
+  // probabilities that weigh its values, so that their roundings cancel as far as they agree (a row of one key is that
+  // key's value); the log-sum-exp, where it is asked for, takes the sum of the unrounded ones.
+  float top = -INFINITY, sum = 0.f, full = 0.f;
 
-  // Lane parts of the operands' LDS addresses.
-  const int v16 = lane & 15, vg = (lane >> 4) & 1;
-  if (end > 0) fetch(0);
-  if (tid < 3) sm.bad[tid] = 0;
-  __syncthreads();
-  int buf = 0, slot = 0;
-  for (int kt = 0; kt < end; kt += kKeys, buf ^= 1, slot = slot == 2 ? 0 : slot + 1) {
+  auto step = [&](int t, auto bufc) {
+    constexpr int buf = decltype(bufc)::value;
+    const int kt = t * kKeys;
+    pipeline_barrier();  // this tile is there, the other buffer read
+    if (kt + kKeys < end) {
+      load(false, kt + kKeys, buf ^ 1);
+      load(true, kt + kKeys, buf ^ 1);
+    }
     const bool part_seen = kt + kKeys > all_see;
+    if (part_seen) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int key = pr + i * kPassRows;
-      if (part_seen) {
+      for (int i = 0; i < kKeys * kC / kThreads; ++i) {
+        const int at = tid + i * kThreads;
+        const uint32_t addr = lds_addr(sm.v[buf][0]) + 16 * at;
+        const u32x4 x = lds_ld<u32x4>(addr);
         u32x4 is;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) is[a] = nonfinite<E>(vr[i][a]);
-        if (cin && (is[0] | is[1] | is[2] | is[3])) atomicOr(&sm.bad[slot], 1ull << key);
-        vr[i] &= ~is;
+        for (int a = 0; a < 4; ++a) is[a] = nonfinite<E>(x[a]);
+        if (is[0] | is[1] | is[2] | is[3]) {
+          lds_st(addr, x & ~is);
+          atomicOr(&sm.bad[buf], 1ull << (at / kC));
+        }
       }
-      sm.k[buf][S::k_at(key, c)] = cin ? kr[i] : u32x4{0, 0, 0, 0};
-      sm.v[buf][S::v_at(key, c)] = cin ? vr[i] : u32x4{0, 0, 0, 0};
+      lds_barrier();
+      if (tid == 0) sm.bad[buf ^ 1] = 0;
     }
-    __syncthreads();
-    if (tid == 0) sm.bad[slot == 0 ? 2 : slot - 1] = 0;  // the tile before's, which the tile after next takes
+    if (kt >= wave_any) return;  // the other waves' rows see this tile
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>(kat[st] + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
     uint64_t exists = ~uint64_t{0};
     if constexpr (kPaged) {
       const int key = kt + lane;
       exists = __ballot(key < end && static_cast<uint32_t>(pages[static_cast<uint32_t>(key) / p.cache.page_size]) < p.cache.n_pages);
     }
-    if (kt + kKeys < end) fetch(kt + kKeys);
-    if (kt >= wave_any) continue;  // the other waves' rows see this tile
-
-    f32x16 s[2];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      s[blk] = f32x16{};
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st) s[blk] = E::mfma32(sm.k[buf][S::k_at(32 * blk + l32, 2 * st + h)], q[st], s[blk]);
-    }
-    const bool whole = kt + kKeys <= wave_all && exists == ~uint64_t{0};
-    if (!whole) {
+    if (!(kt + kKeys <= wave_all && exists == ~uint64_t{0})) {
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -240,50 +271,54 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
           if (kt + key >= vis || !((exists >> key) & 1)) s[blk][r] = -INFINITY;
         }
     }
-    float t = -INFINITY;
+    float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t = fmaxf(t, s[blk][r]);
-    t = fmaxf(top, op_over(t, 32, 64, OpMax{}) * p.scale_log2);
-    const float mm = finite_max(t), f = exp2_fast(top - mm);
-    top = t;
-    float part = 0.f;
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[blk][r] = exp2_fast(s[blk][r] * p.scale_log2 - mm);
-        part += s[blk][r];
-      }
-    sum = sum * f + part;
-    if (__any(f != 1.f)) {
+      for (int blk = 0; blk < 2; ++blk) m2[blk] = fmaxf(m2[blk], s[blk][r]);
+    const float t2 = op_over(fmaxf(m2[0], m2[1]), 32, 64, OpMax{}) * p.scale_log2;
+    if (__any(t2 > top + kSlack)) {
+      const float up = fmaxf(top, t2), f = exp2_fast(top - finite_max(up));
+      top = up;
+      sum *= f;
+      full *= f;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
     }
+    const float mm = finite_max(top);
+    float part[2] = {0.f, 0.f};
+    u32x4 prob[4];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {  // 16 keys
-      u32x4 prob;
+    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int a = 0; a < 4; ++a) prob[a] = pack2<E>(s[kk >> 1][8 * (kk & 1) + 2 * a], s[kk >> 1][8 * (kk & 1) + 2 * a + 1]);
+      for (int a = 0; a < 4; ++a) {
+        const float x = exp2_fast(s[kk >> 1][8 * (kk & 1) + 2 * a] * p.scale_log2 - mm);
+        const float y = exp2_fast(s[kk >> 1][8 * (kk & 1) + 2 * a + 1] * p.scale_log2 - mm);
+        prob[kk][a] = pack2<E>(x, y);
+        sum = E::add2(prob[kk][a], sum);
+        if constexpr (kLse) {
+          part[0] += x;
+          part[1] += y;
+        }
+      }
+    if constexpr (kLse) full += part[0] + part[1];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)  // 16 keys
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        const int key = 16 * kk + 4 * h + (v16 >> 2), cc = 4 * i + 2 * vg + ((v16 & 3) >> 1);
-        const char* base = reinterpret_cast<const char*>(sm.v[buf]) + 8 * (v16 & 1);
-        const u32x2 lo = read_transposed(base + 16 * S::v_at(key, cc)), hi = read_transposed(base + 16 * S::v_at(key + 8, cc));
-        const u32x4 vt{lo[0], lo[1], hi[0], hi[1]};
-        acc[i] = E::mfma32(vt, prob, acc[i]);
+        const uint32_t at = vat[i] + buf * S::kTile + 16 * kk * kRow;
+        const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
+        acc[i] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, prob[kk], acc[i]);
       }
-    }
     if (part_seen) {  // what was cleared, to the rows that see it
-      for (uint64_t bad = sm.bad[slot]; bad; bad &= bad - 1) {
+      for (uint64_t bad = sm.bad[buf]; bad; bad &= bad - 1) {
         const int key = kt + __builtin_ctzll(bad);
         int64_t vo;
         if constexpr (kPaged) {
           const uint32_t pg = static_cast<uint32_t>(key) / p.cache.page_size;
           vo = pages[pg] * p.cache.v_page + (static_cast<uint32_t>(key) - pg * p.cache.page_size) * p.cache.v_row;
         } else {
-          vo = (k0 + key) * p.cache.v_row;
+          vo = key * p.cache.v_row;
         }
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
@@ -301,6 +336,17 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
           }
       }
     }
+  };
+
+  if (end > 0) {
+    if (tid < 2) sm.bad[tid] = 0;
+    load(false, 0, 0);
+    load(true, 0, 0);
+    const int tiles = (end + kKeys - 1) / kKeys;
+    for (int t = 0; t < tiles; t += 2) {
+      step(t, std::integral_constant<int, 0>{});
+      if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>{});
+    }
   }
 
   if (!live) return;
@@ -316,8 +362,10 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
         *reinterpret_cast<u32x2*>(dst + 2 * d) = u32x2{pack2<E>(acc[i][4 * rr] * inv, acc[i][4 * rr + 1] * inv),
                                                        pack2<E>(acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv)};
     }
-  if (p.lse && h == 0)
-    p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+  if constexpr (kLse) {
+    full = op_over(full, 32, 64, OpAdd{});
+    if (h == 0) p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
+  }
 }
 
 int validate(const latent_attn_prompt_args& a) {
@@ -395,10 +443,14 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
     constexpr int kDP = decltype(dp)::value;
     using E = decltype(e);
     const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, tiles) * p.Hkv));
-    if (paged)
-      hipLaunchKernelGGL((prompt_kernel<E, kDP, true>), grid, dim3(kThreads), 0, s, p);
-    else
-      hipLaunchKernelGGL((prompt_kernel<E, kDP, false>), grid, dim3(kThreads), 0, s, p);
+    auto go = [&](auto paged_c) {
+      constexpr bool kPaged = decltype(paged_c)::value;
+      if (p.lse)
+        hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, true>), grid, dim3(kThreads), 0, s, p);
+      else
+        hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, false>), grid, dim3(kThreads), 0, s, p);
+    };
+    paged ? go(std::true_type{}) : go(std::false_type{});
   };
   auto with_type = [&](auto e) {
     if (p.D <= 64)
