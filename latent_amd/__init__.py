@@ -20,6 +20,7 @@ from ._lib import (  # noqa: F401
     lib,
 )
 from .attention import (  # noqa: F401
+    Attention,
     attend_decode,
     attend_decode_workspace_size,
     attend_prompt,

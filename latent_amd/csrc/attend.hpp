@@ -129,7 +129,7 @@ struct Cache {
 
 // ---- host ---------------------------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0; }
+inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s <= int64_t{1} << 40; }
 
 // Sizes every call shares.
 inline int check_heads(int64_t n_head, int64_t n_kv_head, int64_t head_dim, int32_t dtype) {

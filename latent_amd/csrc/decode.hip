@@ -46,6 +46,7 @@ struct DecodeParams {
   uint32_t chunks;     // chunks of a head's query heads
   uint32_t rows;       // query heads of a chunk (the last may have fewer)
   uint32_t U;          // units of a sequence: n_kv_head * chunks
+  bool whole;          // a workgroup a unit
   float scale_log2;
   // Workspace: parts [groups][2][rows] (max, sum), [groups][2][rows][D] rows, and for each unit its first workgroup and number of parts.
   float* part_ml;
@@ -284,24 +285,47 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int n16 = lane & 15, kq = lane >> 4;
 
-  // Sequences without keys: a unit of no parts, a row of zeros.
-  for (uint32_t b = blockIdx.x; b < p.B; b += gridDim.x) {
-    if (length_of(p, b) != 0) continue;
-    for (uint32_t i = threadIdx.x; i < p.Hq * (p.D / 8); i += kThreads) {
-      const uint32_t h = i / (p.D / 8), c = i % (p.D / 8);
+  // Zeros for query heads [h0, h1) of sequence b, which has no keys.
+  auto write_zeros = [&](uint32_t b, uint32_t h0, uint32_t h1) {
+    for (uint32_t i = threadIdx.x; i < (h1 - h0) * (p.D / 8); i += kThreads) {
+      const uint32_t h = h0 + i / (p.D / 8), c = i % (p.D / 8);
       *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = u32x4{0, 0, 0, 0};
       if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = -INFINITY;
     }
-    for (uint32_t u = threadIdx.x; u < p.U; u += kThreads) p.unit_parts[b * p.U + u] = int2{0, 0};
+  };
+  uint32_t cur, last, per = 1, b, u, tile = 0, len, nt;
+  if (p.whole) {
+    b = blockIdx.x / p.U;
+    u = blockIdx.x % p.U;
+    len = length_of(p, b);
+    nt = tiles_of(len);
+    cur = 0;
+    last = nt;
+    if (len == 0) {
+      const uint32_t h0 = u / p.chunks * p.G + (u % p.chunks) * p.rows;
+      write_zeros(b, h0, min(h0 + p.rows, (u / p.chunks + 1) * p.G));
+      return;
+    }
+  } else {
+    // Sequences without keys: units of no parts, rows of zeros.
+    for (b = blockIdx.x; b < p.B; b += gridDim.x) {
+      if (length_of(p, b) != 0) continue;
+      write_zeros(b, 0, p.Hq);
+      for (uint32_t i = threadIdx.x; i < p.U; i += kThreads) p.unit_parts[b * p.U + i] = int2{0, 0};
+    }
+    const Span span = find_span(p, lane);
+    cur = span.begin;
+    last = span.end;
+    per = span.per;
+    if (cur == last) return;
+    b = span.b;
+    len = length_of(p, b);
+    nt = tiles_of(len);
+    u = (cur - span.base * p.U) / nt;
+    tile = (cur - span.base * p.U) % nt;
   }
-
-  const Span span = find_span(p, lane);
-  uint32_t cur = span.begin, b = span.b;
-  if (cur == span.end) return;
-  uint32_t len = length_of(p, b), nt = tiles_of(len);
-  uint32_t u = (cur - span.base * p.U) / nt, tile = (cur - span.base * p.U) % nt;
-  while (cur < span.end) {
-    const uint32_t n = min(nt - tile, span.end - cur);
+  while (cur < last) {
+    const uint32_t n = min(nt - tile, last - cur);
     const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
     Stream<E, kDP, kExact, kMT, kPage8> st{p, lane, kq, len, p.cache.pages + b * p.cache.pages_stride,
                                            p.cache.k + hk * p.cache.k_head, p.cache.v + hk * p.cache.v_head};
@@ -383,11 +407,11 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
       }
       __syncthreads();
     }
-    if (tile == 0 && threadIdx.x == 0)
-      p.unit_parts[b * p.U + u] = int2{static_cast<int>(blockIdx.x), static_cast<int>((cur + nt - 1) / span.per - blockIdx.x + 1)};
+    if (!p.whole && tile == 0 && threadIdx.x == 0)
+      p.unit_parts[b * p.U + u] = int2{static_cast<int>(blockIdx.x), static_cast<int>((cur + nt - 1) / per - blockIdx.x + 1)};
     cur += n;
     tile = 0;
-    if (++u == p.U && cur < span.end) {
+    if (++u == p.U && cur < last) {
       u = 0;
       do len = length_of(p, ++b);
       while (len == 0 && b + 1 < p.B);
@@ -396,71 +420,82 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
   }
 }
 
-// Joins the parts of one unit, a query head a workgroup pass.
+// Joins the parts of a unit: lane i of blockIdx.y holds eight elements of one row, each wave a quarter of the parts.
+// A single pass under a running maximum, four parts in flight.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
-  __shared__ float red[kWaves];
-  __shared__ float weight[kMaxGroups];
-  __shared__ float rows[kThreads / 16][kMaxDim];
+  __shared__ float sm[kWaves][10][kWave];
   const uint32_t unit = blockIdx.x, b = unit / p.U, u = unit % p.U;
   const int2 parts = p.unit_parts[unit];
   if (parts.y < 2) return;
   const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const uint32_t lanes = p.D / 8, sets = kThreads / 32;  // a part's row in at most 32 lanes of 8 elements
-  for (uint32_t row = blockIdx.y; row < nr; row += gridDim.y) {
-    auto at = [&](int i) { return (static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row; };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < parts.y; i += kThreads) m = fmaxf(m, p.part_ml[2 * at(i)]);
-    m = op_over(m, 1, 64, OpMax{});
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    __syncthreads();
-    float l = 0.f;
-    for (int i = threadIdx.x; i < parts.y; i += kThreads) {
-      const float f = exp2_fast(p.part_ml[2 * at(i)] - finite_max(m));
-      weight[i] = f;
-      l += f * p.part_ml[2 * at(i) + 1];
+  const uint32_t pieces = p.D / 8, item = blockIdx.y * kWave + lane, row = min(item / pieces, nr - 1), c = item % pieces;
+  float m = -INFINITY, l = 0.f;
+  f32x4 x[2] = {};
+  for (int i0 = wave; i0 < parts.y; i0 += 4 * kWaves) {
+    float pm[4], pl[4];
+    f32x4 px[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = min(i0 + j * kWaves, parts.y - 1);
+      const int64_t at = (static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
+      pm[j] = i0 + j * kWaves < parts.y ? p.part_ml[2 * at] : -INFINITY;
+      pl[j] = p.part_ml[2 * at + 1];
+      const f32x4* src = reinterpret_cast<const f32x4*>(p.part_acc + at * p.D + 8 * c);
+      px[j][0] = src[0];
+      px[j][1] = src[1];
     }
-    l = op_over(l, 1, 64, OpAdd{});
-    if (lane == 0) red[wave] = l;
-    __syncthreads();
-    l = red[0] + red[1] + red[2] + red[3];
-    const uint32_t set = threadIdx.x / 32, c = threadIdx.x % 32;
-    f32x4 x[2] = {};
-    if (c < lanes) {
-#pragma unroll 4
-      for (uint32_t i = set; i < static_cast<uint32_t>(parts.y); i += sets) {
-        const f32x4* src = reinterpret_cast<const f32x4*>(p.part_acc + at(i) * p.D + 8 * c);
-        x[0] += src[0] * weight[i];
-        x[1] += src[1] * weight[i];
-      }
-      *reinterpret_cast<f32x4*>(&rows[set][8 * c]) = x[0];
-      *reinterpret_cast<f32x4*>(&rows[set][8 * c + 4]) = x[1];
+    const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), mm = finite_max(top), f = exp2_fast(m - mm);
+    m = top;
+    l *= f;
+    x[0] *= f;
+    x[1] *= f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w = exp2_fast(pm[j] - mm);
+      if (pm[j] == -INFINITY && pl[j] == pl[j]) continue;  // no keys (a repeated last part among them), and no NaN to pass on
+      l += w * pl[j];
+      x[0] += px[j][0] * w;
+      x[1] += px[j][1] * w;
     }
-    __syncthreads();
-    if (threadIdx.x < p.D / 2) {
-      float y[2] = {};
-      for (uint32_t s = 0; s < sets; ++s) {
-        y[0] += rows[s][2 * threadIdx.x];
-        y[1] += rows[s][2 * threadIdx.x + 1];
-      }
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-      const uint32_t h = hk * p.G + r0 + row;
-      *reinterpret_cast<uint32_t*>(p.out + b * p.o_token + h * p.o_head + 4 * threadIdx.x) = pack2<E>(y[0] * inv, y[1] * inv);
-      if (p.lse && threadIdx.x == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-    }
-    __syncthreads();
   }
+  sm[wave][0][lane] = m;
+  sm[wave][1][lane] = l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sm[wave][2 + e][lane] = x[e >> 2][e & 3];
+  __syncthreads();
+  if (wave != 0 || item >= nr * pieces) return;
+  float y[8] = {};
+  m = fmaxf(fmaxf(sm[0][0][lane], sm[1][0][lane]), fmaxf(sm[2][0][lane], sm[3][0][lane]));
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float f = exp2_fast(sm[w][0][lane] - finite_max(m));
+    l += f * sm[w][1][lane];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] += f * sm[w][2 + e][lane];
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  const uint32_t h = hk * p.G + r0 + row;
+  u32x4 o;
+#pragma unroll
+  for (int a = 0; a < 4; ++a) o[a] = pack2<E>(y[2 * a] * inv, y[2 * a + 1] * inv);
+  *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = o;
+  if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 struct Plan {
   int mt;
   uint32_t chunks, rows, U, groups;
+  bool whole;
   size_t ml_bytes, acc_bytes, unit_bytes;
-  bool split;  // some unit may be split
 };
+
+// Up to this many tiles of the longest sequence a page table holds, each unit is one workgroup's: the parts and the
+// second launch cost more than the tiles one after the other.
+constexpr int64_t kMaxUnits = 1 << 22;  // workgroups of a launch
+constexpr int64_t kWholeTiles = 4;
 
 Plan plan_for(const latent_attn_decode_args& a) {
   Plan pl{};
@@ -471,8 +506,13 @@ Plan plan_for(const latent_attn_decode_args& a) {
   pl.U = static_cast<uint32_t>(a.n_kv_head) * pl.chunks;
   const int64_t tiles = (a.cache.max_pages * a.cache.page_size + kTile - 1) / kTile;
   const int64_t items = a.cache.n_seq * pl.U * tiles;
-  pl.groups = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(items, kMaxGroups)));
-  pl.split = tiles > 1;
+  const int64_t units = a.cache.n_seq * pl.U;
+  pl.whole = tiles <= kWholeTiles;
+  if (pl.whole) {
+    pl.groups = static_cast<uint32_t>(units);
+    return pl;
+  }
+  pl.groups = static_cast<uint32_t>(std::min<int64_t>(items, kMaxGroups));
   const size_t parts = static_cast<size_t>(pl.groups) * 2 * pl.rows;
   auto up = [](size_t n) { return (n + 15) & ~size_t{15}; };
   pl.ml_bytes = up(parts * 2 * sizeof(float));
@@ -489,6 +529,7 @@ int validate(const latent_attn_decode_args& a) {
   if (sc != LATENT_OK) return sc;
   // Tiles and output rows are counted in 32 bits.
   const Plan pl = plan_for(a);
+  if (a.cache.n_seq * pl.U > kMaxUnits) return LATENT_E_UNSUPPORTED;
   const int64_t tiles = (a.cache.max_pages * a.cache.page_size + kTile - 1) / kTile;
   if (a.cache.n_seq * pl.U > INT32_MAX / std::max<int64_t>(1, tiles) - kMaxGroups) return LATENT_E_UNSUPPORTED;
   return LATENT_OK;
@@ -524,7 +565,7 @@ extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_st
     if (!stride_ok(s)) return LATENT_E_UNSUPPORTED;
   if ((a.n_head > 1 && !a.out_head_stride) || (a.cache.n_seq > 1 && !a.out_token_stride)) return LATENT_E_INVALID;
   const Plan pl = plan_for(a);
-  if (!a.workspace || a.workspace_bytes < pl.ml_bytes + pl.acc_bytes + pl.unit_bytes) return LATENT_E_WORKSPACE;
+  if (!pl.whole && (!a.workspace || a.workspace_bytes < pl.ml_bytes + pl.acc_bytes + pl.unit_bytes)) return LATENT_E_WORKSPACE;
   DecodeParams p{};
   p.cache = device_cache(a.cache);
   if (!keys) p.cache.max_len = 0;
@@ -541,6 +582,7 @@ extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_st
   p.chunks = pl.chunks;
   p.rows = pl.rows;
   p.U = pl.U;
+  p.whole = pl.whole;
   p.scale_log2 = a.scale * kLog2e;
   char* ws = static_cast<char*>(a.workspace);
   p.part_ml = reinterpret_cast<float*>(ws);
@@ -576,10 +618,8 @@ extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_st
   const bool f16 = a.dtype == LATENT_F16;
   f16 ? with_type(F16{}) : with_type(BF16{});
   if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
-  if (pl.split) {
-    // Units that were split have no more than kMaxGroups workgroups between them; where units are few, rows are spread.
-    const uint32_t units = p.B * p.U;
-    const dim3 grid(units, std::max(1u, std::min(p.rows, 2048 / units)));
+  if (!pl.whole) {
+    const dim3 grid(p.B * p.U, (p.rows * (p.D / 8) + kWave - 1) / kWave);
     if (f16)
       hipLaunchKernelGGL(join_kernel<F16>, grid, dim3(kThreads), 0, s, p);
     else

@@ -413,6 +413,8 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
     for (int64_t s : {a.k_token_stride, a.k_head_stride, a.v_token_stride, a.v_head_stride})
       if (!stride_ok(s)) return LATENT_E_UNSUPPORTED;
     if (!aligned16(a.k) || !aligned16(a.v)) return LATENT_E_UNSUPPORTED;
+    // A tile's rows are addressed from its first in 32 bits.
+    if (a.n_keys > 1 && (a.k_token_stride > (1 << 24) || a.v_token_stride > (1 << 24))) return LATENT_E_UNSUPPORTED;
     p.cache.k = static_cast<const char*>(a.k);
     p.cache.v = static_cast<const char*>(a.v);
     p.cache.k_row = a.k_token_stride * 2, p.cache.k_head = a.k_head_stride * 2;

@@ -1,0 +1,147 @@
+"""DecodeStack with attention blocks: its steps are the public calls in their order, replays equal eager
+steps bit for bit, prompts leave the slots ready to decode, idle slots take no part."""
+
+import numpy as np
+import pytest
+
+from oracle import synth
+from tests._attention import assert_attention, visible
+from tests._layers import to_device
+
+pytestmark = pytest.mark.gpu
+
+D_MODEL, HQ, HKV, D, PAGE, PAGES = 256, 4, 2, 64, 16, 40
+
+
+@pytest.fixture(scope="module")
+def parts(gpu):
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    # Rank 256: the tile layout, whose paths sum in a fixed order.
+    layers = [to_device(synth.make_layer(seed=s, n_expert=8, d=D_MODEL, ff=256, max_rank=256)) for s in (1, 2)]
+    assert all(L.layout == "tiles" for L in layers)
+    routers = [gpu.Router(torch.randn((D_MODEL, 8), generator=gen, device="cuda"), 2) for _ in layers]
+    ws = [((torch.randn((D_MODEL, (HQ + 2 * HKV) * D), generator=gen, device="cuda") / 16).bfloat16(),
+           (torch.randn((HQ * D, D_MODEL), generator=gen, device="cuda") / 16).bfloat16()) for _ in layers]
+    return layers, routers, ws, gpu.rope_table(200, D)
+
+
+def _stack(gpu, parts, T, max_pages=8):
+    import torch
+
+    layers, routers, ws, rope = parts
+    blocks = [gpu.Attention(a, b, HQ, HKV, PAGES, PAGE, rope=rope) for a, b in ws]
+    s = gpu.DecodeStack(layers, routers, T, attention=blocks, max_pages=max_pages)
+    order = np.random.default_rng(3).permutation(PAGES).astype(np.int32)
+    s.pages.copy_(torch.from_numpy(order[:T * max_pages].reshape(T, max_pages)).cuda())
+    return s
+
+
+def _x(gen, n):
+    import torch
+
+    return torch.randn((n, D_MODEL), generator=gen, device="cuda")
+
+
+def _ints(v):
+    import torch
+
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def test_step_is_the_public_calls_in_order(gpu, parts):
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    layers, routers, ws, rope = parts
+    s = _stack(gpu, parts, 3)
+    s.positions.copy_(_ints([0, 0, -1]))
+    caches = [tuple(torch.zeros_like(a.k_cache) for _ in range(2)) for a in s.attention]
+    pos = _ints([0, 0, -1])
+    for _ in range(4):
+        x0 = _x(gen, 3)
+        got = s.forward(x0).clone()
+        x = x0
+        for L, r, (wqkv, wo), (kc, vc) in zip(layers, routers, ws, caches):
+            qkv = (x.bfloat16() @ wqkv).view(3, HQ + 2 * HKV, D)
+            q = gpu.kv_append(qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], kc, vc, s.pages, pos, q=qkv[:, :HQ], rope=rope)
+            a = gpu.attend_decode(q, kc, vc, s.pages, pos + 1)
+            assert bool((a[2] == 0).all())  # the idle slot
+            for b in range(2):
+                n = int(pos[b]) + 1
+                at = torch.arange(n, device="cuda")
+                rows = s.pages[b].long()[at // PAGE]
+                assert_attention(a[b:b + 1], None, q[b:b + 1], kc[rows, at % PAGE], vc[rows, at % PAGE],
+                                 visible(1, n, True, "cuda"), D ** -0.5)
+            h = x + a.view(3, -1) @ wo
+            ids, w = r(h)
+            x = h + gpu.moe_forward(h, ids, w, L)
+        assert torch.equal(got, x)
+        pos = pos + (pos >= 0)
+        assert torch.equal(s.positions, pos)
+    for a, (kc, vc) in zip(s.attention, caches):
+        assert torch.equal(a.k_cache, kc) and torch.equal(a.v_cache, vc)
+
+
+def test_captured_steps_equal_eager_steps(gpu, parts):
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    eager, graph = _stack(gpu, parts, 4), _stack(gpu, parts, 4)
+    n = [37, 5, 20]
+    x = _x(gen, sum(n))
+    starts, slots = _ints([0, 37, 42, 62]), _ints([2, 0, 1])  # slot 3 stays idle
+    want = eager.prompt(x, starts, slots)
+    assert torch.equal(graph.prompt(x, starts, slots), want)
+    assert eager.positions.tolist() == [5, 20, 37, -1]
+    graph.capture()
+    assert graph.positions.tolist() == [5, 20, 37, -1]
+    for i in range(5):
+        x0 = _x(gen, 4)
+        graph.load(x0)
+        got = graph.replay()
+        assert torch.equal(got, eager.forward(x0)), i
+        torch.cuda.synchronize()
+    assert graph.positions.tolist() == eager.positions.tolist() == [10, 25, 42, -1]
+
+
+def test_prompt_in_chunks_attends_to_what_is_cached(gpu, parts):
+    """The first layer of a chunked prompt: its cache equals the one of the whole prompt (row by row, as far as the
+    projections of different batches agree), and its queries see the cached part."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    whole, chunks = _stack(gpu, parts, 2), _stack(gpu, parts, 2)
+    x = _x(gen, 100)
+    whole.prompt(x, _ints([0, 60, 100]), _ints([0, 1]))
+    chunks.prompt(torch.cat((x[:33], x[60:75])), _ints([0, 33, 48]), _ints([0, 1]))
+    chunks.prompt(torch.cat((x[75:100], x[33:60])), _ints([0, 25, 52]), _ints([1, 0]))
+    assert whole.positions.tolist() == chunks.positions.tolist() == [60, 40]
+    a, b = whole.attention[0], chunks.attention[0]
+    for got, want in ((b.k_cache, a.k_cache), (b.v_cache, a.v_cache)):
+        # Sums of 256 products in another order, rounded once: 256 * 2^-24 of their size, and a step of bf16.
+        assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+        assert torch.equal(got == 0, want == 0)
+
+
+def test_refusals(gpu, parts):
+    import torch
+
+    layers, routers, ws, rope = parts
+    block = gpu.Attention(*ws[0], HQ, HKV, PAGES, PAGE, rope=rope)
+    with pytest.raises(ValueError):
+        gpu.DecodeStack(layers, routers, 2, attention=[block], max_pages=4)
+    with pytest.raises(ValueError):
+        gpu.DecodeStack(layers, routers, 2, attention=[block, block])
+    with pytest.raises(ValueError):
+        gpu.DecodeStack(layers, routers, 2, max_pages=4)
+    with pytest.raises(RuntimeError):
+        gpu.DecodeStack(layers, routers, 2).prompt(torch.zeros((1, D_MODEL), device="cuda"), _ints([0, 1]), _ints([0]))
+    with pytest.raises(ValueError):
+        gpu.Attention(ws[0][0], ws[0][1], 3, 2, PAGES, PAGE)
+    with pytest.raises(TypeError):
+        gpu.Attention(ws[0][0].float(), ws[0][1].float(), HQ, HKV, PAGES, PAGE)
+    s = _stack(gpu, parts, 2)
+    with pytest.raises(ValueError):
+        s.prompt(torch.zeros((2, D_MODEL), device="cuda"), _ints([0, 2]), _ints([0, 1]))
