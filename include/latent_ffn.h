@@ -515,16 +515,25 @@ typedef struct latent_attn_prompt_args {
   int64_t k_token_stride, k_head_stride;
   int64_t v_token_stride, v_head_stride;
   int64_t n_tokens;
-  int64_t n_keys;
+  int64_t n_keys;   /* rows of k and v; 0 with the cache */
   int64_t n_head;
   int64_t n_kv_head;
   int64_t head_dim;
   int32_t dtype;
   int32_t causal;
-  float scale; /* > 0 */
+  float scale;            /* > 0 */
+  void* workspace;        /* device scratch of latent_attn_prompt_workspace_size() bytes, 16-byte aligned, or NULL */
+  size_t workspace_bytes;
 } latent_attn_prompt_args;
 
-/* Stream ordered; allocates nothing and needs no workspace. */
+/*
+ * Scratch with which a call of few or uneven sequences splits long rows of keys
+ * over the chip; 0 where it would not.  A call given less takes each
+ * 128 rows in one workgroup: the same results to rounding, later.
+ */
+int latent_attn_prompt_workspace_size(const latent_attn_prompt_args* args, size_t* bytes);
+
+/* Stream ordered; allocates nothing; calls that may overlap need workspaces of their own. */
 int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stream);
 
 #ifdef __cplusplus

@@ -25,6 +25,7 @@ from .attention import (  # noqa: F401
     attend_decode_workspace_size,
     attend_prompt,
     attend_prompt_paged,
+    attend_prompt_workspace_size,
     kv_append,
     rope_table,
 )

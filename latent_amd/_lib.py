@@ -58,6 +58,7 @@ EXPORTED = (
     "latent_kv_append",
     "latent_attn_decode_workspace_size",
     "latent_attn_decode",
+    "latent_attn_prompt_workspace_size",
     "latent_attn_prompt",
 )
 
@@ -217,6 +218,8 @@ class LatentAttnPromptArgs(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("causal", ctypes.c_int32),
         ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -280,6 +283,10 @@ def _load() -> ctypes.CDLL:
     ]
     lib.latent_attn_decode.restype = ctypes.c_int
     lib.latent_attn_decode.argtypes = [ctypes.POINTER(LatentAttnDecodeArgs), ctypes.c_void_p]
+    lib.latent_attn_prompt_workspace_size.restype = ctypes.c_int
+    lib.latent_attn_prompt_workspace_size.argtypes = [
+        ctypes.POINTER(LatentAttnPromptArgs), ctypes.POINTER(ctypes.c_size_t),
+    ]
     lib.latent_attn_prompt.restype = ctypes.c_int
     lib.latent_attn_prompt.argtypes = [ctypes.POINTER(LatentAttnPromptArgs), ctypes.c_void_p]
     return lib

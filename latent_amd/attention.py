@@ -66,6 +66,7 @@ _append_args, _append = _packer(LatentKvAppendArgs), _entry("latent_kv_append")
 _decode_args, _decode = _packer(LatentAttnDecodeArgs), _entry("latent_attn_decode")
 _decode_size = _entry("latent_attn_decode_workspace_size")
 _prompt_args, _prompt_call = _packer(LatentAttnPromptArgs), _entry("latent_attn_prompt")
+_prompt_size = _entry("latent_attn_prompt_workspace_size")
 
 
 def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -318,7 +319,7 @@ def attend_decode_workspace_size(n_seq: int, n_head: int, n_kv_head: int, head_d
     return _decode_need(page_size, n_seq, max_pages, n_head, n_kv_head, head_dim)
 
 
-def _prompt(q, starts, cache, Hkv, keys, k_starts, lengths, n_keys, causal, scale, out, lse, dev) -> torch.Tensor:
+def _prompt(q, starts, cache, Hkv, keys, k_starts, lengths, n_keys, causal, scale, out, lse, workspace, dev) -> torch.Tensor:
     """keys: base and strides of k and v, (k, v, k token, k head, v token, v head), zeros for the cache's."""
     q, qp, qt, qh, (T, Hq, D) = q
     B = cache[5]
@@ -329,13 +330,36 @@ def _prompt(q, starts, cache, Hkv, keys, k_starts, lengths, n_keys, causal, scal
     lp = _lse(lse, T, Hq, dev)
     if T == 0 or Hq == 0 or B == 0:
         return out
+    if workspace is None:
+        need = _prompt_need(T, B, n_keys, cache[6] * cache[4], Hq, Hkv, D)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous and on cuda:{dev}")
+    else:
+        need = workspace.numel() * workspace.element_size()
     a = _prompt_args(*cache, qp, op, lp, keys[0], keys[1], starts.data_ptr(), 0 if k_starts is None else k_starts.data_ptr(),
                      0 if lengths is None else lengths.data_ptr(), qt, qh, ot, oh, *keys[2:], T, n_keys, Hq, Hkv, D,
-                     _DTYPE[q.dtype], 1 if causal else 0, _scale(scale, D))
+                     _DTYPE[q.dtype], 1 if causal else 0, _scale(scale, D), workspace.data_ptr() if need else 0, need)
     st = _prompt_call(a, _stream(dev))
     if st:
         check(st, "latent_attn_prompt")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _prompt_need(n_tokens: int, n_seq: int, n_keys: int, cached: int, n_head: int, n_kv_head: int, head_dim: int) -> int:
+    cache = (0, 0, 0, 1, 1, n_seq, cached, cached, 0, 0, 0, 0, 0, 0)
+    n = ctypes.c_size_t()
+    a = _prompt_args(*cache, *(0,) * 16, n_tokens, n_keys, n_head, n_kv_head, head_dim, _lib.LATENT_BF16, 1, 1.0, 0, 0)
+    check(_prompt_size(a, ctypes.addressof(n)), "latent_attn_prompt_workspace_size")
+    return int(n.value)
+
+
+def attend_prompt_workspace_size(n_tokens: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_keys: int = 0,
+                                 max_pages: int = 0, page_size: int = 1) -> int:
+    """Workspace bytes of attend_prompt (n_keys rows of keys) or attend_prompt_paged for these sizes; 0: it takes none."""
+    return _prompt_need(n_tokens, n_seq, n_keys, 0 if n_keys else max_pages * page_size, n_head, n_kv_head, head_dim)
 
 
 def attend_prompt(
@@ -348,6 +372,7 @@ def attend_prompt(
     scale: Optional[float] = None,
     out: Optional[torch.Tensor] = None,
     lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
 ) -> torch.Tensor:
     """Whole prompts, packed: sequence b is rows starts[b] .. starts[b + 1] - 1 (int32 [B + 1], ascending) of
@@ -356,11 +381,13 @@ def attend_prompt(
     Causal with the ends aligned: with n queries and m keys, query i sees keys
     j <= i + m - n.  Rows of out and lse (f32 [T, heads]) that belong to no
     sequence are not written; a row that sees no key is zeros, lse -inf.
+    A workspace that is given (attend_prompt_workspace_size bytes, fewer: the
+    call does without) must not serve calls that may overlap.
     """
     ctx = _here(q, stream)
     if ctx is not None:
         with ctx:
-            return attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse)
+            return attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
     dev = _first(q, "q")
     dt = q.dtype
     q = _heads(q, "q", dt, dev)
@@ -379,7 +406,7 @@ def attend_prompt(
     if Tk == 0:  # a tensor without rows has no base
         kp = vp = q[1]
     cache = (0, 0, 0, 0, 1, B, 0, 0, 0, 0, 0, 0, 0, 0)
-    return _prompt(q, starts, cache, Hkv, (kp, vp, kt, kh, vt, vh), k_starts, None, Tk, causal, scale, out, lse, dev)
+    return _prompt(q, starts, cache, Hkv, (kp, vp, kt, kh, vt, vh), k_starts, None, Tk, causal, scale, out, lse, workspace, dev)
 
 
 def attend_prompt_paged(
@@ -393,6 +420,7 @@ def attend_prompt_paged(
     scale: Optional[float] = None,
     out: Optional[torch.Tensor] = None,
     lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
 ) -> torch.Tensor:
     """attend_prompt with the keys and values of sequence b in the cache: its first lengths[b] (int32 [B])
@@ -400,14 +428,14 @@ def attend_prompt_paged(
     ctx = _here(q, stream)
     if ctx is not None:
         with ctx:
-            return attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse)
+            return attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
     dev = _first(q, "q")
     cache, (_, _, Hkv, cD), dt = _cache(k_cache, v_cache, pages, dev)
     q = _heads(q, "q", dt, dev)
     if q[4][2] != cD:
         raise ValueError(f"q {list(q[4])} does not fit the cache {list(k_cache.shape)}")
     lengths = _ints(lengths, "lengths", cache[5], dev)
-    return _prompt(q, starts, cache, Hkv, (0,) * 6, None, lengths, 0, causal, scale, out, lse, dev)
+    return _prompt(q, starts, cache, Hkv, (0,) * 6, None, lengths, 0, causal, scale, out, lse, workspace, dev)
 
 
 class Attention:

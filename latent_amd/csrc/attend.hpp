@@ -116,6 +116,18 @@ __device__ __forceinline__ void lds_barrier() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// x / d for x < 2^31 as x * mul >> shift: mul = ceil(2^(31 + s) / d) with 2^s >= d.  mul d exceeds 2^(31 + s) by less than d <= 2^s,
+// so x mul / 2^(31 + s) exceeds x / d by less than x / (2^31 d) < 1 / d, and its whole part is the quotient.
+struct Divisor {
+  uint32_t mul, shift;
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return static_cast<uint32_t>(static_cast<uint64_t>(x) * mul >> shift); }
+};
+inline Divisor divisor(int64_t d) {
+  uint32_t s = 0;
+  while ((int64_t{1} << s) < d) ++s;
+  return {static_cast<uint32_t>(((uint64_t{1} << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 // The cache as the kernels address it (byte strides).
 struct Cache {
   const char* k;
@@ -125,6 +137,7 @@ struct Cache {
   int64_t k_page, k_row, k_head;
   int64_t v_page, v_row, v_head;
   uint32_t n_pages, page_size, max_len;  // max_len: positions a page table row has room for
+  Divisor by_page;  // key / page_size
 };
 
 // ---- host ---------------------------------------------------------------------
@@ -166,6 +179,7 @@ inline Cache device_cache(const latent_kv_cache& c) {
   d.n_pages = static_cast<uint32_t>(c.n_pages);
   d.page_size = static_cast<uint32_t>(c.page_size);
   d.max_len = static_cast<uint32_t>(c.max_pages * c.page_size);
+  d.by_page = divisor(c.page_size);
   return d;
 }
 

@@ -147,7 +147,7 @@ struct Stream {
     Place k[kPage8 ? 1 : 2], v[kPage8 ? 1 : 8];
   };
   __device__ __forceinline__ Place place_of(uint32_t key) const {
-    const uint32_t slot = key / p.cache.page_size;
+    const uint32_t slot = p.cache.by_page.of(key);
     return {key < len ? pages[slot] : -1, key - slot * p.cache.page_size};
   }
   // Row m of score block blk is key 8 (m / 4) + 4 blk + m % 4 of the step: lane (query, kq) then holds keys 8 kq .. + 7.

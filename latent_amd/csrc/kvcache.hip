@@ -43,7 +43,7 @@ enum Kind { kHalf, kInterleaved, kScalar };
 __device__ __forceinline__ bool cache_row(const AppendParams& p, uint32_t t, uint32_t pos, int64_t* k, int64_t* v) {
   const uint32_t seq = p.seqs ? static_cast<uint32_t>(p.seqs[t]) : t;
   if (seq >= p.n_seq || pos >= p.cache.max_len) return false;
-  const uint32_t slot = pos / p.cache.page_size, off = pos - slot * p.cache.page_size;
+  const uint32_t slot = p.cache.by_page.of(pos), off = pos - slot * p.cache.page_size;
   const uint32_t page = static_cast<uint32_t>(p.cache.pages[seq * p.cache.pages_stride + slot]);
   if (page >= p.cache.n_pages) return false;
   *k = page * p.cache.k_page + off * p.cache.k_row;

@@ -43,8 +43,13 @@ struct PromptParams {
   const int32_t* lengths;   // paged
   int64_t q_token, q_head, o_token, o_head;  // bytes
   int32_t T, n_keys, B, Hq, Hkv, G, D;
+  Divisor by_group;  // row / G
   bool causal;
   float scale_log2;
+  // Splitting (see find_item): parts that the workspace holds, 0 for none.
+  int32_t max_parts;
+  f32x4* part_acc;  // [max_parts][4 * 32-dimension blocks][256]
+  f32x4* part_ml;   // [max_parts][256]: reference, sum, full sum
 };
 
 // Rows [s0, s0 + n) of sequence b.
@@ -53,32 +58,104 @@ __device__ __forceinline__ int2 rows_of(const int32_t* starts, int b, int most) 
   return int2{s0, s1 - s0};
 }
 
-__device__ __forceinline__ int tiles_of(const PromptParams& p, int b) {
-  return static_cast<int>((static_cast<int64_t>(rows_of(p.starts, b, p.T).y) * p.G + kRowsTile - 1) / kRowsTile);
+// Keys of sequence b: first row (packed) and number.
+template <bool kPaged>
+__device__ __forceinline__ int2 keys_of(const PromptParams& p, int b) {
+  if constexpr (kPaged) return int2{0, min(max(p.lengths[b], 0), static_cast<int>(p.cache.max_len))};
+  return rows_of(p.k_starts, b, p.n_keys);
 }
 
-// Sequence and tile of work item x, or false behind the last.
-__device__ __forceinline__ bool find_tile(const PromptParams& p, int x, int lane, int* b, int* tile) {
-  int base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    upto += base;
-    const uint64_t past = __ballot(upto > x);
-    if (past) {
-      const int first = __builtin_ctzll(past);
-      *b = b0 + first;
-      *tile = __shfl(upto, first) - 1 - x;  // the last rows see the most keys: they start first
-      return true;
-    }
-    base = __shfl(upto, kWave - 1);
+__device__ __forceinline__ int row_tiles(const PromptParams& p, int n) {
+  return (n * p.G + kRowsTile - 1) / kRowsTile;
+}
+__device__ __forceinline__ int key_tiles(int m) { return (m + kKeys - 1) / kKeys; }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// Keys that row r of a sequence of n queries and m keys sees.
+__device__ __forceinline__ int keys_seen(const PromptParams& p, int n, int m, int r) {
+  return p.causal ? max(0, min(m, static_cast<int>(p.by_group.of(min(r, n * p.G - 1))) + m - n + 1)) : m;
+}
+
+// ---- work items ------------------------------------------------------------------
+// A unit is a row tile of one sequence and key/value head.  Sequences go from the longest to the shortest, row tiles
+// from the last (which sees the most keys) to the first, so that short units fill the end of the launch.  Where the units
+// of all sequences are few against their keys, long ones are split: `chunk` key tiles an item, at least kChunk and so many
+// that about kItems items have work; each item of a split unit leaves a part (reference, sums, unnormalised rows), and
+// join_kernel adds them up.  Items of one chunk follow one another: they read the same keys, at about the same time, on the
+// same XCD (equal spans of the line of all key tiles, each workgroup's keys its own, balanced as well and ran three
+// times longer: 14 prompts of up to 2000 tokens 375 us, 190 us a unit a workgroup).
+// Every wave finds its item by itself, from the sequences in its lanes; more than 64 sequences are taken as they come.
+constexpr int kChunk = 8, kItems = 512;
+// Sequence `lane`: its row tiles, keys, and the parts of its units.
+struct Line {
+  int s0, n, k0, m;
+  int tiles, parts, chunk;
+};
+template <bool kPaged>
+__device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
+  Line l{};
+  if (lane < p.B) {
+    const int2 q = rows_of(p.starts, lane, p.T), k = keys_of<kPaged>(p, lane);
+    l = {q.x, q.y, k.x, k.y, row_tiles(p, q.y)};
   }
-  return false;
+  l.parts = 1;
+  l.chunk = INT32_MAX;
+  if (p.max_parts) {
+    const int kt = key_tiles(l.m);
+    float work = static_cast<float>(l.tiles) * static_cast<float>(kt);
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) work += __shfl_xor(work, d);
+    // chunk > work Hkv / kItems: split units are less than kItems, and their parts, kt / chunk + 1 < 2 kt / chunk each, less
+    // than 2 kItems (1.001 is for the rounding of the sum).
+    l.chunk = uniform(max(kChunk, static_cast<int>(min(work * static_cast<float>(p.Hkv) * (1.001f / kItems), 1e9f)) + 1));
+    if (kt > l.chunk) l.parts = (kt + l.chunk - 1) / l.chunk;
+  }
+  return l;
+}
+// Items of the sequences in front of this lane's (longer ones first).
+__device__ __forceinline__ int items_before(const PromptParams& p, const Line& l, int items, int lane) {
+  int before = 0;
+  for (int j = 0; j < p.B; ++j) {
+    const int m = __builtin_amdgcn_readlane(l.m, j), n = __builtin_amdgcn_readlane(items, j);
+    if (m > l.m || (m == l.m && j < lane)) before += n;
+  }
+  return before;
+}
+struct Item {
+  int b, tile, part, chunk;
+  int s0, n, k0, m;  // the sequence's queries and keys
+};
+template <bool kPaged>
+__device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane) {  // b < 0: behind the last
+  if (p.B > kWave) {
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kWave) {
+      const int n = b0 + lane < p.B ? row_tiles(p, rows_of(p.starts, b0 + lane, p.T).y) : 0;
+      int upto = n;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      upto += base;
+      const uint64_t past = __ballot(upto > x);
+      if (past) {
+        const int first = __builtin_ctzll(past);
+        const int b = b0 + first;
+        const int2 q = rows_of(p.starts, b, p.T), k = keys_of<kPaged>(p, b);
+        return {b, __builtin_amdgcn_readlane(upto, first) - 1 - x, 0, INT32_MAX, uniform(q.x), uniform(q.y), uniform(k.x), uniform(k.y)};
+      }
+      base = __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return {-1};
+  }
+  const Line l = line_of<kPaged>(p, lane);
+  const int items = l.tiles * l.parts, before = items_before(p, l, items, lane);
+  const uint64_t mine = __ballot(x >= before && x - before < items);
+  if (!mine) return {-1};
+  const int b = __builtin_ctzll(mine), r = x - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
+  const int part = uniform(r / t);
+  return {b, t - 1 - (r - part * t), part, l.chunk, __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
+          __builtin_amdgcn_readlane(l.k0, b), __builtin_amdgcn_readlane(l.m, b)};
 }
 
 // A tile in LDS: rows of kC 16-byte pieces, permuted so that the lanes of a read spread over all banks: a key row's
@@ -87,7 +164,7 @@ template <int kDP>
 struct Shared {
   static constexpr int kC = kDP / 8;
   static constexpr uint32_t kTile = kKeys * kDP * 2;
-  u32x4 k[2][kKeys * kC];
+  alignas(512) u32x4 k[2][kKeys * kC];
   u32x4 v[2][kKeys * kC];
   // Infinities and NaN among values must not reach the rows that do not see their keys: 0 times them is NaN.  Tiles
   // that some rows see in part hold 0 in their place; the keys they belong to are noted here, and added to
@@ -122,39 +199,31 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   __shared__ S sm;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
   const int hk = blockIdx.x % p.Hkv;
-  int b, tile;
-  if (!find_tile(p, blockIdx.x / p.Hkv, lane, &b, &tile)) return;
-  const int2 qs = rows_of(p.starts, b, p.T);
-  const int n = qs.y;
-  int k0 = 0, m;
-  if constexpr (kPaged) {
-    m = min(max(p.lengths[b], 0), static_cast<int>(p.cache.max_len));
-  } else {
-    const int2 ks = rows_of(p.k_starts, b, p.n_keys);
-    k0 = ks.x;
-    m = ks.y;
-  }
+  const Item it = find_item<kPaged>(p, blockIdx.x / p.Hkv, lane);
+  if (it.b < 0) return;
+  const int b = it.b, tile = it.tile, n = it.n, m = it.m;
   const int32_t* pages = kPaged ? p.cache.pages + b * p.cache.pages_stride : nullptr;
-  const char* kbase = p.cache.k + hk * p.cache.k_head + k0 * p.cache.k_row;
-  const char* vbase = p.cache.v + hk * p.cache.v_head + k0 * p.cache.v_row;
+  const char* kbase = p.cache.k + hk * p.cache.k_head + it.k0 * p.cache.k_row;
+  const char* vbase = p.cache.v + hk * p.cache.v_head + it.k0 * p.cache.v_row;
 
   // This lane's row, and how many keys it sees.
-  const int64_t all = static_cast<int64_t>(n) * p.G, row0 = static_cast<int64_t>(tile) * kRowsTile;
-  const int64_t row = row0 + wave * kRowsWave + l32;
+  const int all = n * p.G, row0 = tile * kRowsTile, w0 = row0 + wave * kRowsWave, row = w0 + l32;
   const bool live = row < all;
-  const int64_t rc = live ? row : all - 1;
-  const int tok = static_cast<int>(rc / p.G), head = hk * p.G + static_cast<int>(rc % p.G);
-  auto sees = [&](int64_t r) { return p.causal ? max(0, min(m, static_cast<int>(min(r, all - 1) / p.G) + m - n + 1)) : m; };
-  const int vis = sees(rc);
-  const int64_t w0 = row0 + wave * kRowsWave;
-  const int all_see = __builtin_amdgcn_readfirstlane(sees(row0));                 // keys that every row of the workgroup sees
-  const int wave_all = __builtin_amdgcn_readfirstlane(sees(w0));                  // of the wave
-  const int wave_any = __builtin_amdgcn_readfirstlane(w0 < all ? sees(w0 + kRowsWave - 1) : 0);
-  const int end = __builtin_amdgcn_readfirstlane(sees(row0 + kRowsTile - 1));     // keys that some row sees
+  const int rc = min(row, all - 1), tok = p.by_group.of(rc), head = hk * p.G + rc - tok * p.G;
+  const int vis = keys_seen(p, n, m, row);
+  const int all_see = uniform(keys_seen(p, n, m, row0));                      // keys that every row of the workgroup sees
+  const int end = uniform(keys_seen(p, n, m, row0 + kRowsTile - 1));          // keys that some row sees
+  const int wave_all = uniform(keys_seen(p, n, m, w0));                       // of the wave
+  const int wave_any = uniform(w0 < all ? keys_seen(p, n, m, w0 + kRowsWave - 1) : 0);
+  // This item's key tiles, and whether they are all of the unit's.
+  const int tiles = key_tiles(end), t0 = it.part ? it.part * it.chunk : 0, t1 = min(tiles, t0 + min(tiles, it.chunk));
+  if (t0 > 0 && t0 >= tiles) return;
+  const bool whole_unit = t0 == 0 && t1 == tiles;
+  const int stop = min(end, t1 * kKeys);
 
   u32x4 q[kSteps];
   {
-    const char* src = p.q + (qs.x + tok) * p.q_token + head * p.q_head;
+    const char* src = p.q + (it.s0 + tok) * p.q_token + head * p.q_head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int d = 16 * s + 8 * h;
@@ -176,46 +245,52 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
   }
   const uint32_t lds_k = lds_addr(sm.k[0][0]) + wave * (S::kTile / kWaves), lds_v = lds_addr(sm.v[0][0]) + wave * (S::kTile / kWaves);
-  const bool exact = p.D == kDP;
-  // K or V rows kt .. kt + 63 into buffer buf.
-  auto load = [&](bool values, int kt, int buf) {
-    const uint32_t to = (values ? lds_v : lds_k) + buf * S::kTile;
+  const bool exact = p.D == kDP, same_strides = p.cache.k_page == p.cache.v_page && p.cache.k_row == p.cache.v_row;
+  // Paged: the page of key kt + lane of the tile that is loaded next, fetched a tile ahead.
+  auto page_of = [&](int kt) -> uint32_t {
+    const int key = kt + lane;
+    return kPaged && key < stop ? static_cast<uint32_t>(pages[p.cache.by_page.of(key)]) : 0xFFFFFFFFu;
+  };
+  // Rows kt .. kt + 63 of K and V into buffer buf.
+  auto load = [&](int kt, int buf, uint32_t page_in_lane) {
+    const uint32_t to_k = lds_k + buf * S::kTile, to_v = lds_v + buf * S::kTile;
     if constexpr (!kPaged) {
       if (kt + kKeys <= end && exact) {
-        const char* from = values ? vbase + kt * p.cache.v_row : kbase + kt * p.cache.k_row;
+        const char *from_k = kbase + kt * p.cache.k_row, *from_v = vbase + kt * p.cache.v_row;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) dma16s(from, values ? voff[i] : koff[i], to + i * (kWave * 16));
+        for (int i = 0; i < kLoads; ++i) dma16s(from_k, koff[i], to_k + i * (kWave * 16));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) dma16s(from_v, voff[i], to_v + i * (kWave * 16));
         return;
       }
     }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int row_in = lrow + i * kRowsLoad, key = kt + row_in, c = lpos ^ (values ? S::v_turn(row_in) : S::k_turn(row_in));
+      const int row_in = lrow + i * kRowsLoad, key = kt + row_in, ck = lpos ^ S::k_turn(row_in), cv = lpos ^ S::v_turn(row_in);
       bool ok = key < end;
-      const char* from;
+      int64_t ko, vo;
       if constexpr (kPaged) {
-        const uint32_t pg = static_cast<uint32_t>(key) / p.cache.page_size, off = static_cast<uint32_t>(key) - pg * p.cache.page_size;
-        const uint32_t page = ok ? static_cast<uint32_t>(pages[pg]) : 0xFFFFFFFFu;
+        const uint32_t page = __shfl(page_in_lane, row_in), off = static_cast<uint32_t>(key) - p.cache.by_page.of(key) * p.cache.page_size;
         ok = page < p.cache.n_pages;
-        from = values ? vbase + page * p.cache.v_page + off * p.cache.v_row : kbase + page * p.cache.k_page + off * p.cache.k_row;
+        ko = page * p.cache.k_page + off * p.cache.k_row;
+        vo = same_strides ? ko : page * p.cache.v_page + off * p.cache.v_row;
       } else {
-        from = values ? vbase + key * p.cache.v_row : kbase + key * p.cache.k_row;
+        ko = key * p.cache.k_row;
+        vo = key * p.cache.v_row;
       }
-      from = ok && 8 * c < p.D ? from + 16 * c : reinterpret_cast<const char*>(kZeroRow);
-      dma16(from, to + i * (kWave * 16));
+      const char* zero = reinterpret_cast<const char*>(kZeroRow);
+      dma16(ok && 8 * ck < p.D ? kbase + ko + 16 * ck : zero, to_k + i * (kWave * 16));
+      dma16(ok && 8 * cv < p.D ? vbase + vo + 16 * cv : zero, to_v + i * (kWave * 16));
+      __builtin_amdgcn_sched_barrier(0);  // all loads' addresses at once would not fit the registers
     }
   };
 
   // Lane parts of the operands' LDS addresses.
-  uint32_t kat[kSteps], vat[kBlocks];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) kat[s] = lds_addr(sm.k[0][0]) + l32 * kRow + 16 * ((2 * s + h) ^ S::k_turn(l32));
-  {
-    const int i16 = lane & 15, row_in = 4 * h + (i16 >> 2);
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i)
-      vat[i] = lds_addr(sm.v[0][0]) + row_in * kRow + 16 * ((4 * i + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ S::v_turn(row_in)) + 8 * (i16 & 1);
-  }
+  // Step s of a key row is 2 s + h pieces on, permuted by a constant: its address is the first's with 2 s put in by xor; block i of
+  // a value row likewise, 4 i pieces on.
+  const uint32_t kat = lds_addr(sm.k[0][0]) + l32 * kRow + 16 * (h ^ S::k_turn(l32));
+  const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2);
+  const uint32_t vat = lds_addr(sm.v[0][0]) + vrow * kRow + 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ S::v_turn(vrow)) + 8 * (i16 & 1);
 
   f32x16 acc[kBlocks];
 #pragma unroll
@@ -224,15 +299,22 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   // probabilities that weigh its values, so that their roundings cancel as far as they agree (a row of one key is that
   // key's value); the log-sum-exp, where it is asked for, takes the sum of the unrounded ones.
   float top = -INFINITY, sum = 0.f, full = 0.f;
+  uint32_t page_now = 0, page_next = 0;  // paged: page_of this tile and the next
 
   auto step = [&](int t, auto bufc) {
     constexpr int buf = decltype(bufc)::value;
     const int kt = t * kKeys;
     pipeline_barrier();  // this tile is there, the other buffer read
-    if (kt + kKeys < end) {
-      load(false, kt + kKeys, buf ^ 1);
-      load(true, kt + kKeys, buf ^ 1);
+    uint64_t exists = ~uint64_t{0};
+    if constexpr (kPaged) {
+      exists = __ballot(page_now < p.cache.n_pages);
+      page_now = page_next;
     }
+    if (kt + kKeys < stop) {
+      load(kt + kKeys, buf ^ 1, page_now);
+      if constexpr (kPaged) page_next = page_of(kt + 2 * kKeys);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the loads' addresses and the products' operands do not share the registers
     const bool part_seen = kt + kKeys > all_see;
     if (part_seen) {
 #pragma unroll
@@ -256,19 +338,18 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>(kat[st] + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
-    uint64_t exists = ~uint64_t{0};
-    if constexpr (kPaged) {
-      const int key = kt + lane;
-      exists = __ballot(key < end && static_cast<uint32_t>(pages[static_cast<uint32_t>(key) / p.cache.page_size]) < p.cache.n_pages);
-    }
+      for (int blk = 0; blk < 2; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
     if (!(kt + kKeys <= wave_all && exists == ~uint64_t{0})) {
+      asm volatile("");  // keeps this a branch: most tiles need none of it
+      const int left = vis - kt - 4 * h;  // of the keys from this lane's first on
+      const uint64_t there = exists >> (4 * h);
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = 32 * blk + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (kt + key >= vis || !((exists >> key) & 1)) s[blk][r] = -INFINITY;
+          const int key = 32 * blk + 8 * (r >> 2) + (r & 3);
+          const uint32_t half = static_cast<uint32_t>(there >> (32 * blk));
+          if (key >= left || (kPaged && !(half & (1u << (key & 31))))) s[blk][r] = -INFINITY;
         }
     }
     float m2[2] = {-INFINITY, -INFINITY};
@@ -306,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     for (int kk = 0; kk < 4; ++kk)  // 16 keys
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        const uint32_t at = vat[i] + buf * S::kTile + 16 * kk * kRow;
+        const uint32_t at = (vat ^ (64 * i)) + buf * S::kTile + 16 * kk * kRow;
         const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
         acc[i] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, prob[kk], acc[i]);
       }
@@ -315,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
         const int key = kt + __builtin_ctzll(bad);
         int64_t vo;
         if constexpr (kPaged) {
-          const uint32_t pg = static_cast<uint32_t>(key) / p.cache.page_size;
+          const uint32_t pg = p.cache.by_page.of(key);
           vo = pages[pg] * p.cache.v_page + (static_cast<uint32_t>(key) - pg * p.cache.page_size) * p.cache.v_row;
         } else {
           vo = key * p.cache.v_row;
@@ -338,21 +419,35 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
   };
 
-  if (end > 0) {
+  if (t0 < t1) {
     if (tid < 2) sm.bad[tid] = 0;
-    load(false, 0, 0);
-    load(true, 0, 0);
-    const int tiles = (end + kKeys - 1) / kKeys;
-    for (int t = 0; t < tiles; t += 2) {
+    if constexpr (kPaged) {
+      page_now = page_of(t0 * kKeys);
+      page_next = page_of((t0 + 1) * kKeys);
+    }
+    load(t0 * kKeys, 0, page_now);
+    for (int t = t0; t < t1; t += 2) {
       step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < tiles) step(t + 1, std::integral_constant<int, 1>{});
+      if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
   }
 
-  if (!live) return;
   sum = op_over(sum, 32, 64, OpAdd{});
+  if constexpr (kLse) full = op_over(full, 32, 64, OpAdd{});
+  if (!whole_unit) {
+    if (static_cast<int>(blockIdx.x) >= p.max_parts) return;  // never, by the choice of chunk
+    f32x4* to = p.part_acc + static_cast<int64_t>(blockIdx.x) * (4 * kBlocks * kThreads) + tid;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr)
+        to[(4 * i + rr) * kThreads] = f32x4{acc[i][4 * rr], acc[i][4 * rr + 1], acc[i][4 * rr + 2], acc[i][4 * rr + 3]};
+    p.part_ml[static_cast<int64_t>(blockIdx.x) * kThreads + tid] = f32x4{top, sum, full, 0.f};
+    return;
+  }
+  if (!live) return;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  char* dst = p.out + (qs.x + tok) * p.o_token + head * p.o_head;
+  char* dst = p.out + (it.s0 + tok) * p.o_token + head * p.o_head;
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -363,9 +458,91 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
                                                        pack2<E>(acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv)};
     }
   if constexpr (kLse) {
-    full = op_over(full, 32, 64, OpAdd{});
-    if (h == 0) p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
+    if (h == 0) p.lse[static_cast<int64_t>(it.s0 + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
   }
+}
+
+// Adds up the parts of a split unit, 32 dimensions a workgroup; threads as in prompt_kernel.
+template <typename E, int kDP, bool kPaged, bool kLse>
+__global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
+  constexpr int kBlocks = kDP / 32;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), h = lane >> 5, i = blockIdx.y, hk = blockIdx.x % p.Hkv;
+  // The split units in the order of their items.
+  const Line l = line_of<kPaged>(p, lane);
+  const int x0 = blockIdx.x / p.Hkv, units = l.parts > 1 ? l.tiles : 0, before = items_before(p, l, units, lane);
+  const uint64_t mine = __ballot(x0 >= before && x0 - before < units);
+  if (!mine) return;
+  const int b = __builtin_ctzll(mine), r = x0 - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
+  const int first = __builtin_amdgcn_readlane(items_before(p, l, l.tiles * l.parts, lane), b) + r, tile = t - 1 - r;
+  const int2 qs = rows_of(p.starts, b, p.T);
+  const int n = qs.y, m = keys_of<kPaged>(p, b).y;
+  const int parts = (key_tiles(keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1)) + l.chunk - 1) / l.chunk;
+  if (parts < 2) return;  // its rows see too little to be split
+  const int at = first * p.Hkv + hk, step = t * p.Hkv;
+  float top = -INFINITY, sum = 0.f, full = 0.f;
+  f32x4 x[4] = {};
+  for (int j0 = 0; j0 < parts; j0 += 4) {
+    f32x4 ml[4], a[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t part = at + static_cast<int64_t>(min(j0 + k, parts - 1)) * step;
+      ml[k] = p.part_ml[part * kThreads + tid];
+      if (j0 + k >= parts) ml[k] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) a[k][rr] = p.part_acc[part * (4 * kBlocks * kThreads) + (4 * i + rr) * kThreads + tid];
+    }
+    const float up = fmaxf(fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0])), top), mm = finite_max(up);
+    const float f = exp2_fast(top - mm);
+    top = up;
+    sum *= f;
+    full *= f;
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) x[rr] *= f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k][0] == -INFINITY && ml[k][1] == ml[k][1]) continue;  // no keys, and no NaN to pass on
+      const float g = exp2_fast(ml[k][0] - mm);
+      sum += g * ml[k][1];
+      full += g * ml[k][2];
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) x[rr] += a[k][rr] * g;
+    }
+  }
+  const int row = tile * kRowsTile + (tid >> 6) * kRowsWave + (lane & 31);
+  if (row >= n * p.G) return;
+  const int tok = p.by_group.of(row), head = hk * p.G + row - tok * p.G;
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  char* dst = p.out + (qs.x + tok) * p.o_token + head * p.o_head;
+#pragma unroll
+  for (int rr = 0; rr < 4; ++rr) {
+    const int d = 32 * i + 8 * rr + 4 * h;
+    if (d < p.D)
+      *reinterpret_cast<u32x2*>(dst + 2 * d) = u32x2{pack2<E>(x[rr][0] * inv, x[rr][1] * inv), pack2<E>(x[rr][2] * inv, x[rr][3] * inv)};
+  }
+  if constexpr (kLse) {
+    if (i == 0 && h == 0) p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
+  }
+}
+
+// Longest keys from which units may be split, and units up to which they are few.
+constexpr int64_t kShortKeys = 1024, kFewUnits = 1024;
+struct Plan {
+  int64_t units;  // at most
+  bool split;
+  size_t acc_bytes, ml_bytes;
+};
+Plan plan_for(const latent_attn_prompt_args& a) {
+  Plan pl{};
+  const int64_t G = a.n_head / a.n_kv_head;
+  // A sequence's rows round up to whole tiles: at most one more each.
+  pl.units = std::max<int64_t>(0, (a.n_tokens * G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1) * a.n_kv_head;
+  const int64_t keys = a.k || a.n_keys ? a.n_keys : a.cache.max_pages * a.cache.page_size;
+  pl.split = keys > kShortKeys && pl.units < kFewUnits && a.cache.n_seq <= kWave;
+  if (!pl.split) return pl;
+  const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+  pl.acc_bytes = size_t{2} * kItems * 4 * blocks * kThreads * sizeof(f32x4);
+  pl.ml_bytes = size_t{2} * kItems * kThreads * sizeof(f32x4);
+  return pl;
 }
 
 int validate(const latent_attn_prompt_args& a) {
@@ -374,11 +551,12 @@ int validate(const latent_attn_prompt_args& a) {
   if (a.n_head == 0 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return LATENT_E_INVALID;
   if (a.n_tokens < 0 || a.n_keys < 0 || a.cache.n_seq < 0) return LATENT_E_INVALID;
   if (a.n_tokens > (1 << 28) || a.n_keys > (1 << 28)) return LATENT_E_UNSUPPORTED;
+  // Rows (tokens times the heads of a group) and, of a launch, threads are counted in 32 bits.
+  if (a.n_tokens * (a.n_head / a.n_kv_head) > (1 << 30)) return LATENT_E_UNSUPPORTED;
   if (a.cache.n_seq > (1 << 20)) return LATENT_E_UNSUPPORTED;
-  // Workgroups are counted in 31 bits.
   const int64_t G = a.n_head / a.n_kv_head, tiles = (a.n_tokens * G + kRowsTile - 1) / kRowsTile + a.cache.n_seq;
-  if (tiles * a.n_kv_head > INT32_MAX) return LATENT_E_UNSUPPORTED;
-  return a.k ? LATENT_OK : check_cache(a.cache);
+  if (tiles * a.n_kv_head > 1 << 23) return LATENT_E_UNSUPPORTED;
+  return a.k || a.n_keys ? LATENT_OK : check_cache(a.cache);
 }
 
 }  // namespace
@@ -387,6 +565,15 @@ int validate(const latent_attn_prompt_args& a) {
 
 using namespace latent;
 using namespace latent::attend;
+
+extern "C" int latent_attn_prompt_workspace_size(const latent_attn_prompt_args* args, size_t* bytes) {
+  if (!args || !bytes) return LATENT_E_INVALID;
+  const int st = validate(*args);
+  if (st != LATENT_OK) return st;
+  const Plan pl = plan_for(*args);
+  *bytes = pl.acc_bytes + pl.ml_bytes;
+  return LATENT_OK;
+}
 
 extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stream) {
   if (!args) return LATENT_E_INVALID;
@@ -402,7 +589,7 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
   PromptParams p{};
   const bool paged = !a.k;
   if (paged) {
-    if (!a.lengths) return LATENT_E_INVALID;
+    if (a.n_keys || !a.lengths) return LATENT_E_INVALID;
     p.cache = device_cache(a.cache);
     if (a.cache.n_pages == 0)
       p.cache.max_len = 0;
@@ -434,25 +621,34 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
   p.Hq = static_cast<int32_t>(a.n_head);
   p.Hkv = static_cast<int32_t>(a.n_kv_head);
   p.G = p.Hq / p.Hkv;
+  p.by_group = divisor(p.G);
   p.D = static_cast<int32_t>(a.head_dim);
   p.causal = a.causal != 0;
   p.scale_log2 = a.scale * kLog2e;
-  // A sequence's rows round up to whole tiles: at most one more each.
-  const int64_t tiles = (a.n_tokens * p.G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1;
+  const Plan pl = plan_for(a);
+  if (pl.split && a.workspace && a.workspace_bytes >= pl.acc_bytes + pl.ml_bytes) {
+    if (!aligned16(a.workspace)) return LATENT_E_UNSUPPORTED;
+    p.max_parts = 2 * kItems;
+    p.part_acc = static_cast<f32x4*>(a.workspace);
+    p.part_ml = reinterpret_cast<f32x4*>(static_cast<char*>(a.workspace) + pl.acc_bytes);
+  }
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   auto launch = [&](auto e, auto dp) {
     constexpr int kDP = decltype(dp)::value;
     using E = decltype(e);
-    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, tiles) * p.Hkv));
-    auto go = [&](auto paged_c) {
-      constexpr bool kPaged = decltype(paged_c)::value;
-      if (p.lse)
-        hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, true>), grid, dim3(kThreads), 0, s, p);
-      else
-        hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, false>), grid, dim3(kThreads), 0, s, p);
+    // Split units have less than kItems parts beyond their first.
+    const int64_t more = (kItems / p.Hkv + 1) * p.Hkv, units = std::max<int64_t>(pl.units, p.Hkv);
+    auto go = [&](auto paged_c, auto lse_c) {
+      constexpr bool kPaged = decltype(paged_c)::value, kLse = decltype(lse_c)::value;
+      const dim3 grid(static_cast<unsigned>(units + (p.max_parts ? more : 0)));
+      hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, kLse>), grid, dim3(kThreads), 0, s, p);
+      if (p.max_parts)
+        hipLaunchKernelGGL((join_kernel<E, kDP, kPaged, kLse>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32),
+                           dim3(kThreads), 0, s, p);
     };
-    paged ? go(std::true_type{}) : go(std::false_type{});
+    auto with_lse = [&](auto paged_c) { p.lse ? go(paged_c, std::true_type{}) : go(paged_c, std::false_type{}); };
+    paged ? with_lse(std::true_type{}) : with_lse(std::false_type{});
   };
   auto with_type = [&](auto e) {
     if (p.D <= 64)

@@ -111,7 +111,14 @@ void prompt() {
   auto call = [](const A& x) { return latent_attn_prompt(&x, nullptr); };
   EXPECT(call(a) == LATENT_E_INVALID);
   sweep(a, kCache, kNCache, fields, sizeof(fields) / sizeof(fields[0]), call);
+  auto size = [](const A& x) {
+    size_t n = 0;
+    return latent_attn_prompt_workspace_size(&x, &n);
+  };
+  EXPECT(size(a) == LATENT_OK);
+  sweep(a, kCache, kNCache, fields, sizeof(fields) / sizeof(fields[0]), size);
   a.k = nullptr;
+  a.n_keys = 0;
   sweep(a, kCache, kNCache, fields, sizeof(fields) / sizeof(fields[0]), call);
 }
 

@@ -101,7 +101,7 @@ def test_decode_cache_checks(L, change, status):
     (dict(scale=0.0), "INVALID"), (dict(n_tokens=-1), "INVALID"), (dict(n_keys=-1), "INVALID"), (dict(starts=None), "INVALID"),
     (dict(k_starts=None), "INVALID"), (dict(v=None), "INVALID"), (dict(v=P + 4), "UNSUPPORTED"), (dict(k_token_stride=4), "UNSUPPORTED"),
     (dict(k_token_stride=(1 << 24) + 8), "UNSUPPORTED"), (dict(n_tokens=1 << 29), "UNSUPPORTED"), (dict(out_token_stride=0), "INVALID"),
-    (dict(k=None, lengths=None), "INVALID"),
+    (dict(k=None, n_keys=0, lengths=None), "INVALID"), (dict(k=None), "INVALID"),
 ])
 def test_prompt_argument_checks(L, change, status):
     _expect(L, L.lib.latent_attn_prompt(ctypes.byref(_prompt(L, **change)), None), status)
@@ -109,7 +109,7 @@ def test_prompt_argument_checks(L, change, status):
 
 @pytest.mark.parametrize("change,status", CACHE + [(dict(pages=None), "INVALID"), (dict(v=None), "INVALID")])
 def test_prompt_cache_checks(L, change, status):
-    _expect(L, L.lib.latent_attn_prompt(ctypes.byref(_prompt(L, cache=_cache(L, **change), k=None)), None), status)
+    _expect(L, L.lib.latent_attn_prompt(ctypes.byref(_prompt(L, cache=_cache(L, **change), k=None, n_keys=0)), None), status)
 
 
 def test_calls_of_no_size_succeed(L):

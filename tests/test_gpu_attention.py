@@ -315,6 +315,38 @@ def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
     _prompt_check(gpu, _gen(D), list(new), [n + ahead for n in new], Hq, Hkv, D, torch.bfloat16, True, page, by=4.0)
 
 
+@pytest.mark.parametrize("new,ahead,Hq,Hkv,D,page,causal", [
+    ((1,), 20001, 8, 1, 128, 64, True),              # one row tile, all the chip
+    ((5, 64, 1, 0, 300), 4000, 6, 3, 64, 48, True),
+    ((40, 3), 9000, 4, 2, 256, 16, False),
+    ((2000, 10), 0, 2, 1, 96, 0, True),              # early rows see too little to be split
+    ((1500,), 0, 4, 2, 128, 0, False),
+    ((3, 700), 1500, 16, 1, 72, 7, True),
+])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_prompt_split_over_the_keys(gpu, new, ahead, Hq, Hkv, D, page, causal, dtype):
+    keys = [n + ahead // (1 + 2 * b) for b, n in enumerate(new)]
+    assert gpu.attend_prompt_workspace_size(sum(new), len(new), Hq, Hkv, D, 0 if page else sum(keys), max(keys), 1) > 0
+    _prompt_check(gpu, _gen(D), list(new), keys, Hq, Hkv, D, _dt(dtype), causal, page, by=3.0)
+
+
+def test_prompt_workspace_given_short_or_whole(gpu):
+    """Without its scratch a call takes each row tile in one workgroup: the same result to rounding."""
+    import torch
+
+    gen, dt, D = _gen(17), torch.bfloat16, 128
+    kc, vc, pages, seqs = paged(gen, [9000], 64, 2, D, dt)
+    q = _randn(gen, 70, 4, D, dt=dt)
+    args = (q, kc, vc, pages, _ints([9000]), _ints([0, 70]))
+    n = gpu.attend_prompt_workspace_size(70, 1, 4, 2, D, 0, pages.shape[1], 64)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    want = gpu.attend_prompt_paged(*args)
+    assert torch.equal(gpu.attend_prompt_paged(*args, workspace=ws), want)
+    short = gpu.attend_prompt_paged(*args, workspace=ws[:n - 16])
+    for got in (want, short):
+        assert_attention(got, None, q, *seqs[0], visible(70, 9000, True, "cuda"), D ** -0.5)
+
+
 def test_prompt_many_sequences(gpu):
     """More sequences than one look of a wave over `starts`."""
     import torch
