@@ -27,7 +27,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRowsWave = 32;
 constexpr int kRowsTile = kRowsWave * kWaves;
-constexpr int kKeys = 64;  // keys of a tile
 // The exponentials' reference follows the running maximum only when it is passed by more than this (log2): the sums are
 // rescaled a few times a row instead of with almost every tile.  Probabilities then reach 2^8 before the
 // division by their sum, which costs no precision (f16 holds up to 2^15).
@@ -68,7 +67,11 @@ __device__ __forceinline__ int2 keys_of(const PromptParams& p, int b) {
 __device__ __forceinline__ int row_tiles(const PromptParams& p, int n) {
   return (n * p.G + kRowsTile - 1) / kRowsTile;
 }
-__device__ __forceinline__ int key_tiles(int m) { return (m + kKeys - 1) / kKeys; }
+// v, computed from here on: what only a rare branch needs is not kept in registers beside the common path's.
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // Keys that row r of a sequence of n queries and m keys sees.
 __device__ __forceinline__ int keys_seen(const PromptParams& p, int n, int m, int r) {
@@ -78,13 +81,13 @@ __device__ __forceinline__ int keys_seen(const PromptParams& p, int n, int m, in
 // ---- work items ------------------------------------------------------------------
 // A unit is a row tile of one sequence and key/value head.  Sequences go from the longest to the shortest, row tiles
 // from the last (which sees the most keys) to the first, so that short units fill the end of the launch.  Where the units
-// of all sequences are few against their keys, long ones are split: `chunk` key tiles an item, at least kChunk and so many
+// of all sequences are few against their keys, long ones are split: `chunk` keys an item (whole tiles), at least kChunk and so many
 // that about kItems items have work; each item of a split unit leaves a part (reference, sums, unnormalised rows), and
 // join_kernel adds them up.  Items of one chunk follow one another: they read the same keys, at about the same time, on the
 // same XCD (equal spans of the line of all key tiles, each workgroup's keys its own, balanced as well and ran three
 // times longer: 14 prompts of up to 2000 tokens 375 us, 190 us a unit a workgroup).
 // Every wave finds its item by itself, from the sequences in its lanes; more than 64 sequences are taken as they come.
-constexpr int kChunk = 8, kItems = 512;
+constexpr int kChunk = 512, kItems = 512, kChunkStep = 64;
 // Sequence `lane`: its row tiles, keys, and the parts of its units.
 struct Line {
   int s0, n, k0, m;
@@ -100,14 +103,13 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
   l.parts = 1;
   l.chunk = INT32_MAX;
   if (p.max_parts) {
-    const int kt = key_tiles(l.m);
-    float work = static_cast<float>(l.tiles) * static_cast<float>(kt);
+    float work = static_cast<float>(l.tiles) * static_cast<float>(l.m);
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) work += __shfl_xor(work, d);
-    // chunk > work Hkv / kItems: split units are less than kItems, and their parts, kt / chunk + 1 < 2 kt / chunk each, less
+    // chunk > work Hkv / kItems: split units are less than kItems, and their parts, m / chunk + 1 < 2 m / chunk each, less
     // than 2 kItems (1.001 is for the rounding of the sum).
-    l.chunk = uniform(max(kChunk, static_cast<int>(min(work * static_cast<float>(p.Hkv) * (1.001f / kItems), 1e9f)) + 1));
-    if (kt > l.chunk) l.parts = (kt + l.chunk - 1) / l.chunk;
+    l.chunk = uniform(max(kChunk, (static_cast<int>(min(work * static_cast<float>(p.Hkv) * (1.001f / kItems), 1e9f)) / kChunkStep + 1) * kChunkStep));
+    if (l.m > l.chunk) l.parts = (l.m + l.chunk - 1) / l.chunk;
   }
   return l;
 }
@@ -121,7 +123,8 @@ __device__ __forceinline__ int items_before(const PromptParams& p, const Line& l
   return before;
 }
 struct Item {
-  int b, tile, part, chunk;
+  int b, tile, part, chunk;  // chunk: keys
+  int place;                 // in the order of all items
   int s0, n, k0, m;  // the sequence's queries and keys
 };
 template <bool kPaged>
@@ -142,25 +145,26 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane
         const int first = __builtin_ctzll(past);
         const int b = b0 + first;
         const int2 q = rows_of(p.starts, b, p.T), k = keys_of<kPaged>(p, b);
-        return {b, __builtin_amdgcn_readlane(upto, first) - 1 - x, 0, INT32_MAX, uniform(q.x), uniform(q.y), uniform(k.x), uniform(k.y)};
+        return {b, __builtin_amdgcn_readlane(upto, first) - 1 - x, 0, INT32_MAX, 0, uniform(q.x), uniform(q.y), uniform(k.x), uniform(k.y)};
       }
       base = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     return {-1};
   }
   const Line l = line_of<kPaged>(p, lane);
-  const int items = l.tiles * l.parts, before = items_before(p, l, items, lane);
+  const int items = l.tiles * l.parts;
+  const int before = items_before(p, l, items, lane);
   const uint64_t mine = __ballot(x >= before && x - before < items);
   if (!mine) return {-1};
   const int b = __builtin_ctzll(mine), r = x - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
   const int part = uniform(r / t);
-  return {b, t - 1 - (r - part * t), part, l.chunk, __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
+  return {b, t - 1 - (r - part * t), part, l.chunk, uniform(x), __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
           __builtin_amdgcn_readlane(l.k0, b), __builtin_amdgcn_readlane(l.m, b)};
 }
 
 // A tile in LDS: rows of kC 16-byte pieces, permuted so that the lanes of a read spread over all banks: a key row's
 // pieces for neighbouring keys; 64 bytes of four neighbouring value rows.  Piece c of row `key` lies at place c ^ *_turn(key).
-template <int kDP>
+template <int kDP, int kKeys>
 struct Shared {
   static constexpr int kC = kDP / 8;
   static constexpr uint32_t kTile = kKeys * kDP * 2;
@@ -190,10 +194,10 @@ __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
   return ((w & kExp) == kExp ? 0xFFFFu : 0u) | ((w >> 16 & kExp) == kExp ? 0xFFFF0000u : 0u);
 }
 
-template <typename E, int kDP, bool kPaged, bool kLse>
+template <typename E, int kDP, int kKeys, bool kPaged, bool kLse>
 __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(PromptParams p) {
-  typedef Shared<kDP> S;
-  constexpr int kC = S::kC, kSteps = kDP / 16, kBlocks = kDP / 32;
+  typedef Shared<kDP, kKeys> S;
+  constexpr int kKeyBlocks = kKeys / 32, kC = S::kC, kSteps = kDP / 16, kBlocks = kDP / 32;
   constexpr int kRowsLoad = kWave / kC, kLoads = kKeys / kWaves / kRowsLoad;  // rows of a direct load; loads of a wave and tile
   constexpr uint32_t kRow = kDP * 2;
   __shared__ S sm;
@@ -207,23 +211,23 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   const char* vbase = p.cache.v + hk * p.cache.v_head + it.k0 * p.cache.v_row;
 
   // This lane's row, and how many keys it sees.
-  const int all = n * p.G, row0 = tile * kRowsTile, w0 = row0 + wave * kRowsWave, row = w0 + l32;
-  const bool live = row < all;
-  const int rc = min(row, all - 1), tok = p.by_group.of(rc), head = hk * p.G + rc - tok * p.G;
-  const int vis = keys_seen(p, n, m, row);
+  const int all = n * p.G, row0 = tile * kRowsTile, w0 = row0 + wave * kRowsWave;
+  const int vis = keys_seen(p, n, m, w0 + l32);
   const int all_see = uniform(keys_seen(p, n, m, row0));                      // keys that every row of the workgroup sees
   const int end = uniform(keys_seen(p, n, m, row0 + kRowsTile - 1));          // keys that some row sees
   const int wave_all = uniform(keys_seen(p, n, m, w0));                       // of the wave
   const int wave_any = uniform(w0 < all ? keys_seen(p, n, m, w0 + kRowsWave - 1) : 0);
-  // This item's key tiles, and whether they are all of the unit's.
-  const int tiles = key_tiles(end), t0 = it.part ? it.part * it.chunk : 0, t1 = min(tiles, t0 + min(tiles, it.chunk));
-  if (t0 > 0 && t0 >= tiles) return;
-  const bool whole_unit = t0 == 0 && t1 == tiles;
-  const int stop = min(end, t1 * kKeys);
+  // This item's keys, and whether they are all of the unit's.
+  const int begin = it.part ? it.part * it.chunk : 0;
+  if (begin > 0 && begin >= end) return;
+  const int stop = begin + min(end - begin, it.chunk);
+  const bool whole_unit = begin == 0 && stop == end;
 
   u32x4 q[kSteps];
   {
-    const char* src = p.q + (it.s0 + tok) * p.q_token + head * p.q_head;
+    const int row = w0 + l32, rc = min(row, all - 1), tok = p.by_group.of(rc);
+    const bool live = row < all;
+    const char* src = p.q + (it.s0 + tok) * p.q_token + (hk * p.G + rc - tok * p.G) * p.q_head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int d = 16 * s + 8 * h;
@@ -232,9 +236,9 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
   }
 
-  // Loading: load i of a wave covers kRowsLoad rows from 16 wave + i kRowsLoad; lane l takes the piece that belongs at place
+  // Loading: load i of a wave covers kRowsLoad rows of its quarter of the tile; lane l takes the piece that belongs at place
   // l % kC of row l / kC.  Offsets within a tile for packed rows; the pieces of a row for any.
-  const int lrow = 16 * wave + lane / kC, lpos = lane % kC;
+  const int lrow = kKeys / kWaves * wave + lane / kC, lpos = lane % kC;
   uint32_t koff[kPaged ? 1 : kLoads], voff[kPaged ? 1 : kLoads];
   if constexpr (!kPaged) {
 #pragma unroll
@@ -255,15 +259,25 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   auto load = [&](int kt, int buf, uint32_t page_in_lane) {
     const uint32_t to_k = lds_k + buf * S::kTile, to_v = lds_v + buf * S::kTile;
     if constexpr (!kPaged) {
-      if (kt + kKeys <= end && exact) {
+      if (kt + kKeys <= end) {
         const char *from_k = kbase + kt * p.cache.k_row, *from_v = vbase + kt * p.cache.v_row;
+        if (exact) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) dma16s(from_k, koff[i], to_k + i * (kWave * 16));
+          for (int i = 0; i < kLoads; ++i) dma16s(from_k, koff[i], to_k + i * (kWave * 16));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) dma16s(from_v, voff[i], to_v + i * (kWave * 16));
+          for (int i = 0; i < kLoads; ++i) dma16s(from_v, voff[i], to_v + i * (kWave * 16));
+        } else {  // pieces beyond D stay the zeros they were set to
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int row_in = lrow + i * kRowsLoad;
+            if (8 * (lpos ^ S::k_turn(row_in)) < p.D) dma16s(from_k, koff[i], to_k + i * (kWave * 16));
+            if (8 * (lpos ^ S::v_turn(row_in)) < p.D) dma16s(from_v, voff[i], to_v + i * (kWave * 16));
+          }
+        }
         return;
       }
     }
+    const int ln = opaque(lane), lrow = kKeys / kWaves * wave + ln / kC, lpos = ln % kC;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row_in = lrow + i * kRowsLoad, key = kt + row_in, ck = lpos ^ S::k_turn(row_in), cv = lpos ^ S::v_turn(row_in);
@@ -301,13 +315,13 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   float top = -INFINITY, sum = 0.f, full = 0.f;
   uint32_t page_now = 0, page_next = 0;  // paged: page_of this tile and the next
 
-  auto step = [&](int t, auto bufc) {
+  auto step = [&](int kt, auto bufc) {
     constexpr int buf = decltype(bufc)::value;
-    const int kt = t * kKeys;
     pipeline_barrier();  // this tile is there, the other buffer read
-    uint64_t exists = ~uint64_t{0};
+    constexpr uint64_t kAll = ~uint64_t{0} >> (64 - kKeys);
+    uint64_t exists = kAll;
     if constexpr (kPaged) {
-      exists = __ballot(page_now < p.cache.n_pages);
+      exists = __ballot(page_now < p.cache.n_pages) & kAll;
       page_now = page_next;
     }
     if (kt + kKeys < stop) {
@@ -319,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     if (part_seen) {
 #pragma unroll
       for (int i = 0; i < kKeys * kC / kThreads; ++i) {
-        const int at = tid + i * kThreads;
+        const int at = opaque(tid) + i * kThreads;
         const uint32_t addr = lds_addr(sm.v[buf][0]) + 16 * at;
         const u32x4 x = lds_ld<u32x4>(addr);
         u32x4 is;
@@ -334,17 +348,20 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
       if (tid == 0) sm.bad[buf ^ 1] = 0;
     }
     if (kt >= wave_any) return;  // the other waves' rows see this tile
-    f32x16 s[2] = {};
+    f32x16 s[kKeyBlocks] = {};
+    
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
-    if (!(kt + kKeys <= wave_all && exists == ~uint64_t{0})) {
+      for (int blk = 0; blk < kKeyBlocks; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
+    
+    
+    if (!(kt + kKeys <= wave_all && exists == kAll)) {
       asm volatile("");  // keeps this a branch: most tiles need none of it
-      const int left = vis - kt - 4 * h;  // of the keys from this lane's first on
+      const int left = vis - kt - 4 * (opaque(lane) >> 5);  // of the keys from this lane's first on
       const uint64_t there = exists >> (4 * h);
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+      for (int blk = 0; blk < kKeyBlocks; ++blk)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = 32 * blk + 8 * (r >> 2) + (r & 3);
@@ -356,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) m2[blk] = fmaxf(m2[blk], s[blk][r]);
+      for (int blk = 0; blk < kKeyBlocks; ++blk) m2[kKeyBlocks == 1 ? r & 1 : blk] = fmaxf(m2[kKeyBlocks == 1 ? r & 1 : blk], s[blk][r]);
     const float t2 = op_over(fmaxf(m2[0], m2[1]), 32, 64, OpMax{}) * p.scale_log2;
     if (__any(t2 > top + kSlack)) {
       const float up = fmaxf(top, t2), f = exp2_fast(top - finite_max(up));
@@ -368,29 +385,32 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
     const float mm = finite_max(top);
     float part[2] = {0.f, 0.f};
-    u32x4 prob[4];
+    float part_sum[2] = {sum, 0.f};
+    u32x4 prob[2 * kKeyBlocks];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
+    for (int kk = 0; kk < 2 * kKeyBlocks; ++kk)
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         const float x = exp2_fast(s[kk >> 1][8 * (kk & 1) + 2 * a] * p.scale_log2 - mm);
         const float y = exp2_fast(s[kk >> 1][8 * (kk & 1) + 2 * a + 1] * p.scale_log2 - mm);
         prob[kk][a] = pack2<E>(x, y);
-        sum = E::add2(prob[kk][a], sum);
+        part_sum[a & 1] = E::add2(prob[kk][a], part_sum[a & 1]);
         if constexpr (kLse) {
           part[0] += x;
           part[1] += y;
         }
       }
+    sum = part_sum[0] + part_sum[1];
     if constexpr (kLse) full += part[0] + part[1];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)  // 16 keys
+    for (int kk = 0; kk < 2 * kKeyBlocks; ++kk)  // 16 keys
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         const uint32_t at = (vat ^ (64 * i)) + buf * S::kTile + 16 * kk * kRow;
         const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
         acc[i] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, prob[kk], acc[i]);
       }
+    
     if (part_seen) {  // what was cleared, to the rows that see it
       for (uint64_t bad = sm.bad[buf]; bad; bad &= bad - 1) {
         const int key = kt + __builtin_ctzll(bad);
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
           for (int rr = 0; rr < 4; ++rr) {
-            const int d = 32 * i + 8 * rr + 4 * h;
+            const int d = 32 * i + 8 * rr + 4 * (opaque(lane) >> 5);
             if (d >= p.D) continue;
             const u32x2 x = *reinterpret_cast<const u32x2*>(vbase + vo + 2 * d);
 #pragma unroll
@@ -419,33 +439,40 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
   };
 
-  if (t0 < t1) {
+  if (begin < stop) {
     if (tid < 2) sm.bad[tid] = 0;
-    if constexpr (kPaged) {
-      page_now = page_of(t0 * kKeys);
-      page_next = page_of((t0 + 1) * kKeys);
+    if (!kPaged && !exact) {
+      for (uint32_t i = tid; i < 4 * S::kTile / 16; i += kThreads) lds_st(lds_addr(sm.k[0][0]) + 16 * i, u32x4{0, 0, 0, 0});
+      lds_barrier();
     }
-    load(t0 * kKeys, 0, page_now);
-    for (int t = t0; t < t1; t += 2) {
-      step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
+    if constexpr (kPaged) {
+      page_now = page_of(begin);
+      page_next = page_of(begin + kKeys);
+    }
+    load(begin, 0, page_now);
+    for (int kt = begin; kt < stop; kt += 2 * kKeys) {
+      step(kt, std::integral_constant<int, 0>{});
+      if (kt + kKeys < stop) step(kt + kKeys, std::integral_constant<int, 1>{});
     }
   }
 
   sum = op_over(sum, 32, 64, OpAdd{});
   if constexpr (kLse) full = op_over(full, 32, 64, OpAdd{});
   if (!whole_unit) {
-    if (static_cast<int>(blockIdx.x) >= p.max_parts) return;  // never, by the choice of chunk
-    f32x4* to = p.part_acc + static_cast<int64_t>(blockIdx.x) * (4 * kBlocks * kThreads) + tid;
+    const int part = it.place * p.Hkv + hk;
+    if (part >= p.max_parts) return;  // never, by the choice of chunk
+    f32x4* to = p.part_acc + static_cast<int64_t>(part) * (4 * kBlocks * kThreads) + tid;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
       for (int rr = 0; rr < 4; ++rr)
         to[(4 * i + rr) * kThreads] = f32x4{acc[i][4 * rr], acc[i][4 * rr + 1], acc[i][4 * rr + 2], acc[i][4 * rr + 3]};
-    p.part_ml[static_cast<int64_t>(blockIdx.x) * kThreads + tid] = f32x4{top, sum, full, 0.f};
+    p.part_ml[static_cast<int64_t>(part) * kThreads + tid] = f32x4{top, sum, full, 0.f};
     return;
   }
-  if (!live) return;
+  const int row = w0 + (opaque(lane) & 31);
+  if (row >= all) return;
+  const int tok = p.by_group.of(row), head = hk * p.G + row - tok * p.G;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   char* dst = p.out + (it.s0 + tok) * p.o_token + head * p.o_head;
 #pragma unroll
@@ -476,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   const int first = __builtin_amdgcn_readlane(items_before(p, l, l.tiles * l.parts, lane), b) + r, tile = t - 1 - r;
   const int2 qs = rows_of(p.starts, b, p.T);
   const int n = qs.y, m = keys_of<kPaged>(p, b).y;
-  const int parts = (key_tiles(keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1)) + l.chunk - 1) / l.chunk;
+  const int parts = (keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1) + l.chunk - 1) / l.chunk;
   if (parts < 2) return;  // its rows see too little to be split
   const int at = first * p.Hkv + hk, step = t * p.Hkv;
   float top = -INFINITY, sum = 0.f, full = 0.f;
@@ -642,7 +669,7 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
     auto go = [&](auto paged_c, auto lse_c) {
       constexpr bool kPaged = decltype(paged_c)::value, kLse = decltype(lse_c)::value;
       const dim3 grid(static_cast<unsigned>(units + (p.max_parts ? more : 0)));
-      hipLaunchKernelGGL((prompt_kernel<E, kDP, kPaged, kLse>), grid, dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL((prompt_kernel<E, kDP, kDP == 256 ? 32 : 64, kPaged, kLse>), grid, dim3(kThreads), 0, s, p);
       if (p.max_parts)
         hipLaunchKernelGGL((join_kernel<E, kDP, kPaged, kLse>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32),
                            dim3(kThreads), 0, s, p);
