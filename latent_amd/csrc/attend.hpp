@@ -102,10 +102,13 @@ __device__ __forceinline__ void lds_st(uint32_t addr, T v) {
   *reinterpret_cast<__attribute__((address_space(3))) T*>(static_cast<uintptr_t>(addr)) = v;
 }
 
-// Workgroup barriers: every wave's direct loads have landed and its LDS accesses are done; or the latter alone.
+// Workgroup barriers: all but the last kLeft of every wave's direct loads have landed and its LDS accesses are done; or the
+// latter alone.
+template <int kLeft = 0>
 __device__ __forceinline__ void pipeline_barrier() {
+  static_assert(kLeft >= 0 && kLeft < 64, "the wait counter's field");
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4) << 14 | 0x0070);  // vmcnt(kLeft) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }

@@ -551,8 +551,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   }
 }
 
-// Longest keys from which units may be split, and units up to which they are few.
-constexpr int64_t kShortKeys = 1024, kFewUnits = 1024;
+// Units may be split where keys are long, and where they are few: packed ones less than the CUs (256 units of 2048 keys 51 us
+// with the parts' second launch, 45 without); sequences in the cache, of which the page table only bounds the lengths, up to four times as many
+// (eight chunks of up to 600 tokens behind up to 4000: 84 us split, 121 not).
+constexpr int64_t kShortKeys = 1024, kFewPacked = 256, kFewPaged = 1024;
 struct Plan {
   int64_t units;  // at most
   bool split;
@@ -563,8 +565,9 @@ Plan plan_for(const latent_attn_prompt_args& a) {
   const int64_t G = a.n_head / a.n_kv_head;
   // A sequence's rows round up to whole tiles: at most one more each.
   pl.units = std::max<int64_t>(0, (a.n_tokens * G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1) * a.n_kv_head;
-  const int64_t keys = a.k || a.n_keys ? a.n_keys : a.cache.max_pages * a.cache.page_size;
-  pl.split = keys > kShortKeys && pl.units < kFewUnits && a.cache.n_seq <= kWave;
+  const bool packed = a.k || a.n_keys;
+  const int64_t keys = packed ? a.n_keys : a.cache.max_pages * a.cache.page_size;
+  pl.split = keys > kShortKeys && keys <= (1 << 28) && pl.units < (packed ? kFewPacked : kFewPaged) && a.cache.n_seq <= kWave;
   if (!pl.split) return pl;
   const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
   pl.acc_bytes = size_t{2} * kItems * 4 * blocks * kThreads * sizeof(f32x4);
