@@ -126,7 +126,14 @@ __device__ __forceinline__ u32x4 pair_rows(const uint32_t (&v)[8][kVec / 2], int
   return r;
 }
 
-template <typename E, int kDP, bool kExact, int kMT, bool kPage8>
+// Rows of a cache that is larger than what the last-level cache keeps from step to step pass it by.
+template <bool kOnce, typename T>
+__device__ __forceinline__ T load_row(const char* at) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const T*>(at));
+  return *reinterpret_cast<const T*>(at);
+}
+
+template <typename E, int kDP, bool kExact, int kMT, bool kPage8, bool kOnce>
 struct Stream {
   static constexpr int kVec = kDP / 16, kK = kDP / 32;
 
@@ -180,9 +187,9 @@ struct Stream {
       for (int s = 0; s < kK; ++s) {
         const int d = 32 * s + 8 * kq;
         if constexpr (kExact) {
-          k[blk][s] = *reinterpret_cast<const u32x4*>(row + 2 * d);
+          k[blk][s] = load_row<kOnce, u32x4>(row + 2 * d);
         } else {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(row + 2 * min(d, static_cast<int>(p.D) - 8));
+          const u32x4 x = load_row<kOnce, u32x4>(row + 2 * min(d, static_cast<int>(p.D) - 8));
           k[blk][s] = d < static_cast<int>(p.D) ? x : u32x4{0, 0, 0, 0};
         }
       }
@@ -200,7 +207,7 @@ struct Stream {
       const char* row = ok ? vbase + pl.page * p.cache.v_page + row_in * p.cache.v_row : reinterpret_cast<const char*>(kZeroRow);
       const int d0 = kVec * (lane & 15);
       if constexpr (kVec == 4) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(row + 2 * (kExact ? d0 : min(d0, static_cast<int>(p.D) - 4)));
+        const u32x2 x = load_row<kOnce, u32x2>(row + 2 * (kExact ? d0 : min(d0, static_cast<int>(p.D) - 4)));
         const bool in = kExact || d0 < static_cast<int>(p.D);
         v[j][0] = in ? x[0] : 0;
         v[j][1] = in ? x[1] : 0;
@@ -208,7 +215,7 @@ struct Stream {
 #pragma unroll
         for (int w = 0; w < kVec / 8; ++w) {
           const int d = d0 + 8 * w;
-          const u32x4 x = *reinterpret_cast<const u32x4*>(row + 2 * (kExact ? d : min(d, static_cast<int>(p.D) - 8)));
+          const u32x4 x = load_row<kOnce, u32x4>(row + 2 * (kExact ? d : min(d, static_cast<int>(p.D) - 8)));
           const bool in = kExact || d < static_cast<int>(p.D);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[j][4 * w + e] = in ? x[e] : 0;
@@ -277,7 +284,7 @@ struct Stream {
   }
 };
 
-template <typename E, int kDP, bool kExact, int kMT, bool kPage8>
+template <typename E, int kDP, bool kExact, int kMT, bool kPage8, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(DecodeParams p) {
   constexpr int kVec = kDP / 16, kK = kDP / 32, kPad = kDP + 4;
   __shared__ float ml[kWaves][kMT * 16][2];
@@ -327,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
   while (cur < last) {
     const uint32_t n = min(nt - tile, last - cur);
     const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
-    Stream<E, kDP, kExact, kMT, kPage8> st{p, lane, kq, len, p.cache.pages + b * p.cache.pages_stride,
+    Stream<E, kDP, kExact, kMT, kPage8, kOnce> st{p, lane, kq, len, p.cache.pages + b * p.cache.pages_stride,
                                            p.cache.k + hk * p.cache.k_head, p.cache.v + hk * p.cache.v_head};
     u32x4 q[kMT][kK];
     Rows<kMT, kVec> r;
@@ -420,11 +427,12 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
   }
 }
 
-// Joins the parts of a unit: lane i of blockIdx.y holds eight elements of one row, each wave a quarter of the parts.
+// Joins the parts of a unit: lane i of blockIdx.y holds eight elements of one row, each wave a share of the parts.
 // A single pass under a running maximum, four parts in flight.
+constexpr int kJoinWaves = 16;
 template <typename E>
-__global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
-  __shared__ float sm[kWaves][10][kWave];
+__global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p) {
+  __shared__ float sm[kJoinWaves][10][kWave];
   const uint32_t unit = blockIdx.x, b = unit / p.U, u = unit % p.U;
   const int2 parts = p.unit_parts[unit];
   if (parts.y < 2) return;
@@ -433,14 +441,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
   const uint32_t pieces = p.D / 8, item = blockIdx.y * kWave + lane, row = min(item / pieces, nr - 1), c = item % pieces;
   float m = -INFINITY, l = 0.f;
   f32x4 x[2] = {};
-  for (int i0 = wave; i0 < parts.y; i0 += 4 * kWaves) {
+  const int waves = blockDim.x / kWave;
+  for (int i0 = wave; i0 < parts.y; i0 += 4 * waves) {
     float pm[4], pl[4];
     f32x4 px[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = min(i0 + j * kWaves, parts.y - 1);
+      const int i = min(i0 + j * waves, parts.y - 1);
       const int64_t at = (static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
-      pm[j] = i0 + j * kWaves < parts.y ? p.part_ml[2 * at] : -INFINITY;
+      pm[j] = i0 + j * waves < parts.y ? p.part_ml[2 * at] : -INFINITY;
       pl[j] = p.part_ml[2 * at + 1];
       const f32x4* src = reinterpret_cast<const f32x4*>(p.part_acc + at * p.D + 8 * c);
       px[j][0] = src[0];
@@ -467,10 +476,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
   __syncthreads();
   if (wave != 0 || item >= nr * pieces) return;
   float y[8] = {};
-  m = fmaxf(fmaxf(sm[0][0][lane], sm[1][0][lane]), fmaxf(sm[2][0][lane], sm[3][0][lane]));
+  m = -INFINITY;
+  for (int w = 0; w < waves; ++w) m = fmaxf(m, sm[w][0][lane]);
   l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < waves; ++w) {
     const float f = exp2_fast(sm[w][0][lane] - finite_max(m));
     l += f * sm[w][1][lane];
 #pragma unroll
@@ -488,14 +497,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(DecodeParams p) {
 struct Plan {
   int mt;
   uint32_t chunks, rows, U, groups;
-  bool whole;
+  bool whole, once;
   size_t ml_bytes, acc_bytes, unit_bytes;
 };
 
-// Up to this many tiles of the longest sequence a page table holds, each unit is one workgroup's: the parts and the
-// second launch cost more than the tiles one after the other.
+// Up to kWholeTiles tiles of the longest sequence a page table holds each unit is one workgroup's: the parts and the second
+// launch cost more than the tiles one after the other (301 tokens: 13.6 us in parts, 8.7 whole).  Twice as many where
+// the units alone fill the chip (32 sequences of up to 1000 tokens, 8 heads: 22.9 and 21.1 us; 12 sequences 13.4 and 20.0).
+constexpr int64_t kWholeTiles = 4, kManyWholeTiles = 8;
+// A call that may read more than this finds nothing of it in the last-level cache (256 MB) at the next step, and its loads leave
+// what others keep there alone (131071 tokens, 537 MB: 113 -> 103 us; 3.8 GB: 684 -> 658; 32 MB would go from 18.0 to 19.6).
+constexpr int64_t kOnceBytes = 256 << 20;
 constexpr int64_t kMaxUnits = 1 << 22;  // workgroups of a launch
-constexpr int64_t kWholeTiles = 4;
 
 Plan plan_for(const latent_attn_decode_args& a) {
   Plan pl{};
@@ -507,7 +520,9 @@ Plan plan_for(const latent_attn_decode_args& a) {
   const int64_t tiles = (a.cache.max_pages * a.cache.page_size + kTile - 1) / kTile;
   const int64_t items = a.cache.n_seq * pl.U * tiles;
   const int64_t units = a.cache.n_seq * pl.U;
-  pl.whole = tiles <= kWholeTiles;
+  const int64_t row = 4 * a.n_kv_head * a.head_dim;  // bytes of a position
+  pl.once = std::min(a.cache.n_seq * a.cache.max_pages, a.cache.n_pages) > kOnceBytes / (row * a.cache.page_size);
+  pl.whole = tiles <= kWholeTiles || (tiles <= kManyWholeTiles && units >= 256 && units <= 1024);
   if (pl.whole) {
     pl.groups = static_cast<uint32_t>(units);
     return pl;
@@ -591,8 +606,15 @@ extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_st
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   auto launch = [&](auto e, auto dp, auto exact, auto mt, auto page8) {
-    hipLaunchKernelGGL((decode_kernel<decltype(e), decltype(dp)::value, decltype(exact)::value, decltype(mt)::value, decltype(page8)::value>),
-                       dim3(pl.groups), dim3(kThreads), 0, s, p);
+    auto go = [&](auto once) {
+      hipLaunchKernelGGL((decode_kernel<decltype(e), decltype(dp)::value, decltype(exact)::value, decltype(mt)::value,
+                                        decltype(page8)::value, decltype(once)::value>),
+                         dim3(pl.groups), dim3(kThreads), 0, s, p);
+    };
+    if constexpr (decltype(exact)::value && decltype(page8)::value)
+      pl.once ? go(std::true_type{}) : go(std::false_type{});
+    else
+      go(std::false_type{});
   };
   using std::integral_constant;
   auto with_dim = [&](auto e, auto dp) {
@@ -619,11 +641,13 @@ extern "C" int latent_attn_decode(const latent_attn_decode_args* args, latent_st
   f16 ? with_type(F16{}) : with_type(BF16{});
   if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
   if (!pl.whole) {
-    const dim3 grid(p.B * p.U, (p.rows * (p.D / 8) + kWave - 1) / kWave);
+    // A unit has about groups / units parts, four in flight a wave.
+    const uint32_t units = p.B * p.U;
+    const dim3 grid(units, (p.rows * (p.D / 8) + kWave - 1) / kWave), block(kWave * (pl.groups > 16 * units ? kJoinWaves : 4));
     if (f16)
-      hipLaunchKernelGGL(join_kernel<F16>, grid, dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL(join_kernel<F16>, grid, block, 0, s, p);
     else
-      hipLaunchKernelGGL(join_kernel<BF16>, grid, dim3(kThreads), 0, s, p);
+      hipLaunchKernelGGL(join_kernel<BF16>, grid, block, 0, s, p);
     if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
   }
   return LATENT_OK;
