@@ -79,6 +79,10 @@ def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cu
     return torch.stack((angle.cos(), angle.sin()), 1).float().contiguous()
 
 
+def _no_grad():
+    raise RuntimeError("attention here has no backward pass: call it under torch.no_grad()")
+
+
 def _heads(t: torch.Tensor, name: str, dt: torch.dtype, dev: int):
     """[T, heads, D] as the kernels read it (a copy where strides or base do not fit), its base, strides and shape."""
     shape = t.shape
@@ -88,6 +92,8 @@ def _heads(t: torch.Tensor, name: str, dt: torch.dtype, dev: int):
         raise TypeError(f"{name} must be {dt}, as the queries and the cache are")
     if t.get_device() != dev:
         raise ValueError(f"{name} must be on cuda:{dev}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _no_grad()
     st, sh, sd = t.stride()
     p = t.data_ptr()
     if (sd != 1 and shape[2] > 1) or (st | sh) & 7 or p & 15 or st >= _FAR:
@@ -114,6 +120,8 @@ def _out(t: Optional[torch.Tensor], like: torch.Tensor, name: str):
         return t, t.data_ptr(), *t.stride()[:2]
     if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must be {like.dtype} {list(like.shape)} on {like.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _no_grad()
     st, sh, sd = t.stride()
     if (sd != 1 and t.shape[2] > 1) or (st | sh) & 7 or t.data_ptr() & 15:
         raise ValueError(f"{name} must have adjacent D, strides that are multiples of 8 and a 16-byte aligned base")
@@ -135,6 +143,8 @@ def _cache(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, dev: int):
         raise ValueError("k_cache and v_cache must be [pages, page rows, kv heads, D], of one shape")
     if dt not in _DTYPE or v.dtype is not dt:
         raise TypeError("the cache must be f16 or bf16, keys and values alike")
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _no_grad()
     if k.get_device() != dev or v.get_device() != dev or pages.get_device() != dev:
         raise ValueError(f"the cache and its page table must be on cuda:{dev}")
     B_most = pages.shape
@@ -162,8 +172,6 @@ def _first(t: torch.Tensor, name: str) -> int:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DTYPE:
         raise TypeError(f"{name} must be f16 or bf16")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("attention here has no backward pass: call it under torch.no_grad()")
     return t.get_device()
 
 
@@ -454,6 +462,8 @@ class Attention:
         if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head or w_o.shape[0] % n_head:
             raise ValueError("n_head must be a multiple of n_kv_head, and w_o's rows one of n_head")
         D = w_o.shape[0] // n_head
+        if D % 8 or not 0 < D <= 256:
+            raise ValueError(f"heads of {D} dimensions: a multiple of 8 up to 256 is supported")
         if w_qkv.shape[1] != (n_head + 2 * n_kv_head) * D or w_o.shape[1] != w_qkv.shape[0] or w_o.device != w_qkv.device:
             raise ValueError(f"w_qkv {list(w_qkv.shape)} and w_o {list(w_o.shape)} do not fit {n_head} and {n_kv_head} heads")
         self.w_qkv, self.w_o = w_qkv.detach().contiguous(), w_o.detach().contiguous()
@@ -469,8 +479,9 @@ class Attention:
     def _append(self, x: torch.Tensor, pages, positions, seqs) -> torch.Tensor:
         qkv = (x.to(self.w_qkv.dtype) @ self.w_qkv).view(x.shape[0], -1, self.head_dim)
         H, K = self.n_head, self.n_kv_head
+        q = qkv[:, :H]
         return kv_append(qkv[:, H:H + K], qkv[:, H + K:], self.k_cache, self.v_cache, pages, positions, seqs=seqs,
-                         q=qkv[:, :H], rope=self.rope, interleaved=self.interleaved)
+                         q=q, rope=self.rope, interleaved=self.interleaved, q_out=q)
 
     def _project(self, a: torch.Tensor) -> torch.Tensor:
         return a.view(a.shape[0], -1) @ self.w_o
@@ -484,6 +495,8 @@ class Attention:
     def prompt(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor,
                lengths: torch.Tensor) -> torch.Tensor:
         """New tokens of several sequences, packed: x [T, d], token t of sequence seqs[t] (row of pages) at positions[t],
-        sequence b's being rows starts[b] .. starts[b + 1] - 1 and the last of its lengths[b]."""
+        sequence b's being rows starts[b] .. starts[b + 1] - 1 and the last of its lengths[b].  Rows of no sequence
+        (padding, at negative positions) give zeros."""
         q = self._append(x, pages, positions, seqs)
-        return self._project(attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale))
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        return self._project(attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out))

@@ -18,7 +18,12 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 
 // The two element types: conversions and the fp32-accumulating products.  Eight
 // elements of an operand travel as four dwords.
+//
+// Probabilities that are to be rounded to f16 are held times 2^kLift, so that the largest come near the type's
+// largest: unlifted, those below 2^-14 of the largest would lose their bits, and a hundred thousand of them are not little.
+// bf16 has fp32's range and needs none.
 struct F16 {
+  static constexpr float kLift = 15.f;
   typedef _Float16 T;
   typedef _Float16 T2 __attribute__((ext_vector_type(2)));
   typedef _Float16 T8 __attribute__((ext_vector_type(8)));
@@ -34,6 +39,7 @@ struct F16 {
   }
 };
 struct BF16 {
+  static constexpr float kLift = 0.f;
   typedef __bf16 T;
   typedef __bf16 T2 __attribute__((ext_vector_type(2)));
   typedef __bf16 T8 __attribute__((ext_vector_type(8)));
@@ -102,13 +108,10 @@ __device__ __forceinline__ void lds_st(uint32_t addr, T v) {
   *reinterpret_cast<__attribute__((address_space(3))) T*>(static_cast<uintptr_t>(addr)) = v;
 }
 
-// Workgroup barriers: all but the last kLeft of every wave's direct loads have landed and its LDS accesses are done; or the
-// latter alone.
-template <int kLeft = 0>
+// Workgroup barriers: every wave's direct loads have landed and its LDS accesses are done; or the latter alone.
 __device__ __forceinline__ void pipeline_barrier() {
-  static_assert(kLeft >= 0 && kLeft < 64, "the wait counter's field");
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4) << 14 | 0x0070);  // vmcnt(kLeft) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }

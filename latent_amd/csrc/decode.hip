@@ -112,7 +112,7 @@ __device__ __forceinline__ Span find_span(const DecodeParams& p, int lane) {
 
 template <int kMT, int kVec>
 struct Rows {  // a wave's running softmax: lane (query lane & 15, dims 4 kVec (lane >> 4) ..)
-  float m[kMT], l[kMT];  // l: this lane's keys
+  float m[kMT], l[kMT];  // l: this lane's keys; sums and rows are times 2^kLift
   f32x4 acc[kMT][kVec];
 };
 
@@ -256,12 +256,12 @@ struct Stream {
           top = fmaxf(top, x[j]);
         }
         top = fmaxf(r.m[mt], op_over(top, 16, 64, OpMax{}));
-        const float mm = finite_max(top), f = exp2_fast(r.m[mt] - mm);
+        const float mm = finite_max(top), f = exp2_fast(r.m[mt] - mm), from = mm - E::kLift;
         r.m[mt] = top;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[j] = exp2_fast(x[j] - mm);
+          x[j] = exp2_fast(x[j] - from);
           sum += x[j];
         }
         r.l[mt] = r.l[mt] * f + sum;
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
 #pragma unroll
           for (int a = 0; a < 4; ++a) y[a] = pack2<E>(x[a >> 1][2 * (a & 1)] * inv, x[a >> 1][2 * (a & 1) + 1] * inv);
           *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = y;
-          if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+          if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m - E::kLift + __log2f(l)) * kLn2;
         } else {
           f32x4* dst = reinterpret_cast<f32x4*>(p.part_acc + (part + row) * p.D + 8 * c);
           dst[0] = x[0];
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p
 #pragma unroll
   for (int a = 0; a < 4; ++a) o[a] = pack2<E>(y[2 * a] * inv, y[2 * a + 1] * inv);
   *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = o;
-  if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+  if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m - E::kLift + __log2f(l)) * kLn2;
 }
 
 struct Plan {

@@ -7,7 +7,7 @@
 // token r / G, query head r % G of the group: all heads that read the same keys
 // share the tiles, and a few tokens of many heads fill a tile as well as many of
 // one.  Keys come in tiles of 64 through LDS, one pass, with the running maximum
-// and sum of the softmax; the next tile is on its way into registers meanwhile.
+// and sum of the softmax; direct loads fill the other buffer with the next tile meanwhile.
 //
 // Each wave owns 32 rows.  scores^T = K Q^T on 32x32x16 products leaves every
 // lane the scores of one row (lane % 32) for keys 8 (r / 4) + 4 (lane / 32) + r % 4,
@@ -27,10 +27,13 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRowsWave = 32;
 constexpr int kRowsTile = kRowsWave * kWaves;
-// The exponentials' reference follows the running maximum only when it is passed by more than this (log2): the sums are
-// rescaled a few times a row instead of with almost every tile.  Probabilities then reach 2^8 before the
-// division by their sum, which costs no precision (f16 holds up to 2^15).
-constexpr float kSlack = 8.f;
+// The exponentials' reference follows the running maximum only when it is passed by more than kSlack (log2): the sums are
+// rescaled a few times a row instead of with almost every tile.  Probabilities are taken times 2^kUp so that with
+// that they end at f16's 2^15, where the small ones keep their bits, and at bf16's 1, where no product with a value can overflow.
+template <typename E>
+struct Scale {
+  static constexpr float kSlack = __is_same(E, F16) ? 2.f : 8.f, kUp = E::kLift - kSlack;
+};
 
 struct PromptParams {
   Cache cache;  // packed keys: k, v, k_row, k_head, v_row, v_head alone
@@ -124,8 +127,7 @@ __device__ __forceinline__ int items_before(const PromptParams& p, const Line& l
 }
 struct Item {
   int b, tile, part, chunk;  // chunk: keys
-  int place;                 // in the order of all items
-  int s0, n, k0, m;  // the sequence's queries and keys
+  int s0, n, k0, m;          // the sequence's queries and keys
 };
 template <bool kPaged>
 __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane) {  // b < 0: behind the last
@@ -145,7 +147,7 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane
         const int first = __builtin_ctzll(past);
         const int b = b0 + first;
         const int2 q = rows_of(p.starts, b, p.T), k = keys_of<kPaged>(p, b);
-        return {b, __builtin_amdgcn_readlane(upto, first) - 1 - x, 0, INT32_MAX, 0, uniform(q.x), uniform(q.y), uniform(k.x), uniform(k.y)};
+        return {b, __builtin_amdgcn_readlane(upto, first) - 1 - x, 0, INT32_MAX, uniform(q.x), uniform(q.y), uniform(k.x), uniform(k.y)};
       }
       base = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
@@ -158,7 +160,7 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane
   if (!mine) return {-1};
   const int b = __builtin_ctzll(mine), r = x - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
   const int part = uniform(r / t);
-  return {b, t - 1 - (r - part * t), part, l.chunk, uniform(x), __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
+  return {b, t - 1 - (r - part * t), part, l.chunk, __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
           __builtin_amdgcn_readlane(l.k0, b), __builtin_amdgcn_readlane(l.m, b)};
 }
 
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     const int key = kt + lane;
     return kPaged && key < stop ? static_cast<uint32_t>(pages[p.cache.by_page.of(key)]) : 0xFFFFFFFFu;
   };
-  // Rows kt .. kt + 63 of K and V into buffer buf.
+  // Rows kt .. kt + kKeys - 1 of K and V into buffer buf.
   auto load = [&](int kt, int buf, uint32_t page_in_lane) {
     const uint32_t to_k = lds_k + buf * S::kTile, to_v = lds_v + buf * S::kTile;
     if constexpr (!kPaged) {
@@ -349,13 +351,10 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     }
     if (kt >= wave_any) return;  // the other waves' rows see this tile
     f32x16 s[kKeyBlocks] = {};
-    
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int blk = 0; blk < kKeyBlocks; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
-    
-    
     if (!(kt + kKeys <= wave_all && exists == kAll)) {
       asm volatile("");  // keeps this a branch: most tiles need none of it
       const int left = vis - kt - 4 * (opaque(lane) >> 5);  // of the keys from this lane's first on
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
 #pragma unroll
       for (int blk = 0; blk < kKeyBlocks; ++blk) m2[kKeyBlocks == 1 ? r & 1 : blk] = fmaxf(m2[kKeyBlocks == 1 ? r & 1 : blk], s[blk][r]);
     const float t2 = op_over(fmaxf(m2[0], m2[1]), 32, 64, OpMax{}) * p.scale_log2;
-    if (__any(t2 > top + kSlack)) {
+    if (__any(t2 > top + Scale<E>::kSlack)) {
       const float up = fmaxf(top, t2), f = exp2_fast(top - finite_max(up));
       top = up;
       sum *= f;
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
     }
-    const float mm = finite_max(top);
+    const float mm = finite_max(top) - Scale<E>::kUp;
     float part[2] = {0.f, 0.f};
     float part_sum[2] = {sum, 0.f};
     u32x4 prob[2 * kKeyBlocks];
@@ -410,7 +409,6 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
         const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
         acc[i] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, prob[kk], acc[i]);
       }
-    
     if (part_seen) {  // what was cleared, to the rows that see it
       for (uint64_t bad = sm.bad[buf]; bad; bad &= bad - 1) {
         const int key = kt + __builtin_ctzll(bad);
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   sum = op_over(sum, 32, 64, OpAdd{});
   if constexpr (kLse) full = op_over(full, 32, 64, OpAdd{});
   if (!whole_unit) {
-    const int part = it.place * p.Hkv + hk;
+    const int part = blockIdx.x;  // items in their order, heads within
     if (part >= p.max_parts) return;  // never, by the choice of chunk
     f32x4* to = p.part_acc + static_cast<int64_t>(part) * (4 * kBlocks * kThreads) + tid;
 #pragma unroll
@@ -485,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
                                                        pack2<E>(acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv)};
     }
   if constexpr (kLse) {
-    if (h == 0) p.lse[static_cast<int64_t>(it.s0 + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
+    if (h == 0) p.lse[static_cast<int64_t>(it.s0 + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top - Scale<E>::kUp + __log2f(full)) * kLn2;
   }
 }
 
@@ -547,7 +545,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
       *reinterpret_cast<u32x2*>(dst + 2 * d) = u32x2{pack2<E>(x[rr][0] * inv, x[rr][1] * inv), pack2<E>(x[rr][2] * inv, x[rr][3] * inv)};
   }
   if constexpr (kLse) {
-    if (i == 0 && h == 0) p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top + __log2f(full)) * kLn2;
+    if (i == 0 && h == 0) p.lse[static_cast<int64_t>(qs.x + tok) * p.Hq + head] = full == 0.f ? -INFINITY : (top - Scale<E>::kUp + __log2f(full)) * kLn2;
   }
 }
 

@@ -265,6 +265,96 @@ def test_decode_strided_operands_and_given_buffers(gpu):
     assert torch.equal(gpu.attend_decode(odd, kc, vc, pages, _ints(lens)), got)
 
 
+@pytest.mark.parametrize("Hq,D,dtype", [(8, 128, "bf16"), (160, 128, "f16"), (24, 64, "f16"), (8, 256, "bf16")])
+def test_decode_of_a_cache_larger_than_the_last_level_cache(gpu, Hq, D, dtype):
+    """Page tables and pages of more than 256 MB: the rows' loads differ, the results do not."""
+    import torch
+
+    gen, dt, Hkv, page, lens = _gen(D + Hq), _dt(dtype), 8, 16, [300, 0, 2049, 1]
+    n_pages = (256 << 20) // (4 * Hkv * D * page) + 1
+    kc, vc, pages, seqs = paged(gen, lens, page, Hkv, D, dt, spare=n_pages, width=n_pages // 4 + 1)
+    q, L = _randn(gen, 4, Hq, D, dt=dt), _ints(lens)
+    out = _decode_check(gpu, q, kc, vc, pages, L, seqs, lens)
+    used = -(-max(lens) // page)
+    few = torch.cat((pages[:, :used], torch.full((4, pages.shape[1] // 2), -1, dtype=torch.int32, device="cuda")), 1)
+    assert torch.equal(gpu.attend_decode(q, kc, vc, few, L), out)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,most", [(64, 8, 4, 128, 1000), (43, 6, 6, 64, 641), (256, 40, 1, 72, 513)])
+def test_decode_units_of_several_tiles_that_fill_the_chip(gpu, B, Hq, Hkv, D, most):
+    import torch
+
+    gen, dt = _gen(B), torch.bfloat16
+    lens = [(97 * b + most) % (most + 1) for b in range(B)]
+    lens[0] = most
+    kc, vc, pages, seqs = paged(gen, lens, 16, Hkv, D, dt)
+    q = _randn(gen, B, Hq, D, dt=dt)
+    assert gpu.attend_decode_workspace_size(B, Hq, Hkv, D, pages.shape[1], 16) == 0
+    _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(1024, 1), (1024, 1024), (1024, 8), (1, 1)])
+def test_most_and_fewest_heads(gpu, Hq, Hkv):
+    import torch
+
+    gen, dt, D, lens = _gen(Hq + Hkv), torch.float16, 8, [700, 3]
+    kc, vc, pages, seqs = paged(gen, lens, 5, Hkv, D, dt)
+    q = _randn(gen, 2, Hq, D, dt=dt)
+    out = _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+    k, v = (_randn(gen, 4, Hkv, D, dt=dt) for _ in range(2))
+    pos = _ints([p - 1 for p in lens])  # over their last rows
+    q2 = gpu.kv_append(k[:2], v[:2], kc, vc, pages, pos, q=q)
+    assert torch.equal(q2, q)
+    seqs = [(torch.cat((a[:-1], k[b:b + 1])), torch.cat((c[:-1], v[b:b + 1]))) for b, (a, c) in enumerate(seqs)]
+    _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+    lse = torch.empty((2, Hq), device="cuda")
+    out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints(lens), _ints([0, 1, 2]), lse=lse)
+    for b, n in enumerate(lens):
+        assert_attention(out[b:b + 1], lse[b:b + 1], q[b:b + 1], *seqs[b], visible(1, n, True, "cuda"), D ** -0.5)
+
+
+# ---- numerics of both -----------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("score", [-9.0, -17.0])
+def test_many_small_probabilities_keep_their_bits(gpu, dtype, score):
+    """One key of weight 1 and value 0, 60000 of weight e^score and value 1: the result is all theirs.  e^-17 is 1.4 * 2^-25
+    of the largest, below f16's smallest normal number."""
+    import torch
+
+    gen, dt, D, n, page = _gen(18), _dt(dtype), 64, 60001, 64
+    kc, vc, pages, seqs = paged(gen, [n], page, 1, D, dt)
+    k, v = seqs[0]
+    k.zero_(), v.fill_(1.0)
+    k[:, 0, 0] = score
+    k[30, 0, 0], v[30] = 0.0, 0.0
+    rows, at = pages[0].long(), torch.arange(n, device="cuda")
+    kc[rows[at // page], at % page], vc[rows[at // page], at % page] = k, v
+    q = torch.zeros((3, 2, D), dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    _decode_check(gpu, q[:1], kc, vc, pages, _ints([n]), seqs, [n], scale=1.0)
+    seen = visible(3, n, True, "cuda")
+    lse = torch.empty((3, 2), device="cuda")
+    out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints([n]), _ints([0, 3]), scale=1.0, lse=lse)
+    assert_attention(out, lse, q, k, v, seen, 1.0)
+    whole = gpu.attend_prompt(q, k, v, _ints([0, 3]), k_starts=_ints([0, n]), scale=1.0,
+                              workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    assert_attention(whole, None, q, k, v, seen, 1.0)
+
+
+def test_prompt_large_values_under_rising_scores(gpu):
+    """Values of 2^115 under scores that rise by 0.05 a key (weights to 2^7 of the first tile's): the sums stay finite
+    (200 weights of at most 1 are less than 2^8, the products' sums less than 2^123)."""
+    import torch
+
+    gen, dt, D, n = _gen(19), torch.bfloat16, 64, 200
+    k, v = torch.zeros((n, 1, D), dtype=dt, device="cuda"), _randn(gen, n, 1, D, dt=dt).clamp(-4, 4) * 2.0 ** 113
+    k[:, 0, 0] = torch.arange(n, device="cuda") * 0.05
+    q = torch.zeros((n, 2, D), dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    out = gpu.attend_prompt(q, k, v, _ints([0, n]), scale=1.0)
+    assert_attention(out, None, q, k, v, visible(n, n, True, "cuda"), 1.0)
+
+
 # ---- prompt -------------------------------------------------------------------
 def _prompt_check(gpu, gen, new, keys, Hq, Hkv, D, dt, causal, page=0, pad=0, by=2.0):
     import torch
@@ -353,6 +443,7 @@ def test_prompt_many_sequences(gpu):
 
     new = [(7 * i) % 5 for i in range(150)]
     _prompt_check(gpu, _gen(9), new, new, 4, 2, 64, torch.float16, True)
+    _prompt_check(gpu, _gen(20), new, [n + 13 * (i % 9) for i, n in enumerate(new)], 4, 2, 64, torch.float16, True, page=16, pad=2)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -462,6 +553,76 @@ def test_captured_step_replays(gpu):
         assert torch.equal(a["out"], eager["out"]) and torch.equal(b["out"], eager["out"]), i
         assert torch.equal(a["pos"], eager["pos"])
         torch.randn((1000, 1000), device="cuda") @ torch.randn((1000, 1000), device="cuda")
+
+
+def test_captured_prompts_replay_over_other_lengths(gpu):
+    """A chunk of two prompts, split over the keys, in a graph: replayed as the cache grows and the chunk divides otherwise."""
+    import torch
+
+    gen, dt, D, page = _gen(21), torch.float16, 128, 16
+    kc, vc, pages, _ = paged(gen, [6000, 4000], page, 2, D, dt)
+    q, starts, lengths = _randn(gen, 100, 8, D, dt=dt), _ints([0, 60, 100]), _ints([5000, 40])
+    out, lse = torch.zeros_like(q), torch.zeros((100, 8), device="cuda")
+    call = lambda: gpu.attend_prompt_paged(q, kc, vc, pages, lengths, starts, out=out, lse=lse)
+    call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for new, keys in (([0, 60, 100], [5000, 40]), ([0, 1, 100], [6000, 4000]), ([0, 0, 90], [0, 3333]), ([5, 100, 100], [700, 0])):
+        starts.copy_(_ints(new)), lengths.copy_(_ints(keys)), q.copy_(_randn(gen, 100, 8, D, dt=dt))
+        out.fill_(9.0), lse.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), lse.clone()
+        out.fill_(9.0), lse.fill_(9.0)
+        call()
+        assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+        torch.randn((1000, 1000), device="cuda") @ torch.randn((1000, 1000), device="cuda")
+
+
+def test_two_calls_at_once(gpu):
+    """Calls on two streams, each with scratch of its own, as the calls take it when none is given."""
+    import torch
+
+    gen, dt, D, lens = _gen(22), torch.bfloat16, 128, [9000, 100]
+    kc, vc, pages, _ = paged(gen, lens, 16, 2, D, dt)
+    L, starts = _ints(lens), _ints([0, 30, 50])
+    q = [_randn(gen, 2, 16, D, dt=dt) for _ in range(2)]
+    p = [_randn(gen, 50, 16, D, dt=dt) for _ in range(2)]
+    want = [(gpu.attend_decode(a, kc, vc, pages, L), gpu.attend_prompt_paged(b, kc, vc, pages, L, starts)) for a, b in zip(q, p)]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(sides):
+            got[i].append((gpu.attend_decode(q[i], kc, vc, pages, L, stream=s),
+                           gpu.attend_prompt_paged(p[i], kc, vc, pages, L, starts, stream=s)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+
+
+def test_operands_that_want_gradients_are_refused(gpu):
+    import torch
+
+    gen, dt = _gen(23), torch.bfloat16
+    kc, vc, pages, _ = paged(gen, [20], 16, 1, 32, dt)
+    q, k, v = (_randn(gen, 1, 1, 32, dt=dt) for _ in range(3))
+    L, starts = _ints([20]), _ints([0, 1])
+    calls = (lambda q, k, v, kc, vc: gpu.kv_append(k, v, kc, vc, pages, _ints([3]), q=q),
+             lambda q, k, v, kc, vc: gpu.attend_prompt(q, k, v, starts),
+             lambda q, k, v, kc, vc: gpu.attend_prompt_paged(q, kc, vc, pages, L, starts),
+             lambda q, k, v, kc, vc: gpu.attend_decode(q, kc, vc, pages, L))
+    used = ((0, 1, 2, 3, 4), (0, 1, 2), (0, 3, 4), (0, 3, 4))
+    for call, which in zip(calls, used):
+        for i in which:
+            args = [q, k, v, kc, vc]
+            args[i] = args[i].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no_grad"):
+                call(*args)
+            with torch.no_grad():
+                call(*args)
 
 
 # ---- a run of them together -----------------------------------------------------
