@@ -115,9 +115,10 @@ class DecodeStack:
 
     def prompt(self, x: torch.Tensor, starts: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
         """New tokens of several sequences through every layer: x [N, d], packed; sequence b is rows starts[b] ..
-        starts[b + 1] - 1 (int32 [B + 1], from 0 to N) and goes on in slot slots[b] (int32 [B], different ones)
-        at that slot's position, or from 0 where the slot is idle.  The slots' pages have to have room.
-        Returns the output rows f32 [N, d]; the slots then decode what follows."""
+        starts[b + 1] - 1 (int32 [B + 1], ascending, up to N) and goes on in slot slots[b] (int32 [B], different
+        ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle.  The slots' pages have to
+        have room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
+        (padding) reach no cache and pass the experts alone."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")
         if x.dim() != 2 or x.shape[1] != self.d:
@@ -133,6 +134,7 @@ class DecodeStack:
         row = torch.arange(N, dtype=torch.int32, device=x.device)
         seqs = torch.searchsorted(starts[1:].contiguous(), row, right=True, out_int32=True).clamp_max(slots.numel() - 1)
         positions = row - starts[seqs.long()] + first[seqs.long()]
+        positions = torch.where((row >= starts[0]) & (row < starts[-1]), positions, -1)
         lengths = first + starts[1:] - starts[:-1]
         ws = torch.zeros((max(max(workspace_size(L, N, self.k) for L in self.layers), 256),), dtype=torch.uint8, device=x.device)
         for L, r, a in zip(self.layers, self.routers, self.attention):

@@ -125,6 +125,28 @@ def test_prompt_in_chunks_attends_to_what_is_cached(gpu, parts):
         assert torch.equal(got == 0, want == 0)
 
 
+def test_padded_prompt(gpu, parts):
+    """Rows in front of the first and behind the last sequence reach no cache; the sequences' own rows are those of the call without."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    a, b = _stack(gpu, parts, 3), _stack(gpu, parts, 3)
+    x = _x(gen, 40)
+    for s in (a, b):  # what the padding must not touch
+        s.prompt(_x(torch.Generator(device="cuda").manual_seed(5), 30), _ints([0, 20, 30]), _ints([0, 2]))
+    want = a.prompt(x, _ints([4, 20, 20, 33]), _ints([0, 1, 2]))
+    first = a.positions.clone()
+    got = b.prompt(x[4:33], _ints([0, 16, 16, 29]), _ints([0, 1, 2]))
+    assert a.positions.tolist() == [36, 0, 23] == b.positions.tolist() and torch.equal(first, a.positions)
+    assert bool(torch.isfinite(want).all())
+    for p, q in zip(a.attention, b.attention):
+        assert torch.equal(p.k_cache == 0, q.k_cache == 0) and torch.equal(p.v_cache == 0, q.v_cache == 0)
+    # The first layer's keys are the same, but for the projections' sums in another order.
+    k, l = a.attention[0].k_cache.float(), b.attention[0].k_cache.float()
+    assert float((k - l).abs().max()) <= 2.0 ** -7 * float(l.abs().max())
+    assert want.shape == x.shape and got.shape == (29, D_MODEL)
+
+
 def test_refusals(gpu, parts):
     import torch
 
@@ -140,6 +162,9 @@ def test_refusals(gpu, parts):
         gpu.DecodeStack(layers, routers, 2).prompt(torch.zeros((1, D_MODEL), device="cuda"), _ints([0, 1]), _ints([0]))
     with pytest.raises(ValueError):
         gpu.Attention(ws[0][0], ws[0][1], 3, 2, PAGES, PAGE)
+    with pytest.raises(ValueError):
+        gpu.Attention(torch.zeros((64, 3 * 20), dtype=torch.bfloat16, device="cuda"),
+                      torch.zeros((20, 64), dtype=torch.bfloat16, device="cuda"), 1, 1, PAGES, PAGE)  # heads of 20
     with pytest.raises(TypeError):
         gpu.Attention(ws[0][0].float(), ws[0][1].float(), HQ, HKV, PAGES, PAGE)
     s = _stack(gpu, parts, 2)
