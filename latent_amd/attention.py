@@ -23,50 +23,25 @@ for the product with the values, outputs once.  There is no backward pass.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
-import struct
-from typing import Optional, Tuple
+from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import LatentAttnDecodeArgs, LatentAttnPromptArgs, LatentKvAppendArgs, check, lib
+from ._lib import LatentAttnDecodeArgs, LatentAttnPromptArgs, LatentError, LatentKvCache, check, lib
 
-try:  # the current stream's handle without a Stream object: 0.1 instead of 1.9 us of a call
-    from torch._C import _cuda_getCurrentRawStream as _stream
-except ImportError:
-    def _stream(device: int) -> int:
-        return torch.cuda.current_stream(device).cuda_stream
+try:
+    from . import _attend
+except ImportError as e:
+    raise ImportError(
+        "latent_amd/_attend.so is missing or does not fit this torch: build it with `python latent_amd/build.py`"
+    ) from e
 
-_DTYPE = {torch.float16: _lib.LATENT_F16, torch.bfloat16: _lib.LATENT_BF16}
+_attend.entries(*(ctypes.cast(lib[f"latent_{n}"], ctypes.c_void_p).value for n in (
+    "kv_append", "attn_decode_workspace_size", "attn_decode", "attn_prompt_workspace_size", "attn_prompt")), LatentError)
 
-
-def _packer(args):
-    """The argument struct of ctypes class `args` from its values in field order, as bytes (0.3 us; a nested ctypes
-    structure takes 1.5)."""
-    codes = {ctypes.c_void_p: "q", ctypes.c_int64: "q", ctypes.c_size_t: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
-
-    def fields(c):
-        return "".join(fields(t) if issubclass(t, ctypes.Structure) else codes[t] for _, t in c._fields_)
-
-    s = struct.Struct("@" + fields(args) + "0q")
-    assert s.size == ctypes.sizeof(args)
-    return s.pack
-
-
-def _entry(name: str):
-    """The library's function on packed arguments."""
-    f = lib[name]
-    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
-    return f
-
-
-_append_args, _append = _packer(LatentKvAppendArgs), _entry("latent_kv_append")
-_decode_args, _decode = _packer(LatentAttnDecodeArgs), _entry("latent_attn_decode")
-_decode_size = _entry("latent_attn_decode_workspace_size")
-_prompt_args, _prompt_call = _packer(LatentAttnPromptArgs), _entry("latent_attn_prompt")
-_prompt_size = _entry("latent_attn_prompt_workspace_size")
+_DTYPE = (torch.float16, torch.bfloat16)
 
 
 def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -77,118 +52,6 @@ def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cu
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
     angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * base ** (-i / rot_dim)
     return torch.stack((angle.cos(), angle.sin()), 1).float().contiguous()
-
-
-def _no_grad():
-    raise RuntimeError("attention here has no backward pass: call it under torch.no_grad()")
-
-
-def _heads(t: torch.Tensor, name: str, dt: torch.dtype, dev: int):
-    """[T, heads, D] as the kernels read it (a copy where strides or base do not fit), its base, strides and shape."""
-    shape = t.shape
-    if len(shape) != 3:
-        raise ValueError(f"{name} must be [tokens, heads, D]")
-    if t.dtype is not dt:
-        raise TypeError(f"{name} must be {dt}, as the queries and the cache are")
-    if t.get_device() != dev:
-        raise ValueError(f"{name} must be on cuda:{dev}")
-    if t.requires_grad and torch.is_grad_enabled():
-        _no_grad()
-    st, sh, sd = t.stride()
-    p = t.data_ptr()
-    if (sd != 1 and shape[2] > 1) or (st | sh) & 7 or p & 15 or st >= _FAR:
-        t = t.clone(memory_format=torch.contiguous_format)
-        st, sh, sd = t.stride()
-        p = t.data_ptr()
-    return t, p, st, sh, shape
-
-
-# Tokens further apart than this (elements) are copied together: the kernels step over a tile of them in 32 bits.
-_FAR = 1 << 22
-
-
-def _ints(t: torch.Tensor, name: str, n: int, dev: int) -> torch.Tensor:
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != dev:
-        raise ValueError(f"{name} must be int32 [{n}] on cuda:{dev}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _out(t: Optional[torch.Tensor], like: torch.Tensor, name: str):
-    """The output, its base and strides."""
-    if t is None:
-        t = torch.empty_like(like, memory_format=torch.contiguous_format)
-        return t, t.data_ptr(), *t.stride()[:2]
-    if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device():
-        raise ValueError(f"{name} must be {like.dtype} {list(like.shape)} on {like.device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        _no_grad()
-    st, sh, sd = t.stride()
-    if (sd != 1 and t.shape[2] > 1) or (st | sh) & 7 or t.data_ptr() & 15:
-        raise ValueError(f"{name} must have adjacent D, strides that are multiples of 8 and a 16-byte aligned base")
-    return t, t.data_ptr(), st, sh
-
-
-def _lse(t: Optional[torch.Tensor], T: int, Hq: int, dev: int) -> int:
-    if t is None:
-        return 0
-    if t.dtype is not torch.float32 or tuple(t.shape) != (T, Hq) or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"lse must be contiguous f32 {[T, Hq]} on cuda:{dev}")
-    return t.data_ptr()
-
-
-def _cache(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, dev: int):
-    """The fields of a LatentKvCache, and the cache's shape and type."""
-    shape, dt = k.shape, k.dtype
-    if len(shape) != 4 or v.shape != shape:
-        raise ValueError("k_cache and v_cache must be [pages, page rows, kv heads, D], of one shape")
-    if dt not in _DTYPE or v.dtype is not dt:
-        raise TypeError("the cache must be f16 or bf16, keys and values alike")
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        _no_grad()
-    if k.get_device() != dev or v.get_device() != dev or pages.get_device() != dev:
-        raise ValueError(f"the cache and its page table must be on cuda:{dev}")
-    B_most = pages.shape
-    if pages.dtype is not torch.int32 or len(B_most) != 2:
-        raise ValueError("pages must be int32 [sequences, max_pages]")
-    B, most = B_most
-    ps, one = pages.stride()
-    n, page, heads, D = shape
-    k0, k1, k2, k3 = k.stride()
-    v0, v1, v2, v3 = v.stride()
-    if ((k3 != 1 or v3 != 1) and D > 1) or (one != 1 and most > 1):
-        raise ValueError("the last dimensions of k_cache, v_cache and pages must be adjacent")
-    # A size of one makes its stride meaningless to torch, and so to the library.
-    if B < 2 or n < 2 or page < 2 or heads < 2:
-        ps = ps if B > 1 else most
-        k0, v0 = (k0, v0) if n > 1 else (0, 0)
-        k1, v1 = (k1, v1) if page > 1 else (0, 0)
-        k2, v2 = (k2, v2) if heads > 1 else (0, 0)
-    return (k.data_ptr(), v.data_ptr(), pages.data_ptr(), n, page, B, most, ps, k0, k1, k2, v0, v1, v2), shape, dt
-
-
-def _first(t: torch.Tensor, name: str) -> int:
-    """The device of a call's first tensor."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype not in _DTYPE:
-        raise TypeError(f"{name} must be f16 or bf16")
-    return t.get_device()
-
-
-def _here(t: torch.Tensor, stream: Optional[torch.cuda.Stream]):
-    """The context a call has to enter first: its stream's or its tensors' device's; None when both are current."""
-    if stream is not None:
-        return torch.cuda.stream(stream)
-    if t.is_cuda and t.get_device() != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return None
-
-
-def _scale(scale: Optional[float], D: int) -> float:
-    s = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < s < math.inf:
-        raise ValueError("scale must be positive and finite")
-    return s
 
 
 def kv_append(
@@ -216,52 +79,10 @@ def kv_append(
     Tokens of one call must not name the same cache row twice: what it holds
     then is unspecified.
     """
-    ctx = _here(k, stream)
-    if ctx is not None:
-        with ctx:
-            return kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
-    dev = _first(k, "k")
-    dt = k.dtype
-    cache, (_, _, cHkv, cD), cdt = _cache(k_cache, v_cache, pages, dev)
-    k, kp, kt, kh, kshape = _heads(k, "k", dt, dev)
-    v, vp, vt, vh, vshape = _heads(v, "v", dt, dev)
-    T, Hkv, D = kshape
-    if cdt is not dt or cHkv != Hkv or cD != D or vshape != kshape:
-        raise ValueError(f"k {list(k.shape)}, v {list(v.shape)} and the cache {list(k_cache.shape)} {k_cache.dtype} do not fit")
-    sp = rows = rot = rp = 0
-    if seqs is not None:
-        seqs = _ints(seqs, "seqs", T, dev)
-        sp = seqs.data_ptr()
-    elif T > cache[5]:
-        raise ValueError("more tokens than sequences: give seqs")
-    positions = _ints(positions, "positions", T, dev)
-    if rope is not None:
-        if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[1] != 2 or rope.get_device() != dev:
-            raise ValueError(f"rope must be f32 [positions, 2, rot / 2] on cuda:{dev}")
-        rp = rope.data_ptr()
-        if not rope.is_contiguous() or rp & 15:
-            rope = rope.clone(memory_format=torch.contiguous_format)
-            rp = rope.data_ptr()
-        rows, _, rot = rope.shape
-        rot *= 2
-        if not 0 < rot <= D:
-            raise ValueError(f"rope turns {rot} dimensions of {D}")
-    qp = qt = qh = op = ot = oh = Hq = 0
-    if q is not None:
-        q, qp, qt, qh, (Tq, Hq, Dq) = _heads(q, "q", dt, dev)
-        if Tq != T or Dq != D:
-            raise ValueError(f"q {list(q.shape)} does not fit k {list(k.shape)}")
-        q_out, op, ot, oh = _out(q_out, q, "q_out")
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    if T == 0:
-        return q_out
-    a = _append_args(*cache, qp, op, kp, vp, qt, qh, ot, oh, kt, kh, vt, vh, positions.data_ptr(), sp, rp, rows, rot, T, Hq,
-                     Hkv, D, _DTYPE[dt], 1 if interleaved else 0)
-    st = _append(a, _stream(dev))
-    if st:
-        check(st, "latent_kv_append")
-    return q_out
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
+    return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
 
 
 def attend_decode(
@@ -284,90 +105,31 @@ def attend_decode(
     of several caches needs it.  A workspace that is given
     (attend_decode_workspace_size bytes) must not serve calls that may overlap.
     """
-    ctx = _here(q, stream)
-    if ctx is not None:
-        with ctx:
-            return attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
-    dev = _first(q, "q")
-    cache, (_, _, Hkv, cD), dt = _cache(k_cache, v_cache, pages, dev)
-    q, qp, qt, qh, (B, Hq, D) = _heads(q, "q", dt, dev)
-    if B != cache[5] or D != cD or not Hkv or Hq % Hkv:
-        raise ValueError(f"q {list(q.shape)} does not fit the cache {list(k_cache.shape)} of {cache[5]} sequences")
-    lengths = _ints(lengths, "lengths", B, dev)
-    out, op, ot, oh = _out(out, q, "out")
-    lp = _lse(lse, B, Hq, dev)
-    if B == 0 or Hq == 0:
-        return out
-    a = (*cache, qp, op, lp, lengths.data_ptr(), qt, qh, ot, oh, Hq, Hkv, D, _DTYPE[dt], _scale(scale, D))
-    if workspace is None:
-        n = _decode_need(*cache[4:7], Hq, Hkv, D)
-        if n:
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous and on cuda:{dev}")
-    else:
-        n = workspace.numel() * workspace.element_size()
-    st = _decode(_decode_args(*a, workspace.data_ptr() if n else 0, n), _stream(dev))
-    if st:
-        check(st, "latent_attn_decode")
-    return out
-
-
-@functools.lru_cache(maxsize=256)
-def _decode_need(page_size: int, n_seq: int, max_pages: int, n_head: int, n_kv_head: int, head_dim: int) -> int:
-    cache = (0, 0, 0, 1, page_size, n_seq, max_pages, max_pages, 0, 0, 0, 0, 0, 0)
-    n = ctypes.c_size_t()
-    a = _decode_args(*cache, *(0,) * 8, n_head, n_kv_head, head_dim, _lib.LATENT_BF16, 1.0, 0, 0)
-    check(_decode_size(a, ctypes.addressof(n)), "latent_attn_decode_workspace_size")
-    return int(n.value)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
+    return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
 
 
 def attend_decode_workspace_size(n_seq: int, n_head: int, n_kv_head: int, head_dim: int, max_pages: int, page_size: int) -> int:
     """Workspace bytes of attend_decode for these sizes."""
-    return _decode_need(page_size, n_seq, max_pages, n_head, n_kv_head, head_dim)
-
-
-def _prompt(q, starts, cache, Hkv, keys, k_starts, lengths, n_keys, causal, scale, out, lse, workspace, dev) -> torch.Tensor:
-    """keys: base and strides of k and v, (k, v, k token, k head, v token, v head), zeros for the cache's."""
-    q, qp, qt, qh, (T, Hq, D) = q
-    B = cache[5]
-    if not Hkv or Hq % Hkv:
-        raise ValueError(f"{Hq} heads are no multiple of {Hkv} key and value heads")
-    starts = _ints(starts, "starts", B + 1, dev)
-    out, op, ot, oh = _out(out, q, "out")
-    lp = _lse(lse, T, Hq, dev)
-    if T == 0 or Hq == 0 or B == 0:
-        return out
-    if workspace is None:
-        need = _prompt_need(T, B, n_keys, cache[6] * cache[4], Hq, Hkv, D)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous and on cuda:{dev}")
-    else:
-        need = workspace.numel() * workspace.element_size()
-    a = _prompt_args(*cache, qp, op, lp, keys[0], keys[1], starts.data_ptr(), 0 if k_starts is None else k_starts.data_ptr(),
-                     0 if lengths is None else lengths.data_ptr(), qt, qh, ot, oh, *keys[2:], T, n_keys, Hq, Hkv, D,
-                     _DTYPE[q.dtype], 1 if causal else 0, _scale(scale, D), workspace.data_ptr() if need else 0, need)
-    st = _prompt_call(a, _stream(dev))
-    if st:
-        check(st, "latent_attn_prompt")
-    return out
-
-
-@functools.lru_cache(maxsize=1024)
-def _prompt_need(n_tokens: int, n_seq: int, n_keys: int, cached: int, n_head: int, n_kv_head: int, head_dim: int) -> int:
-    cache = (0, 0, 0, 1, 1, n_seq, cached, cached, 0, 0, 0, 0, 0, 0)
+    cache = LatentKvCache(n_pages=1, page_size=page_size, n_seq=n_seq, max_pages=max_pages, pages_stride=max_pages)
+    a = LatentAttnDecodeArgs(cache=cache, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, dtype=_lib.LATENT_BF16, scale=1.0)
     n = ctypes.c_size_t()
-    a = _prompt_args(*cache, *(0,) * 16, n_tokens, n_keys, n_head, n_kv_head, head_dim, _lib.LATENT_BF16, 1, 1.0, 0, 0)
-    check(_prompt_size(a, ctypes.addressof(n)), "latent_attn_prompt_workspace_size")
+    check(lib.latent_attn_decode_workspace_size(ctypes.byref(a), ctypes.byref(n)), "latent_attn_decode_workspace_size")
     return int(n.value)
 
 
 def attend_prompt_workspace_size(n_tokens: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_keys: int = 0,
                                  max_pages: int = 0, page_size: int = 1) -> int:
     """Workspace bytes of attend_prompt (n_keys rows of keys) or attend_prompt_paged for these sizes; 0: it takes none."""
-    return _prompt_need(n_tokens, n_seq, n_keys, 0 if n_keys else max_pages * page_size, n_head, n_kv_head, head_dim)
+    cache = LatentKvCache(n_pages=1, page_size=page_size, n_seq=n_seq, max_pages=0 if n_keys else max_pages,
+                          pages_stride=max_pages)
+    a = LatentAttnPromptArgs(cache=cache, n_tokens=n_tokens, n_keys=n_keys, n_head=n_head, n_kv_head=n_kv_head,
+                             head_dim=head_dim, dtype=_lib.LATENT_BF16, causal=1, scale=1.0)
+    n = ctypes.c_size_t()
+    check(lib.latent_attn_prompt_workspace_size(ctypes.byref(a), ctypes.byref(n)), "latent_attn_prompt_workspace_size")
+    return int(n.value)
 
 
 def attend_prompt(
@@ -392,29 +154,10 @@ def attend_prompt(
     A workspace that is given (attend_prompt_workspace_size bytes, fewer: the
     call does without) must not serve calls that may overlap.
     """
-    ctx = _here(q, stream)
-    if ctx is not None:
-        with ctx:
-            return attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
-    dev = _first(q, "q")
-    dt = q.dtype
-    q = _heads(q, "q", dt, dev)
-    k, kp, kt, kh, (Tk, Hkv, D) = _heads(k, "k", dt, dev)
-    v, vp, vt, vh, vshape = _heads(v, "v", dt, dev)
-    if vshape != k.shape or D != q[4][2]:
-        raise ValueError(f"q {list(q[4])}, k {list(k.shape)} and v {list(vshape)} do not fit")
-    if starts.dim() != 1 or starts.shape[0] == 0:
-        raise ValueError("starts must be int32 [sequences + 1]")
-    B = starts.shape[0] - 1
-    if k_starts is None:
-        if Tk != q[4][0]:
-            raise ValueError("k has other rows than q: give k_starts")
-        k_starts = starts
-    k_starts = _ints(k_starts, "k_starts", B + 1, dev)
-    if Tk == 0:  # a tensor without rows has no base
-        kp = vp = q[1]
-    cache = (0, 0, 0, 0, 1, B, 0, 0, 0, 0, 0, 0, 0, 0)
-    return _prompt(q, starts, cache, Hkv, (kp, vp, kt, kh, vt, vh), k_starts, None, Tk, causal, scale, out, lse, workspace, dev)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _attend.attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
+    return _attend.attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
 
 
 def attend_prompt_paged(
@@ -433,17 +176,10 @@ def attend_prompt_paged(
 ) -> torch.Tensor:
     """attend_prompt with the keys and values of sequence b in the cache: its first lengths[b] (int32 [B])
     positions, the new tokens' own (appended before the call) the last of them."""
-    ctx = _here(q, stream)
-    if ctx is not None:
-        with ctx:
-            return attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
-    dev = _first(q, "q")
-    cache, (_, _, Hkv, cD), dt = _cache(k_cache, v_cache, pages, dev)
-    q = _heads(q, "q", dt, dev)
-    if q[4][2] != cD:
-        raise ValueError(f"q {list(q[4])} does not fit the cache {list(k_cache.shape)}")
-    lengths = _ints(lengths, "lengths", cache[5], dev)
-    return _prompt(q, starts, cache, Hkv, (0,) * 6, None, lengths, 0, causal, scale, out, lse, workspace, dev)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
+    return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
 
 
 class Attention:

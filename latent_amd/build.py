@@ -1,4 +1,4 @@
-"""Build liblatent_hip.so (gfx950) in-tree with hipcc.
+"""Build liblatent_hip.so (gfx950) and the attention calls' binding, _attend.so, in-tree.
 
     python latent_amd/build.py
 
@@ -7,15 +7,19 @@
 The library links only against the HIP runtime; no torch headers.  When the
 Python binding loads it after `import torch`, the dynamic linker binds it to
 the HIP runtime torch already loaded (same SONAME), so torch's streams and
-device pointers are valid in it.
+device pointers are valid in it.  _attend.so (bind_attend.cpp, host code) is a
+Python extension over torch's C++ interface, for the calls of a decode step whose
+arguments take longer to look at from Python than the GPU needs for them.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +28,7 @@ CSRC = PKG / "csrc"
 SOURCES = ["chain32.hip", "codec.hip", "decode.hip", "expert.hip", "kvcache.hip", "moe.hip", "noalloc.hip", "prefill.hip",
            "prompt.hip", "route.hip", "rows.hip", "stream.hip"]
 LIB = PKG / "liblatent_hip.so"
+BINDING = PKG / "_attend.so"
 ARCH = os.environ.get("LATENT_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -45,8 +50,17 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (set HIPCC)")
 
 
+def binding_command(out: Path) -> list:
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    rocm = Path(hipcc()).resolve().parent.parent / "include"
+    include = [torch / "include", rocm, sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            *[f"-I{i}" for i in include], str(CSRC / "bind_attend.cpp"), "-o", str(out), f"-L{torch / 'lib'}",
+            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile every source and link the shared library; always rebuilds."""
+    """Compile every source and link the shared library and the binding; always rebuilds."""
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
     cc = hipcc()
@@ -55,6 +69,8 @@ def build(verbose: bool = False) -> Path:
         obj = objdir / (Path(src).stem + ".o")
         cmds.append([cc, *HIPCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(str(obj))
+    tmp_binding = BINDING.with_suffix(".so.tmp")
+    cmds.append(binding_command(tmp_binding))
     # One compiler process per source, at most `jobs` at a time.
     jobs = max(1, min(len(cmds), int(os.environ.get("MAX_JOBS", os.cpu_count() or 1))))
     with ThreadPoolExecutor(max_workers=jobs) as pool:
@@ -71,6 +87,7 @@ def build(verbose: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+    os.replace(tmp_binding, BINDING)
     return LIB
 
 

@@ -138,26 +138,6 @@ def test_decode_workspace_grows_to_a_bound(L):
         latent_amd.attend_decode_workspace_size(1, 3, 2, 128, 40, 16)
 
 
-def test_packed_arguments_are_the_structures(L):
-    """The binding packs arguments itself: the bytes of the structure with the same values."""
-    from latent_amd import attention as A
-
-    for cls, pack in ((L.LatentKvAppendArgs, A._append_args), (L.LatentAttnDecodeArgs, A._decode_args),
-                      (L.LatentAttnPromptArgs, A._prompt_args)):
-        s, values = cls(), []
-
-        def fill(obj, values=values):
-            for name, t in obj._fields_:
-                if issubclass(t, ctypes.Structure):
-                    fill(getattr(obj, name))
-                else:
-                    values.append(len(values) + 1)
-                    setattr(obj, name, values[-1])
-
-        fill(s)
-        assert pack(*values) == bytes(s)
-
-
 # ---- the Python calls -----------------------------------------------------------
 def _t(*shape, dt=torch.bfloat16):
     return torch.zeros(shape, dtype=dt)
@@ -179,6 +159,13 @@ def _calls():
 def test_cpu_tensors_are_refused(name):
     with pytest.raises(ValueError, match="CUDA"):
         _calls()[name](_t(3, 2, 64))
+
+
+@pytest.mark.parametrize("name", ["kv_append", "attend_decode", "attend_prompt", "attend_prompt_paged"])
+def test_what_is_no_tensor_is_refused(name):
+    for bad in (None, 3, np.zeros((3, 2, 64), np.float16)):
+        with pytest.raises(TypeError, match="must be a tensor"):
+            _calls()[name](bad)
 
 
 def test_rope_table_on_the_cpu():

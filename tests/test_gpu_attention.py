@@ -625,6 +625,103 @@ def test_operands_that_want_gradients_are_refused(gpu):
                 call(*args)
 
 
+def _refusal_operands():
+    import torch
+
+    dt = torch.bfloat16
+    t = lambda *shape, dt=dt: torch.zeros(shape, dtype=dt, device="cuda")
+    return dict(q=t(3, 4, 64), k=t(3, 2, 64), v=t(3, 2, 64), kc=t(4, 8, 2, 64), vc=t(4, 8, 2, 64), pages=t(3, 2, dt=torch.int32),
+                ints=t(3, dt=torch.int32), starts=t(4, dt=torch.int32))
+
+
+REFUSED = [  # which operand, what it becomes
+    ("q", lambda t, o: t[0], ValueError), ("q", lambda t, o: t.half(), TypeError), ("q", lambda t, o: t.float(), TypeError),
+    ("q", lambda t, o: t[..., :56], ValueError), ("q", lambda t, o: t.cpu(), ValueError),
+    ("kc", lambda t, o: t[0], ValueError), ("kc", lambda t, o: t.half(), TypeError), ("kc", lambda t, o: t[:2], ValueError),
+    ("vc", lambda t, o: t.half(), TypeError), ("vc", lambda t, o: t.cpu(), ValueError),
+    ("vc", lambda t, o: t.transpose(2, 3).contiguous().transpose(2, 3), ValueError),
+    ("kc", lambda t, o: t.expand(4, 8, 2, 64)[..., ::2], ValueError),
+    ("pages", lambda t, o: t.long(), ValueError), ("pages", lambda t, o: t[0], ValueError), ("pages", lambda t, o: t.cpu(), ValueError),
+    ("pages", lambda t, o: t.T.contiguous().T, ValueError),
+    ("ints", lambda t, o: t.long(), ValueError), ("ints", lambda t, o: t[:2], ValueError), ("ints", lambda t, o: t.cpu(), ValueError),
+]
+
+
+@pytest.mark.parametrize("at", range(len(REFUSED)))
+def test_operands_that_do_not_fit_are_refused(gpu, at):
+    which, change, error = REFUSED[at]
+    calls = (lambda q, k, v, kc, vc, pages, ints, starts: gpu.kv_append(k, v, kc, vc, pages, ints, q=q),
+             lambda q, k, v, kc, vc, pages, ints, starts: gpu.attend_decode(q, kc, vc, pages, ints),
+             lambda q, k, v, kc, vc, pages, ints, starts: gpu.attend_prompt_paged(q, kc, vc, pages, ints, starts))
+    for call in calls:
+        o = _refusal_operands()
+        call(**o)
+        o[which] = change(o[which], o)
+        with pytest.raises(error):
+            call(**o)
+
+
+def test_options_that_do_not_fit_are_refused(gpu):
+    import torch
+
+    o = _refusal_operands()
+    q, k, v, kc, vc, pages, ints, starts = o.values()
+    decode = lambda **kw: gpu.attend_decode(q, kc, vc, pages, ints, **kw)
+    prompt = lambda **kw: gpu.attend_prompt(q, k, v, starts, **kw)
+    paged_ = lambda **kw: gpu.attend_prompt_paged(q, kc, vc, pages, ints, starts, **kw)
+    for call in (decode, prompt, paged_):
+        for scale in (0.0, -1.0, math.inf, math.nan):
+            with pytest.raises(ValueError, match="scale"):
+                call(scale=scale)
+        with pytest.raises(TypeError):
+            call(scale="x")
+        for out in (q[:2], q.half(), q.cpu(), torch.zeros((3, 4, 128), dtype=q.dtype, device="cuda")[..., ::2],
+                    torch.zeros(3 * 4 * 64 + 1, dtype=q.dtype, device="cuda")[1:].view(3, 4, 64)):
+            with pytest.raises(ValueError, match="out"):
+                call(out=out)
+        with pytest.raises(TypeError, match="out"):
+            call(out=3)
+        with pytest.raises(gpu.LatentError):
+            call(out=torch.zeros((3, 1, 64), dtype=q.dtype, device="cuda").expand(3, 4, 64))  # heads of one place
+        for lse in (torch.zeros((3, 3), device="cuda"), torch.zeros((3, 4)), torch.zeros((4, 3), device="cuda").T,
+                    torch.zeros((3, 4), dtype=torch.float64, device="cuda")):
+            with pytest.raises(ValueError, match="lse"):
+                call(lse=lse)
+        with pytest.raises(ValueError, match="workspace"):
+            call(workspace=torch.zeros(64, dtype=torch.uint8))
+        with pytest.raises(gpu.LatentError):
+            call(workspace=None, scale=1.0, out=torch.zeros((3, 4, 64 + 8), dtype=q.dtype, device="cuda")[..., :64][:, :1].expand(3, 4, 64))
+    for bad in (starts[:0], starts.view(2, 2), starts.long(), starts.cpu(), torch.zeros(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            gpu.attend_prompt_paged(q, kc, vc, pages, ints, bad)
+    for bad in (starts[:0], starts.view(2, 2), starts.long(), starts.cpu()):
+        with pytest.raises(ValueError):
+            gpu.attend_prompt(q, k, v, bad)
+    with pytest.raises(ValueError, match="k_starts"):
+        gpu.attend_prompt(q, k[:2], v[:2], starts)
+    with pytest.raises(ValueError, match="k_starts"):
+        gpu.attend_prompt(q, k[:2], v[:2], starts, k_starts=starts[:3])
+    with pytest.raises(ValueError):
+        gpu.attend_prompt(q[:, :3], k, v, starts)  # 3 heads over 2
+    with pytest.raises(ValueError):
+        gpu.attend_prompt(q, k, v[:2], starts)
+    append = lambda **kw: gpu.kv_append(k, v, kc, vc, pages, ints, **kw)
+    for rope in (torch.zeros((4, 2, 33), device="cuda"), torch.zeros((4, 2, 0), device="cuda"), torch.zeros((4, 32), device="cuda"),
+                 torch.zeros((4, 2, 32)), torch.zeros((4, 2, 32), device="cuda").half()):
+        with pytest.raises(ValueError, match="rope"):
+            append(rope=rope)
+    with pytest.raises(ValueError, match="q_out"):
+        append(q_out=q)
+    with pytest.raises(ValueError, match="seqs"):
+        append(seqs=ints[:2])
+    with pytest.raises(ValueError, match="seqs"):
+        gpu.kv_append(k, v, kc, vc, pages[:2], ints)
+    with pytest.raises(gpu.LatentError):  # pages of one place
+        gpu.kv_append(k, v, kc[:1].expand(4, 8, 2, 64), vc, pages, ints)
+    with pytest.raises(gpu.LatentError):  # heads of 20
+        gpu.attend_prompt(q[..., :20].contiguous(), k[..., :20].contiguous(), v[..., :20].contiguous(), starts)
+
+
 # ---- a run of them together -----------------------------------------------------
 def test_prompt_then_tokens_equal_one_prompt(gpu):
     """Prompts appended in chunks and continued token by token see what one packed causal pass sees."""
