@@ -288,7 +288,8 @@ template <typename E, int kDP, bool kExact, int kMT, bool kPage8, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(DecodeParams p) {
   constexpr int kVec = kDP / 16, kK = kDP / 32, kPad = kDP + 4;
   __shared__ float ml[kWaves][kMT * 16][2];
-  __shared__ float rows[kWaves][16][kPad];
+  constexpr int kRound = kDP <= 128 ? kMT : 1;  // row blocks that the waves exchange at once
+  __shared__ float rows[kWaves][kRound * 16][kPad];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int n16 = lane & 15, kq = lane >> 4;
 
@@ -370,19 +371,23 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
     }
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt) {
-      float top = -INFINITY;
+    for (int mt0 = 0; mt0 < kMT; mt0 += kRound) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[w][mt * 16 + n16][0]);
-      const float f = exp2_fast(r.m[mt] - finite_max(top));
+      for (int mm = 0; mm < kRound; ++mm) {
+        const int mt = mt0 + mm;
+        float top = -INFINITY;
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr)
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[w][mt * 16 + n16][0]);
+        const float f = exp2_fast(r.m[mt] - finite_max(top));
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) rows[wave][n16][4 * kVec * kq + kVec * rr + i] = r.acc[mt][i][rr] * f;
+        for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) rows[wave][mm * 16 + n16][4 * kVec * kq + kVec * rr + i] = r.acc[mt][i][rr] * f;
+      }
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < 16 * (p.D / 8); i += kThreads) {
-        const uint32_t row = mt * 16 + i / (p.D / 8), c = i % (p.D / 8);
-        if (row >= nr) continue;
+      const uint32_t live = min(kRound * 16, max(0, static_cast<int>(nr) - mt0 * 16));
+      for (uint32_t i = threadIdx.x; i < live * (p.D / 8); i += kThreads) {
+        const uint32_t row = mt0 * 16 + i / (p.D / 8), c = i % (p.D / 8);
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[w][row][0]);
@@ -391,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) decode_kernel(De
         f32x4 x[2] = {};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          x[0] += *reinterpret_cast<const f32x4*>(&rows[w][row & 15][8 * c]);
-          x[1] += *reinterpret_cast<const f32x4*>(&rows[w][row & 15][8 * c + 4]);
+          x[0] += *reinterpret_cast<const f32x4*>(&rows[w][row - mt0 * 16][8 * c]);
+          x[1] += *reinterpret_cast<const f32x4*>(&rows[w][row - mt0 * 16][8 * c + 4]);
         }
         if (whole) {
           const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
