@@ -14,6 +14,14 @@
 // so maximum and sum are per-lane loops and one exchange between lane halves, and
 // eight consecutive registers, rounded, are the operand of out^T = V^T P^T as
 // they stand; the value operand is read transposed from LDS in that key order.
+//
+// Measured (bf16, heads of 128): 8192 tokens of 64 heads over 8 in 1030 us, 1070
+// TFLOP/s; 14 prompts of 162 to 2000 tokens, 32 heads, 186 us.  The long ones are
+// bound by the power the products draw: the same instructions over zeros take
+// 832 us (the card's 8192^3 matrix product: 1360 TFLOP/s, 1800 over zeros), and
+// neither waits nor the order of products and exponentials shows in the time
+// (scores a tile ahead with a few exponentials behind every product: 1049 us;
+// three and four LDS buffers: the same; no wait for the loads at all: the same).
 #include "attend.hpp"
 
 #include <algorithm>
@@ -279,25 +287,46 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
         return;
       }
     }
+    if constexpr (kPaged) {
+      // Lane l finds where row l lies, once for the tile; whoever loads a piece of the row asks it (four chunks of up to 517
+      // tokens: 28.7 us with every load's address worked out by itself, 27.4 so).
+      const uint32_t key = kt + opaque(lane), off = key - p.cache.by_page.of(key) * p.cache.page_size;
+      const bool there = page_in_lane < p.cache.n_pages;
+      const int64_t ko = there ? page_in_lane * p.cache.k_page + off * p.cache.k_row : 0;
+      const int64_t vo = same_strides ? ko : there ? page_in_lane * p.cache.v_page + off * p.cache.v_row : 0;
+      auto row = [](int64_t o, int of) {
+        const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * of, static_cast<int>(o)), hi = __builtin_amdgcn_ds_bpermute(4 * of, static_cast<int>(o >> 32));
+        return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+      };
+      const uint64_t have = __ballot(there) | ~(~uint64_t{0} >> (64 - kKeys));
+      const bool all = have == ~uint64_t{0} && exact;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row_in = lrow + i * kRowsLoad, ck = lpos ^ S::k_turn(row_in), cv = lpos ^ S::v_turn(row_in);
+        const int64_t kr = row(ko, row_in), vr = same_strides ? kr : row(vo, row_in);
+        const char *from_k = kbase + kr + 16 * ck, *from_v = vbase + vr + 16 * cv;
+        if (!all) {
+          asm volatile("");
+          const bool ok = have >> row_in & 1;
+          const char* zero = reinterpret_cast<const char*>(kZeroRow);
+          from_k = ok && 8 * ck < p.D ? from_k : zero;
+          from_v = ok && 8 * cv < p.D ? from_v : zero;
+        }
+        dma16(from_k, to_k + i * (kWave * 16));
+        dma16(from_v, to_v + i * (kWave * 16));
+        __builtin_amdgcn_sched_barrier(0);  // all loads' addresses at once would not fit the registers
+      }
+      return;
+    }
     const int ln = opaque(lane), lrow = kKeys / kWaves * wave + ln / kC, lpos = ln % kC;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row_in = lrow + i * kRowsLoad, key = kt + row_in, ck = lpos ^ S::k_turn(row_in), cv = lpos ^ S::v_turn(row_in);
-      bool ok = key < end;
-      int64_t ko, vo;
-      if constexpr (kPaged) {
-        const uint32_t page = __shfl(page_in_lane, row_in), off = static_cast<uint32_t>(key) - p.cache.by_page.of(key) * p.cache.page_size;
-        ok = page < p.cache.n_pages;
-        ko = page * p.cache.k_page + off * p.cache.k_row;
-        vo = same_strides ? ko : page * p.cache.v_page + off * p.cache.v_row;
-      } else {
-        ko = key * p.cache.k_row;
-        vo = key * p.cache.v_row;
-      }
+      const bool ok = key < end;
       const char* zero = reinterpret_cast<const char*>(kZeroRow);
-      dma16(ok && 8 * ck < p.D ? kbase + ko + 16 * ck : zero, to_k + i * (kWave * 16));
-      dma16(ok && 8 * cv < p.D ? vbase + vo + 16 * cv : zero, to_v + i * (kWave * 16));
-      __builtin_amdgcn_sched_barrier(0);  // all loads' addresses at once would not fit the registers
+      dma16(ok && 8 * ck < p.D ? kbase + key * p.cache.k_row + 16 * ck : zero, to_k + i * (kWave * 16));
+      dma16(ok && 8 * cv < p.D ? vbase + key * p.cache.v_row + 16 * cv : zero, to_v + i * (kWave * 16));
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
