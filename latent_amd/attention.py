@@ -44,6 +44,12 @@ _attend.entries(*(ctypes.cast(lib[f"latent_{n}"], ctypes.c_void_p).value for n i
 _DTYPE = (torch.float16, torch.bfloat16)
 
 
+def _on(stream: torch.cuda.Stream, t: torch.Tensor):
+    if t.device != stream.device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {t.device}")
+    return torch.cuda.stream(stream)
+
+
 def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
     """cos and sin of position p times base^(-2i / rot_dim), f32 [n_positions, 2, rot_dim / 2]
     (angles in 64 bits: in 32 a far position's angle is off by more than the table's rounding)."""
@@ -80,7 +86,7 @@ def kv_append(
     then is unspecified.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, k):
             return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
     return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
 
@@ -106,7 +112,7 @@ def attend_decode(
     (attend_decode_workspace_size bytes) must not serve calls that may overlap.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, q):
             return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
     return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
 
@@ -155,7 +161,7 @@ def attend_prompt(
     call does without) must not serve calls that may overlap.
     """
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, q):
             return _attend.attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
     return _attend.attend_prompt(q, k, v, starts, k_starts, causal, scale, out, lse, workspace)
 
@@ -177,7 +183,7 @@ def attend_prompt_paged(
     """attend_prompt with the keys and values of sequence b in the cache: its first lengths[b] (int32 [B])
     positions, the new tokens' own (appended before the call) the last of them."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, q):
             return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
     return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
 

@@ -10,7 +10,7 @@
 // written once.  A thread moves 2 x 16 bytes of a head (the two halves of eight
 // pairs, or 16 neighbours) and goes on to the next heads of its token with the
 // same 16 table values: read again for each head they would be twice the bytes
-// of the data itself.  Measured: 8190 tokens of 48 heads of 128 bf16 68 us (5.0 TB/s,
+// of the data itself.  Measured: 8190 tokens of 80 heads of 128 bf16 68 us (5.0 TB/s,
 // a copy's rate); one token 2.9 us of GPU, 5.1 a call.
 #include "attend.hpp"
 

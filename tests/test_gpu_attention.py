@@ -511,6 +511,18 @@ def test_calls_on_another_stream(gpu):
     assert torch.equal(got, want) and torch.equal(got_p, want_p)
 
 
+def test_stream_of_another_device_is_refused(gpu):
+    import torch
+
+    side = torch.cuda.Stream()
+    kc = torch.zeros((2, 4, 1, 8), dtype=torch.float16)
+    q, pages, one = torch.zeros((1, 1, 8), dtype=torch.float16), torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for call in (lambda: gpu.kv_append(q, q, kc, kc, pages, one, stream=side), lambda: gpu.attend_decode(q, kc, kc, pages, one, stream=side),
+                 lambda: gpu.attend_prompt(q, q, q, one, stream=side), lambda: gpu.attend_prompt_paged(q, kc, kc, pages, one, one, stream=side)):
+        with pytest.raises(ValueError, match="stream"):
+            call()
+
+
 def test_captured_step_replays(gpu):
     """Append, attend and count in one graph, replayed with the host's own work between; two graphs in turn."""
     import torch
