@@ -14,6 +14,8 @@ caches (the new token's own key and value among them):
 
 and h_l takes x_l's place above.  Row b of a step is the next token of the
 sequence in slot b, at positions[b]; a slot whose position is negative is idle.
+A slot whose pages (or whose rotation table) end before its position keeps what
+is cached and stores nothing more.
 `prompt` runs whole prompts, or chunks of them, through the same layers and
 leaves the slots ready to decode.
 
@@ -125,6 +127,9 @@ class DecodeStack:
             raise ValueError(f"expected x [N, {self.d}]")
         if starts.dtype != torch.int32 or slots.dtype != torch.int32 or starts.shape != (slots.numel() + 1,) or slots.dim() != 1:
             raise ValueError("starts must be int32 [B + 1] and slots int32 [B]")
+        dev = self.positions.device
+        if x.device != dev or starts.device != dev or slots.device != dev:
+            raise ValueError(f"x, starts and slots must be on {dev}")
         x = x.to(torch.float32)
         N = x.shape[0]
         if N == 0 or slots.numel() == 0:

@@ -246,6 +246,45 @@ def test_decode_cache_beyond_32_bit_offsets(gpu):
     assert_attention(out, None, q, k, v, visible(1, 300, True, "cuda"), D ** -0.5)
 
 
+def test_prompt_tokens_far_apart(gpu):
+    """Packed rows 2 MB apart (offsets beyond 2^32), and rows so far apart that they are copied."""
+    import torch
+
+    gen, dt, n, D = _gen(24), torch.float16, 2504, 64
+    room = torch.empty(n << 20, dtype=dt, device="cuda").view(n, 1 << 20)
+    q, k, v = (room[:, i * 128:(i + 1) * 128].view(n, 2, D) for i in range(3))
+    for t in (q, k, v):
+        t.copy_(_randn(gen, n, 2, D, dt=dt))
+    out = room[:, 512:640].view(n, 2, D)
+    assert gpu.attend_prompt(q, k, v, _ints([0, 7, n]), out=out) is out
+    for a, b in ((0, 7), (7, n)):
+        assert_attention(out[a:b], None, q[a:b], k[a:b], v[a:b], visible(b - a, b - a, True, "cuda"), D ** -0.5)
+    few = room.view(-1, 8 << 20)[:100, :384].view(100, 6, D)  # 16 MB apart
+    q, k, v = few[:, :2], few[:, 2:4], few[:, 4:]
+    got = gpu.attend_prompt(q, k, v, _ints([0, 100]))
+    assert_attention(got, None, q, k, v, visible(100, 100, True, "cuda"), D ** -0.5)
+
+
+def test_sequences_that_share_pages(gpu):
+    """Two sequences with one prefix, their last pages their own: each reads the shared pages as its own."""
+    import torch
+
+    gen, dt, D, page = _gen(25), torch.bfloat16, 128, 16
+    kc, vc, pages, seqs = paged(gen, [330, 50], page, 2, D, dt, width=21)
+    k0, v0 = seqs[0]
+    own = pages[1, :4].clone()
+    pages[1] = pages[0]
+    pages[1, 17:21] = own  # 272 shared rows, then the second's
+    lens = [330, 272 + 50]
+    seqs = [seqs[0], (torch.cat((k0[:272], seqs[1][0])), torch.cat((v0[:272], seqs[1][1])))]
+    q = _randn(gen, 2, 8, D, dt=dt)
+    _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+    q = _randn(gen, 70, 8, D, dt=dt)
+    out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints(lens), _ints([0, 30, 70]))
+    for b, (i, j) in enumerate(((0, 30), (30, 70))):
+        assert_attention(out[i:j], None, q[i:j], *seqs[b], visible(j - i, lens[b], True, "cuda"), D ** -0.5)
+
+
 def test_decode_strided_operands_and_given_buffers(gpu):
     import torch
 

@@ -170,3 +170,26 @@ def test_refusals(gpu, parts):
     s = _stack(gpu, parts, 2)
     with pytest.raises(ValueError):
         s.prompt(torch.zeros((2, D_MODEL), device="cuda"), _ints([0, 2]), _ints([0, 1]))
+    for change in (0, 1, 2):
+        args = [torch.zeros((2, D_MODEL), device="cuda"), _ints([0, 1, 2]), _ints([0, 1])]
+        args[change] = args[change].cpu()
+        with pytest.raises(ValueError, match="cuda"):
+            s.prompt(*args)
+
+
+def test_slots_without_room_store_nothing_more(gpu, parts):
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    s = _stack(gpu, parts, 2, max_pages=2)  # 32 positions a slot
+    s.prompt(_x(gen, 50), _ints([0, 30, 50]), _ints([0, 1]))
+    for i in range(4):
+        if i == 2:
+            before = [(a.k_cache.clone(), a.v_cache.clone()) for a in s.attention]
+        out = s.forward(_x(gen, 2)).clone()
+        assert bool(torch.isfinite(out).all())
+    assert s.positions.tolist() == [34, 24]
+    mine = s.pages[0].long()
+    for a, (k, v) in zip(s.attention, before):
+        assert torch.equal(a.k_cache[mine], k[mine]) and torch.equal(a.v_cache[mine], v[mine])
+        assert not torch.equal(a.k_cache[s.pages[1].long()], k[s.pages[1].long()])
