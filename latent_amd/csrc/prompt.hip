@@ -96,9 +96,10 @@ __device__ __forceinline__ int keys_seen(const PromptParams& p, int n, int m, in
 // that about kItems items have work; each item of a split unit leaves a part (reference, sums, unnormalised rows), and
 // join_kernel adds them up.  Items of one chunk follow one another: they read the same keys, at about the same time, on the
 // same XCD (equal spans of the line of all key tiles, each workgroup's keys its own, balanced as well and ran three
-// times longer: 14 prompts of up to 2000 tokens 375 us, 190 us a unit a workgroup).
+// times longer: 14 prompts of up to 2000 tokens 375 us, 190 us a unit a workgroup).  Against chunks of 512 those of 256 took
+// 29.0 us instead of 39.7 (two prompts of 699 tokens, 4 heads of 256), 18.0 of 20.9 (2000 tokens, 2 heads); of 128, 27.5 and 20.4.
 // Every wave finds its item by itself, from the sequences in its lanes; more than 64 sequences are taken as they come.
-constexpr int kChunk = 512, kItems = 512, kChunkStep = 64;
+constexpr int kChunk = 256, kItems = 512, kChunkStep = 64;
 // Sequence `lane`: its row tiles, keys, and the parts of its units.
 struct Line {
   int s0, n, k0, m;
@@ -578,10 +579,12 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   }
 }
 
-// Units may be split where keys are long, and where they are few: packed ones less than the CUs (256 units of 2048 keys 51 us
-// with the parts' second launch, 45 without); sequences in the cache, of which the page table only bounds the lengths, up to four times as many
-// (eight chunks of up to 600 tokens behind up to 4000: 84 us split, 121 not).
-constexpr int64_t kShortKeys = 1024, kFewPacked = 256, kFewPaged = 1024;
+// Units may be split where keys are long and units few.  Up to kShortKeys, where splitting saves little, the units have to leave
+// CUs idle (717 tokens behind cached ones, 184 units: 24.1 us split, 25.8 not; four chunks of up to 517, 448 units: 35.8 and
+// 27.4).  Beyond it too for packed ones (256 units of 2048 keys 51 us with the parts' second launch, 45 without); sequences in
+// the cache, of which the page table only bounds the lengths, up to four times as many (eight chunks of up to 600 tokens behind up
+// to 4000: 80 us split, 121 not).
+constexpr int64_t kFewKeys = 512, kShortKeys = 1024, kFew = 256, kFewPaged = 1024;
 struct Plan {
   int64_t units;  // at most
   bool split;
@@ -594,7 +597,8 @@ Plan plan_for(const latent_attn_prompt_args& a) {
   pl.units = std::max<int64_t>(0, (a.n_tokens * G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1) * a.n_kv_head;
   const bool packed = a.k || a.n_keys;
   const int64_t keys = packed ? a.n_keys : a.cache.max_pages * a.cache.page_size;
-  pl.split = keys > kShortKeys && keys <= (1 << 28) && pl.units < (packed ? kFewPacked : kFewPaged) && a.cache.n_seq <= kWave;
+  pl.split = keys > kFewKeys && keys <= (1 << 28) && pl.units < (packed || keys <= kShortKeys ? kFew : kFewPaged) &&
+             a.cache.n_seq <= kWave;
   if (!pl.split) return pl;
   const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
   pl.acc_bytes = size_t{2} * kItems * 4 * blocks * kThreads * sizeof(f32x4);
