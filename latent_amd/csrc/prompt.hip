@@ -104,6 +104,7 @@ constexpr int kChunk = 256, kItems = 512, kChunkStep = 64;
 struct Line {
   int s0, n, k0, m;
   int tiles, parts, chunk;
+  uint64_t order;  // longer sequences first, equal ones as they come
 };
 template <bool kPaged>
 __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
@@ -112,6 +113,7 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
     const int2 q = rows_of(p.starts, lane, p.T), k = keys_of<kPaged>(p, lane);
     l = {q.x, q.y, k.x, k.y, row_tiles(p, q.y)};
   }
+  l.order = static_cast<uint64_t>(l.m) << 6 | (kWave - 1 - lane);
   l.parts = 1;
   l.chunk = INT32_MAX;
   if (p.max_parts) {
@@ -126,11 +128,11 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
   return l;
 }
 // Items of the sequences in front of this lane's (longer ones first).
-__device__ __forceinline__ int items_before(const PromptParams& p, const Line& l, int items, int lane) {
+__device__ __forceinline__ int items_before(const PromptParams& p, const Line& l, int items) {
   int before = 0;
   for (int j = 0; j < p.B; ++j) {
-    const int m = __builtin_amdgcn_readlane(l.m, j), n = __builtin_amdgcn_readlane(items, j);
-    if (m > l.m || (m == l.m && j < lane)) before += n;
+    const uint64_t other = static_cast<uint64_t>(__builtin_amdgcn_readlane(l.m, j)) << 6 | (kWave - 1 - j);
+    before += other > l.order ? __builtin_amdgcn_readlane(items, j) : 0;
   }
   return before;
 }
@@ -164,7 +166,7 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane
   }
   const Line l = line_of<kPaged>(p, lane);
   const int items = l.tiles * l.parts;
-  const int before = items_before(p, l, items, lane);
+  const int before = items_before(p, l, items);
   const uint64_t mine = __ballot(x >= before && x - before < items);
   if (!mine) return {-1};
   const int b = __builtin_ctzll(mine), r = x - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
@@ -486,6 +488,8 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
 
   sum = op_over(sum, 32, 64, OpAdd{});
   if constexpr (kLse) full = op_over(full, 32, 64, OpAdd{});
+  const int row = w0 + (opaque(lane) & 31);
+  if (row >= all) return;
   if (!whole_unit) {
     const int part = blockIdx.x;  // items in their order, heads within
     if (part >= p.max_parts) return;  // never, by the choice of chunk
@@ -498,8 +502,6 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     p.part_ml[static_cast<int64_t>(part) * kThreads + tid] = f32x4{top, sum, full, 0.f};
     return;
   }
-  const int row = w0 + (opaque(lane) & 31);
-  if (row >= all) return;
   const int tok = p.by_group.of(row), head = hk * p.G + row - tok * p.G;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   char* dst = p.out + (it.s0 + tok) * p.o_token + head * p.o_head;
@@ -524,15 +526,22 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), h = lane >> 5, i = blockIdx.y, hk = blockIdx.x % p.Hkv;
   // The split units in the order of their items.
   const Line l = line_of<kPaged>(p, lane);
-  const int x0 = blockIdx.x / p.Hkv, units = l.parts > 1 ? l.tiles : 0, before = items_before(p, l, units, lane);
+  const int x0 = blockIdx.x / p.Hkv, units = l.parts > 1 ? l.tiles : 0;
+  int count = units;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) count += __shfl_xor(count, d);
+  if (x0 >= count) return;  // most of the grid, which has room for as many as there can be
+  const int before = items_before(p, l, units);
   const uint64_t mine = __ballot(x0 >= before && x0 - before < units);
   if (!mine) return;
   const int b = __builtin_ctzll(mine), r = x0 - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
-  const int first = __builtin_amdgcn_readlane(items_before(p, l, l.tiles * l.parts, lane), b) + r, tile = t - 1 - r;
+  const int first = __builtin_amdgcn_readlane(items_before(p, l, l.tiles * l.parts), b) + r, tile = t - 1 - r;
   const int2 qs = rows_of(p.starts, b, p.T);
   const int n = qs.y, m = keys_of<kPaged>(p, b).y;
   const int parts = (keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1) + l.chunk - 1) / l.chunk;
   if (parts < 2) return;  // its rows see too little to be split
+  const int row = tile * kRowsTile + (tid >> 6) * kRowsWave + (lane & 31);
+  if (row >= n * p.G) return;
   const int at = first * p.Hkv + hk, step = t * p.Hkv;
   float top = -INFINITY, sum = 0.f, full = 0.f;
   f32x4 x[4] = {};
@@ -563,8 +572,6 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
       for (int rr = 0; rr < 4; ++rr) x[rr] += a[k][rr] * g;
     }
   }
-  const int row = tile * kRowsTile + (tid >> 6) * kRowsWave + (lane & 31);
-  if (row >= n * p.G) return;
   const int tok = p.by_group.of(row), head = hk * p.G + row - tok * p.G;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   char* dst = p.out + (qs.x + tok) * p.o_token + head * p.o_head;
