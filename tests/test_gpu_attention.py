@@ -451,6 +451,8 @@ def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
     ((2000, 10), 0, 2, 1, 96, 0, True),              # early rows see too little to be split
     ((1500,), 0, 4, 2, 128, 0, False),
     ((3, 700), 1500, 16, 1, 72, 7, True),
+    ((700,), 0, 8, 1, 128, 0, True),                 # fewer units than CUs
+    ((3, 20), 600, 4, 2, 64, 16, True),
 ])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_prompt_split_over_the_keys(gpu, new, ahead, Hq, Hkv, D, page, causal, dtype):
@@ -483,6 +485,13 @@ def test_prompt_many_sequences(gpu):
     new = [(7 * i) % 5 for i in range(150)]
     _prompt_check(gpu, _gen(9), new, new, 4, 2, 64, torch.float16, True)
     _prompt_check(gpu, _gen(20), new, [n + 13 * (i % 9) for i, n in enumerate(new)], 4, 2, 64, torch.float16, True, page=16, pad=2)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [(8, 2, 128, "bf16"), (3, 1, 64, "f16"), (4, 4, 256, "bf16")])
+def test_prompt_many_short_chunks_behind_cached_tokens(gpu, Hq, Hkv, D, dtype):
+    """Row tiles that are partly rows, some of their sequences split over the keys."""
+    new = [(5 * i) % 13 for i in range(40)]
+    _prompt_check(gpu, _gen(26), new, [n + (97 * i) % 1500 for i, n in enumerate(new)], Hq, Hkv, D, _dt(dtype), True, page=16, pad=2)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
