@@ -58,6 +58,8 @@ struct PromptParams {
   float scale_log2;
   // Splitting (see find_item): parts that the workspace holds, 0 for none.
   int32_t max_parts;
+  float items;      // that are to have work
+  int32_t least;    // keys of a sequence up to which it stays whole
   f32x4* part_acc;  // [max_parts][4 * 32-dimension blocks][256]
   f32x4* part_ml;   // [max_parts][256]: reference, sum, full sum
 };
@@ -93,13 +95,13 @@ __device__ __forceinline__ int keys_seen(const PromptParams& p, int n, int m, in
 // A unit is a row tile of one sequence and key/value head.  Sequences go from the longest to the shortest, row tiles
 // from the last (which sees the most keys) to the first, so that short units fill the end of the launch.  Where the units
 // of all sequences are few against their keys, long ones are split: `chunk` keys an item (whole tiles), at least kChunk and so many
-// that about kItems items have work; each item of a split unit leaves a part (reference, sums, unnormalised rows), and
+// that about `items` items have work; each item of a split unit leaves a part (reference, sums, unnormalised rows), and
 // join_kernel adds them up.  Items of one chunk follow one another: they read the same keys, at about the same time, on the
 // same XCD (equal spans of the line of all key tiles, each workgroup's keys its own, balanced as well and ran three
 // times longer: 14 prompts of up to 2000 tokens 375 us, 190 us a unit a workgroup).  Against chunks of 512 those of 256 took
 // 29.0 us instead of 39.7 (two prompts of 699 tokens, 4 heads of 256), 18.0 of 20.9 (2000 tokens, 2 heads); of 128, 27.5 and 20.4.
 // Every wave finds its item by itself, from the sequences in its lanes; more than 64 sequences are taken as they come.
-constexpr int kChunk = 256, kItems = 512, kChunkStep = 64;
+constexpr int kChunk = 256, kChunkStep = 64;
 // Sequence `lane`: its row tiles, keys, and the parts of its units.
 struct Line {
   int s0, n, k0, m;
@@ -120,10 +122,10 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
     float work = static_cast<float>(l.tiles) * static_cast<float>(l.m);
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) work += __shfl_xor(work, d);
-    // chunk > work Hkv / kItems: split units are less than kItems, and their parts, m / chunk + 1 < 2 m / chunk each, less
-    // than 2 kItems (1.001 is for the rounding of the sum).
-    l.chunk = uniform(max(kChunk, (static_cast<int>(min(work * static_cast<float>(p.Hkv) * (1.001f / kItems), 1e9f)) / kChunkStep + 1) * kChunkStep));
-    if (l.m > l.chunk) l.parts = (l.m + l.chunk - 1) / l.chunk;
+    // chunk > work Hkv / items: split units are less than `items`, and their parts, m / chunk + 1 < 2 m / chunk each, less
+    // than twice that (1.001 is for the rounding of the sum).
+    l.chunk = uniform(max(kChunk, (static_cast<int>(min(work * static_cast<float>(p.Hkv) * 1.001f / p.items, 1e9f)) / kChunkStep + 1) * kChunkStep));
+    if (l.m > l.chunk && l.m > p.least) l.parts = (l.m + l.chunk - 1) / l.chunk;
   }
   return l;
 }
@@ -586,15 +588,24 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   }
 }
 
-// Units may be split where keys are long and units few.  Up to kShortKeys, where splitting saves little, the units have to leave
-// CUs idle (717 tokens behind cached ones, 184 units: 24.1 us split, 25.8 not; four chunks of up to 517, 448 units: 35.8 and
-// 27.4).  Beyond it too for packed ones (256 units of 2048 keys 51 us with the parts' second launch, 45 without); sequences in
-// the cache, of which the page table only bounds the lengths, up to four times as many (eight chunks of up to 600 tokens behind up
-// to 4000: 80 us split, 121 not).
+// Units may be split where keys are long and units few, as measured at D = 128 unless said otherwise, split and not:
+//  - up to kShortKeys, where it saves little, units that leave CUs idle (717 tokens behind cached ones, 184 units: 24.1 and 25.8 us;
+//    four chunks of up to 517, 448 units: 35.8 and 27.4);
+//  - beyond it long packed prompts, where the last rows see all keys and the first almost none, into more items than fit the chip
+//    at once (8192 tokens, 256 units: 104 and 154 us; 512 units: 162 and 180; 2048 tokens, 384 units: 47.0 and 47.9; but 1300 tokens,
+//    256 units: 37.5 and 32.0), fewer where a CU holds one workgroup (D = 256, 2048 tokens, 300 units: 95 and 110; 128 units
+//    into 384 items 54, into 512 71);
+//  - without the causal mask, where all units are alike, only those less than the CUs (256 units of 2048 keys: 51 and 45);
+//  - sequences in the cache, of which the page table only bounds the lengths, up to 1024 (eight chunks of up to 600 tokens behind up to
+//    4000: 80 and 121).
 constexpr int64_t kFewKeys = 512, kShortKeys = 1024, kFew = 256, kFewPaged = 1024;
+constexpr int64_t kLong = 1536, kLongMean = 1024;  // keys of one prompt; of several
+constexpr int kItems = 512, kItemsCausal = 640, kFewCausal = 640, kItemsWide = 384, kFewWide = 320;
 struct Plan {
   int64_t units;  // at most
   bool split;
+  int items;
+  int64_t least;
   size_t acc_bytes, ml_bytes;
 };
 Plan plan_for(const latent_attn_prompt_args& a) {
@@ -604,12 +615,16 @@ Plan plan_for(const latent_attn_prompt_args& a) {
   pl.units = std::max<int64_t>(0, (a.n_tokens * G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1) * a.n_kv_head;
   const bool packed = a.k || a.n_keys;
   const int64_t keys = packed ? a.n_keys : a.cache.max_pages * a.cache.page_size;
-  pl.split = keys > kFewKeys && keys <= (1 << 28) && pl.units < (packed || keys <= kShortKeys ? kFew : kFewPaged) &&
-             a.cache.n_seq <= kWave;
+  const bool wide = a.head_dim > 128, slanted = packed && a.causal && keys >= (a.cache.n_seq == 1 ? kLong : kLongMean * a.cache.n_seq);
+  const int64_t few = slanted ? (wide ? kFewWide : kFewCausal) : packed || keys <= kShortKeys ? kFew : kFewPaged;
+  pl.split = keys > kFewKeys && keys <= (1 << 28) && pl.units < few && a.cache.n_seq <= kWave;
   if (!pl.split) return pl;
-  const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
-  pl.acc_bytes = size_t{2} * kItems * 4 * blocks * kThreads * sizeof(f32x4);
-  pl.ml_bytes = size_t{2} * kItems * kThreads * sizeof(f32x4);
+  pl.least = slanted && pl.units >= kFew ? kLong : 0;
+  pl.items = slanted ? (wide ? kItemsWide : kItemsCausal) : kItems;
+  // The size is that of the most items, with the mask or without.
+  const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8, parts = 2 * (wide ? kItems : kItemsCausal);
+  pl.acc_bytes = parts * 4 * blocks * kThreads * sizeof(f32x4);
+  pl.ml_bytes = parts * kThreads * sizeof(f32x4);
   return pl;
 }
 
@@ -696,7 +711,9 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
   const Plan pl = plan_for(a);
   if (pl.split && a.workspace && a.workspace_bytes >= pl.acc_bytes + pl.ml_bytes) {
     if (!aligned16(a.workspace)) return LATENT_E_UNSUPPORTED;
-    p.max_parts = 2 * kItems;
+    p.max_parts = 2 * pl.items;
+    p.items = static_cast<float>(pl.items);
+    p.least = static_cast<int32_t>(pl.least);
     p.part_acc = static_cast<f32x4*>(a.workspace);
     p.part_ml = reinterpret_cast<f32x4*>(static_cast<char*>(a.workspace) + pl.acc_bytes);
   }
@@ -705,8 +722,8 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
   auto launch = [&](auto e, auto dp) {
     constexpr int kDP = decltype(dp)::value;
     using E = decltype(e);
-    // Split units have less than kItems parts beyond their first.
-    const int64_t more = (kItems / p.Hkv + 1) * p.Hkv, units = std::max<int64_t>(pl.units, p.Hkv);
+    // Split units have less than pl.items parts beyond their first.
+    const int64_t more = (pl.items / p.Hkv + 1) * p.Hkv, units = std::max<int64_t>(pl.units, p.Hkv);
     auto go = [&](auto paged_c, auto lse_c) {
       constexpr bool kPaged = decltype(paged_c)::value, kLse = decltype(lse_c)::value;
       const dim3 grid(static_cast<unsigned>(units + (p.max_parts ? more : 0)));

@@ -453,6 +453,9 @@ def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
     ((3, 700), 1500, 16, 1, 72, 7, True),
     ((700,), 0, 8, 1, 128, 0, True),                 # fewer units than CUs
     ((3, 20), 600, 4, 2, 64, 16, True),
+    ((2100, 30), 0, 16, 16, 64, 0, True),            # more units than CUs: the long sequence alone
+    ((1200, 1100, 1600), 0, 8, 8, 128, 0, True),
+    ((2050,), 0, 16, 16, 168, 0, True),
 ])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_prompt_split_over_the_keys(gpu, new, ahead, Hq, Hkv, D, page, causal, dtype):
