@@ -173,7 +173,7 @@ __device__ __forceinline__ Item find_item(const PromptParams& p, int x, int lane
   if (!mine) return {-1};
   const int b = __builtin_ctzll(mine), r = x - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
   const int part = uniform(r / t);
-  return {b, t - 1 - (r - part * t), part, l.chunk, __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
+  return {b, t - 1 - (r - part * t), part, __builtin_amdgcn_readlane(l.parts, b) > 1 ? l.chunk : INT32_MAX, __builtin_amdgcn_readlane(l.s0, b), __builtin_amdgcn_readlane(l.n, b),
           __builtin_amdgcn_readlane(l.k0, b), __builtin_amdgcn_readlane(l.m, b)};
 }
 
