@@ -593,13 +593,13 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
 //    four chunks of up to 517, 448 units: 35.8 and 27.4);
 //  - beyond it long packed prompts, where the last rows see all keys and the first almost none, into more items than fit the chip
 //    at once (8192 tokens, 256 units: 104 and 154 us; 512 units: 162 and 180; 2048 tokens, 384 units: 47.0 and 47.9; but 1300 tokens,
-//    256 units: 37.5 and 32.0), fewer where a CU holds one workgroup (D = 256, 2048 tokens, 300 units: 95 and 110; 128 units
-//    into 384 items 54, into 512 71);
+//    256 units: 37.5 and 32.0, and five prompts of 1300, 440 units: 51.2 and 41.1), fewer where a CU holds one workgroup (D = 256, 2048 tokens, 300 units: 98 and 110; 128 units
+//    into 384 items 55, into 512 71);
 //  - without the causal mask, where all units are alike, only those less than the CUs (256 units of 2048 keys: 51 and 45);
 //  - sequences in the cache, of which the page table only bounds the lengths, up to 1024 (eight chunks of up to 600 tokens behind up to
 //    4000: 80 and 121).
 constexpr int64_t kFewKeys = 512, kShortKeys = 1024, kFew = 256, kFewPaged = 1024;
-constexpr int64_t kLong = 1536, kLongMean = 1024;  // keys of one prompt; of several
+constexpr int64_t kLong = 1536;  // keys of a prompt, or of several on average
 constexpr int kItems = 512, kItemsCausal = 640, kFewCausal = 640, kItemsWide = 384, kFewWide = 320;
 struct Plan {
   int64_t units;  // at most
@@ -615,7 +615,7 @@ Plan plan_for(const latent_attn_prompt_args& a) {
   pl.units = std::max<int64_t>(0, (a.n_tokens * G + kRowsTile - 1) / kRowsTile + std::min<int64_t>(a.cache.n_seq, a.n_tokens) - 1) * a.n_kv_head;
   const bool packed = a.k || a.n_keys;
   const int64_t keys = packed ? a.n_keys : a.cache.max_pages * a.cache.page_size;
-  const bool wide = a.head_dim > 128, slanted = packed && a.causal && keys >= (a.cache.n_seq == 1 ? kLong : kLongMean * a.cache.n_seq);
+  const bool wide = a.head_dim > 128, slanted = packed && a.causal && keys >= kLong * std::max<int64_t>(1, a.cache.n_seq);
   const int64_t few = slanted ? (wide ? kFewWide : kFewCausal) : packed || keys <= kShortKeys ? kFew : kFewPaged;
   pl.split = keys > kFewKeys && keys <= (1 << 28) && pl.units < few && a.cache.n_seq <= kWave;
   if (!pl.split) return pl;

@@ -437,6 +437,7 @@ def test_prompt_matches_plain_attention(gpu, Hq, Hkv, D, dtype, new, keys, causa
 
 @pytest.mark.parametrize("new,ahead,Hq,Hkv,D,page", [
     ((1500, 3, 700), 0, 8, 2, 128, 0), ((2000,), 0, 3, 3, 64, 0), ((600, 100), 3000, 8, 1, 128, 32), ((900,), 0, 2, 2, 256, 0),
+    ((2100, 30), 0, 16, 16, 64, 0), ((1200, 1100, 1600), 0, 8, 8, 128, 0),
 ])
 def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
     import torch
@@ -453,8 +454,8 @@ def test_prompt_long(gpu, new, ahead, Hq, Hkv, D, page):
     ((3, 700), 1500, 16, 1, 72, 7, True),
     ((700,), 0, 8, 1, 128, 0, True),                 # fewer units than CUs
     ((3, 20), 600, 4, 2, 64, 16, True),
-    ((2100, 30), 0, 16, 16, 64, 0, True),            # more units than CUs: the long sequence alone
-    ((1200, 1100, 1600), 0, 8, 8, 128, 0, True),
+    ((2100, 1000), 0, 16, 16, 64, 0, True),          # more units than CUs: the long sequence alone
+    ((1400, 1100, 2200), 0, 8, 8, 128, 0, True),
     ((2050,), 0, 16, 16, 168, 0, True),
 ])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
