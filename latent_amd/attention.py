@@ -225,20 +225,35 @@ class Attention:
         return kv_append(qkv[:, H:H + K], qkv[:, H + K:], self.k_cache, self.v_cache, pages, positions, seqs=seqs,
                          q=q, rope=self.rope, interleaved=self.interleaved, q_out=q)
 
+    def _stored_limit(self, max_pages: int) -> Optional[int]:
+        """How many positions tokens are stored at, where the rotation table ends before a page table row of max_pages does
+        (else None).  A token behind it is left out of the cache, so nothing may read its row: lengths are cut off there, a
+        launch more that a table of as many positions as the pages spares."""
+        if self.rope is None or self.rope.shape[0] >= max_pages * self.k_cache.shape[1]:
+            return None
+        return int(self.rope.shape[0])
+
+    def _stored(self, lengths: torch.Tensor, pages: torch.Tensor) -> torch.Tensor:
+        limit = self._stored_limit(pages.shape[1])
+        return lengths if limit is None else lengths.clamp_max(limit)
+
     def _project(self, a: torch.Tensor) -> torch.Tensor:
         return a.view(a.shape[0], -1) @ self.w_o
 
     def decode(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """One new token a sequence: x [B, d] at positions [B]; lengths [B] count it.  Returns [B, d] in the weights' type."""
+        """One new token a sequence: x [B, d] at positions [B]; lengths [B] count it.  Returns [B, d] in the weights' type.
+        A token behind the rotation table is not stored, and attends, unrotated, to those that are."""
         q = self._append(x, pages, positions, None)
+        lengths = self._stored(lengths, pages)
         return self._project(attend_decode(q, self.k_cache, self.v_cache, pages, lengths, scale=self.scale, workspace=workspace))
 
     def prompt(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor,
                lengths: torch.Tensor) -> torch.Tensor:
         """New tokens of several sequences, packed: x [T, d], token t of sequence seqs[t] (row of pages) at positions[t],
         sequence b's being rows starts[b] .. starts[b + 1] - 1 and the last of its lengths[b].  Rows of no sequence
-        (padding, at negative positions) give zeros."""
+        (padding, at negative positions) give zeros.  The pages and the rotation table have to have room for all lengths[b]."""
         q = self._append(x, pages, positions, seqs)
+        lengths = self._stored(lengths, pages)
         out = torch.zeros_like(q, memory_format=torch.contiguous_format)
         return self._project(attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out))

@@ -193,3 +193,39 @@ def test_slots_without_room_store_nothing_more(gpu, parts):
     for a, (k, v) in zip(s.attention, before):
         assert torch.equal(a.k_cache[mine], k[mine]) and torch.equal(a.v_cache[mine], v[mine])
         assert not torch.equal(a.k_cache[s.pages[1].long()], k[s.pages[1].long()])
+
+
+def test_slots_behind_their_rotation_table_read_what_is_stored(gpu, parts):
+    """A table that ends (at 20) before the pages do (at 32): its slot's later tokens are not stored, so the rows behind it, here NaN,
+    are not read; a step is append and attention over the 20 tokens that are there.  Eager and captured."""
+    import torch
+
+    layers, routers, ws, _ = parts
+    short = (layers, routers, ws, gpu.rope_table(20, D))
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x, steps = _x(gen, 23), [_x(gen, 2) for _ in range(5)]
+    for captured in (False, True):
+        s = _stack(gpu, short, 2, max_pages=2)
+        for a in s.attention:
+            a.k_cache.fill_(float("nan")), a.v_cache.fill_(float("nan"))
+        s.prompt(x, _ints([0, 18, 23]), _ints([0, 1]))
+        if captured:
+            s.capture()
+        for i, x0 in enumerate(steps):
+            s.load(x0)
+            out = s.replay() if captured else s.forward()
+            torch.cuda.synchronize()
+            assert bool(torch.isfinite(out).all()), i
+            a = s.attention[0]
+            qkv = (x0.bfloat16() @ a.w_qkv).view(2, HQ + 2 * HKV, D)
+            q = gpu.kv_append(qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], a.k_cache.clone(), a.v_cache.clone(), s.pages, _ints([18 + i, 5 + i]),
+                              q=qkv[:, :HQ], rope=a.rope, q_out=qkv[:, :HQ])
+            y = gpu.attend_decode(q, a.k_cache, a.v_cache, s.pages, _ints([min(19 + i, 20), 6 + i]))
+            assert torch.equal(s.h[0], x0 + y.view(2, -1) @ a.w_o), i
+        assert s.positions.tolist() == [23, 10]
+        for a in s.attention:
+            for t in (a.k_cache, a.v_cache):
+                rows = t[s.pages[0].long()].view(32, HKV, D)
+                assert bool(torch.isfinite(rows[:20]).all()) and bool(torch.isnan(rows[20:]).all())
+        # A prompt that passes the table reads no such row either.
+        assert bool(torch.isfinite(s.prompt(x, _ints([0, 2, 23]), _ints([0, 1]))).all())
