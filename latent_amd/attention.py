@@ -31,15 +31,25 @@ import torch
 from . import _lib
 from ._lib import LatentAttnDecodeArgs, LatentAttnPromptArgs, LatentError, LatentKvCache, check, lib
 
+
+class _NoBinding:
+    """In the binding's place where it cannot be loaded: the rest of the package works, an attention call raises."""
+
+    def __init__(self, cause: ImportError):
+        self._cause = cause
+
+    def __getattr__(self, name: str):
+        raise ImportError("latent_amd/_attend.so is missing or does not fit this torch: build it with "
+                          f"`python latent_amd/build.py` ({self._cause})") from self._cause
+
+
 try:
     from . import _attend
 except ImportError as e:
-    raise ImportError(
-        "latent_amd/_attend.so is missing or does not fit this torch: build it with `python latent_amd/build.py`"
-    ) from e
-
-_attend.entries(*(ctypes.cast(lib[f"latent_{n}"], ctypes.c_void_p).value for n in (
-    "kv_append", "attn_decode_workspace_size", "attn_decode", "attn_prompt_workspace_size", "attn_prompt")), LatentError)
+    _attend = _NoBinding(e)
+else:
+    _attend.entries(*(ctypes.cast(lib[f"latent_{n}"], ctypes.c_void_p).value for n in (
+        "kv_append", "attn_decode_workspace_size", "attn_decode", "attn_prompt_workspace_size", "attn_prompt")), LatentError)
 
 _DTYPE = (torch.float16, torch.bfloat16)
 

@@ -22,6 +22,7 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -50,8 +51,12 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (set HIPCC)")
 
 
-def binding_command(out: Path) -> list:
-    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+def binding_command(out: Path) -> Optional[list]:
+    """None without torch: there is nothing to bind to."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    torch = Path(spec.submodule_search_locations[0])
     rocm = Path(hipcc()).resolve().parent.parent / "include"
     include = [torch / "include", rocm, sysconfig.get_paths()["include"]]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
@@ -60,7 +65,11 @@ def binding_command(out: Path) -> list:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every source and link the shared library and the binding; always rebuilds."""
+    """Compile every source and link the shared library and the binding; always rebuilds.
+
+    The library needs hipcc alone and is in place before an error of the binding's (torch's headers, g++) is raised;
+    a binding that cannot be built leaves none, and without it everything but the attention calls works.
+    """
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
     cc = hipcc()
@@ -70,14 +79,22 @@ def build(verbose: bool = False) -> Path:
         cmds.append([cc, *HIPCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(str(obj))
     tmp_binding = BINDING.with_suffix(".so.tmp")
-    cmds.append(binding_command(tmp_binding))
+    binding = binding_command(tmp_binding)
+
+    def run(cmd):
+        try:
+            return subprocess.run(cmd, capture_output=True, text=True)
+        except OSError as e:  # no such program
+            return subprocess.CompletedProcess(cmd, 127, "", f"{cmd[0]}: {e}\n")
+
     # One compiler process per source, at most `jobs` at a time.
-    jobs = max(1, min(len(cmds), int(os.environ.get("MAX_JOBS", os.cpu_count() or 1))))
+    jobs = max(1, min(len(cmds) + 1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 1))))
     with ThreadPoolExecutor(max_workers=jobs) as pool:
-        for cmd in cmds:
-            if verbose:
+        for cmd in cmds + [binding or []]:
+            if verbose and cmd:
                 print(" ".join(cmd), flush=True)
-        for result in pool.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds):
+        bound = pool.submit(run, binding) if binding else None
+        for result in pool.map(run, cmds):
             sys.stderr.write(result.stderr)
             if result.returncode != 0:
                 raise subprocess.CalledProcessError(result.returncode, result.args, result.stdout, result.stderr)
@@ -87,7 +104,14 @@ def build(verbose: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    os.replace(tmp_binding, BINDING)
+    if bound is not None and bound.result().returncode == 0:
+        sys.stderr.write(bound.result().stderr)
+        os.replace(tmp_binding, BINDING)
+        return LIB
+    BINDING.unlink(missing_ok=True)  # an older one may not fit the library
+    if bound is not None:
+        raise RuntimeError(f"{LIB.name} is built, the binding {BINDING.name} is not:\n{bound.result().stderr}")
+    print(f"torch not found: {BINDING.name}, the binding of the attention calls, is not built", file=sys.stderr)
     return LIB
 
 

@@ -4,10 +4,16 @@ Only calls that return before any HIP runtime call are made here.
 """
 
 import ctypes
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
 import torch
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 @pytest.fixture(scope="module")
@@ -180,3 +186,44 @@ def test_rope_table_on_the_cpu():
     for bad in ((5, 7), (5, 0), (-1, 8)):
         with pytest.raises(ValueError):
             la.rope_table(*bad, device="cpu")
+
+
+# ---- without the binding --------------------------------------------------------
+def test_the_package_imports_without_the_binding():
+    """Only the attention calls need _attend.so; where it is missing or does not load, they say so."""
+    code = """
+import sys
+sys.modules["latent_amd._attend"] = None
+import torch, latent_amd as la, latent_amd.gguf
+assert la.moe_forward and la.Router and la.library_version() >= 100
+assert la.attend_decode_workspace_size(1, 4, 2, 64, 400, 16) > 0
+t = torch.zeros((1, 1, 8))
+for call in (lambda: la.kv_append(t, t, t, t, t, t), lambda: la.attend_decode(t, t, t, t, t), lambda: la.attend_prompt(t, t, t, t),
+             lambda: la.attend_prompt_paged(t, t, t, t, t, t)):
+    try:
+        call()
+    except ImportError as e:
+        assert "_attend.so" in str(e) and "build.py" in str(e)
+    else:
+        raise AssertionError("no error")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("why", ["no torch", "no compiler", "an error"])
+def test_the_library_is_built_whatever_becomes_of_the_binding(tmp_path, monkeypatch, why):
+    from latent_amd import build as b
+
+    if not os.path.exists(b.hipcc()):
+        pytest.skip("hipcc not found")
+    for name, value in (("PKG", tmp_path), ("LIB", tmp_path / "lib.so"), ("BINDING", tmp_path / "binding.so"), ("SOURCES", ["noalloc.hip"])):
+        monkeypatch.setattr(b, name, value)
+    if why == "no torch":
+        monkeypatch.setattr(b.importlib.util, "find_spec", lambda name: None)
+        b.build()
+    else:
+        monkeypatch.setenv("CXX", "/nowhere/g++" if why == "no compiler" else "false")
+        with pytest.raises(RuntimeError, match="_attend|binding"):
+            b.build()
+    assert b.LIB.exists() and not b.BINDING.exists()
