@@ -75,6 +75,9 @@ class DecodeStack:
         for a in blocks:
             if a.n_embd != self.d or a.k_cache.shape[:2] != blocks[0].k_cache.shape[:2] or a.w_qkv.device != dev:
                 raise ValueError("attention blocks must share d, the pages' number and size, and the layers' device")
+        caches = [t.data_ptr() for a in blocks for t in (a.k_cache, a.v_cache) if t.numel()]
+        if len(set(caches)) != len(caches):
+            raise ValueError("each layer's attention block needs a cache of its own: layers that share one overwrite each other's keys")
         if max_pages <= 0:
             raise ValueError("max_pages must be positive")
         self.attention = blocks

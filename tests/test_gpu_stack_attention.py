@@ -229,3 +229,22 @@ def test_slots_behind_their_rotation_table_read_what_is_stored(gpu, parts):
                 assert bool(torch.isfinite(rows[:20]).all()) and bool(torch.isnan(rows[20:]).all())
         # A prompt that passes the table reads no such row either.
         assert bool(torch.isfinite(s.prompt(x, _ints([0, 2, 23]), _ints([0, 1]))).all())
+
+
+def test_blocks_that_share_a_cache_are_refused(gpu, parts):
+    """Layers that store into one cache would read each other's keys."""
+    layers, routers, ws, rope = parts
+    make = lambda i: gpu.Attention(*ws[i], HQ, HKV, PAGES, PAGE, rope=rope)
+    block = make(0)
+    with pytest.raises(ValueError, match="cache of its own"):
+        gpu.DecodeStack(layers, routers, 2, attention=[block, block], max_pages=4)
+    for name in ("k_cache", "v_cache"):
+        other = make(1)
+        setattr(other, name, getattr(block, name).view(PAGES, PAGE, HKV, D))
+        with pytest.raises(ValueError, match="cache of its own"):
+            gpu.DecodeStack(layers, routers, 2, attention=[block, other], max_pages=4)
+    other = make(1)
+    other.v_cache = other.k_cache
+    with pytest.raises(ValueError, match="cache of its own"):
+        gpu.DecodeStack(layers, routers, 2, attention=[block, other], max_pages=4)
+    gpu.DecodeStack(layers, routers, 2, attention=[make(0), make(0)], max_pages=4)  # shared weights are no matter
