@@ -7,6 +7,7 @@
 // keeps its C ABI and knows no torch: its entry points come as addresses.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
@@ -45,6 +46,8 @@ const Tensor& tensor(PyObject* o, const char* name) {
 void check_grad(const Tensor& t) {
   TORCH_CHECK(!t.requires_grad() || !c10::GradMode::is_enabled(),
               "attention here has no backward pass: call it under torch.no_grad()");
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+              "attention here has no forward-mode derivative: its operands may not carry tangents");
 }
 
 // The device of a call's first tensor.
@@ -121,6 +124,7 @@ float* lse_of(PyObject* o, const Heads& q) {
   TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == q.tokens && t.size(1) == q.heads &&
                         t.device() == q.t.device() && t.is_contiguous(),
                     "lse must be contiguous f32 [", q.tokens, ", ", q.heads, "] on ", q.t.device());
+  check_grad(t);
   return static_cast<float*>(t.data_ptr());
 }
 

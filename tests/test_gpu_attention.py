@@ -689,6 +689,34 @@ def test_operands_that_want_gradients_are_refused(gpu):
                 call(*args)
 
 
+def test_operands_with_tangents_are_refused(gpu):
+    """Forward-mode derivatives would be dropped: operands that carry one are refused, lse and out among them."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+
+    gen, dt = _gen(27), torch.bfloat16
+    kc, vc, pages, _ = paged(gen, [20], 16, 1, 32, dt)
+    q, k, v, out = (_randn(gen, 1, 1, 32, dt=dt) for _ in range(4))
+    rope, lse, L, starts = gpu.rope_table(20, 32), torch.zeros((1, 1), device="cuda"), _ints([20]), _ints([0, 1])
+    calls = (lambda q, k, v, kc, vc, out, lse, rope: gpu.kv_append(k, v, kc, vc, pages, _ints([3]), q=q, q_out=out, rope=rope),
+             lambda q, k, v, kc, vc, out, lse, rope: gpu.attend_prompt(q, k, v, starts, out=out, lse=lse),
+             lambda q, k, v, kc, vc, out, lse, rope: gpu.attend_prompt_paged(q, kc, vc, pages, L, starts, out=out, lse=lse),
+             lambda q, k, v, kc, vc, out, lse, rope: gpu.attend_decode(q, kc, vc, pages, L, out=out, lse=lse))
+    used = ((0, 1, 2, 3, 4, 5, 7), (0, 1, 2, 5, 6), (0, 3, 4, 5, 6), (0, 3, 4, 5, 6))
+    for call, which in zip(calls, used):
+        for i in which:
+            args = [q, k, v, kc, vc, out, lse, rope]
+            with fwd.dual_level():
+                args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="derivative"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="derivative"):  # which does not stop tangents
+                    call(*args)
+            call(q, k, v, kc, vc, out, lse, rope)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        gpu.attend_decode(q, kc, vc, pages, L, lse=lse.clone().requires_grad_())
+
+
 def _refusal_operands():
     import torch
 
