@@ -50,6 +50,14 @@ void check_grad(const Tensor& t) {
               "attention here has no forward-mode derivative: its operands may not carry tangents");
 }
 
+// What a call wrote in place, for autograd's check of what it saved.  Inference tensors have no counter.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject* o) {
+  if (o != Py_None) written(THPVariable_Unpack(o));
+}
+
 // The device of a call's first tensor.
 c10::Device first(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
@@ -276,6 +284,7 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         a.dtype = dtype_of(k.t);
         a.rope_kind = truth(args[9]) ? LATENT_ROPE_INTERLEAVED : LATENT_ROPE_HALF;
         launch(append_entry, a, stream, "latent_kv_append");
+        written(args[2]), written(args[3]), written(args[10]);
       }
       if (args[7] == Py_None) Py_RETURN_NONE;
       return result(args[10], out);
@@ -311,6 +320,7 @@ PyObject* attend_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Scratch s = scratch(args[8], a, decode_size_entry, "latent_attn_decode", q.t);
         a.workspace = s.p, a.workspace_bytes = s.bytes;
         launch(decode_entry, a, stream, "latent_attn_decode");
+        written(args[6]), written(args[7]);
       }
       return result(args[6], out);
     });
@@ -336,6 +346,7 @@ PyObject* prompt(latent_attn_prompt_args& a, const Heads& q, PyObject* starts_ar
     const Scratch s = scratch(rest[3], a, prompt_size_entry, "latent_attn_prompt", q.t);
     a.workspace = s.p, a.workspace_bytes = s.bytes;
     launch(prompt_entry, a, stream, "latent_attn_prompt");
+    written(rest[1]), written(rest[2]);
   }
   return result(rest[1], out);
 }

@@ -717,6 +717,36 @@ def test_operands_with_tangents_are_refused(gpu):
         gpu.attend_decode(q, kc, vc, pages, L, lse=lse.clone().requires_grad_())
 
 
+def test_what_is_written_counts_as_changed(gpu):
+    """A buffer that autograd saved and a call then fills is noticed at the backward pass, as with torch's own in-place operations."""
+    import torch
+
+    gen, dt = _gen(28), torch.bfloat16
+    kc, vc, pages, _ = paged(gen, [20], 16, 1, 32, dt)
+    q, k, v, out, q_out = (_randn(gen, 1, 1, 32, dt=dt) for _ in range(5))
+    lse, L, starts = torch.zeros((1, 1), device="cuda"), _ints([20]), _ints([0, 1])
+    calls = ((lambda: gpu.kv_append(k, v, kc, vc, pages, _ints([3]), q=q, q_out=q_out), (kc, vc, q_out)),
+             (lambda: gpu.attend_prompt(q, k, v, starts, out=out, lse=lse), (out, lse)),
+             (lambda: gpu.attend_prompt_paged(q, kc, vc, pages, L, starts, out=out, lse=lse), (out, lse)),
+             (lambda: gpu.attend_decode(q, kc, vc, pages, L, out=out, lse=lse), (out, lse)))
+    read = (q, k, v, pages, L, starts)
+    for call, written in calls:
+        before = [t._version for t in (*written, *read)]
+        call()
+        assert [t._version for t in written] == [n + 1 for n in before[:len(written)]]
+        assert [t._version for t in read] == before[len(written):]
+    w = torch.ones(32, dtype=dt, device="cuda", requires_grad=True)
+    y = (w * out).sum()
+    gpu.attend_decode(q, kc, vc, pages, L, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        mine = torch.empty_like(out)
+        gpu.attend_decode(q, kc, vc, pages, L, out=mine)
+    gpu.attend_decode(q, kc, vc, pages, L, out=mine)  # inference tensors have no counter
+    assert torch.equal(mine, out)
+
+
 def _refusal_operands():
     import torch
 
