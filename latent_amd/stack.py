@@ -121,8 +121,9 @@ class DecodeStack:
     def prompt(self, x: torch.Tensor, starts: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
         """New tokens of several sequences through every layer: x [N, d], packed; sequence b is rows starts[b] ..
         starts[b + 1] - 1 (int32 [B + 1], ascending, up to N) and goes on in slot slots[b] (int32 [B], different
-        ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle.  The slots' pages, and the
-        blocks' rotation tables, have to have room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
+        ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle (also
+        with no tokens: a slot that is to stay idle is left out).  The slots' pages, and the blocks' rotation tables, have
+        to have room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
         (padding) reach no cache and pass the experts alone."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")
@@ -134,21 +135,24 @@ class DecodeStack:
         if x.device != dev or starts.device != dev or slots.device != dev:
             raise ValueError(f"x, starts and slots must be on {dev}")
         x = x.to(torch.float32)
-        N = x.shape[0]
-        if N == 0 or slots.numel() == 0:
-            return x.clone()
+        N, B = x.shape[0], slots.numel()
         at = slots.long()
         first, pages = self.positions[at].clamp_min(0), self.pages[at]
-        row = torch.arange(N, dtype=torch.int32, device=x.device)
-        seqs = torch.searchsorted(starts[1:].contiguous(), row, right=True, out_int32=True).clamp_max(slots.numel() - 1)
-        positions = row - starts[seqs.long()] + first[seqs.long()]
-        positions = torch.where((row >= starts[0]) & (row < starts[-1]), positions, -1)
         lengths = first + starts[1:] - starts[:-1]
-        ws = torch.zeros((max(max(workspace_size(L, N, self.k) for L in self.layers), 256),), dtype=torch.uint8, device=x.device)
-        for L, r, a in zip(self.layers, self.routers, self.attention):
-            x = x + a.prompt(x, pages, positions, seqs, starts, lengths)
-            ids, w = route(r.k, x=x, router=r.weight, drop=r.drop, drop_param=r.drop_param)
-            x = x + moe_forward(x, ids, w, L, workspace=ws)
+        if N and B:
+            row = torch.arange(N, dtype=torch.int32, device=x.device)
+            seqs = torch.searchsorted(starts[1:].contiguous(), row, right=True, out_int32=True).clamp_max(B - 1)
+            positions = row - starts[seqs.long()] + first[seqs.long()]
+            positions = torch.where((row >= starts[0]) & (row < starts[-1]), positions, -1)
+        if N:
+            ws = torch.zeros((max(max(workspace_size(L, N, self.k) for L in self.layers), 256),), dtype=torch.uint8, device=x.device)
+            for L, r, a in zip(self.layers, self.routers, self.attention):
+                if B:
+                    x = x + a.prompt(x, pages, positions, seqs, starts, lengths)
+                ids, w = route(r.k, x=x, router=r.weight, drop=r.drop, drop_param=r.drop_param)
+                x = x + moe_forward(x, ids, w, L, workspace=ws)
+        else:
+            x = x.clone()
         self.positions.index_copy_(0, at, lengths)
         return x
 

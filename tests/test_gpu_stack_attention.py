@@ -248,3 +248,30 @@ def test_blocks_that_share_a_cache_are_refused(gpu, parts):
     with pytest.raises(ValueError, match="cache of its own"):
         gpu.DecodeStack(layers, routers, 2, attention=[block, other], max_pages=4)
     gpu.DecodeStack(layers, routers, 2, attention=[make(0), make(0)], max_pages=4)  # shared weights are no matter
+
+
+def test_prompts_without_slots_or_tokens(gpu, parts):
+    """Rows of no sequence pass the experts alone, also where there is no sequence at all; a sequence of no tokens starts an idle
+    slot at 0, whether or not other rows come with it."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    layers, routers, _, _ = parts
+    s = _stack(gpu, parts, 3)
+    s.prompt(_x(gen, 9), _ints([0, 9]), _ints([2]))
+    before = [(a.k_cache.clone(), a.v_cache.clone()) for a in s.attention]
+    x = _x(gen, 7)
+    got = s.prompt(x, _ints([0]), _ints([]))
+    want = x
+    for L, r in zip(layers, routers):
+        ids, w = gpu.route(r.k, x=want, router=r.weight)
+        want = want + gpu.moe_forward(want, ids, w, L)
+    assert torch.equal(got, want)
+    assert s.positions.tolist() == [-1, -1, 9]
+    assert s.prompt(x[:0], _ints([0, 0, 0]), _ints([2, 0])).shape == (0, D_MODEL)
+    assert s.positions.tolist() == [0, -1, 9]
+    assert torch.equal(s.prompt(x, _ints([7, 7]), _ints([1])), want)
+    assert s.positions.tolist() == [0, 0, 9]
+    assert s.prompt(x[:0], _ints([0]), _ints([])).shape == (0, D_MODEL)
+    for a, (k, v) in zip(s.attention, before):
+        assert torch.equal(a.k_cache, k) and torch.equal(a.v_cache, v)
