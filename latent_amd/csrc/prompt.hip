@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   if (row >= all) return;
   if (!whole_unit) {
     const int part = blockIdx.x;  // items in their order, heads within
-    if (part >= p.max_parts) return;  // never, by the choice of chunk
+    if (part >= p.max_parts) return;  // never, by the choice of chunk and of max_parts, but for `starts` that descend
     f32x4* to = p.part_acc + static_cast<int64_t>(part) * (4 * kBlocks * kThreads) + tid;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
@@ -545,6 +545,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   const int row = tile * kRowsTile + (tid >> 6) * kRowsWave + (lane & 31);
   if (row >= n * p.G) return;
   const int at = first * p.Hkv + hk, step = t * p.Hkv;
+  if (at + (parts - 1) * step >= p.max_parts) return;  // never, but for `starts` that descend
   float top = -INFINITY, sum = 0.f, full = 0.f;
   f32x4 x[4] = {};
   for (int j0 = 0; j0 < parts; j0 += 4) {
@@ -606,6 +607,7 @@ struct Plan {
   bool split;
   int items;
   int64_t least;
+  int parts;  // at most
   size_t acc_bytes, ml_bytes;
 };
 Plan plan_for(const latent_attn_prompt_args& a) {
@@ -621,8 +623,12 @@ Plan plan_for(const latent_attn_prompt_args& a) {
   if (!pl.split) return pl;
   pl.least = slanted && pl.units >= kFew ? kLong : 0;
   pl.items = slanted ? (wide ? kItemsWide : kItemsCausal) : kItems;
+  // Parts are less than twice the items, and a unit has no more than chunks of kChunk in the keys.
+  const int64_t by_unit = pl.units * ((keys + kChunk - 1) / kChunk);
+  pl.parts = static_cast<int>(std::min<int64_t>(2 * pl.items, by_unit));
   // The size is that of the most items, with the mask or without.
-  const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8, parts = 2 * (wide ? kItems : kItemsCausal);
+  const size_t blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+  const size_t parts = std::min<int64_t>(2 * (wide ? kItems : kItemsCausal), by_unit);
   pl.acc_bytes = parts * 4 * blocks * kThreads * sizeof(f32x4);
   pl.ml_bytes = parts * kThreads * sizeof(f32x4);
   return pl;
@@ -711,7 +717,7 @@ extern "C" int latent_attn_prompt(const latent_attn_prompt_args* args, latent_st
   const Plan pl = plan_for(a);
   if (pl.split && a.workspace && a.workspace_bytes >= pl.acc_bytes + pl.ml_bytes) {
     if (!aligned16(a.workspace)) return LATENT_E_UNSUPPORTED;
-    p.max_parts = 2 * pl.items;
+    p.max_parts = pl.parts;
     p.items = static_cast<float>(pl.items);
     p.least = static_cast<int32_t>(pl.least);
     p.part_acc = static_cast<f32x4*>(a.workspace);

@@ -144,6 +144,24 @@ def test_decode_workspace_grows_to_a_bound(L):
         latent_amd.attend_decode_workspace_size(1, 3, 2, 128, 40, 16)
 
 
+def test_prompt_workspace_follows_the_call(L):
+    """A part is 128 rows of D rounded up to 64, 128 or 256 in fp32, and 16 bytes for each of 256 threads: 68 KB at D = 128.  A call
+    has no more of them than row tiles times chunks of 256 keys, nor than 1280."""
+    import latent_amd as la
+
+    size = la.attend_prompt_workspace_size
+    part = 128 * 128 * 4 + 256 * 16
+    assert 0 < size(600, 1, 1, 1, 128, n_keys=600) <= 5 * 3 * part
+    assert 0 < size(5, 1, 8, 8, 64, max_pages=40, page_size=32) <= 8 * 5 * part  # 8 row tiles, 1280 keys
+    assert 0 < size(600, 1, 1, 1, 256, n_keys=600) <= 5 * 3 * 2 * part
+    last = 0
+    for keys in (600, 6000, 60000, 600000):
+        n = size(64, 4, 8, 2, 128, max_pages=keys // 100, page_size=100)
+        assert last <= n <= 1280 * part
+        last = n
+    assert last == 1280 * part  # long keys: the most there are
+
+
 # ---- the Python calls -----------------------------------------------------------
 def _t(*shape, dt=torch.bfloat16):
     return torch.zeros(shape, dtype=dt)
