@@ -119,6 +119,8 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
   l.parts = 1;
   l.chunk = INT32_MAX;
   if (p.max_parts) {
+    // Both kernels cut the keys by this sum and have to agree to the last bit, whatever the compiler makes of either: no contraction.
+#pragma clang fp contract(off)
     float work = static_cast<float>(l.tiles) * static_cast<float>(l.m);
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) work += __shfl_xor(work, d);
