@@ -82,9 +82,9 @@ __device__ const u32x4 kZeroRow[kMaxDim * 2 / 16] = {};
 
 // Direct global -> LDS loads: lane l's 16 bytes land at LDS byte address lds + 16 l; lds is wave-uniform.  Inline
 // assembly, so that the compiler does not make every later LDS read wait for them; whoever issues them waits
-// (pipeline_barrier).  The second form takes a wave-uniform base and a 32-bit lane offset.
+// (pipeline_barrier).  They write memory, so no access of the program's own moves across them.  The second form takes a wave-uniform base and a 32-bit lane offset.
 __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "m0", "memory");
 }
 __device__ __forceinline__ void dma16s(const void* base, uint32_t off, uint32_t lds) {
   const uint64_t v = reinterpret_cast<uintptr_t>(base);
@@ -92,7 +92,7 @@ __device__ __forceinline__ void dma16s(const void* base, uint32_t off, uint32_t 
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(u),
                "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "m0");
+               : "m0", "memory");
 }
 
 template <typename T>
