@@ -229,6 +229,21 @@ def test_decode_infinite_and_nan_keys_reach_their_own_rows_only(gpu):
     assert bool((gpu.attend_decode(q0, kc2, vc2, pages2, _ints([40]), lse=lse) == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("length", [100, 3000])
+def test_decode_infinite_and_nan_values_reach_their_own_rows_only(gpu, length):
+    import torch
+
+    gen, dt, D = _gen(30), torch.float16, 128
+    lens = [length, length - 1]
+    kc, vc, pages, seqs = paged(gen, lens, 16, 2, D, dt)
+    q = _randn(gen, 2, 6, D, dt=dt)
+    for key, x in ((length - 2, math.nan), (17, math.inf), (0, -math.inf)):
+        seqs[1][1][key, 1, 5] = x
+        vc[pages[1, key // 16].long(), key % 16, 1, 5] = x
+    vc[pages[1, (length - 1) // 16].long(), (length - 1) % 16] = math.nan  # behind its last row
+    _decode_check(gpu, q, kc, vc, pages, _ints(lens), seqs, lens)
+
+
 def test_decode_cache_beyond_32_bit_offsets(gpu):
     """Rows whose byte offsets pass 2^32."""
     import torch
@@ -512,6 +527,45 @@ def test_prompt_nan_and_infinity_do_not_reach_rows_that_do_not_see_them(gpu, D):
     got = gpu.attend_prompt(q, k, v, starts)
     assert torch.equal(got[:70], out[:70]) and torch.equal(got[70:80, 1], out[70:80, 1])
     assert torch.isnan(got[80:, 1]).all()
+
+
+@pytest.mark.parametrize("page", [0, 16, 7])
+@pytest.mark.parametrize("n,ahead,Hq,Hkv,D,dtype", [
+    (150, 0, 6, 2, 64, "bf16"), (150, 40, 3, 1, 128, "f16"), (70, 1500, 6, 2, 128, "bf16"), (90, 1300, 5, 1, 256, "bf16"),
+    (200, 900, 4, 4, 96, "f16"), (33, 700, 7, 1, 72, "bf16"),
+])
+def test_prompt_nan_and_infinity_among_cached_and_split_values(gpu, n, ahead, Hq, Hkv, D, dtype, page):
+    """The same in the cache, for grouped heads and where the keys are split: in tiles that all rows see, that some do, and that
+    only the last does."""
+    import torch
+
+    gen, dt, m = _gen(29), _dt(dtype), n + ahead
+    q = _randn(gen, n, Hq, D, dt=dt)
+    kc, vc, pages, seqs = paged(gen, [m], page or 64, Hkv, D, dt)
+    k, v = seqs[0]
+    split = gpu.attend_prompt_workspace_size(n, 1, Hq, Hkv, D, 0 if page else m, m, 1) > 0
+    assert split == (m > 512)
+
+    def check(at):
+        v2 = v.clone()
+        for i, (key, h, d, x) in enumerate(at):
+            v2[key, h, d] = x
+        starts = _ints([0, n])
+        if page:
+            rows = torch.arange(m, device="cuda")
+            vc[pages[0].long()[rows // page], rows % page] = v2
+        for ws in (None, torch.empty(16, dtype=torch.uint8, device="cuda")):  # with scratch, and in whole units
+            lse = torch.empty((n, Hq), device="cuda")
+            if page:
+                out = gpu.attend_prompt_paged(q, kc, vc, pages, _ints([m]), starts, lse=lse, workspace=ws)
+            else:
+                out = gpu.attend_prompt(q, k, v2, starts, k_starts=_ints([0, m]), lse=lse, workspace=ws)
+            assert_attention(out, lse, q, k, v2, visible(n, m, True, "cuda"), D ** -0.5)
+
+    check([(m - 1, 0, 3, math.inf), (m - 1, Hkv - 1, D - 1, math.nan)])
+    check([(ahead + n // 2, Hkv - 1, 0, math.nan), (ahead + 5, 0, D - 2, -math.inf), (ahead + 6, 0, D - 2, math.inf), (m - 2, 0, 1, math.nan)])
+    if ahead:
+        check([(ahead - 1, 0, 5, math.nan), (0, Hkv - 1, 6, math.inf)])
 
 
 def test_prompt_masks_pages_that_do_not_exist(gpu):

@@ -275,3 +275,42 @@ def test_prompts_without_slots_or_tokens(gpu, parts):
     assert s.prompt(x[:0], _ints([0]), _ints([])).shape == (0, D_MODEL)
     for a, (k, v) in zip(s.attention, before):
         assert torch.equal(a.k_cache, k) and torch.equal(a.v_cache, v)
+
+
+def test_prompt_is_the_public_calls_in_order(gpu, parts):
+    """A padded batch behind cached tokens, one sequence without any: rows, caches and attention of every layer, rebuilt from the
+    public calls, the attention against 64 bits."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    layers, routers, ws, rope = parts
+    s = _stack(gpu, parts, 4)
+    s.prompt(_x(gen, 33), _ints([0, 20, 33]), _ints([3, 1]))
+    caches = [(a.k_cache.clone(), a.v_cache.clone()) for a in s.attention]
+    new, first, slots, lead, tail = [17, 0, 40, 1], [0, 13, 20, 0], [0, 1, 3, 2], 2, 3
+    starts = [lead]
+    for n in new:
+        starts.append(starts[-1] + n)
+    N = starts[-1] + tail
+    x = x0 = _x(gen, N)
+    got = s.prompt(x0, _ints(starts), _ints(slots))
+    rows = [b for b, n in enumerate(new) for _ in range(n)]
+    seqs = _ints([0] * lead + rows + [0] * tail)
+    pos = _ints([-1] * lead + [first[b] + i for b, n in enumerate(new) for i in range(n)] + [-1] * tail)
+    pages, lengths = s.pages[_ints(slots).long()], _ints([a + n for a, n in zip(first, new)])
+    for L, r, (wqkv, wo), (kc, vc), a in zip(layers, routers, ws, caches, s.attention):
+        qkv = (x.bfloat16() @ wqkv).view(N, HQ + 2 * HKV, D)
+        q = gpu.kv_append(qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], kc, vc, pages, pos, seqs=seqs, q=qkv[:, :HQ], rope=rope, q_out=qkv[:, :HQ])
+        y = gpu.attend_prompt_paged(q, kc, vc, pages, lengths, _ints(starts), out=torch.zeros((N, HQ, D), dtype=q.dtype, device="cuda"))
+        assert bool((y[:lead] == 0).all()) and bool((y[starts[-1]:] == 0).all())
+        for b, n in enumerate(new):
+            at = torch.arange(first[b] + n, device="cuda")
+            p, o = pages[b].long()[at // PAGE], at % PAGE
+            assert_attention(y[starts[b]:starts[b + 1]], None, q[starts[b]:starts[b + 1]], kc[p, o], vc[p, o],
+                             visible(n, first[b] + n, True, "cuda"), D ** -0.5)
+        h = x + y.view(N, -1) @ wo
+        ids, w = gpu.route(r.k, x=h, router=r.weight)
+        x = h + gpu.moe_forward(h, ids, w, L)
+        assert torch.equal(a.k_cache, kc) and torch.equal(a.v_cache, vc)
+    assert torch.equal(got, x)
+    assert s.positions[_ints(slots).long()].tolist() == lengths.tolist()
