@@ -597,6 +597,67 @@ def test_prompt_fused_projection_views_and_bad_starts(gpu):
     assert torch.equal(room[:40], out[:40])
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,page,dtype", [(8, 2, 128, 16, "bf16"), (6, 3, 72, 5, "f16"), (4, 2, 256, 8, "bf16"), (5, 1, 64, 24, "f16")])
+def test_keys_and_values_in_caches_of_other_strides(gpu, Hq, Hkv, D, page, dtype):
+    """Keys by rows, values by heads, each a part of something wider."""
+    import torch
+
+    gen, dt, lens = _gen(31), _dt(dtype), [70, 1100, 0, 1]
+    kc, vc, pages, seqs = paged(gen, lens, page, Hkv, D, dt)
+    wide = torch.full((kc.shape[0], 2, page, Hkv + 1, D + 8), math.nan, dtype=dt, device="cuda")
+    k2 = wide[:, 1, :, 1:, 8:]
+    k2.copy_(kc)
+    v2 = torch.full((kc.shape[0], Hkv, 3, page, D), math.nan, dtype=dt, device="cuda")[:, :, 1].transpose(1, 2)
+    v2.copy_(vc)
+    q = _randn(gen, 4, Hq, D, dt=dt)
+    _decode_check(gpu, q, k2, v2, pages, _ints(lens), seqs, lens)
+    starts = [0, 33, 93, 95, 96]
+    q = _randn(gen, 96, Hq, D, dt=dt)
+    lse = torch.empty((96, Hq), device="cuda")
+    out = gpu.attend_prompt_paged(q, k2, v2, pages, _ints(lens), _ints(starts), lse=lse)
+    for b, n in enumerate(lens):
+        r = slice(starts[b], starts[b + 1])
+        assert_attention(out[r], lse[r], q[r], *seqs[b], visible(starts[b + 1] - starts[b], n, True, "cuda"), D ** -0.5)
+    k, v = (_randn(gen, 3, Hkv, D, dt=dt) for _ in range(2))
+    before = wide.clone()
+    gpu.kv_append(k, v, k2, v2, pages, _ints([3, 69, 1099]), seqs=_ints([0, 0, 1]))
+    for t, (b, p) in enumerate(((0, 3), (0, 69), (1, 1099))):
+        at = int(pages[b, p // page]), p % page
+        assert torch.equal(k2[at], k[t]) and torch.equal(v2[at], v[t])
+        before[at[0], 1, at[1], 1:, 8:] = k[t]
+    assert torch.equal(wide.view(torch.int16), before.view(torch.int16))
+
+
+def test_prompt_broadcast_operands(gpu):
+    """Heads and tokens of one place, among the operands that are read."""
+    import torch
+
+    gen, dt, T, D = _gen(32), torch.bfloat16, 140, 64
+    q, k, v = _randn(gen, 1, 4, D, dt=dt).expand(T, 4, D), _randn(gen, T, 1, D, dt=dt).expand(T, 2, D), _randn(gen, T, 1, D, dt=dt).expand(T, 2, D)
+    out = gpu.attend_prompt(q, k, v, _ints([0, 100, T]))
+    for a, b in ((0, 100), (100, T)):
+        assert_attention(out[a:b], None, q[a:b], k[a:b], v[a:b], visible(b - a, b - a, True, "cuda"), D ** -0.5)
+    kc, vc, pages, _ = paged(gen, [T], 16, 2, D, dt)
+    gpu.kv_append(k, v, kc, vc, pages, _ints(list(range(T))), seqs=_ints([0] * T))
+    assert torch.equal(gpu.attend_prompt_paged(q, kc, vc, pages, _ints([T]), _ints([0, T]))[:100], out[:100])
+    one = kc[:, :, :1].expand(-1, -1, 2, -1), vc[:, :, :1].expand(-1, -1, 2, -1)
+    L = _ints([T])
+    assert torch.equal(gpu.attend_decode(q[:1], *one, pages, L), gpu.attend_decode(q[:1], kc, vc, pages, L))
+
+
+@pytest.mark.parametrize("B", [63, 64, 65])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 64), (4, 2, 256)])
+def test_prompt_one_long_sequence_among_as_many_as_a_wave_has_lanes(gpu, B, Hq, Hkv, D):
+    new = [1 + (11 * i) % 7 for i in range(B)]
+    new[B - 2] = 90
+    keys = [n + (B - i) % 40 for i, n in enumerate(new)]
+    keys[B - 2] = 2600
+    split = gpu.attend_prompt_workspace_size(sum(new), B, Hq, Hkv, D, 0, 2600, 1) > 0
+    assert split == (B <= 64)
+    _prompt_check(gpu, _gen(33), new, keys, Hq, Hkv, D, _dt("bf16"), True, page=16, pad=1)
+    _prompt_check(gpu, _gen(34), new, keys, Hq, Hkv, D, _dt("f16"), True, pad=1)
+
+
 # ---- streams, graphs ------------------------------------------------------------
 def test_calls_on_another_stream(gpu):
     import torch
