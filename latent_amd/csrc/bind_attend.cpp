@@ -261,7 +261,8 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           "rope must be f32 [positions, 2, rot / 2] on ", dev);
         check_grad(rope);
         if (!rope.is_contiguous() || (reinterpret_cast<uintptr_t>(rope.data_ptr()) & 15)) rope = rope.clone(at::MemoryFormat::Contiguous);
-        a.rope = static_cast<const float*>(rope.data_ptr());
+        // A table without rows has no base, and no base would mean no rotation: any address serves, none of it is read.
+        a.rope = static_cast<const float*>(rope.numel() ? rope.data_ptr() : k.p);
         a.rope_rows = rope.size(0);
         a.rot_dim = 2 * rope.size(2);
         TORCH_CHECK_VALUE(0 < a.rot_dim && a.rot_dim <= k.D, "rope turns ", a.rot_dim, " dimensions of ", k.D);

@@ -127,6 +127,22 @@ def test_append_leaves_out_what_has_no_place(gpu, D):
     assert float(((out[fine].double() - q64).abs() - tol).max()) <= 0
 
 
+@pytest.mark.parametrize("D", [32, 24])
+def test_append_with_an_empty_table_leaves_all_out(gpu, D):
+    """No position is in a table without rows: nothing is stored, q_out stays."""
+    import torch
+
+    gen, dt = _gen(35), torch.bfloat16
+    kc, vc, pages, _ = paged(gen, [12], 4, 1, D, dt)
+    before = kc.clone(), vc.clone()
+    q, k, v = (_randn(gen, 3, 1, D, dt=dt) for _ in range(3))
+    out = torch.full_like(q, 7.0)
+    gpu.kv_append(k, v, kc, vc, pages, _ints([0, 1, 5]), seqs=_ints([0, 0, 0]), q=q, rope=gpu.rope_table(0, 8), q_out=out)
+    assert bool((out == 7.0).all())
+    for got, want in zip((kc, vc), before):
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
 def test_append_without_tokens_or_sequences(gpu):
     import torch
 
