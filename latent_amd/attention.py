@@ -229,8 +229,8 @@ class Attention:
         return int(self.w_qkv.shape[0])
 
     def _append(self, x: torch.Tensor, pages, positions, seqs) -> torch.Tensor:
-        qkv = (x.to(self.w_qkv.dtype) @ self.w_qkv).view(x.shape[0], -1, self.head_dim)
         H, K = self.n_head, self.n_kv_head
+        qkv = (x.to(self.w_qkv.dtype) @ self.w_qkv).view(x.shape[0], H + 2 * K, self.head_dim)
         q = qkv[:, :H]
         return kv_append(qkv[:, H:H + K], qkv[:, H + K:], self.k_cache, self.v_cache, pages, positions, seqs=seqs,
                          q=q, rope=self.rope, interleaved=self.interleaved, q_out=q)
@@ -248,7 +248,7 @@ class Attention:
         return lengths if limit is None else lengths.clamp_max(limit)
 
     def _project(self, a: torch.Tensor) -> torch.Tensor:
-        return a.view(a.shape[0], -1) @ self.w_o
+        return a.view(a.shape[0], self.w_o.shape[0]) @ self.w_o
 
     def decode(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -314,3 +314,17 @@ def test_prompt_is_the_public_calls_in_order(gpu, parts):
         assert torch.equal(a.k_cache, kc) and torch.equal(a.v_cache, vc)
     assert torch.equal(got, x)
     assert s.positions[_ints(slots).long()].tolist() == lengths.tolist()
+
+
+def test_blocks_without_sequences_or_tokens(gpu, parts):
+    import torch
+
+    _, _, ws, rope = parts
+    a = gpu.Attention(*ws[0], HQ, HKV, PAGES, PAGE, rope=rope)
+    x, pages, none = torch.empty((0, D_MODEL), device="cuda"), torch.zeros((2, 3), dtype=torch.int32, device="cuda"), _ints([])
+    assert a.decode(x, pages[:0], none, none).shape == (0, D_MODEL)
+    assert a.prompt(x, pages, none, none, _ints([0, 0, 0]), _ints([0, 5])).shape == (0, D_MODEL)
+    assert a.prompt(x, pages[:0], none, none, _ints([0]), none).shape == (0, D_MODEL)
+    y = a.prompt(torch.ones((2, D_MODEL), device="cuda"), pages[:0], _ints([-1, -1]), _ints([0, 0]), _ints([0]), none)  # padding alone
+    assert y.shape == (2, D_MODEL) and bool((y == 0).all())
+    assert bool((a.k_cache == 0).all()) and bool((a.v_cache == 0).all())
