@@ -271,7 +271,7 @@ def _host_subset(torch, layer, ids, ref):
 def cpu_baseline(torch, layer, routes, xs, batch, steps, prefill_inputs, prefill_tokens):
     """The oracle (numpy restatement of loader/latent_runtime.py, each routed
     expert dequantized once per step) on the same workloads, timed on the
-    host: decode steps at `batch` with all host threads the GPU box grants
+    host: decode steps at `batch` with all host threads that are granted
     (OMP_NUM_THREADS) and with one, median of `steps` steps each; and one
     prefill step on the first `prefill_tokens` tokens of the prefill batch
     (all threads)."""

@@ -495,7 +495,8 @@ int latent_attn_decode(const latent_attn_decode_args* args, latent_stream_t stre
  * Whole prompts, packed: sequence b's queries are rows starts[b] ..
  * starts[b + 1] - 1 of q (starts ascends from >= 0; what passes n_tokens is cut
  * off), its keys either rows k_starts[b] .. k_starts[b + 1] - 1 of k and v, or
- * (k NULL) positions 0 .. lengths[b] - 1 of the cache.  With n queries and m
+ * (k NULL) positions 0 .. lengths[b] - 1 of the cache (lengths outside
+ * [0, max_pages * page_size] are clamped to it first).  With n queries and m
  * keys, query i sees keys j <= i + m - n when causal (the last query sees all),
  * every key otherwise.  A row that sees none gives zeros and lse -inf.  Rows of
  * out and lse that belong to no sequence are left as they are.

@@ -16,8 +16,10 @@ strides that are multiples of 8 elements, D adjacent: permuted views work), with
 a page table int32 [B, max_pages]: position p of sequence b is row p % page of
 page pages[b, p // page].  A page id outside [0, pages) names no page.  Query
 head h reads kv head h // (n_head / n_kv_head).  D is a multiple of 8 up to 256.
-Scores, softmax and sums are fp32; probabilities are rounded to the element type
+Scores, softmax and sums are fp32 (a row's sum of values times weights of at most
+one has to stay finite there); probabilities are rounded to the element type
 for the product with the values, outputs once.  There is no backward pass.
+Lengths are cut off at what a row of the page table has room for, and at 0.
 """
 
 from __future__ import annotations
@@ -191,7 +193,8 @@ def attend_prompt_paged(
     stream: Optional[torch.cuda.Stream] = None,
 ) -> torch.Tensor:
     """attend_prompt with the keys and values of sequence b in the cache: its first lengths[b] (int32 [B])
-    positions, the new tokens' own (appended before the call) the last of them."""
+    positions, the new tokens' own (appended before the call) the last of them.  lengths[b] is at most what a row of
+    pages has room for: what is beyond is cut off, and the last query then stands at the last position that is left."""
     if stream is not None:
         with _on(stream, q):
             return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)

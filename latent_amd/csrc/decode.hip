@@ -21,9 +21,14 @@
 // operand covers those keys.  A value row arrives as VEC = D / 16 neighbours a lane
 // for eight keys; eight rows are paired into operand dwords by byte permutes.
 //
-// Measured (bf16, heads of 128, 8 of them with keys): 131071 tokens 102 us (5.2 TB/s),
-// 32 sequences of 500 to 16000 tokens 59 us (4.8 TB/s), 64 of up to 20000 658 us (5.7 TB/s);
-// 301 tokens 7.1 us, of which the launch alone is 5.
+// A probability is rounded to the element type for its product with the values, at most half a step of its own size; the sum
+// that divides takes them unrounded, as the log-sum-exp needs it, so a row may be off by those half steps
+// (in bf16 0.0018 of a row's size against 0.0017 with them in 32 bits; the output's own rounding is as much).
+//
+// Measured (bf16, heads of 128, 8 of them with keys): 131071 tokens 102 us (5.2 TB/s), 35 sequences of 16 to 16000
+// tokens, 69502 in all, 60 us (4.8 TB/s), 64 of 10000 to 20000 656 us (5.7 TB/s); 301 tokens 7.0 us, of
+// which the launch alone is 5, and 9.4 where the page table is wider than what is taken whole (kWholeTiles).
+// Heads of 72 and 96: 3.8 and 4.8 TB/s (16 sequences of 12000), padded to 128 and with the usual loads.
 #include "attend.hpp"
 
 #include <algorithm>

@@ -11,7 +11,9 @@
 // pairs, or 16 neighbours) and goes on to the next heads of its token with the
 // same 16 table values: read again for each head they would be twice the bytes
 // of the data itself.  Measured: 8190 tokens of 80 heads of 128 bf16 68 us (5.0 TB/s,
-// a copy's rate); one token 2.9 us of GPU, 5.1 a call.
+// a copy's rate); one token 2.9 us of GPU, 5.1 a call.  Heads or rotations that are no multiples of 16 take a kernel of one pair a
+// thread in accesses of two bytes (8192 tokens of 48 heads: rotation of 20 of 128 dimensions 191 us, of 128 41; heads of 72 62,
+// of 80 31): one step's tokens cost a launch either way (32 tokens of heads of 72: 4.6 us).
 #include "attend.hpp"
 
 #include <algorithm>

@@ -15,10 +15,10 @@
 // eight consecutive registers, rounded, are the operand of out^T = V^T P^T as
 // they stand; the value operand is read transposed from LDS in that key order.
 //
-// Measured (bf16, heads of 128): 8192 tokens of 64 heads over 8 in 1030 us, 1070
-// TFLOP/s; 14 prompts of 162 to 2000 tokens, 32 heads, 186 us.  The long ones are
-// bound by the power the products draw: the same instructions over zeros take
-// 832 us (the card's 8192^3 matrix product: 1360 TFLOP/s, 1800 over zeros), and
+// Measured (bf16, heads of 128): 8192 tokens of 64 heads over 8 in 1030 to 1130 us by the
+// card, 970 to 1070 TFLOP/s; 14 prompts of 162 to 2000 tokens, 32 heads, 191 us.  The long ones are
+// bound by the power the products draw: where the 8192 took 1024 us, the same instructions over zeros took
+// 832 (the card's 8192^3 matrix product: 1360 TFLOP/s, 1800 over zeros), and
 // neither waits nor the order of products and exponentials shows in the time
 // (scores a tile ahead with a few exponentials behind every product: 1049 us;
 // three and four LDS buffers: the same; no wait for the loads at all: the same).
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
       }
     }
     if constexpr (kPaged) {
-      // Lane l finds where row l lies, once for the tile; whoever loads a piece of the row asks it (four chunks of up to 517
+      // Lane l finds where row l lies, once for the tile; whoever loads a piece of the row asks it (four chunks of 354 to 517
       // tokens: 28.7 us with every load's address worked out by itself, 27.4 so).
       const uint32_t key = kt + opaque(lane), off = key - p.cache.by_page.of(key) * p.cache.page_size;
       const bool there = page_in_lane < p.cache.n_pages;
@@ -592,15 +592,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
 }
 
 // Units may be split where keys are long and units few, as measured at D = 128 unless said otherwise, split and not:
-//  - up to kShortKeys, where it saves little, units that leave CUs idle (717 tokens behind cached ones, 184 units: 24.1 and 25.8 us;
-//    four chunks of up to 517, 448 units: 35.8 and 27.4);
+//  - up to kShortKeys, where it saves little, units that leave CUs idle (716 tokens behind 6 cached ones, 184 units: 24.5 and 25.7 us;
+//    four chunks of 354 to 517 tokens behind 5 to 210, 448 units: 35.5 and 27.8);
 //  - beyond it long packed prompts, where the last rows see all keys and the first almost none, into more items than fit the chip
 //    at once (8192 tokens, 256 units: 104 and 154 us; 512 units: 162 and 180; 2048 tokens, 384 units: 47.0 and 47.9; but 1300 tokens,
 //    256 units: 37.5 and 32.0, and five prompts of 1300, 440 units: 51.2 and 41.1), fewer where a CU holds one workgroup (D = 256, 2048 tokens, 300 units: 98 and 110; 128 units
 //    into 384 items 55, into 512 71);
 //  - without the causal mask, where all units are alike, only those less than the CUs (256 units of 2048 keys: 51 and 45);
-//  - sequences in the cache, of which the page table only bounds the lengths, up to 1024 (eight chunks of up to 600 tokens behind up to
-//    4000: 80 and 121).
+//  - sequences in the cache, of which the page table only bounds the lengths, up to 1024 (a chunk of 512 tokens behind 4000: 59 and
+//    112, two of them 103 and 113, four 182 and 178; behind 30000: 305 and 706; 30 tokens behind 8000: 28 and 185).  Keys that
+//    are fewer than the table has room for are split as well: the four chunks of the first line in a wider table take 35.5 us.
 constexpr int64_t kFewKeys = 512, kShortKeys = 1024, kFew = 256, kFewPaged = 1024;
 constexpr int64_t kLong = 1536;  // keys of a prompt, or of several on average
 constexpr int kItems = 512, kItemsCausal = 640, kFewCausal = 640, kItemsWide = 384, kFewWide = 320;

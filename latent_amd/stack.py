@@ -19,8 +19,9 @@ is cached, stores nothing more and attends to what is there.
 `prompt` runs whole prompts, or chunks of them, through the same layers and
 leaves the slots ready to decode.
 
-The residual stream stays fp32 on the device; every buffer is allocated once,
-so the whole stack (2 router kernels + the expert FFN + one add per layer, and
+The residual stream stays fp32 on the device; the stack's own buffers are
+allocated once (an attention block's projections come from torch's allocator,
+from a graph's pool when captured), so the whole stack (2 router kernels + the expert FFN + one add per layer, and
 the attention's) can be captured in a torch.cuda.CUDAGraph (a HIP graph) and
 replayed.  This is the stacked decode of a llama.cpp graph built by
 build_moe_ffn_latent (README.md:111-113): the MoE blocks alone, or with the
