@@ -240,15 +240,11 @@ class Attention:
 
     def _stored_limit(self, max_pages: int) -> Optional[int]:
         """How many positions tokens are stored at, where the rotation table ends before a page table row of max_pages does
-        (else None).  A token behind it is left out of the cache, so nothing may read its row: lengths are cut off there, a
-        launch more that a table of as many positions as the pages spares."""
+        (else None).  A token behind it is left out of the cache and its query is not rotated, so its attention is zeros: a
+        launch or two more, which a table of as many positions as the pages spares."""
         if self.rope is None or self.rope.shape[0] >= max_pages * self.k_cache.shape[1]:
             return None
         return int(self.rope.shape[0])
-
-    def _stored(self, lengths: torch.Tensor, pages: torch.Tensor) -> torch.Tensor:
-        limit = self._stored_limit(pages.shape[1])
-        return lengths if limit is None else lengths.clamp_max(limit)
 
     def _project(self, a: torch.Tensor) -> torch.Tensor:
         return a.view(a.shape[0], self.w_o.shape[0]) @ self.w_o
@@ -256,17 +252,23 @@ class Attention:
     def decode(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One new token a sequence: x [B, d] at positions [B]; lengths [B] count it.  Returns [B, d] in the weights' type.
-        A token behind the rotation table is not stored, and attends, unrotated, to those that are."""
+        A token behind the rotation table is not stored, and its attention is zeros."""
         q = self._append(x, pages, positions, None)
-        lengths = self._stored(lengths, pages)
+        limit = self._stored_limit(pages.shape[1])
+        if limit is not None:
+            lengths = lengths.masked_fill(positions >= limit, 0)
         return self._project(attend_decode(q, self.k_cache, self.v_cache, pages, lengths, scale=self.scale, workspace=workspace))
 
     def prompt(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor,
                lengths: torch.Tensor) -> torch.Tensor:
         """New tokens of several sequences, packed: x [T, d], token t of sequence seqs[t] (row of pages) at positions[t],
         sequence b's being rows starts[b] .. starts[b + 1] - 1 and the last of its lengths[b].  Rows of no sequence
-        (padding, at negative positions) give zeros.  The pages and the rotation table have to have room for all lengths[b]."""
+        (padding, at negative positions) and tokens behind the rotation table, which are not stored, give zeros; the pages
+        have to have room for lengths[b]."""
         q = self._append(x, pages, positions, seqs)
-        lengths = self._stored(lengths, pages)
         out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-        return self._project(attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out))
+        attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out)
+        limit = self._stored_limit(pages.shape[1])
+        if limit is not None:  # only these rows see what was not stored: the others' positions are in front of it
+            out.masked_fill_((positions >= limit)[:, None, None], 0)
+        return self._project(out)

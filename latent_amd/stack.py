@@ -15,7 +15,8 @@ caches (the new token's own key and value among them):
 and h_l takes x_l's place above.  Row b of a step is the next token of the
 sequence in slot b, at positions[b]; a slot whose position is negative is idle.
 A slot whose pages (or whose rotation table) end before its position keeps what
-is cached, stores nothing more and attends to what is there.
+is cached and stores nothing more; behind its pages it attends to what is there,
+behind the table its attention is zeros.
 `prompt` runs whole prompts, or chunks of them, through the same layers and
 leaves the slots ready to decode.
 
@@ -123,8 +124,8 @@ class DecodeStack:
         """New tokens of several sequences through every layer: x [N, d], packed; sequence b is rows starts[b] ..
         starts[b + 1] - 1 (int32 [B + 1], ascending, up to N) and goes on in slot slots[b] (int32 [B], different
         ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle (also
-        with no tokens: a slot that is to stay idle is left out).  The slots' pages, and the blocks' rotation tables, have
-        to have room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
+        with no tokens: a slot that is to stay idle is left out).  The slots' pages have to have
+        room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
         (padding) reach no cache and pass the experts alone."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")

@@ -196,8 +196,8 @@ def test_slots_without_room_store_nothing_more(gpu, parts):
 
 
 def test_slots_behind_their_rotation_table_read_what_is_stored(gpu, parts):
-    """A table that ends (at 20) before the pages do (at 32): its slot's later tokens are not stored, so the rows behind it, here NaN,
-    are not read; a step is append and attention over the 20 tokens that are there.  Eager and captured."""
+    """A table that ends (at 20) before the pages do (at 32): its slot's later tokens are not stored, and the rows behind it, here
+    NaN, reach nothing: those tokens' attention is zeros, the other slot's its own.  Eager and captured."""
     import torch
 
     layers, routers, ws, _ = parts
@@ -220,8 +220,9 @@ def test_slots_behind_their_rotation_table_read_what_is_stored(gpu, parts):
             qkv = (x0.bfloat16() @ a.w_qkv).view(2, HQ + 2 * HKV, D)
             q = gpu.kv_append(qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], a.k_cache.clone(), a.v_cache.clone(), s.pages, _ints([18 + i, 5 + i]),
                               q=qkv[:, :HQ], rope=a.rope, q_out=qkv[:, :HQ])
-            y = gpu.attend_decode(q, a.k_cache, a.v_cache, s.pages, _ints([min(19 + i, 20), 6 + i]))
+            y = gpu.attend_decode(q, a.k_cache, a.v_cache, s.pages, _ints([19 + i if i < 2 else 0, 6 + i]))
             assert torch.equal(s.h[0], x0 + y.view(2, -1) @ a.w_o), i
+            assert i < 2 or torch.equal(s.h[0][0], x0[0])
         assert s.positions.tolist() == [23, 10]
         for a in s.attention:
             for t in (a.k_cache, a.v_cache):
@@ -229,6 +230,39 @@ def test_slots_behind_their_rotation_table_read_what_is_stored(gpu, parts):
                 assert bool(torch.isfinite(rows[:20]).all()) and bool(torch.isnan(rows[20:]).all())
         # A prompt that passes the table reads no such row either.
         assert bool(torch.isfinite(s.prompt(x, _ints([0, 2, 23]), _ints([0, 1]))).all())
+
+
+def test_prompts_that_pass_the_rotation_table(gpu, parts):
+    """Tokens in the table see what they would in a longer one; those behind it get zeros; other sequences are their own."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    w_qkv, eye = parts[2][0][0], torch.eye(D_MODEL, dtype=torch.bfloat16, device="cuda")  # w_o: the attention as it is
+    order = torch.randperm(PAGES, generator=gen, device="cuda").int()
+    pages = torch.stack((order[:4], order[4:8]))
+    blocks = [gpu.Attention(w_qkv, eye, HQ, HKV, PAGES, PAGE, rope=gpu.rope_table(n, D)) for n in (41, 64)]
+    for a in blocks:
+        a.k_cache.fill_(float("nan")), a.v_cache.fill_(float("nan"))
+    first = [0, 0]
+    for new in ([30, 12], [25, 7]):  # positions 30 .. 54 and 12 .. 18: the first passes 41
+        T, starts = sum(new), _ints([0, new[0], sum(new)])
+        x = _x(gen, T)
+        pos = _ints([f + i for f, n in zip(first, new) for i in range(n)])
+        seqs, lengths = _ints([0] * new[0] + [1] * new[1]), _ints([f + n for f, n in zip(first, new)])
+        got, whole = (a.prompt(x, pages, pos, seqs, starts, lengths).view(T, HQ, D) for a in blocks)
+        b = blocks[1]
+        q = (x.bfloat16() @ w_qkv).view(T, HQ + 2 * HKV, D)[:, :HQ]
+        q = gpu.kv_append(q[:, :HKV], q[:, :HKV], b.k_cache.clone(), b.v_cache.clone(), pages, pos, seqs=seqs, q=q, rope=b.rope)
+        for i, (f, n) in enumerate(zip(first, new)):
+            at = torch.arange(f + n, device="cuda")
+            p, o = pages[i].long()[at // PAGE], at % PAGE
+            r, seen = int(starts[i]), min(n, 41 - f)
+            for y, m in ((got, seen), (whole, n)):
+                assert_attention(y[r:r + m], None, q[r:r + m], b.k_cache[p, o], b.v_cache[p, o], visible(n, f + n, True, "cuda")[:m], D ** -0.5)
+            assert bool((got[r + seen:r + n] == 0).all())
+        first = [f + n for f, n in zip(first, new)]
+    rows = blocks[0].k_cache[pages[0].long()].view(64, HKV, D)
+    assert bool(torch.isfinite(rows[:41]).all()) and bool(torch.isnan(rows[41:]).all())
 
 
 def test_blocks_that_share_a_cache_are_refused(gpu, parts):
