@@ -362,3 +362,39 @@ def test_blocks_without_sequences_or_tokens(gpu, parts):
     y = a.prompt(torch.ones((2, D_MODEL), device="cuda"), pages[:0], _ints([-1, -1]), _ints([0, 0]), _ints([0]), none)  # padding alone
     assert y.shape == (2, D_MODEL) and bool((y == 0).all())
     assert bool((a.k_cache == 0).all()) and bool((a.v_cache == 0).all())
+
+
+def test_prompts_between_replays_and_steps_on_another_stream(gpu, parts):
+    """A slot is filled, retired and filled anew between the replays of one graph; an eager stack on another stream agrees."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    eager, graph = _stack(gpu, parts, 3), _stack(gpu, parts, 3)
+    graph.capture()
+    side = torch.cuda.Stream()
+
+    def both(f):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            a = f(eager, eager.forward)
+        torch.cuda.current_stream().wait_stream(side)
+
+        def replay(x0):
+            graph.load(x0)
+            return graph.replay()
+
+        return a, f(graph, replay)
+
+    for starts, slots, n in (([0, 30], [1], 30), ([0, 5, 26], [2, 1], 26), ([0, 1], [0], 1), ([0, 40], [1], 40)):
+        if slots == [1] and n == 40:  # retired: its pages are another sequence's
+            eager.positions[1] = graph.positions[1] = -1
+        x, st, sl = _x(gen, n), _ints(starts), _ints(slots)
+        a, b = both(lambda s, step: s.prompt(x, st, sl))
+        assert torch.equal(a, b)
+        for _ in range(3):
+            x0 = _x(gen, 3)
+            a, b = both(lambda s, step: step(x0).clone())
+            assert torch.equal(a, b) and eager.positions.tolist() == graph.positions.tolist()
+    assert eager.positions.tolist() == [7, 43, 14]
+    for p, q in zip(eager.attention, graph.attention):
+        assert torch.equal(p.k_cache, q.k_cache) and torch.equal(p.v_cache, q.v_cache)
