@@ -537,6 +537,129 @@ int latent_attn_prompt_workspace_size(const latent_attn_prompt_args* args, size_
 /* Stream ordered; allocates nothing; calls that may overlap need workspaces of their own. */
 int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stream);
 
+/* ---- 8-bit caches --------------------------------------------------------- */
+/*
+ * A cache whose keys and values are codes of 8 bits, with one scale for each
+ * position and key/value head: a row x of D numbers is held as
+ *     m = max(max |x|, 2^-100),  scale = m / top,  code = x * (top / m)
+ * in fp32, the code rounded to the nearest (ties to even): whole numbers with
+ * top 127, or OCP e4m3 with top 448.  A row with an infinity or a NaN has a NaN
+ * as its scale and codes of zero: whoever reads it gets NaN.  The number held is
+ * code * scale.
+ *
+ * In the calls below, latent_kv_cache holds codes: strides count them and are
+ * multiples of 16; page_size is a multiple of 8, head_dim of 16.  Scales of a
+ * page's rows are adjacent; their other strides are multiples of 4 and their
+ * bases 16-byte aligned.  Everything else is as in the calls for 16-bit caches;
+ * queries, new keys and values and outputs have dtype (LATENT_F16 | LATENT_BF16).
+ */
+#define LATENT_CODE_INT8 0
+#define LATENT_CODE_E4M3 1
+typedef struct latent_kv_scales {
+  float* k; /* [n_pages][n_kv_head][page_size] */
+  float* v;
+  int64_t k_page_stride, k_head_stride;
+  int64_t v_page_stride, v_head_stride;
+  int32_t code; /* LATENT_CODE_* */
+} latent_kv_scales;
+
+/* latent_kv_append into an 8-bit cache: keys are rotated in fp32 (products and sums rounded one by one) and
+ * rounded once, to their codes.  Stream ordered; allocates nothing. */
+int latent_kv_append_q8(const latent_kv_append_args* args, const latent_kv_scales* scales, latent_stream_t stream);
+
+/*
+ * Reading a cache back: the key and value rows of token t, position positions[t]
+ * of sequence seqs[t] (t itself when seqs is NULL), rounded to dtype from an
+ * 8-bit cache, as they are from a 16-bit one of that type (scales NULL).  Rows
+ * whose position, sequence or page does not exist are zeros.
+ */
+typedef struct latent_kv_read_args {
+  latent_kv_cache cache;
+  void* k; /* [T][n_kv_head][D] */
+  void* v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int32_t* positions; /* [T] */
+  const int32_t* seqs;      /* [T] or NULL */
+  int64_t n_tokens;
+  int64_t n_kv_head;
+  int64_t head_dim;
+  int32_t dtype;
+} latent_kv_read_args;
+
+/* Stream ordered; allocates nothing. */
+int latent_kv_read(const latent_kv_read_args* args, const latent_kv_scales* scales, latent_stream_t stream);
+
+/* latent_attn_decode over an 8-bit cache.  Scores and probabilities take the scales in fp32; a probability times
+ * its value's scale is rounded once to dtype. */
+int latent_attn_decode_q8_workspace_size(const latent_attn_decode_args* args, size_t* bytes);
+int latent_attn_decode_q8(const latent_attn_decode_args* args, const latent_kv_scales* scales, latent_stream_t stream);
+
+/* latent_attn_prompt over an 8-bit cache (k NULL); its scratch is latent_attn_prompt_workspace_size(). */
+int latent_attn_prompt_q8(const latent_attn_prompt_args* args, const latent_kv_scales* scales, latent_stream_t stream);
+
+/* ---- one new token for each of a batch that shares its first positions ---- */
+/*
+ * latent_attn_decode for sequences whose first n_prefix pages are the same:
+ * positions 0 .. n_prefix * page_size - 1 of every sequence are in the pages that
+ * prefix names, which are read once for all of them; from there on positions
+ * are in the sequence's own row of decode.cache.pages, whose first n_prefix ids
+ * are not looked at.  lengths count all positions (one within the prefix sees
+ * that many of its keys).  One softmax over both.  scales NULL: a 16-bit cache.
+ */
+typedef struct latent_attn_shared_args {
+  latent_attn_decode_args decode;
+  const latent_kv_scales* scales; /* or NULL */
+  const int32_t* prefix;          /* [n_prefix] page ids */
+  int64_t n_prefix;               /* <= decode.cache.max_pages */
+} latent_attn_shared_args;
+
+int latent_attn_decode_shared_workspace_size(const latent_attn_shared_args* args, size_t* bytes);
+
+/* Stream ordered; allocates nothing; calls that may overlap need workspaces of their own. */
+int latent_attn_decode_shared(const latent_attn_shared_args* args, latent_stream_t stream);
+
+/* ---- between two blocks of a layer ---------------------------------------- */
+/*
+ * The residual stream after a block, and what the next block reads:
+ *
+ *     x' = x + scale * gate * post(y),   n = pre(x')
+ *
+ * row by row of d numbers; post and pre are norms
+ *     (v - mean(v)) / sqrt(var(v) + eps) * weight + bias   (LATENT_NORM_LAYER)
+ *     v / sqrt(mean(v^2) + eps) * weight + bias            (LATENT_NORM_RMS)
+ * or nothing (LATENT_NORM_NONE).  Statistics and sums are fp32; n is taken from x'
+ * before x' is rounded to its type.
+ */
+#define LATENT_NORM_NONE 0
+#define LATENT_NORM_RMS 1
+#define LATENT_NORM_LAYER 2
+typedef struct latent_norm {
+  int32_t kind;        /* LATENT_NORM_* */
+  float eps;           /* >= 0 */
+  const void* weight;  /* [d], or NULL: ones */
+  const void* bias;    /* [d], or NULL: zeros */
+  int32_t dtype;       /* of weight and bias */
+} latent_norm;
+
+typedef struct latent_residual_norm_args {
+  const void* x;    /* [T][d] of x_dtype */
+  const void* y;    /* [T][d] of y_dtype, or NULL: x' = x */
+  const void* gate; /* [T][d] of gate_dtype (row stride 0: one row for all), or NULL */
+  void* x_out;      /* [T][d] of x_dtype, may be x; or NULL: not written */
+  void* n_out;      /* [T][d] of n_dtype, or NULL: not written */
+  int64_t x_stride, y_stride, gate_stride, x_out_stride, n_out_stride; /* of rows, in elements */
+  int64_t n_tokens;
+  int64_t n_embd;   /* d <= 32768 */
+  int32_t x_dtype, y_dtype, gate_dtype, n_dtype; /* LATENT_F32 | LATENT_F16 | LATENT_BF16 */
+  float scale;
+  latent_norm post;
+  latent_norm pre;
+} latent_residual_norm_args;
+
+/* Stream ordered; allocates nothing. */
+int latent_residual_norm(const latent_residual_norm_args* args, latent_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

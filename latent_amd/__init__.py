@@ -4,6 +4,7 @@
     from latent_amd.runtime import load_pair, swiglu_expert # loader/latent_runtime.py
     from latent_amd import route, Router, DecodeStack        # GPU routing, stacked decode
     from latent_amd import kv_append, attend_decode, attend_prompt  # attention over a paged cache
+    from latent_amd import residual_norm, Norm               # between a layer's blocks
 
 The compute runs in `liblatent_hip.so` (hand-written HIP for gfx950, C ABI in
 include/latent_ffn.h); torch provides device memory and streams.  Importing
@@ -22,11 +23,15 @@ from ._lib import (  # noqa: F401
 from .attention import (  # noqa: F401
     Attention,
     attend_decode,
+    attend_decode_shared,
+    attend_decode_shared_workspace_size,
     attend_decode_workspace_size,
     attend_prompt,
     attend_prompt_paged,
     attend_prompt_workspace_size,
     kv_append,
+    kv_read,
+    kv_scales,
     rope_table,
 )
 from .moe import (  # noqa: F401
@@ -40,6 +45,7 @@ from .moe import (  # noqa: F401
     workspace_error,
     workspace_size,
 )
+from .norm import Norm, residual_norm  # noqa: F401
 from .router import Router, route  # noqa: F401
 from .stack import DecodeStack  # noqa: F401
 

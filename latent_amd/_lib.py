@@ -60,6 +60,14 @@ EXPORTED = (
     "latent_attn_decode",
     "latent_attn_prompt_workspace_size",
     "latent_attn_prompt",
+    "latent_kv_append_q8",
+    "latent_kv_read",
+    "latent_attn_decode_q8_workspace_size",
+    "latent_attn_decode_q8",
+    "latent_attn_prompt_q8",
+    "latent_attn_decode_shared_workspace_size",
+    "latent_attn_decode_shared",
+    "latent_residual_norm",
 )
 
 LATENT_NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -223,6 +231,65 @@ class LatentAttnPromptArgs(ctypes.Structure):
     ]
 
 
+LATENT_CODE_INT8 = 0
+LATENT_CODE_E4M3 = 1
+
+
+class LatentKvScales(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        *[(n, ctypes.c_int64) for n in ("k_page_stride", "k_head_stride", "v_page_stride", "v_head_stride")],
+        ("code", ctypes.c_int32),
+    ]
+
+
+class LatentKvReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", LatentKvCache),
+        *[(n, ctypes.c_void_p) for n in ("k", "v")],
+        *[(n, ctypes.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")],
+        *[(n, ctypes.c_void_p) for n in ("positions", "seqs")],
+        *[(n, ctypes.c_int64) for n in ("n_tokens", "n_kv_head", "head_dim")],
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class LatentAttnSharedArgs(ctypes.Structure):
+    _fields_ = [
+        ("decode", LatentAttnDecodeArgs),
+        ("scales", ctypes.POINTER(LatentKvScales)),
+        ("prefix", ctypes.c_void_p),
+        ("n_prefix", ctypes.c_int64),
+    ]
+
+
+LATENT_NORM_NONE = 0
+LATENT_NORM_RMS = 1
+LATENT_NORM_LAYER = 2
+
+
+class LatentNorm(ctypes.Structure):
+    _fields_ = [
+        ("kind", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class LatentResidualNormArgs(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("x", "y", "gate", "x_out", "n_out")],
+        *[(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "gate_stride", "x_out_stride", "n_out_stride", "n_tokens", "n_embd")],
+        *[(n, ctypes.c_int32) for n in ("x_dtype", "y_dtype", "gate_dtype", "n_dtype")],
+        ("scale", ctypes.c_float),
+        ("post", LatentNorm),
+        ("pre", LatentNorm),
+    ]
+
+
 class LatentError(RuntimeError):
     def __init__(self, status: int, what: str):
         super().__init__(f"{what}: {status_string(status)} ({status})")
@@ -289,6 +356,20 @@ def _load() -> ctypes.CDLL:
     ]
     lib.latent_attn_prompt.restype = ctypes.c_int
     lib.latent_attn_prompt.argtypes = [ctypes.POINTER(LatentAttnPromptArgs), ctypes.c_void_p]
+    size = ctypes.POINTER(ctypes.c_size_t)
+    for name, args in (
+        ("kv_append_q8", (ctypes.POINTER(LatentKvAppendArgs), ctypes.POINTER(LatentKvScales), ctypes.c_void_p)),
+        ("kv_read", (ctypes.POINTER(LatentKvReadArgs), ctypes.POINTER(LatentKvScales), ctypes.c_void_p)),
+        ("attn_decode_q8_workspace_size", (ctypes.POINTER(LatentAttnDecodeArgs), size)),
+        ("attn_decode_q8", (ctypes.POINTER(LatentAttnDecodeArgs), ctypes.POINTER(LatentKvScales), ctypes.c_void_p)),
+        ("attn_prompt_q8", (ctypes.POINTER(LatentAttnPromptArgs), ctypes.POINTER(LatentKvScales), ctypes.c_void_p)),
+        ("attn_decode_shared_workspace_size", (ctypes.POINTER(LatentAttnSharedArgs), size)),
+        ("attn_decode_shared", (ctypes.POINTER(LatentAttnSharedArgs), ctypes.c_void_p)),
+        ("residual_norm", (ctypes.POINTER(LatentResidualNormArgs), ctypes.c_void_p)),
+    ):
+        f = lib[f"latent_{name}"]
+        setattr(lib, f"latent_{name}", f)
+        f.restype, f.argtypes = ctypes.c_int, list(args)
     return lib
 
 

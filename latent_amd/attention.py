@@ -6,6 +6,9 @@
     attend_prompt        whole prompts, packed, causal
     attend_prompt_paged  the same with keys and values in the cache (a chunk of a
                          prompt behind the part that is cached)
+    attend_decode_shared one new token a sequence, the sequences' first positions
+                         being the same: read once for all of them
+    kv_read              rows of the cache, as 16-bit numbers
     Attention            projections, cache and these calls as one block, which
                          DecodeStack puts before each layer's experts
 
@@ -20,18 +23,29 @@ Scores, softmax and sums are fp32 (a row's sum of values times weights of at mos
 one has to stay finite there); probabilities are rounded to the element type
 for the product with the values, outputs once.  There is no backward pass.
 Lengths are cut off at what a row of the page table has room for, and at 0.
+
+Caches of int8 or float8_e4m3fn take half the bytes: a row x of D numbers is held
+as codes and one scale, f32 in k_scale and v_scale [pages, kv heads, page rows],
+
+    m = max(max |x|, 2^-100),  scale = m / top,  code = x (top / m)
+
+computed in fp32, the code rounded to nearest; top is 127 for int8, 448 for
+float8_e4m3fn.  A row with an infinity or a NaN is a NaN wherever it is read.
+There D and the strides are multiples of 16 (bytes; of the scales 4 elements, and
+a page's rows adjacent) and page rows of 8; kv_scales makes the scales.
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import LatentAttnDecodeArgs, LatentAttnPromptArgs, LatentError, LatentKvCache, check, lib
+from ._lib import (LatentAttnDecodeArgs, LatentAttnPromptArgs, LatentAttnSharedArgs, LatentError, LatentKvCache, LatentKvScales, check,
+                   lib)
 
 
 class _NoBinding:
@@ -50,9 +64,9 @@ try:
 except ImportError as e:
     _attend = _NoBinding(e)
 else:
-    _attend.entries(*(ctypes.cast(lib[f"latent_{n}"], ctypes.c_void_p).value for n in (
-        "kv_append", "attn_decode_workspace_size", "attn_decode", "attn_prompt_workspace_size", "attn_prompt")), LatentError)
+    _attend.entries({n: ctypes.cast(lib[n], ctypes.c_void_p).value for n in _lib.EXPORTED}, LatentError)
 
+_CODES = (torch.int8, torch.float8_e4m3fn)
 _DTYPE = (torch.float16, torch.bfloat16)
 
 
@@ -72,6 +86,13 @@ def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cu
     return torch.stack((angle.cos(), angle.sin()), 1).float().contiguous()
 
 
+def kv_scales(cache: torch.Tensor) -> torch.Tensor:
+    """Scales for a cache of int8 or float8_e4m3fn codes, zeros: f32 [pages, kv heads, page rows]."""
+    if cache.dim() != 4 or cache.dtype not in _CODES:
+        raise TypeError("expected a cache [pages, page rows, kv heads, D] of int8 or float8_e4m3fn")
+    return torch.zeros((cache.shape[0], cache.shape[2], cache.shape[1]), dtype=torch.float32, device=cache.device)
+
+
 def kv_append(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -85,6 +106,8 @@ def kv_append(
     interleaved: bool = False,
     q_out: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> Optional[torch.Tensor]:
     """Stores keys and values [T, kv heads, D] in the cache, keys rotated; returns q rotated (None without q).
 
@@ -95,12 +118,36 @@ def kv_append(
     A token whose position is negative or beyond the table is left out, q_out
     row and all; one whose sequence or page does not exist is not stored.
     Tokens of one call must not name the same cache row twice: what it holds
-    then is unspecified.
+    then is unspecified.  Into an 8-bit cache keys (rotated in fp32) and values go
+    as codes, their scales into k_scale and v_scale.
     """
     if stream is not None:
         with _on(stream, k):
-            return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
-    return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out)
+            return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out, k_scale, v_scale)
+    return _attend.kv_append(k, v, k_cache, v_cache, pages, positions, seqs, q, rope, interleaved, q_out, k_scale, v_scale)
+
+
+def kv_read(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    pages: torch.Tensor,
+    positions: torch.Tensor,
+    seqs: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    dtype: Optional[torch.dtype] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [T, kv heads, D] as the cache holds them: row t is position positions[t] (int32 [T]) of sequence seqs[t]
+    (int32 [T]; t itself when None).  From an 8-bit cache code times scale, rounded once to dtype (f16 or bf16); a 16-bit
+    cache's rows are copied, and dtype may only be its own.  Rows whose position, sequence or page does not exist are zeros."""
+    if dtype is not None and dtype not in _DTYPE:
+        raise TypeError("dtype must be float16 or bfloat16")
+    want = 0 if dtype is None else _lib.LATENT_F16 if dtype == torch.float16 else _lib.LATENT_BF16
+    if stream is not None:
+        with _on(stream, k_cache):
+            return _attend.kv_read(k_cache, v_cache, pages, positions, seqs, k_scale, v_scale, want)
+    return _attend.kv_read(k_cache, v_cache, pages, positions, seqs, k_scale, v_scale, want)
 
 
 def attend_decode(
@@ -114,6 +161,8 @@ def attend_decode(
     lse: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """One new token a sequence: q [B, heads, D] over the first lengths[b] (int32 [B]) positions of the cache.
 
@@ -125,16 +174,63 @@ def attend_decode(
     """
     if stream is not None:
         with _on(stream, q):
-            return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
-    return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace)
+            return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace, k_scale, v_scale)
+    return _attend.attend_decode(q, k_cache, v_cache, pages, lengths, scale, out, lse, workspace, k_scale, v_scale)
 
 
-def attend_decode_workspace_size(n_seq: int, n_head: int, n_kv_head: int, head_dim: int, max_pages: int, page_size: int) -> int:
-    """Workspace bytes of attend_decode for these sizes."""
+def attend_decode_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    prefix: torch.Tensor,
+    pages: torch.Tensor,
+    lengths: torch.Tensor,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """attend_decode for sequences whose first positions are the same: those are in the pages that prefix (int32 [P]) names,
+    P * page rows of them, and are read once for the whole batch.
+
+    pages is as in attend_decode, its rows' first P ids (P <= max_pages) those of
+    the prefix, which are not looked at here; lengths count all positions, the
+    prefix's too (a sequence that ends within it sees what its length says).
+    The result is that of attend_decode to rounding.  A workspace that is given
+    (attend_decode_shared_workspace_size bytes) must not serve calls that may
+    overlap.
+    """
+    if stream is not None:
+        with _on(stream, q):
+            return _attend.attend_decode_shared(q, k_cache, v_cache, prefix, pages, lengths, scale, out, lse, workspace, k_scale, v_scale)
+    return _attend.attend_decode_shared(q, k_cache, v_cache, prefix, pages, lengths, scale, out, lse, workspace, k_scale, v_scale)
+
+
+def attend_decode_workspace_size(n_seq: int, n_head: int, n_kv_head: int, head_dim: int, max_pages: int, page_size: int,
+                                 codes: bool = False) -> int:
+    """Workspace bytes of attend_decode for these sizes; codes: over an 8-bit cache."""
     cache = LatentKvCache(n_pages=1, page_size=page_size, n_seq=n_seq, max_pages=max_pages, pages_stride=max_pages)
     a = LatentAttnDecodeArgs(cache=cache, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, dtype=_lib.LATENT_BF16, scale=1.0)
     n = ctypes.c_size_t()
-    check(lib.latent_attn_decode_workspace_size(ctypes.byref(a), ctypes.byref(n)), "latent_attn_decode_workspace_size")
+    name = "latent_attn_decode_q8_workspace_size" if codes else "latent_attn_decode_workspace_size"
+    check(getattr(lib, name)(ctypes.byref(a), ctypes.byref(n)), name)
+    return int(n.value)
+
+
+def attend_decode_shared_workspace_size(n_seq: int, n_head: int, n_kv_head: int, head_dim: int, max_pages: int, page_size: int,
+                                        prefix_pages: int, codes: bool = False) -> int:
+    """Workspace bytes of attend_decode_shared for these sizes; codes: over an 8-bit cache."""
+    cache = LatentKvCache(n_pages=1, page_size=page_size, n_seq=n_seq, max_pages=max_pages, pages_stride=max_pages)
+    decode = LatentAttnDecodeArgs(cache=cache, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, dtype=_lib.LATENT_BF16, scale=1.0)
+    a = LatentAttnSharedArgs(decode=decode, n_prefix=prefix_pages)
+    if codes:
+        scales = LatentKvScales()
+        a.scales = ctypes.pointer(scales)
+    n = ctypes.c_size_t()
+    check(lib.latent_attn_decode_shared_workspace_size(ctypes.byref(a), ctypes.byref(n)), "latent_attn_decode_shared_workspace_size")
     return int(n.value)
 
 
@@ -191,14 +287,17 @@ def attend_prompt_paged(
     lse: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """attend_prompt with the keys and values of sequence b in the cache: its first lengths[b] (int32 [B])
     positions, the new tokens' own (appended before the call) the last of them.  lengths[b] is at most what a row of
     pages has room for: what is beyond is cut off, and the last query then stands at the last position that is left."""
     if stream is not None:
         with _on(stream, q):
-            return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
-    return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace)
+            return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace,
+                                               k_scale, v_scale)
+    return _attend.attend_prompt_paged(q, k_cache, v_cache, pages, lengths, starts, causal, scale, out, lse, workspace, k_scale, v_scale)
 
 
 class Attention:

@@ -26,8 +26,8 @@ from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
-SOURCES = ["chain32.hip", "codec.hip", "decode.hip", "expert.hip", "kvcache.hip", "moe.hip", "noalloc.hip", "prefill.hip",
-           "prompt.hip", "route.hip", "rows.hip", "stream.hip"]
+SOURCES = ["chain32.hip", "codec.hip", "decode.hip", "decode8.hip", "expert.hip", "kvcache.hip", "moe.hip", "noalloc.hip", "norm.hip",
+           "prefill.hip", "prompt.hip", "prompt8.hip", "route.hip", "rows.hip", "shared.hip", "stream.hip"]
 LIB = PKG / "liblatent_hip.so"
 BINDING = PKG / "_attend.so"
 ARCH = os.environ.get("LATENT_OFFLOAD_ARCH", "gfx950")

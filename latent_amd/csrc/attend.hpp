@@ -146,6 +146,68 @@ struct Cache {
   Divisor by_page;  // key / page_size
 };
 
+// ---- 8-bit caches --------------------------------------------------------------
+// The scales as the kernels address them (byte strides; rows of a page are adjacent).
+struct Scales {
+  const char* k;
+  const char* v;
+  int64_t k_page, k_head, v_page, v_head;
+};
+
+// Codes as operands: four of them in a dword become element pairs (0, 1) and (2, 3), both exactly.
+struct Int8 {
+  static constexpr float kTop = 127.f;
+  template <typename E, bool kHi>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    if constexpr (__is_same(E, F16)) {  // 1024 + 128 + x has x's bits for its last, in the type
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      const h2 up = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, kHi ? 0x04030402u : 0x04010400u));
+      return __builtin_bit_cast(uint32_t, up - h2{1152, 1152});
+    }
+    return pack2<E>(static_cast<float>(static_cast<int8_t>(w >> (kHi ? 16 : 0))), static_cast<float>(static_cast<int8_t>(w >> (kHi ? 24 : 8))));
+  }
+  // The same times a power of two (up to 2^15 for f16), rounded once.
+  template <typename E, bool kHi>
+  static __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {
+    if constexpr (__is_same(E, F16)) {  // in two steps, the first exact: a power below f16's least would be none
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      const float first = fmaxf(power, 0x1p-14f), second = power * (1.f / first);
+      const _Float16 a = static_cast<_Float16>(first), b = static_cast<_Float16>(second);
+      return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair<E, kHi>(w)) * h2{a, a} * h2{b, b});
+    }
+    return pack2<E>(value(w, kHi ? 2 : 0) * power, value(w, kHi ? 3 : 1) * power);
+  }
+  static __device__ __forceinline__ float value(uint32_t w, int i) { return static_cast<float>(static_cast<int8_t>(w >> (8 * i))); }
+  // Four numbers of magnitude up to kTop (and a rounding of the scaling) as codes.
+  static __device__ __forceinline__ uint32_t codes(const float x[4]) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (static_cast<uint32_t>(static_cast<int>(rintf(x[i]))) & 0xFFu) << (8 * i);
+    return w;
+  }
+};
+struct E4M3 {
+  static constexpr float kTop = 448.f;
+  template <typename E, bool kHi>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    if constexpr (__is_same(E, F16)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHi));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHi));
+  }
+  template <typename E, bool kHi>
+  static __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {
+    if constexpr (__is_same(E, F16)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, kHi));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, kHi));
+  }
+  static __device__ __forceinline__ float value(uint32_t w, int i) {
+    const uint32_t two = i >> 1 ? pair<BF16, true>(w) : pair<BF16, false>(w);
+    return i & 1 ? unpack_hi<BF16>(two) : unpack_lo<BF16>(two);
+  }
+  static __device__ __forceinline__ uint32_t codes(const float x[4]) {
+    const uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+  }
+};
+
 // ---- host ---------------------------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s <= int64_t{1} << 40; }
@@ -170,23 +232,39 @@ inline int check_cache(const latent_kv_cache& c) {
   return LATENT_OK;
 }
 
-inline Cache device_cache(const latent_kv_cache& c) {
+inline Cache device_cache(const latent_kv_cache& c, int64_t size = 2) {  // size: bytes of an element
   Cache d{};
   d.k = static_cast<const char*>(c.k);
   d.v = static_cast<const char*>(c.v);
   d.pages = c.pages;
   d.pages_stride = c.pages_stride;
-  d.k_page = c.k_page_stride * 2;
-  d.k_row = c.k_row_stride * 2;
-  d.k_head = c.k_head_stride * 2;
-  d.v_page = c.v_page_stride * 2;
-  d.v_row = c.v_row_stride * 2;
-  d.v_head = c.v_head_stride * 2;
+  d.k_page = c.k_page_stride * size;
+  d.k_row = c.k_row_stride * size;
+  d.k_head = c.k_head_stride * size;
+  d.v_page = c.v_page_stride * size;
+  d.v_row = c.v_row_stride * size;
+  d.v_head = c.v_head_stride * size;
   d.n_pages = static_cast<uint32_t>(c.n_pages);
   d.page_size = static_cast<uint32_t>(c.page_size);
   d.max_len = static_cast<uint32_t>(c.max_pages * c.page_size);
   d.by_page = divisor(c.page_size);
   return d;
+}
+
+// The cache and the scales of an 8-bit call: what it asks for beyond the 16-bit one's checks.
+inline int check_codes(const latent_kv_cache& c, const latent_kv_scales& s, int64_t head_dim) {
+  if (s.code != LATENT_CODE_INT8 && s.code != LATENT_CODE_E4M3) return LATENT_E_INVALID;
+  if (head_dim % 16 || c.page_size % 8) return LATENT_E_UNSUPPORTED;
+  for (int64_t x : {c.k_page_stride, c.k_row_stride, c.k_head_stride, c.v_page_stride, c.v_row_stride, c.v_head_stride})
+    if (x % 16) return LATENT_E_UNSUPPORTED;
+  for (int64_t x : {s.k_page_stride, s.k_head_stride, s.v_page_stride, s.v_head_stride})
+    if (x < 0 || x % 4 || x > int64_t{1} << 40) return LATENT_E_UNSUPPORTED;
+  return aligned16(s.k) && aligned16(s.v) ? LATENT_OK : LATENT_E_UNSUPPORTED;
+}
+
+inline Scales device_scales(const latent_kv_scales& s) {
+  return {reinterpret_cast<const char*>(s.k), reinterpret_cast<const char*>(s.v), s.k_page_stride * 4, s.k_head_stride * 4, s.v_page_stride * 4,
+          s.v_head_stride * 4};
 }
 
 }  // namespace attend

@@ -1,0 +1,70 @@
+"""Between two blocks of a layer: norms before and after a block, with its gate and the residual stream, in one pass.
+
+    residual_norm   x' = x + scale gate post(y),  n = pre(x')
+
+y is what a block gave for the stream x, n what the next block reads.  The
+reference leaves norms to llama.cpp's graph (README.md:111-113).
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .attention import _attend, _on
+
+_KINDS = {"rms": _lib.LATENT_NORM_RMS, "layer": _lib.LATENT_NORM_LAYER}
+_DTYPES = {torch.float32: _lib.LATENT_F32, torch.float16: _lib.LATENT_F16, torch.bfloat16: _lib.LATENT_BF16}
+
+
+class Norm:
+    """A norm of rows of d numbers: kind "rms", v / sqrt(mean(v^2) + eps) weight + bias, or "layer", the same of v - mean(v).
+
+    weight and bias: [d], f32, f16 or bf16 (both of one type), either None for ones and zeros.
+    """
+
+    __slots__ = ("weight", "bias", "kind", "eps", "_args")
+
+    def __init__(self, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, kind: str = "rms", eps: float = 1e-6):
+        if kind not in _KINDS:
+            raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+        if not 0.0 <= eps < float("inf"):
+            raise ValueError("eps must be finite and not negative")
+        self.weight, self.bias, self.kind, self.eps = weight, bias, kind, float(eps)
+        self._args = (_KINDS[kind], self.eps, weight, bias)
+
+
+def residual_norm(
+    x: torch.Tensor,
+    y: Optional[torch.Tensor] = None,
+    post: Optional[Norm] = None,
+    gate: Optional[torch.Tensor] = None,
+    scale: float = 1.0,
+    pre: Optional[Norm] = None,
+    dtype: Optional[torch.dtype] = None,
+    x_out: Optional[torch.Tensor] = None,
+    n_out: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """x' = x + scale gate post(y) and n = pre(x'), row by row: x, y [T, d] (d <= 32768), each f32, f16 or bf16.
+
+    gate: [d], [T, 1] or [T, d]; post, gate: None for none.  Without y, x' is x
+    itself; without pre there is no n (None).  x' has x's type, n dtype (default:
+    x's); x_out may be x.  Sums are fp32, and n is taken from x' before x' is
+    rounded to its type.  There is no backward pass.
+    """
+    for name, n in (("post", post), ("pre", pre)):
+        if n is not None and not isinstance(n, Norm):
+            raise TypeError(f"{name} must be a Norm")
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a tensor")
+    want = _DTYPES.get(x.dtype if dtype is None else dtype)
+    if want is None:
+        raise TypeError("x and dtype must be float32, float16 or bfloat16")
+    args = (x, y, None if post is None else post._args, gate, scale, None if pre is None else pre._args, want, x_out, n_out)
+    if stream is not None:
+        with _on(stream, x):
+            return _attend.residual_norm(*args)
+    return _attend.residual_norm(*args)
