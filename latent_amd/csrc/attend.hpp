@@ -33,10 +33,11 @@ struct F16 {
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
   }
-  // c plus the dword's two elements.
-  static __device__ __forceinline__ float add2(uint32_t w, float c) {
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(T2, w), __builtin_bit_cast(T2, 0x3C003C00u), c, false);
+  // c plus the products of two dwords' elements; plus the dword's two elements.
+  static __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(T2, a), __builtin_bit_cast(T2, b), c, false);
   }
+  static __device__ __forceinline__ float add2(uint32_t w, float c) { return dot2(w, 0x3C003C00u, c); }
 };
 struct BF16 {
   static constexpr float kLift = 0.f;
@@ -49,9 +50,10 @@ struct BF16 {
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ float add2(uint32_t w, float c) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(T2, w), __builtin_bit_cast(T2, 0x3F803F80u), c, false);
+  static __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(T2, a), __builtin_bit_cast(T2, b), c, false);
   }
+  static __device__ __forceinline__ float add2(uint32_t w, float c) { return dot2(w, 0x3F803F80u, c); }
 };
 
 // Two fp32 values rounded to nearest even, the first in the low half.

@@ -6,8 +6,8 @@
 // Codes are loaded a tile ahead into registers (a tile's keys and values are 64 bytes a thread at D = 128), made exact
 // elements of the queries' type there and written to the LDS buffer that the waves do not read: each code is
 // converted once for the four waves, and the operands' reads are the 16-bit kernel's.  The scales of a tile's keys lie in LDS beside
-// it, in fp32: a key's multiplies its score; of a value's the power of two goes into the elements, exactly, and the rest multiplies
-// the probability, which is rounded to the element type after it.
+// it.  A value's scale is a power of two, which its elements take exactly, times a rest from 1 to 2, which its weight takes: as the
+// logarithm added to the score (the product with the key's scale becomes a multiply-add), so that one exponential gives p[j] rest[j].
 #include "prompt.hpp"
 
 namespace latent {
@@ -21,20 +21,19 @@ struct Split {
     const uint32_t e = __float_as_uint(s) & 0x7F800000u;
     return e >= 0x7F000000u ? 1.f : __uint_as_float(e);  // a NaN's codes are zeros; 0 for 0
   }
-  static __device__ __forceinline__ float rest(float s) {
+  static __device__ __forceinline__ float rest(float s) {  // of a finite one
     const float p = power(s);
     return p == 0.f ? 1.f : s * __uint_as_float(0x7F000000u - __float_as_uint(p));
   }
 };
 
-// Sixteen codes as 32 bytes of elements, times a power of two (kScaled).
+// Eight codes as 16 bytes of elements, times a power of two (kScaled).
 template <typename E, typename Q, bool kScaled>
-__device__ __forceinline__ void convert16(const u32x4& w, float power, u32x4 (&out)[2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i >> 1][2 * (i & 1)] = kScaled ? Q::template scaled_pair<E, false>(w[i], power) : Q::template pair<E, false>(w[i]);
-    out[i >> 1][2 * (i & 1) + 1] = kScaled ? Q::template scaled_pair<E, true>(w[i], power) : Q::template pair<E, true>(w[i]);
-  }
+__device__ __forceinline__ u32x4 convert8(uint32_t a, uint32_t b, float power) {
+  if constexpr (kScaled)
+    return {Q::template scaled_pair<E, false>(a, power), Q::template scaled_pair<E, true>(a, power), Q::template scaled_pair<E, false>(b, power),
+            Q::template scaled_pair<E, true>(b, power)};
+  return {Q::template pair<E, false>(a), Q::template pair<E, true>(a), Q::template pair<E, false>(b), Q::template pair<E, true>(b)};
 }
 
 template <int kDP, int kKeys>
@@ -43,10 +42,16 @@ struct Shared8 {
   static constexpr uint32_t kTile = kKeys * kDP * 2;
   alignas(512) u32x4 k[2][kKeys * kC];
   u32x4 v[2][kKeys * kC];
-  float ks[2][kKeys], vs[2][kKeys], over[2][kKeys];  // a score's factor, base 2; a probability's, and one over it
+  float ks[2][kKeys], add[2][kKeys];  // a score's factor, base 2, and what is added: the log2 of its value's rest
+  u32x4 over[2][kKeys / 4];           // one over the rests of four keys as two summands of the element type: (0, 1), (2, 3), then the smaller
   static __device__ __forceinline__ int k_turn(int key) { return kC >= 16 ? key & 15 : (key >> 1) & 7; }
   static __device__ __forceinline__ int v_turn(int key) { return kC >= 16 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 };
+
+template <typename T>
+__device__ __forceinline__ T load_global(uint64_t at) {  // which a pointer that may be the zeros' would not be seen to be
+  return *reinterpret_cast<const __attribute__((address_space(1))) T*>(at);
+}
 
 template <typename E, typename Q, int kDP, int kKeys, bool kLse, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(PromptParams p) {
@@ -54,7 +59,6 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
   constexpr int kKeyBlocks = kKeys / 32, kSteps = kDP / 16, kBlocks = kDP / 32;
   constexpr int kPieces = kDP / 16, kLoads = kKeys * kPieces / kThreads, kRowsLoad = kThreads / kPieces;  // 16 codes a piece
   constexpr uint32_t kRow = kDP * 2;
-  constexpr float kRoom = E::kLift != 0.f ? 1.f : 0.f;  // for Split's rest, below two: probabilities are taken so much (log2) lower
   __shared__ S sm;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
   const int hk = blockIdx.x % p.Hkv;
@@ -62,10 +66,6 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
   if (it.b < 0) return;
   const int tile = it.tile, n = it.n, m = it.m;
   const int32_t* pages = p.cache.pages + it.b * p.cache.pages_stride;
-  const char* kbase = p.cache.k + hk * p.cache.k_head;
-  const char* vbase = p.cache.v + hk * p.cache.v_head;
-  const char* kscale = p.scales.k + hk * p.scales.k_head;
-  const char* vscale = p.scales.v + hk * p.scales.v_head;
 
   // This lane's row, and how many keys it sees.
   const int all = n * p.G, row0 = tile * kRowsTile, w0 = row0 + wave * kRowsWave;
@@ -100,61 +100,86 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
     }
   }
 
-  // Loading: load i of a thread is piece tid % kPieces of row tid / kPieces + i kRowsLoad, and lane l of the first two waves has the
-  // key's and the value's scale of row l.  Pages are looked up a tile before.
-  const int piece = tid % kPieces, lrow = tid / kPieces;
+  // Loading: load i of a thread is piece tid % kPieces of row tid / kPieces + i kRowsLoad.  Eight rows from a multiple of eight share a page, so
+  // a wave's rows of a load lie behind one wave-uniform address (two at D = 64), and what a lane adds to it never changes; every lane's
+  // address worked out by itself was half of the vector instructions that this kernel has beyond the 16-bit one's.  Lane g holds the
+  // page of rows 8 g .. and where in it they are, looked up a tile before; lane l of the first wave takes the scales of row l.
+  constexpr int kRowsHere = kWave / kPieces, kGroups = kRowsHere > 8 ? 2 : 1;
+  const int piece = tid % kPieces, lrow = tid / kPieces, in_group = lrow & 7;
+  const int64_t lane_k = in_group * p.cache.k_row + 16 * piece, lane_v = in_group * p.cache.v_row + 16 * piece;
+  const uint64_t kbase = reinterpret_cast<uint64_t>(p.cache.k + hk * p.cache.k_head), vbase = reinterpret_cast<uint64_t>(p.cache.v + hk * p.cache.v_head);
+  const uint64_t kscale = reinterpret_cast<uint64_t>(p.scales.k + hk * p.scales.k_head), vscale = reinterpret_cast<uint64_t>(p.scales.v + hk * p.scales.v_head);
+  const bool exact = p.D == kDP;
   u32x4 raw_k[kLoads], raw_v[kLoads];
-  float scale_v[kLoads], raw_scale = 0.f;
-  uint32_t piece_page[kLoads], lane_page;
+  float scale_v[kLoads], raw_ks = 0.f, raw_vs = 0.f;
+  uint32_t group_page, group_off;
   uint64_t exists_next = 0;
   auto find_pages = [&](int kt) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int key = kt + lrow + i * kRowsLoad;
-      piece_page[i] = key < stop ? static_cast<uint32_t>(pages[p.cache.by_page.of(key)]) : 0xFFFFFFFFu;
-    }
-    const int key = kt + lane;
-    lane_page = lane < kKeys && key < stop ? static_cast<uint32_t>(pages[p.cache.by_page.of(key)]) : 0xFFFFFFFFu;
+    const int key = kt + 8 * lane;
+    const uint32_t slot = p.cache.by_page.of(key);
+    group_page = lane < kKeys / 8 && key < stop ? static_cast<uint32_t>(pages[slot]) : 0xFFFFFFFFu;
+    group_off = key - slot * p.cache.page_size;
   };
   auto load = [&](int kt) {
+    const uint64_t zero = reinterpret_cast<uint64_t>(kZeroRow);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t key = kt + lrow + i * kRowsLoad, off = key - p.cache.by_page.of(key) * p.cache.page_size, page = piece_page[i];
-      const bool ok = page < p.cache.n_pages && 16 * piece < p.D;
-      const char* zero = reinterpret_cast<const char*>(kZeroRow);
-      raw_k[i] = *reinterpret_cast<const u32x4*>(ok ? kbase + page * p.cache.k_page + off * p.cache.k_row + 16 * piece : zero);
-      raw_v[i] = *reinterpret_cast<const u32x4*>(ok ? vbase + page * p.cache.v_page + off * p.cache.v_row + 16 * piece : zero);
-      scale_v[i] = *reinterpret_cast<const float*>(ok ? vscale + page * p.scales.v_page + 4 * off : zero);
+      uint64_t k[kGroups], v[kGroups], sc[kGroups];
+      bool there[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const int g = (wave * kRowsHere + i * kRowsLoad) / 8 + j;
+        const uint32_t page = __builtin_amdgcn_readlane(group_page, g), off = __builtin_amdgcn_readlane(group_off, g);
+        k[j] = kbase + page * p.cache.k_page + off * p.cache.k_row;
+        v[j] = vbase + page * p.cache.v_page + off * p.cache.v_row;
+        sc[j] = vscale + page * p.scales.v_page + 4 * off;
+        there[j] = page < p.cache.n_pages;
+      }
+      const bool second = kGroups > 1 && lane >= 32;
+      uint64_t ka = (second ? k[kGroups - 1] : k[0]) + lane_k, va = (second ? v[kGroups - 1] : v[0]) + lane_v;
+      uint64_t sa = (second ? sc[kGroups - 1] : sc[0]) + 4 * in_group;
+      if (!(exact && there[0] && there[kGroups - 1] && kt + kKeys <= stop)) {
+        const bool ok = (second ? there[kGroups - 1] : there[0]) && 16 * piece < p.D && kt + lrow + i * kRowsLoad < stop;
+        ka = ok ? ka : zero;
+        va = ok ? va : zero;
+        sa = ok ? sa : zero;
+      }
+      raw_k[i] = load_global<u32x4>(ka);
+      raw_v[i] = load_global<u32x4>(va);
+      scale_v[i] = load_global<float>(sa);
     }
-    const bool there = lane_page < p.cache.n_pages;
+    const uint32_t page = __builtin_amdgcn_ds_bpermute(4 * (lane >> 3), group_page);
+    const bool there = page < p.cache.n_pages && lane < kKeys && kt + lane < stop;
     exists_next = __ballot(there);
-    if (wave < 2) {
-      const uint32_t key = kt + lane, off = key - p.cache.by_page.of(key) * p.cache.page_size;
-      const char* at = wave == 0 ? kscale + lane_page * p.scales.k_page : vscale + lane_page * p.scales.v_page;
-      raw_scale = *reinterpret_cast<const float*>(there ? at + 4 * off : reinterpret_cast<const char*>(kZeroRow));
+    if (wave == 0) {
+      const uint32_t off = __builtin_amdgcn_ds_bpermute(4 * (lane >> 3), group_off) + (lane & 7);
+      raw_ks = load_global<float>(there ? kscale + page * p.scales.k_page + 4 * off : zero);
+      raw_vs = load_global<float>(there ? vscale + page * p.scales.v_page + 4 * off : zero);
     }
   };
   const uint32_t lds_k = lds_addr(sm.k[0][0]), lds_v = lds_addr(sm.v[0][0]);
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = lrow + i * kRowsLoad;
-      u32x4 x[2];
-      convert16<E, Q, false>(raw_k[i], 1.f, x);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) lds_st(lds_k + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::k_turn(row)), x[j]);
-      convert16<E, Q, true>(raw_v[i], Split::power(scale_v[i]), x);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) lds_st(lds_v + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::v_turn(row)), x[j]);
-    }
-    if (lane < kKeys && wave < 2) {
-      if (wave == 0) {
-        sm.ks[buf][lane] = raw_scale * p.scale_log2;
-      } else {
-        const float f = Split::rest(raw_scale);
-        sm.vs[buf][lane] = f;
-        sm.over[buf][lane] = f > 0.f ? 1.f / f : 0.f;
-      }
+  // What was loaded into buffer buf, a half of a piece at a time: keys' halves, then values'.
+  constexpr int kHalves = 4 * kLoads;
+  auto store_half = [&](int buf, int half) {
+    const int i = half / 2 % kLoads, j = half % 2, row = lrow + i * kRowsLoad;
+    if (half < kHalves / 2)
+      lds_st(lds_k + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::k_turn(row)), convert8<E, Q, false>(raw_k[i][2 * j], raw_k[i][2 * j + 1], 1.f));
+    else
+      lds_st(lds_v + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::v_turn(row)),
+             convert8<E, Q, true>(raw_v[i][2 * j], raw_v[i][2 * j + 1], Split::power(scale_v[i])));
+  };
+  auto store_scales = [&](int buf) {
+    if (wave == 0 && lane < kKeys) {
+      // A value row that is a NaN makes the scores of its key one: the rows that see the key take it, and no others.
+      const bool is = raw_vs == raw_vs;
+      const float f = is ? Split::rest(raw_vs) : 1.f, over = 1.f / f;
+      sm.ks[buf][lane] = is ? raw_ks * p.scale_log2 : raw_vs;
+      sm.add[buf][lane] = __log2f(f);
+      const uint32_t hi = pack2<E>(over, 0.f);
+      const uint32_t lo = pack2<E>(over - unpack_lo<E>(hi), 0.f);
+      uint16_t* to = reinterpret_cast<uint16_t*>(&sm.over[buf][lane >> 2]) + (lane & 3);
+      to[0] = static_cast<uint16_t>(hi);
+      to[4] = static_cast<uint16_t>(lo);
     }
   };
 
@@ -166,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
   f32x16 acc[kBlocks];
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) acc[i] = f32x16{};
-  // top: what the exponentials are taken against, within kSlack of the maximum.  The row is divided by the sum of the probabilities that the
+  // top: what the exponentials are taken against, within kSlack of the largest weight.  The row is divided by the sum of the probabilities that the
   // rounded weights of its values stand for, so that their roundings cancel as far as they agree (a row of one key is that key's
   // value); the log-sum-exp, where it is asked for, takes the sum of the unrounded ones.
   float top = -INFINITY, sum = 0.f, full = 0.f;
@@ -177,32 +202,53 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
     constexpr uint64_t kAll = ~uint64_t{0} >> (64 - kKeys);
     lds_barrier();  // this tile is there, the other buffer read
     const uint64_t exists = exists_now & kAll;
-    if (kt + kKeys < stop) {
-      store(buf ^ 1);
+    const bool more = kt + kKeys < stop, busy = kt < wave_any;
+    auto follow = [&] {  // what the stores left free takes the tile after the next
+      store_scales(buf ^ 1);
       exists_now = exists_next;
       if (kt + 2 * kKeys < stop) {
         load(kt + 2 * kKeys);
         find_pages(kt + 3 * kKeys);
       }
+    };
+    if (!busy) {  // the other waves' rows see this tile
+      if (more) {
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) store_half(buf ^ 1, half);
+        follow();
+      }
+      return;
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (kt >= wave_any) return;  // the other waves' rows see this tile
+    // Scores; the next tile's codes are converted in the products' shadow (two prompts of 4099 behind up to 8000: 1031 us before them).
     f32x16 s[kKeyBlocks] = {};
+    auto scores = [&](auto converting) {
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st)
+      for (int st = 0; st < kSteps; ++st) {
 #pragma unroll
-      for (int blk = 0; blk < kKeyBlocks; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
-    const uint32_t ks_at = lds_addr(sm.ks[buf][0]) + 16 * h, vs_at = lds_addr(sm.vs[buf][0]) + 16 * h, over_at = lds_addr(sm.over[buf][0]) + 16 * h;
+        for (int blk = 0; blk < kKeyBlocks; ++blk) s[blk] = E::mfma32(lds_ld<u32x4>((kat ^ (32 * st)) + buf * S::kTile + blk * 32 * kRow), q[st], s[blk]);
+        if constexpr (decltype(converting)::value) {
+          if (st < kHalves) store_half(buf ^ 1, st);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if constexpr (decltype(converting)::value) {
+#pragma unroll
+        for (int half = kSteps; half < kHalves; ++half) store_half(buf ^ 1, half);
+        follow();
+      }
+    };
+    more ? scores(std::true_type{}) : scores(std::false_type{});
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t ks_at = lds_addr(sm.ks[buf][0]) + 16 * h, add_at = lds_addr(sm.add[buf][0]) + 16 * h, over_at = lds_addr(sm.over[buf][0]) + 16 * h;
 #pragma unroll
     for (int blk = 0; blk < kKeyBlocks; ++blk)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 f = lds_ld<f32x4>(ks_at + 4 * (32 * blk + 8 * g));
+        const f32x4 f = lds_ld<f32x4>(ks_at + 4 * (32 * blk + 8 * g)), add = lds_ld<f32x4>(add_at + 4 * (32 * blk + 8 * g));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[blk][4 * g + r] *= f[r];
+        for (int r = 0; r < 4; ++r) s[blk][4 * g + r] = __builtin_fmaf(s[blk][4 * g + r], f[r], add[r]);
       }
-    const bool part_seen = !(kt + kKeys <= wave_all && exists == kAll);
-    if (part_seen) {
+    if (!(kt + kKeys <= wave_all && exists == kAll)) {
       asm volatile("");  // keeps this a branch: most tiles need none of it
       const int left = vis - kt - 4 * h;  // of the keys from this lane's first on
       const uint64_t there = exists >> (4 * h);
@@ -229,28 +275,24 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) acc[i] *= f;
     }
-    const float mm = finite_max(top) - Scale<E>::kUp + kRoom;
+    const float mm = finite_max(top) - Scale<E>::kUp;
     float part[2] = {sum, 0.f}, part_full[2] = {full, 0.f};
     u32x4 prob[2 * kKeyBlocks];
 #pragma unroll
     for (int kk = 0; kk < 2 * kKeyBlocks; ++kk)
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const f32x4 f = lds_ld<f32x4>(vs_at + 4 * (16 * kk + 8 * g)), over = lds_ld<f32x4>(over_at + 4 * (16 * kk + 8 * g));
+        const u32x4 over = lds_ld<u32x4>(over_at + 4 * (16 * kk + 8 * g));
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          float x[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            x[r] = exp2_fast(s[kk >> 1][8 * (kk & 1) + 4 * g + 2 * a + r] - mm);
-            if constexpr (kLse) part_full[r] += x[r];
-            // A row that does not see a key takes nothing of it, whatever its scale (a NaN, for a row that held one).
-            x[r] = part_seen && x[r] == 0.f ? 0.f : x[r] * f[2 * a + r];
-          }
-          const uint32_t w = pack2<E>(x[0], x[1]);
+          const float x = exp2_fast(s[kk >> 1][8 * (kk & 1) + 4 * g + 2 * a] - mm), y = exp2_fast(s[kk >> 1][8 * (kk & 1) + 4 * g + 2 * a + 1] - mm);
+          const uint32_t w = pack2<E>(x, y);
           prob[kk][2 * g + a] = w;
-          part[0] += unpack_lo<E>(w) * over[2 * a];
-          part[1] += unpack_hi<E>(w) * over[2 * a + 1];
+          part[a] = E::dot2(w, over[2 + a], E::dot2(w, over[a], part[a]));
+          if constexpr (kLse) {
+            part_full[0] += x * (unpack_lo<E>(over[a]) + unpack_lo<E>(over[2 + a]));
+            part_full[1] += y * (unpack_hi<E>(over[a]) + unpack_hi<E>(over[2 + a]));
+          }
         }
       }
     sum = part[0] + part[1];
@@ -269,7 +311,9 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
     find_pages(begin);
     load(begin);
     find_pages(begin + kKeys);
-    store(0);
+#pragma unroll
+    for (int half = 0; half < kHalves; ++half) store_half(0, half);
+    store_scales(0);
     exists_now = exists_next;
     if (begin + kKeys < stop) {
       load(begin + kKeys);
@@ -283,7 +327,6 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
 
   sum = op_over(sum, 32, 64, OpAdd{});
   if constexpr (kLse) full = op_over(full, 32, 64, OpAdd{});
-  top += kRoom;  // as if taken against that, with the 16-bit kernel's factor
   const int row = w0 + l32;
   if (row >= all) return;
   if (!whole_unit) {
