@@ -45,7 +45,7 @@ from .moe import (  # noqa: F401
     workspace_error,
     workspace_size,
 )
-from .norm import Norm, residual_norm  # noqa: F401
+from .norm import BlockNorm, Norm, residual_norm  # noqa: F401
 from .router import Router, route  # noqa: F401
 from .stack import DecodeStack  # noqa: F401
 

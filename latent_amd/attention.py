@@ -305,12 +305,15 @@ class Attention:
 
     w_qkv [d, (n_head + 2 n_kv_head) D] holds the columns of q, k and v one after
     the other, w_o [n_head D, d] the output projection; both f16 or bf16, the
-    cache's type too.  The cache has n_pages pages of page_size positions; which
-    sequence owns which page is the caller's, in the page table of each call.
+    cache's type too unless cache_dtype asks for codes of 8 bits (int8,
+    float8_e4m3fn; D then a multiple of 16, page_size of 8).  The cache has n_pages
+    pages of page_size positions; which sequence owns which page is the caller's,
+    in the page table of each call.
     """
 
     def __init__(self, w_qkv: torch.Tensor, w_o: torch.Tensor, n_head: int, n_kv_head: int, n_pages: int, page_size: int,
-                 rope: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None):
+                 rope: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None,
+                 cache_dtype: Optional[torch.dtype] = None):
         if w_qkv.dim() != 2 or w_o.dim() != 2 or w_qkv.dtype not in _DTYPE or w_o.dtype != w_qkv.dtype or not w_qkv.is_cuda:
             raise TypeError("w_qkv and w_o must be CUDA f16 or bf16 matrices")
         if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head or w_o.shape[0] % n_head:
@@ -324,7 +327,17 @@ class Attention:
         self.n_head, self.n_kv_head, self.head_dim = int(n_head), int(n_kv_head), int(D)
         self.rope, self.interleaved, self.scale = rope, bool(interleaved), scale
         shape = (int(n_pages), int(page_size), self.n_kv_head, self.head_dim)
-        self.k_cache, self.v_cache = (torch.zeros(shape, dtype=w_qkv.dtype, device=w_qkv.device) for _ in range(2))
+        dtype = w_qkv.dtype if cache_dtype is None else cache_dtype
+        self.k_scale = self.v_scale = None
+        if dtype in _CODES:
+            if D % 16 or shape[1] % 8:
+                raise ValueError(f"8-bit caches take heads of a multiple of 16 dimensions and pages of a multiple of 8 positions, not {D} and {shape[1]}")
+            self.k_cache, self.v_cache = (torch.zeros(shape, dtype=torch.uint8, device=w_qkv.device).view(dtype) for _ in range(2))
+            self.k_scale, self.v_scale = kv_scales(self.k_cache), kv_scales(self.v_cache)
+        elif dtype == w_qkv.dtype:
+            self.k_cache, self.v_cache = (torch.zeros(shape, dtype=dtype, device=w_qkv.device) for _ in range(2))
+        else:
+            raise TypeError(f"the cache holds {w_qkv.dtype}, as the weights do, int8 or float8_e4m3fn, not {dtype}")
 
     @property
     def n_embd(self) -> int:
@@ -335,7 +348,7 @@ class Attention:
         qkv = (x.to(self.w_qkv.dtype) @ self.w_qkv).view(x.shape[0], H + 2 * K, self.head_dim)
         q = qkv[:, :H]
         return kv_append(qkv[:, H:H + K], qkv[:, H + K:], self.k_cache, self.v_cache, pages, positions, seqs=seqs,
-                         q=q, rope=self.rope, interleaved=self.interleaved, q_out=q)
+                         q=q, rope=self.rope, interleaved=self.interleaved, q_out=q, k_scale=self.k_scale, v_scale=self.v_scale)
 
     def _stored_limit(self, max_pages: int) -> Optional[int]:
         """How many positions tokens are stored at, where the rotation table ends before a page table row of max_pages does
@@ -348,15 +361,25 @@ class Attention:
     def _project(self, a: torch.Tensor) -> torch.Tensor:
         return a.view(a.shape[0], self.w_o.shape[0]) @ self.w_o
 
+    def workspace_size(self, n_seq: int, max_pages: int, prefix_pages: int = 0) -> int:
+        """Workspace bytes of decode for so many sequences and page table columns, prefix_pages of them shared."""
+        args = (n_seq, self.n_head, self.n_kv_head, self.head_dim, max_pages, self.k_cache.shape[1])
+        codes = self.k_scale is not None
+        return attend_decode_shared_workspace_size(*args, prefix_pages, codes) if prefix_pages else attend_decode_workspace_size(*args, codes)
+
     def decode(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
-               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+               workspace: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One new token a sequence: x [B, d] at positions [B]; lengths [B] count it.  Returns [B, d] in the weights' type.
-        A token behind the rotation table is not stored, and its attention is zeros."""
+        A token behind the rotation table is not stored, and its attention is zeros.  prefix (int32 [P]): the first P pages
+        of every row of pages, which attend_decode_shared then reads once."""
         q = self._append(x, pages, positions, None)
         limit = self._stored_limit(pages.shape[1])
         if limit is not None:
             lengths = lengths.masked_fill(positions >= limit, 0)
-        return self._project(attend_decode(q, self.k_cache, self.v_cache, pages, lengths, scale=self.scale, workspace=workspace))
+        more = dict(scale=self.scale, workspace=workspace, k_scale=self.k_scale, v_scale=self.v_scale)
+        if prefix is not None:
+            return self._project(attend_decode_shared(q, self.k_cache, self.v_cache, prefix, pages, lengths, **more))
+        return self._project(attend_decode(q, self.k_cache, self.v_cache, pages, lengths, **more))
 
     def prompt(self, x: torch.Tensor, pages: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor,
                lengths: torch.Tensor) -> torch.Tensor:
@@ -366,7 +389,8 @@ class Attention:
         have to have room for lengths[b]."""
         q = self._append(x, pages, positions, seqs)
         out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-        attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out)
+        attend_prompt_paged(q, self.k_cache, self.v_cache, pages, lengths, starts, scale=self.scale, out=out, k_scale=self.k_scale,
+                            v_scale=self.v_scale)
         limit = self._stored_limit(pages.shape[1])
         if limit is not None:  # only these rows see what was not stored: the others' positions are in front of it
             out.masked_fill_((positions >= limit)[:, None, None], 0)

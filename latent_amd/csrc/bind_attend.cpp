@@ -575,6 +575,9 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         norm(args[2], &a.post, held, "post");
         if (args[3] != Py_None) {
           const Tensor& g = tensor(args[3], "gate");
+          TORCH_CHECK_VALUE(g.dim() == 1 ? g.size(0) == d : g.dim() == 2 && g.size(0) == T && (g.size(1) == d || g.size(1) == 1), "gate must be [", d, "], [",
+                            T, ", 1] or [", T, ", ", d, "]");
+          check_norm_grad(g);
           gate = rows(g.dim() == 1 ? g.unsqueeze(0).expand({T, d}) : g.dim() == 2 && g.size(1) == 1 && d != 1 ? g.expand({g.size(0), d}) : g, "gate", T, d, dev);
           a.gate_dtype = any_dtype(gate, "gate");
           a.gate = gate.data_ptr(), a.gate_stride = row_stride(gate);

@@ -60,10 +60,10 @@ extern "C" int latent_attn_decode_shared(const latent_attn_shared_args* args, la
   if (a.cache.n_pages > 0 && (!a.cache.k || !a.cache.v || !a.cache.pages || (args->scales && (!args->scales->k || !args->scales->v))))
     return LATENT_E_INVALID;
   if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.workspace)) return LATENT_E_UNSUPPORTED;
-  if (!a.workspace || a.workspace_bytes < l.all()) return LATENT_E_WORKSPACE;
   for (int64_t s : {a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride})
     if (!stride_ok(s)) return LATENT_E_UNSUPPORTED;
   if ((a.n_head > 1 && !a.out_head_stride) || (a.cache.n_seq > 1 && !a.out_token_stride)) return LATENT_E_INVALID;
+  if (!a.workspace || a.workspace_bytes < l.all()) return LATENT_E_WORKSPACE;
   char* ws = static_cast<char*>(a.workspace);
   const Prior prior{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + l.out)};
   void* scratch = ws + l.out + l.lse;  // one half's, then the other's

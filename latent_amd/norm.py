@@ -36,6 +36,27 @@ class Norm:
         self._args = (_KINDS[kind], self.eps, weight, bias)
 
 
+class BlockNorm:
+    """A block's place in the residual stream: it reads pre(x) and adds scale gate post(y); each of pre, post, gate may be None.
+
+    gate: [d] (one for all tokens).  DecodeStack takes one for each of its blocks.
+    """
+
+    __slots__ = ("pre", "post", "gate", "scale")
+
+    def __init__(self, pre: Optional[Norm] = None, post: Optional[Norm] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0):
+        if gate is not None and gate.dim() != 1:
+            raise ValueError("gate must be [d]")
+        self.pre, self.post, self.gate, self.scale = pre, post, gate, float(scale)
+
+    def add(self, x: torch.Tensor, y: torch.Tensor, following: "Optional[BlockNorm]", dtype: torch.dtype,
+            x_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The stream after the block gave y for it, and what the following block reads (the stream itself, where it has no pre)."""
+        x, n = residual_norm(x, y, post=self.post, gate=self.gate, scale=self.scale, pre=None if following is None else following.pre,
+                             dtype=dtype, x_out=x_out)
+        return x, x if n is None else n
+
+
 def residual_norm(
     x: torch.Tensor,
     y: Optional[torch.Tensor] = None,

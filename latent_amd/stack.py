@@ -18,7 +18,14 @@ A slot whose pages (or whose rotation table) end before its position keeps what
 is cached and stores nothing more; behind its pages it attends to what is there,
 behind the table its attention is zeros.
 `prompt` runs whole prompts, or chunks of them, through the same layers and
-leaves the slots ready to decode.
+leaves the slots ready to decode.  After `share` the slots' first pages are the
+same ones, which a step reads once for all slots (latent_attn_decode_shared).
+
+With norms each block, attention and experts alike, reads pre(x) and adds
+scale gate post(y) to the stream, in one launch with the next block's pre
+(latent_residual_norm):
+
+    x' = x + s g post(Block(pre(x)))
 
 The residual stream stays fp32 on the device; the stack's own buffers are
 allocated once (an attention block's projections come from torch's allocator,
@@ -35,14 +42,17 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from .attention import Attention, attend_decode_workspace_size
+from .attention import Attention
 from .moe import StackedLayer, moe_forward, workspace_size
+from .norm import BlockNorm, residual_norm
 from .router import Router, route
 
 
 class DecodeStack:
     def __init__(self, layers: Sequence[StackedLayer], routers: Sequence[Router], n_tokens: int,
-                 attention: Optional[Sequence[Attention]] = None, max_pages: int = 0):
+                 attention: Optional[Sequence[Attention]] = None, max_pages: int = 0,
+                 norms: Optional[Sequence[BlockNorm]] = None):
+        """norms: one for each block in their order, a layer's attention (if there is any) and its experts."""
         if len(layers) != len(routers) or not layers:
             raise ValueError("need one router per layer")
         d, k = layers[0].d, routers[0].k
@@ -70,6 +80,14 @@ class DecodeStack:
             self._add_attention(list(attention), int(max_pages), dev)
         elif max_pages:
             raise ValueError("max_pages without attention")
+        self.norms: Optional[List[BlockNorm]] = None
+        if norms is not None:
+            self.norms = list(norms)
+            per = 1 if self.attention is None else 2
+            if len(self.norms) != per * n:
+                raise ValueError(f"need {per * n} norms, one for each block")
+            if not all(isinstance(b, BlockNorm) for b in self.norms):
+                raise TypeError("norms must be BlockNorm")
 
     def _add_attention(self, blocks: List[Attention], max_pages: int, dev: torch.device) -> None:
         if len(blocks) != len(self.layers):
@@ -88,9 +106,30 @@ class DecodeStack:
         self.positions = torch.full((self.T,), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros((self.T,), dtype=torch.int32, device=dev)
         self.h = [torch.empty((self.T, self.d), dtype=torch.float32, device=dev) for _ in blocks]
-        need = max(attend_decode_workspace_size(self.T, a.n_head, a.n_kv_head, a.head_dim, max_pages, a.k_cache.shape[1])
-                   for a in blocks)
-        self.attention_workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=dev)
+        self.prefix: Optional[torch.Tensor] = None
+        self._attention_scratch()
+
+    def _attention_scratch(self) -> None:
+        prefix = 0 if self.prefix is None else self.prefix.numel()
+        need = max(a.workspace_size(self.T, self.pages.shape[1], prefix) for a in self.attention)
+        self.attention_workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=self.pages.device)
+
+    def share(self, prefix: Optional[torch.Tensor]) -> None:
+        """From now on the first P pages of every slot are those that prefix (int32 [P], P <= max_pages) names, of every
+        layer's cache alike: pages[:, :P] is set to them, and steps read them once for all slots.  Whoever fills them does so
+        through a slot, by `prompt`; a slot that goes on behind them has positions >= P times the page size.  None:
+        slots have pages of their own again.  A captured graph is dropped."""
+        if self.attention is None:
+            raise RuntimeError("this stack has no attention")
+        if prefix is not None:
+            if prefix.dtype != torch.int32 or prefix.dim() != 1 or prefix.device != self.pages.device or prefix.numel() > self.pages.shape[1]:
+                raise ValueError(f"prefix must be int32 [pages] on {self.pages.device}, at most {self.pages.shape[1]} of them")
+            prefix = prefix.clone() if prefix.numel() else None
+        self.graph = None
+        self.prefix = prefix
+        if prefix is not None:
+            self.pages[:, :prefix.numel()] = prefix
+        self._attention_scratch()
 
     @property
     def output(self) -> torch.Tensor:
@@ -99,16 +138,45 @@ class DecodeStack:
     def _body(self) -> None:
         if self.attention is not None:
             torch.add(self.positions, 1, out=self.lengths)
-        for l, (L, r) in enumerate(zip(self.layers, self.routers)):
-            x = self.x[l]
-            if self.attention is not None:
-                a = self.attention[l].decode(x, self.pages, self.positions, self.lengths, workspace=self.attention_workspace)
-                x = torch.add(x, a, out=self.h[l])
-            r(x, ids=self.ids[l], weights=self.w[l], logits_out=self.logits[l])
-            moe_forward(x, self.ids[l], self.w[l], L, out=self.y[l], workspace=self.workspace)
-            torch.add(x, self.y[l], out=self.x[l + 1])
+        if self.norms is not None:
+            self._normed_layers()
+        else:
+            for l, (L, r) in enumerate(zip(self.layers, self.routers)):
+                x = self.x[l]
+                if self.attention is not None:
+                    x = torch.add(x, self._attend(l, x), out=self.h[l])
+                torch.add(x, self._experts(l, x), out=self.x[l + 1])
         if self.attention is not None:
             self.positions.add_(self.positions >= 0)
+
+    def _attend(self, l: int, x: torch.Tensor) -> torch.Tensor:
+        return self.attention[l].decode(x, self.pages, self.positions, self.lengths, workspace=self.attention_workspace, prefix=self.prefix)
+
+    def _experts(self, l: int, x: torch.Tensor) -> torch.Tensor:
+        self.routers[l](x, ids=self.ids[l], weights=self.w[l], logits_out=self.logits[l])
+        return moe_forward(x, self.ids[l], self.w[l], self.layers[l], out=self.y[l], workspace=self.workspace)
+
+    def _reads(self, i: int) -> torch.dtype:
+        """What block i reads: an attention block its weights' type, experts the stream's."""
+        return torch.float32 if self.attention is None or i % 2 else self.attention[i // 2].w_qkv.dtype
+
+    def _first(self, x: torch.Tensor) -> torch.Tensor:
+        pre = self.norms[0].pre
+        return x if pre is None else residual_norm(x, pre=pre, dtype=self._reads(0))[1]
+
+    def _add(self, i: int, x: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None):
+        last = i + 1 == len(self.norms)
+        return self.norms[i].add(x, y, None if last else self.norms[i + 1], torch.float32 if last else self._reads(i + 1), x_out=out)
+
+    def _normed_layers(self) -> None:
+        x = self.x[0]
+        n, i = self._first(x), 0
+        for l in range(len(self.layers)):
+            if self.attention is not None:
+                x, n = self._add(i, x, self._attend(l, n), out=self.h[l])
+                i += 1
+            x, n = self._add(i, x, self._experts(l, n), out=self.x[l + 1])
+            i += 1
 
     def load(self, x0: torch.Tensor) -> None:
         self.x[0].copy_(x0)
@@ -126,7 +194,7 @@ class DecodeStack:
         ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle (also
         with no tokens: a slot that is to stay idle is left out).  The slots' pages have to have
         room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
-        (padding) reach no cache and pass the experts alone."""
+        (padding) reach no cache, their attention is zeros, and they pass the experts."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")
         if x.dim() != 2 or x.shape[1] != self.d:
@@ -148,11 +216,14 @@ class DecodeStack:
             positions = torch.where((row >= starts[0]) & (row < starts[-1]), positions, -1)
         if N:
             ws = torch.zeros((max(max(workspace_size(L, N, self.k) for L in self.layers), 256),), dtype=torch.uint8, device=x.device)
-            for L, r, a in zip(self.layers, self.routers, self.attention):
-                if B:
-                    x = x + a.prompt(x, pages, positions, seqs, starts, lengths)
-                ids, w = route(r.k, x=x, router=r.weight, drop=r.drop, drop_param=r.drop_param)
-                x = x + moe_forward(x, ids, w, L, workspace=ws)
+            n = x if self.norms is None else self._first(x)
+            for l, (L, r, a) in enumerate(zip(self.layers, self.routers, self.attention)):
+                if B or self.norms is not None:
+                    y = a.prompt(n, pages, positions, seqs, starts, lengths) if B else x.new_zeros(x.shape)
+                    x, n = (x + y,) * 2 if self.norms is None else self._add(2 * l, x, y)
+                ids, w = route(r.k, x=n, router=r.weight, drop=r.drop, drop_param=r.drop_param)
+                y = moe_forward(n, ids, w, L, workspace=ws)
+                x, n = (x + y,) * 2 if self.norms is None else self._add(2 * l + 1, x, y)
         else:
             x = x.clone()
         self.positions.index_copy_(0, at, lengths)
