@@ -168,14 +168,17 @@ struct Int8 {
     }
     return pack2<E>(static_cast<float>(static_cast<int8_t>(w >> (kHi ? 16 : 0))), static_cast<float>(static_cast<int8_t>(w >> (kHi ? 24 : 8))));
   }
-  // The same times a power of two (up to 2^15 for f16), rounded once.
-  template <typename E, bool kHi>
+  // The same times a power of two (up to 2^15 for f16), rounded once.  kSmall: for f16, the power may be below its normal numbers.
+  template <typename E, bool kHi, bool kSmall>
   static __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {
-    if constexpr (__is_same(E, F16)) {  // in two steps, the first exact: a power below f16's least would be none
+    if constexpr (__is_same(E, F16)) {
       typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-      const float first = fmaxf(power, 0x1p-14f), second = power * (1.f / first);
-      const _Float16 a = static_cast<_Float16>(first), b = static_cast<_Float16>(second);
-      return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair<E, kHi>(w)) * h2{a, a} * h2{b, b});
+      const h2 x = __builtin_bit_cast(h2, pair<E, kHi>(w));
+      const _Float16 a = static_cast<_Float16>(kSmall ? fmaxf(power, 0x1p-14f) : power);
+      if constexpr (!kSmall) return __builtin_bit_cast(uint32_t, x * h2{a, a});
+      // In two steps, the first exact: a power below the type's least would be none.
+      const _Float16 b = static_cast<_Float16>(power < 0x1p-14f ? power * 0x1p14f : 1.f);
+      return __builtin_bit_cast(uint32_t, x * h2{a, a} * h2{b, b});
     }
     return pack2<E>(value(w, kHi ? 2 : 0) * power, value(w, kHi ? 3 : 1) * power);
   }
@@ -195,8 +198,8 @@ struct E4M3 {
     if constexpr (__is_same(E, F16)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHi));
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHi));
   }
-  template <typename E, bool kHi>
-  static __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {
+  template <typename E, bool kHi, bool kSmall>
+  static __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {  // in the conversion, whatever the power
     if constexpr (__is_same(E, F16)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, kHi));
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, kHi));
   }

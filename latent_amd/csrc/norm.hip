@@ -213,7 +213,8 @@ extern "C" int latent_residual_norm(const latent_residual_norm_args* args, laten
   if (!(a.scale > -INFINITY) || !(a.scale < INFINITY)) return LATENT_E_INVALID;
   if (!a.y && (a.gate || a.post.kind != LATENT_NORM_NONE)) return LATENT_E_INVALID;
   if (!a.n_out && a.pre.kind != LATENT_NORM_NONE) return LATENT_E_INVALID;
-  if (a.n_embd > kMaxNormDim || a.n_tokens > INT32_MAX) return LATENT_E_UNSUPPORTED;
+  // A launch's threads are counted in 32 bits: a wave, four or sixteen a row.
+  if (a.n_embd > kMaxNormDim || a.n_tokens > (int64_t{1} << 32) / (a.n_embd <= 1024 ? 64 : a.n_embd <= 8192 ? 256 : 1024) - 8) return LATENT_E_UNSUPPORTED;
   constexpr int64_t kFar = int64_t{1} << 40;
   for (int64_t s : {a.x_stride, a.y_stride, a.gate_stride, a.x_out_stride, a.n_out_stride})
     if (s < 0 || s > kFar) return LATENT_E_UNSUPPORTED;

@@ -6,7 +6,7 @@
 // Codes are loaded a tile ahead into registers (a tile's keys and values are 64 bytes a thread at D = 128), made exact
 // elements of the queries' type there and written to the LDS buffer that the waves do not read: each code is
 // converted once for the four waves, and the operands' reads are the 16-bit kernel's.  The scales of a tile's keys lie in LDS beside
-// it.  A value's scale is a power of two, which its elements take exactly, times a rest from 1 to 2, which its weight takes: as the
+// it.  A value's scale is a power of two, which its elements take exactly, times a rest, which its weight takes: as the
 // logarithm added to the score (the product with the key's scale becomes a multiply-add), so that one exponential gives p[j] rest[j].
 #include "prompt.hpp"
 
@@ -14,12 +14,16 @@ namespace latent {
 namespace attend {
 namespace {
 
-// A value row of scale s: its codes times `power`, of two, are the elements; the probability takes `rest`, from 1 to 2.  s = power
-// rest.  The elements are exact but for f16's below its normal numbers, which are as near as f16 has them.
+// A value row of scale s: its codes times `power`, of two, are the elements; the probability takes `rest`.  s = power rest.  f16: rest
+// is from 1 to 2, so that a weight has the bits of its probability, whatever the values' size; the elements are exact but for those
+// below the type's normal numbers, which are as near as it has them.  bf16 has fp32's range: the weight takes all of a scale that is
+// not tiny.
+template <typename E>
 struct Split {
   static __device__ __forceinline__ float power(float s) {
     const uint32_t e = __float_as_uint(s) & 0x7F800000u;
-    return e >= 0x7F000000u ? 1.f : __uint_as_float(e);  // a NaN's codes are zeros; 0 for 0
+    if (e >= 0x7F000000u || (E::kLift == 0.f && e >= 0x21800000u)) return 1.f;  // a NaN's codes are zeros; 2^-60
+    return __uint_as_float(e);  // 0 for 0
   }
   static __device__ __forceinline__ float rest(float s) {  // of a finite one
     const float p = power(s);
@@ -27,13 +31,25 @@ struct Split {
   }
 };
 
-// Eight codes as 16 bytes of elements, times a power of two (kScaled).
-template <typename E, typename Q, bool kScaled>
-__device__ __forceinline__ u32x4 convert8(uint32_t a, uint32_t b, float power) {
-  if constexpr (kScaled)
-    return {Q::template scaled_pair<E, false>(a, power), Q::template scaled_pair<E, true>(a, power), Q::template scaled_pair<E, false>(b, power),
-            Q::template scaled_pair<E, true>(b, power)};
+// Eight codes as 16 bytes of elements, and times a power of two.
+template <typename E, typename Q>
+__device__ __forceinline__ u32x4 convert8(uint32_t a, uint32_t b) {
   return {Q::template pair<E, false>(a), Q::template pair<E, true>(a), Q::template pair<E, false>(b), Q::template pair<E, true>(b)};
+}
+template <typename E, typename Q, bool kSmall>
+__device__ __forceinline__ u32x4 convert8(uint32_t a, uint32_t b, float power) {
+  return {Q::template scaled_pair<E, false, kSmall>(a, power), Q::template scaled_pair<E, true, kSmall>(a, power),
+          Q::template scaled_pair<E, false, kSmall>(b, power), Q::template scaled_pair<E, true, kSmall>(b, power)};
+}
+template <typename E, typename Q>
+__device__ __forceinline__ u32x4 convert_value8(uint32_t a, uint32_t b, float power) {
+  if constexpr (__is_same(Q, E4M3)) return convert8<E, Q, true>(a, b, power);
+  if constexpr (E::kLift == 0.f) {
+    if (__all(power == 1.f)) return convert8<E, Q>(a, b);
+  } else {
+    if (__all(power >= 0x1p-14f)) return convert8<E, Q, false>(a, b, power);
+  }
+  return convert8<E, Q, true>(a, b, power);
 }
 
 template <int kDP, int kKeys>
@@ -43,6 +59,7 @@ struct Shared8 {
   alignas(512) u32x4 k[2][kKeys * kC];
   u32x4 v[2][kKeys * kC];
   float ks[2][kKeys], add[2][kKeys];  // a score's factor, base 2, and what is added: the log2 of its value's rest
+  float whole[2][kKeys];              // one over the rest; the log-sum-exp takes it unrounded
   u32x4 over[2][kKeys / 4];           // one over the rests of four keys as two summands of the element type: (0, 1), (2, 3), then the smaller
   static __device__ __forceinline__ int k_turn(int key) { return kC >= 16 ? key & 15 : (key >> 1) & 7; }
   static __device__ __forceinline__ int v_turn(int key) { return kC >= 16 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
@@ -163,18 +180,19 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
   auto store_half = [&](int buf, int half) {
     const int i = half / 2 % kLoads, j = half % 2, row = lrow + i * kRowsLoad;
     if (half < kHalves / 2)
-      lds_st(lds_k + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::k_turn(row)), convert8<E, Q, false>(raw_k[i][2 * j], raw_k[i][2 * j + 1], 1.f));
+      lds_st(lds_k + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::k_turn(row)), convert8<E, Q>(raw_k[i][2 * j], raw_k[i][2 * j + 1]));
     else
       lds_st(lds_v + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::v_turn(row)),
-             convert8<E, Q, true>(raw_v[i][2 * j], raw_v[i][2 * j + 1], Split::power(scale_v[i])));
+             convert_value8<E, Q>(raw_v[i][2 * j], raw_v[i][2 * j + 1], Split<E>::power(scale_v[i])));
   };
   auto store_scales = [&](int buf) {
     if (wave == 0 && lane < kKeys) {
       // A value row that is a NaN makes the scores of its key one: the rows that see the key take it, and no others.
       const bool is = raw_vs == raw_vs;
-      const float f = is ? Split::rest(raw_vs) : 1.f, over = 1.f / f;
+      const float f = is ? Split<E>::rest(raw_vs) : 1.f, over = 1.f / f;
       sm.ks[buf][lane] = is ? raw_ks * p.scale_log2 : raw_vs;
       sm.add[buf][lane] = __log2f(f);
+      if constexpr (kLse) sm.whole[buf][lane] = over;
       const uint32_t hi = pack2<E>(over, 0.f);
       const uint32_t lo = pack2<E>(over - unpack_lo<E>(hi), 0.f);
       uint16_t* to = reinterpret_cast<uint16_t*>(&sm.over[buf][lane >> 2]) + (lane & 3);
@@ -283,6 +301,8 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const u32x4 over = lds_ld<u32x4>(over_at + 4 * (16 * kk + 8 * g));
+        f32x4 whole{};
+        if constexpr (kLse) whole = lds_ld<f32x4>(lds_addr(sm.whole[buf][0]) + 16 * h + 4 * (16 * kk + 8 * g));
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
           const float x = exp2_fast(s[kk >> 1][8 * (kk & 1) + 4 * g + 2 * a] - mm), y = exp2_fast(s[kk >> 1][8 * (kk & 1) + 4 * g + 2 * a + 1] - mm);
@@ -290,8 +310,8 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
           prob[kk][2 * g + a] = w;
           part[a] = E::dot2(w, over[2 + a], E::dot2(w, over[a], part[a]));
           if constexpr (kLse) {
-            part_full[0] += x * (unpack_lo<E>(over[a]) + unpack_lo<E>(over[2 + a]));
-            part_full[1] += y * (unpack_hi<E>(over[a]) + unpack_hi<E>(over[2 + a]));
+            part_full[0] += x * whole[2 * a];
+            part_full[1] += y * whole[2 * a + 1];
           }
         }
       }

@@ -137,7 +137,7 @@ def test_shared_prefix_sizes(L):
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(n_tokens=-1), "INVALID"), (dict(n_embd=-1), "INVALID"), (dict(n_embd=32769), "UNSUPPORTED"), (dict(x=None), "INVALID"), (dict(x_dtype=3), "INVALID"),
+    (dict(n_tokens=-1), "INVALID"), (dict(n_embd=-1), "INVALID"), (dict(n_embd=32769), "UNSUPPORTED"), (dict(n_tokens=1 << 27), "UNSUPPORTED"), (dict(n_tokens=1 << 22, n_embd=16384), "UNSUPPORTED"), (dict(x=None), "INVALID"), (dict(x_dtype=3), "INVALID"),
     (dict(n_dtype=7), "INVALID"), (dict(gate_dtype=-1), "INVALID"), (dict(scale=float("nan")), "INVALID"), (dict(scale=float("inf")), "INVALID"), (dict(y=None), "INVALID"),
     (dict(y=None, gate=None), "INVALID"), (dict(n_out=None), "INVALID"), (dict(x_out_stride=63), "INVALID"), (dict(n_out_stride=0), "INVALID"), (dict(x_stride=-1), "UNSUPPORTED"),
     (dict(post=dict(kind=3)), "INVALID"), (dict(post=dict(kind=0)), "INVALID"), (dict(pre=dict(eps=-1.0)), "INVALID"), (dict(pre=dict(eps=float("nan"))), "INVALID"),
