@@ -79,21 +79,14 @@ int launch16(const latent_attn_decode_args& a, const Plan& pl, const DecodeParam
 }  // namespace
 
 size_t after_workspace(const latent_attn_decode_args& a, int64_t n_prefix, bool codes) {
-  const latent_attn_decode_args own = behind(a, n_prefix);
-  const Plan pl = codes ? plan_for(own, 1, kMaxGroups8) : plan_for(own);
-  return pl.ml_bytes + pl.acc_bytes + pl.unit_bytes;
+  return plan_after(behind(a, n_prefix), codes ? 1 : 2, codes ? kMaxGroups8 : kMaxGroups).all();
 }
 
 int launch_after16(const latent_attn_decode_args& a, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s) {
-  latent_attn_decode_args own = behind(a, n_prefix);
-  own.workspace = workspace;
-  own.workspace_bytes = SIZE_MAX;
-  const Plan pl = plan_for(own);
+  const After w = plan_after(behind(a, n_prefix), 2, kMaxGroups);
   DecodeParams p{};
-  const int st = decode_params(own, 2, pl, &p);
-  if (st != LATENT_OK) return st;
-  set_prior(a, n_prefix, prior, &p);
-  return launch16<true>(own, pl, p, s);
+  const int st = after_params(a, n_prefix, 2, w, prior, workspace, &p);
+  return st == LATENT_OK ? launch16<true>(a, w.plan, p, s) : st;
 }
 
 }  // namespace attend

@@ -39,10 +39,11 @@ struct DecodeParams {
   float* part_acc;
   int2* unit_parts;
   Scales scales;  // of an 8-bit cache
-  // What each row has seen already, elsewhere (kAfter): its normalised outputs [B][Hq][D] and the log2 of its sum of exponentials
-  // [B][Hq].  Its keys here begin at position `ahead`, which cache.pages and cache.max_len leave out.
-  const float* prior_out;
-  const float* prior_lse;
+  // kAfter: keys here begin at position `ahead`, which cache.pages and cache.max_len leave out; what rows have seen before it is `prior`.  Every
+  // unit leaves its rows, those that one workgroup has whole by themselves: sums [units][rows][2] and rows [units][rows][D].
+  Prior prior;
+  float* unit_ml;
+  float* unit_acc;
   uint32_t ahead;
 };
 
@@ -288,37 +289,15 @@ struct Stream {
   }
 };
 
-// The output of a row: sums x and l under the maximum m (times 2^kLift), joined with what the row has seen before (kAfter).
-template <typename E, bool kAfter>
+// The output of a row: sums x and l under the maximum m (times 2^kLift).
+template <typename E>
 __device__ __forceinline__ void finish(const DecodeParams& p, uint32_t b, uint32_t h, uint32_t c, const f32x4 (&x)[2], float m, float l) {
-  const int64_t row = static_cast<int64_t>(b) * p.Hq + h;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   u32x4 y;
-  float lse;
-  if constexpr (kAfter) {
-    const float z = p.prior_lse[row];
-    const f32x4* was = reinterpret_cast<const f32x4*>(p.prior_out + row * p.D + 8 * c);
-    const f32x4 w0 = was[0], w1 = was[1];
-    const float top = fmaxf(m, z), t = finite_max(top), f = exp2_fast(m - t - E::kLift), g = z == -INFINITY ? 0.f : exp2_fast(z - t);
-    const float sum = l == 0.f ? g : l * f + g;  // l is 0 where this row has no key here, its m -inf
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    const float fx = l == 0.f ? 0.f : f * inv, gx = g * inv;
-    const f32x4 a = x[0] * fx, d = x[1] * fx;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 &s = i < 2 ? a : d, &w = i < 2 ? w0 : w1;
-      const int e = 2 * (i & 1);
-      // A row that has seen nothing elsewhere has zeros there.
-      y[i] = pack2<E>(s[e] + w[e] * gx, s[e + 1] + w[e + 1] * gx);
-    }
-    lse = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
-  } else {
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-#pragma unroll
-    for (int a = 0; a < 4; ++a) y[a] = pack2<E>(x[a >> 1][2 * (a & 1)] * inv, x[a >> 1][2 * (a & 1) + 1] * inv);
-    lse = l == 0.f ? -INFINITY : (m - E::kLift + __log2f(l)) * kLn2;
-  }
+  for (int a = 0; a < 4; ++a) y[a] = pack2<E>(x[a >> 1][2 * (a & 1)] * inv, x[a >> 1][2 * (a & 1) + 1] * inv);
   *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = y;
-  if (p.lse && c == 0) p.lse[row] = lse;
+  if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = l == 0.f ? -INFINITY : (m - E::kLift + __log2f(l)) * kLn2;
 }
 
 template <typename S, bool kAfter>
@@ -331,17 +310,12 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int n16 = lane & 15, kq = lane >> 4;
 
-  // Zeros (or what was seen before) for query heads [h0, h1) of sequence b, which has no keys.
+  // Zeros for query heads [h0, h1) of sequence b, which has no keys.
   auto write_zeros = [&](uint32_t b, uint32_t h0, uint32_t h1) {
     for (uint32_t i = threadIdx.x; i < (h1 - h0) * (p.D / 8); i += kThreads) {
       const uint32_t h = h0 + i / (p.D / 8), c = i % (p.D / 8);
-      if constexpr (kAfter) {
-        const f32x4 none[2] = {};
-        finish<E, true>(p, b, h, c, none, -INFINITY, 0.f);
-      } else {
-        *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = u32x4{0, 0, 0, 0};
-        if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = -INFINITY;
-      }
+      *reinterpret_cast<u32x4*>(p.out + b * p.o_token + h * p.o_head + 16 * c) = u32x4{0, 0, 0, 0};
+      if (p.lse && c == 0) p.lse[static_cast<int64_t>(b) * p.Hq + h] = -INFINITY;
     }
   };
   uint32_t cur, last, per = 1, b, u, tile = 0, len, nt;
@@ -352,6 +326,8 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
     nt = tiles_of(len);
     cur = 0;
     last = nt;
+    if (kAfter && threadIdx.x == 0) p.unit_parts[blockIdx.x] = int2{0, len != 0};
+    if (kAfter && len == 0) return;
     if (len == 0) {
       const uint32_t h0 = u / p.chunks * p.G + (u % p.chunks) * p.rows;
       write_zeros(b, h0, min(h0 + p.rows, (u / p.chunks + 1) * p.G));
@@ -361,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
     // Sequences without keys: units of no parts, rows of zeros.
     for (b = blockIdx.x; b < p.B; b += gridDim.x) {
       if (length_of<kAfter>(p, b) != 0) continue;
-      write_zeros(b, 0, p.Hq);
+      if (!kAfter) write_zeros(b, 0, p.Hq);
       for (uint32_t i = threadIdx.x; i < p.U; i += kThreads) p.unit_parts[b * p.U + i] = int2{0, 0};
     }
     const Span span = find_span<kAfter>(p, lane);
@@ -441,15 +417,18 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
           x[0] += *reinterpret_cast<const f32x4*>(&rows[w][row - mt0 * 16][8 * c]);
           x[1] += *reinterpret_cast<const f32x4*>(&rows[w][row - mt0 * 16][8 * c + 4]);
         }
-        if (whole) {
-          finish<E, kAfter>(p, b, hk * p.G + r0 + row, c, x, m, l);
+        if (!kAfter && whole) {
+          finish<E>(p, b, hk * p.G + r0 + row, c, x, m, l);
         } else {
-          f32x4* dst = reinterpret_cast<f32x4*>(p.part_acc + (part + row) * p.D + 8 * c);
+          const bool alone = kAfter && whole;
+          const int64_t at = (alone ? (static_cast<int64_t>(b) * p.U + u) * p.rows : part) + row;
+          f32x4* dst = reinterpret_cast<f32x4*>((alone ? p.unit_acc : p.part_acc) + at * p.D + 8 * c);
+          float* ml = (alone ? p.unit_ml : p.part_ml) + 2 * at;
           dst[0] = x[0];
           dst[1] = x[1];
           if (c == 0) {
-            p.part_ml[2 * (part + row)] = m;
-            p.part_ml[2 * (part + row) + 1] = l;
+            ml[0] = m;
+            ml[1] = l;
           }
         }
       }
@@ -476,25 +455,49 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p
   __shared__ float sm[kJoinWaves][10][kWave];
   const uint32_t unit = blockIdx.x, b = unit / p.U, u = unit % p.U;
   const int2 parts = p.unit_parts[unit];
-  if (parts.y < 2) return;
+  if (!kAfter && parts.y < 2) return;
+  const int count = kAfter ? parts.y + p.prior.parts : parts.y;
   const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const uint32_t pieces = p.D / 8, item = blockIdx.y * kWave + lane, row = min(item / pieces, nr - 1), c = item % pieces;
+  // A part's pieces of one row are neighbours, the prior's those of neighbouring rows (kAfter).
+  const uint32_t pieces = p.D / 8, item = blockIdx.y * kWave + lane, row_at = kAfter ? item % p.rows : item / pieces;
+  const uint32_t row = min(row_at, nr - 1), c = kAfter ? min(item / p.rows, pieces - 1) : item % pieces;
   float m = -INFINITY, l = 0.f;
   f32x4 x[2] = {};
   const int waves = blockDim.x / kWave;
-  for (int i0 = wave; i0 < parts.y; i0 += 4 * waves) {
+  // kAfter: the prior's parts of this row lie in the prompt kernels' layout: thread 64 wave + 32 half + row % 32 has dimensions 8 c + 4 half ..
+  const uint32_t pr = b * p.G + r0 + row, tile = pr / 128, thread = pr % 128 / 32 * 64 + pr % 32, Hkv = p.Hq / p.G, width = p.D <= 64 ? 64 : p.D <= 128 ? 128 : 256;
+  const int64_t pfirst = static_cast<int64_t>(p.prior.tiles - 1 - static_cast<int>(tile)) * Hkv + hk, pstep = static_cast<int64_t>(p.prior.tiles) * Hkv;
+  for (int i0 = wave; i0 < count; i0 += 4 * waves) {
     float pm[4], pl[4];
     f32x4 px[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = min(i0 + j * waves, parts.y - 1);
-      const int64_t at = (static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
-      pm[j] = i0 + j * waves < parts.y ? p.part_ml[2 * at] : -INFINITY;
-      pl[j] = p.part_ml[2 * at + 1];
-      const f32x4* src = reinterpret_cast<const f32x4*>(p.part_acc + at * p.D + 8 * c);
-      px[j][0] = src[0];
-      px[j][1] = src[1];
+      const int i = min(i0 + j * waves, count - 1);
+      if (kAfter && i >= parts.y) {
+        const int64_t at = pfirst + (i - parts.y) * pstep;
+        const f32x4 ml = reinterpret_cast<const f32x4*>(p.prior.ml)[at * 256 + thread];
+        const f32x4* src = reinterpret_cast<const f32x4*>(p.prior.acc) + at * (width / 8 * 256) + c * 256 + thread;
+        // Its rows are to be divided by the sum of the rounded weights, the second of ml, and count with the full one.
+        const float by = ml[1] > 0.f ? ml[2] / ml[1] : ml[1] == 0.f ? 0.f : ml[1];
+        pm[j] = ml[0] - p.prior.up + E::kLift;
+        pl[j] = ml[2];
+        px[j][0] = src[0] * by;
+        px[j][1] = src[32] * by;
+      } else {
+        const bool alone = kAfter && parts.y == 1;
+        const int64_t at = (alone ? static_cast<int64_t>(unit) : static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
+        const float* ml = (alone ? p.unit_ml : p.part_ml) + 2 * at;
+        pm[j] = ml[0];
+        pl[j] = ml[1];
+        const f32x4* src = reinterpret_cast<const f32x4*>((alone ? p.unit_acc : p.part_acc) + at * p.D + 8 * c);
+        px[j][0] = src[0];
+        px[j][1] = src[1];
+      }
+      if (i0 + j * waves >= count) {
+        pm[j] = -INFINITY;
+        pl[j] = 0.f;
+      }
     }
     const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), mm = finite_max(top), f = exp2_fast(m - mm);
     m = top;
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p
 #pragma unroll
   for (int e = 0; e < 8; ++e) sm[wave][2 + e][lane] = x[e >> 2][e & 3];
   __syncthreads();
-  if (wave != 0 || item >= nr * pieces) return;
+  if (wave != 0 || item >= p.rows * pieces || row_at >= nr) return;
   float y[8] = {};
   m = -INFINITY;
   for (int w = 0; w < waves; ++w) m = fmaxf(m, sm[w][0][lane]);
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p
     for (int e = 0; e < 8; ++e) y[e] += f * sm[w][2 + e][lane];
   }
   const f32x4 sums[2] = {{y[0], y[1], y[2], y[3]}, {y[4], y[5], y[6], y[7]}};
-  finish<E, kAfter>(p, b, hk * p.G + r0 + row, c, sums, m, l);
+  finish<E>(p, b, hk * p.G + r0 + row, c, sums, m, l);
 }
 
 struct Plan {
@@ -626,10 +629,13 @@ int decode_params(const latent_attn_decode_args& a, int64_t size, const Plan& pl
 // The second launch, where units were left in parts.
 template <bool kAfter>
 void launch_join(const Plan& pl, const DecodeParams& p, bool f16, hipStream_t s) {
-  if (pl.whole) return;
+  if (pl.whole && !kAfter) return;
   // A unit has about groups / units parts, four in flight a wave.  Of few parts two waves join soonest (96 units of six:
   // 16.8 us the whole call, 17.1 with one or four), of hundreds sixteen (one unit of 235: 16.6, 23.1 with four).
-  const uint32_t units = p.B * p.U, waves = pl.groups > 16 * units ? kJoinWaves : pl.groups > 8 * units ? 4 : 2;
+  const uint32_t units = p.B * p.U;
+  uint32_t waves = pl.groups > 16 * units ? kJoinWaves : pl.groups > 8 * units ? 4 : 2;
+  // The prior's parts are as many for each unit (5 sequences, 16 parts, 40 units: 5.1 us by eight waves, 7.2 by four; 512 units 12.0 and 10.0).
+  if (kAfter && p.prior.parts > 8) waves = std::max<uint32_t>(waves, units <= 256 ? 8 : 4);
   const dim3 grid(units, (p.rows * (p.D / 8) + kWave - 1) / kWave), block(kWave * waves);
   if (f16)
     hipLaunchKernelGGL((join_kernel<F16, kAfter>), grid, block, 0, s, p);
@@ -644,10 +650,33 @@ latent_attn_decode_args behind(const latent_attn_decode_args& a, int64_t n_prefi
   if (r.cache.pages) r.cache.pages += n_prefix;
   return r;
 }
-void set_prior(const latent_attn_decode_args& a, int64_t n_prefix, const Prior& prior, DecodeParams* p) {
-  p->prior_out = prior.out;
-  p->prior_lse = prior.lse;
+// The workspace behind a shared prefix: a decode's, every unit's parts among it, and the rows of units that one workgroup has whole.
+struct After {
+  Plan plan;
+  size_t unit_bytes, ml_bytes, acc_bytes;
+  size_t all() const { return plan.ml_bytes + plan.acc_bytes + unit_bytes + ml_bytes + acc_bytes; }
+};
+After plan_after(const latent_attn_decode_args& own, int64_t size, uint32_t most) {
+  After r{plan_for(own, size, most), 0, 0, 0};
+  auto up = [](size_t n) { return (n + 15) & ~size_t{15}; };
+  const size_t units = static_cast<size_t>(own.cache.n_seq) * r.plan.U, rows = units * r.plan.rows;
+  r.unit_bytes = up(units * sizeof(int2));
+  r.ml_bytes = up(rows * 2 * sizeof(float));
+  r.acc_bytes = rows * own.head_dim * sizeof(float);
+  return r;
+}
+int after_params(const latent_attn_decode_args& a, int64_t n_prefix, int64_t size, const After& w, const Prior& prior, void* workspace, DecodeParams* p) {
+  latent_attn_decode_args own = behind(a, n_prefix);
+  own.workspace = workspace;
+  own.workspace_bytes = SIZE_MAX;
+  const int st = decode_params(own, size, w.plan, p);
+  char* more = static_cast<char*>(workspace) + w.plan.ml_bytes + w.plan.acc_bytes;
+  p->unit_parts = reinterpret_cast<int2*>(more);
+  p->unit_ml = reinterpret_cast<float*>(more + w.unit_bytes);
+  p->unit_acc = reinterpret_cast<float*>(more + w.unit_bytes + w.ml_bytes);
+  p->prior = prior;
   p->ahead = static_cast<uint32_t>(n_prefix * a.cache.page_size);
+  return st;
 }
 
 }  // namespace

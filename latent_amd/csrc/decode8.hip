@@ -20,16 +20,12 @@ int launch8(const latent_attn_decode_args& a, int32_t code, const Plan& pl, cons
 }  // namespace
 
 int launch_after8(const latent_attn_decode_args& a, const latent_kv_scales& scales, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s) {
-  latent_attn_decode_args own = behind(a, n_prefix);
-  own.workspace = workspace;
-  own.workspace_bytes = SIZE_MAX;
-  const Plan pl = plan_for(own, 1, kMaxGroups8);
+  const After w = plan_after(behind(a, n_prefix), 1, kMaxGroups8);
   DecodeParams p{};
-  const int st = decode_params(own, 1, pl, &p);
+  const int st = after_params(a, n_prefix, 1, w, prior, workspace, &p);
   if (st != LATENT_OK) return st;
   p.scales = device_scales(scales);
-  set_prior(a, n_prefix, prior, &p);
-  return launch8<true>(own, scales.code, pl, p, s);
+  return launch8<true>(a, scales.code, w.plan, p, s);
 }
 
 }  // namespace attend

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
   const int begin = it.part ? it.part * it.chunk : 0;
   if (begin > 0 && begin >= end) return;
   const int stop = begin + min(end - begin, it.chunk);
-  const bool whole_unit = begin == 0 && stop == end;
+  const bool whole_unit = !kPrefix && begin == 0 && stop == end;
 
   u32x4 q[kSteps];
   {
@@ -347,10 +347,10 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt_kernel(Pr
     for (int rr = 0; rr < 4; ++rr) {
       const int d = 32 * i + 8 * rr + 4 * h;
       if (d < p.D)
-        store4<E, kPrefix>(p, it.s0 + tok, head, d, acc[i][4 * rr] * inv, acc[i][4 * rr + 1] * inv, acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv);
+        store4<E>(p, it.s0 + tok, head, d, acc[i][4 * rr] * inv, acc[i][4 * rr + 1] * inv, acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv);
     }
   if constexpr (kLse) {
-    if (h == 0) store_lse<E, kPrefix>(p, it.s0 + tok, head, top, full);
+    if (h == 0) store_lse<E>(p, it.s0 + tok, head, top, full);
   }
 }
 
@@ -364,10 +364,10 @@ int launch16(const latent_attn_prompt_args& a, const Plan& pl, const PromptParam
     const int64_t more = (pl.items / p.Hkv + 1) * p.Hkv, units = std::max<int64_t>(pl.units, p.Hkv);
     auto go = [&](auto paged_c, auto lse_c) {
       constexpr bool kPaged = decltype(paged_c)::value, kLse = decltype(lse_c)::value;
-      const dim3 grid(static_cast<unsigned>(units + (p.max_parts ? more : 0)));
+      const dim3 grid(static_cast<unsigned>(kPrefix ? p.max_parts : units + (p.max_parts ? more : 0)));
       hipLaunchKernelGGL((prompt_kernel<E, kDP, kDP == 256 ? 32 : 64, kPaged, kLse, kPrefix>), grid, dim3(kThreads), 0, s, p);
-      if (p.max_parts)
-        hipLaunchKernelGGL((join_kernel<E, kDP, kPaged, kLse, kPrefix>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32),
+      if (!kPrefix && p.max_parts)
+        hipLaunchKernelGGL((join_kernel<E, kDP, kPaged, kLse>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32),
                            dim3(kThreads), 0, s, p);
     };
     if constexpr (kPrefix) {
@@ -391,19 +391,25 @@ int launch16(const latent_attn_prompt_args& a, const Plan& pl, const PromptParam
 
 }  // namespace
 
-size_t prefix_workspace(const latent_attn_decode_args& a, int64_t n_prefix) {
-  const Plan pl = plan_for(prefix_args(a, a.cache.pages, n_prefix));
-  return pl.acc_bytes + pl.ml_bytes;
+// As many items of a row tile and key/value head as the chip holds at once (one workgroup a CU above D = 128), of 256 keys at least.
+PriorBytes plan_prior(const latent_attn_decode_args& a, int64_t n_prefix, Prior* prior) {
+  const int64_t rows = a.cache.n_seq * (a.n_head / a.n_kv_head), keys = n_prefix * a.cache.page_size;
+  const int64_t tiles = (rows + kRowsTile - 1) / kRowsTile, units = std::max<int64_t>(1, tiles * a.n_kv_head);
+  const int64_t most = std::max<int64_t>(1, (a.head_dim > 128 ? 256 : 512) / units), least = (keys + most - 1) / most;
+  const int64_t chunk = std::max<int64_t>(kChunk, (least + kChunkStep - 1) / kChunkStep * kChunkStep);
+  prior->parts = static_cast<int32_t>(std::max<int64_t>(1, a.cache.n_pages ? (keys + chunk - 1) / chunk : 0));
+  prior->chunk = static_cast<int32_t>(chunk);
+  prior->tiles = static_cast<int32_t>(tiles);
+  prior->up = a.dtype == LATENT_F16 ? Scale<F16>::kUp : Scale<BF16>::kUp;
+  const size_t parts = static_cast<size_t>(prior->parts) * units, blocks = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+  return {parts * 4 * blocks * kThreads * sizeof(f32x4), parts * kThreads * sizeof(f32x4)};
 }
 
-int launch_prefix16(const latent_attn_decode_args& a, const int32_t* prefix, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s) {
-  latent_attn_prompt_args r = prefix_args(a, prefix, n_prefix);
-  r.workspace = workspace;
-  r.workspace_bytes = SIZE_MAX;
-  const Plan pl = plan_for(r);
+int launch_prefix16(const latent_attn_decode_args& a, const int32_t* prefix, int64_t n_prefix, const Prior& prior, hipStream_t s) {
+  const latent_attn_prompt_args r = prefix_args(a, prefix, n_prefix);
   PromptParams p{};
-  const int st = prefix_params(r, 2, pl, prior, &p);
-  return st == LATENT_OK ? launch16<true>(r, pl, p, s) : st;
+  const int st = prefix_params(r, 2, prior, &p);
+  return st == LATENT_OK ? launch16<true>(r, Plan{}, p, s) : st;
 }
 
 }  // namespace attend

@@ -43,10 +43,9 @@ struct PromptParams {
   f32x4* part_acc;  // [max_parts][4 * 32-dimension blocks][256]
   f32x4* part_ml;   // [max_parts][256]: reference, sum, full sum
   Scales scales;    // of an 8-bit cache
-  // kPrefix: one sequence of all T tokens over the first n_keys positions of the cache, of which token t sees lengths[t]; outputs are fp32
-  // [T][Hq][D], and the log2 of each row's sum of exponentials [T][Hq].
-  float* prior_out;
-  float* prior_lse;
+  // kPrefix: one sequence of all T tokens over the first n_keys positions of the cache, of which token t sees lengths[t]; every item
+  // of prefix_chunk keys leaves a part.
+  int32_t prefix_chunk;
 };
 
 // Rows [s0, s0 + n) of sequence b.
@@ -109,7 +108,10 @@ __device__ __forceinline__ Line line_of(const PromptParams& p, int lane) {
   l.order = static_cast<uint64_t>(l.m) << 6 | (kWave - 1 - lane);
   l.parts = 1;
   l.chunk = INT32_MAX;
-  if (p.max_parts) {
+  if constexpr (kPrefix) {
+    l.chunk = p.prefix_chunk;
+    l.parts = max(1, (l.m + l.chunk - 1) / l.chunk);
+  } else if (p.max_parts) {
     // Both kernels cut the keys by this sum and have to agree to the last bit, whatever the compiler makes of either: no contraction.
 #pragma clang fp contract(off)
     float work = static_cast<float>(l.tiles) * static_cast<float>(l.m);
@@ -181,18 +183,13 @@ __device__ __forceinline__ int least_of(int v) {
 }
 
 // Four outputs from dimension d on of a row of token t and head h, and its log-sum-exp.
-template <typename E, bool kPrefix>
+template <typename E>
 __device__ __forceinline__ void store4(const PromptParams& p, int t, int h, int d, float a, float b, float c, float e) {
-  if constexpr (kPrefix) {
-    *reinterpret_cast<f32x4*>(p.prior_out + (static_cast<int64_t>(t) * p.Hq + h) * p.D + d) = f32x4{a, b, c, e};
-  } else {
-    *reinterpret_cast<u32x2*>(p.out + t * p.o_token + h * p.o_head + 2 * d) = u32x2{pack2<E>(a, b), pack2<E>(c, e)};
-  }
+  *reinterpret_cast<u32x2*>(p.out + t * p.o_token + h * p.o_head + 2 * d) = u32x2{pack2<E>(a, b), pack2<E>(c, e)};
 }
-template <typename E, bool kPrefix>
+template <typename E>
 __device__ __forceinline__ void store_lse(const PromptParams& p, int t, int h, float top, float full) {
-  const float z = top - Scale<E>::kUp + __log2f(full);
-  (kPrefix ? p.prior_lse : p.lse)[static_cast<int64_t>(t) * p.Hq + h] = full == 0.f ? -INFINITY : kPrefix ? z : z * kLn2;
+  p.lse[static_cast<int64_t>(t) * p.Hq + h] = full == 0.f ? -INFINITY : (top - Scale<E>::kUp + __log2f(full)) * kLn2;
 }
 
 // A tile in LDS: rows of kC 16-byte pieces, permuted so that the lanes of a read spread over all banks: a key row's
@@ -221,12 +218,12 @@ __device__ __forceinline__ u32x2 read_transposed(uint32_t at) {
 }
 
 // Adds up the parts of a split unit, 32 dimensions a workgroup; threads as in prompt_kernel.
-template <typename E, int kDP, bool kPaged, bool kLse, bool kPrefix>
+template <typename E, int kDP, bool kPaged, bool kLse>
 __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   constexpr int kBlocks = kDP / 32;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), h = lane >> 5, i = blockIdx.y, hk = blockIdx.x % p.Hkv;
   // The split units in the order of their items.
-  const Line l = line_of<kPaged, kPrefix>(p, lane);
+  const Line l = line_of<kPaged, false>(p, lane);
   const int x0 = blockIdx.x / p.Hkv, units = l.parts > 1 ? l.tiles : 0;
   int count = units;
 #pragma unroll
@@ -237,9 +234,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
   if (!mine) return;
   const int b = __builtin_ctzll(mine), r = x0 - __builtin_amdgcn_readlane(before, b), t = __builtin_amdgcn_readlane(l.tiles, b);
   const int first = __builtin_amdgcn_readlane(items_before(p, l, l.tiles * l.parts), b) + r, tile = t - 1 - r;
-  const int2 qs = queries_of<kPrefix>(p, b);
-  const int n = qs.y, m = keys_of<kPaged, kPrefix>(p, b).y;
-  const int parts = ((kPrefix ? m : keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1)) + l.chunk - 1) / l.chunk;
+  const int2 qs = queries_of<false>(p, b);
+  const int n = qs.y, m = keys_of<kPaged, false>(p, b).y;
+  const int parts = (keys_seen(p, n, m, tile * kRowsTile + kRowsTile - 1) + l.chunk - 1) / l.chunk;
   if (parts < 2) return;  // its rows see too little to be split
   const int row = tile * kRowsTile + (tid >> 6) * kRowsWave + (lane & 31);
   if (row >= n * p.G) return;
@@ -279,10 +276,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(PromptParams p) {
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
     const int d = 32 * i + 8 * rr + 4 * h;
-    if (d < p.D) store4<E, kPrefix>(p, qs.x + tok, head, d, x[rr][0] * inv, x[rr][1] * inv, x[rr][2] * inv, x[rr][3] * inv);
+    if (d < p.D) store4<E>(p, qs.x + tok, head, d, x[rr][0] * inv, x[rr][1] * inv, x[rr][2] * inv, x[rr][3] * inv);
   }
   if constexpr (kLse) {
-    if (i == 0 && h == 0) store_lse<E, kPrefix>(p, qs.x + tok, head, top, full);
+    if (i == 0 && h == 0) store_lse<E>(p, qs.x + tok, head, top, full);
   }
 }
 
@@ -411,7 +408,7 @@ latent_attn_prompt_args prefix_args(const latent_attn_decode_args& a, const int3
   r.cache.n_seq = 1;
   r.cache.max_pages = r.cache.pages_stride = n_prefix;
   r.q = a.q;
-  r.out = a.out;          // not written: the prior is
+  r.out = a.out;          // not written: parts are
   r.starts = a.lengths;   // not read
   r.lengths = a.lengths;  // one a token
   r.q_token_stride = a.q_token_stride, r.q_head_stride = a.q_head_stride;
@@ -422,12 +419,14 @@ latent_attn_prompt_args prefix_args(const latent_attn_decode_args& a, const int3
   r.scale = a.scale;
   return r;
 }
-int prefix_params(const latent_attn_prompt_args& a, int64_t size, const Plan& pl, const Prior& prior, PromptParams* p) {
-  const int st = prompt_params(a, size, pl, p);
+int prefix_params(const latent_attn_prompt_args& a, int64_t size, const Prior& prior, PromptParams* p) {
+  const int st = prompt_params(a, size, Plan{}, p);
   if (st != LATENT_OK) return st;
   p->n_keys = static_cast<int32_t>(p->cache.max_len);
-  p->prior_out = prior.out;
-  p->prior_lse = prior.lse;
+  p->prefix_chunk = prior.chunk;
+  p->max_parts = prior.parts * prior.tiles * p->Hkv;
+  p->part_acc = reinterpret_cast<f32x4*>(prior.acc);
+  p->part_ml = reinterpret_cast<f32x4*>(prior.ml);
   return LATENT_OK;
 }
 

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
   const int begin = it.part ? it.part * it.chunk : 0;
   if (begin > 0 && begin >= end) return;
   const int stop = begin + min(end - begin, it.chunk);
-  const bool whole_unit = begin == 0 && stop == end;
+  const bool whole_unit = !kPrefix && begin == 0 && stop == end;
 
   u32x4 q[kSteps];
   {
@@ -369,10 +369,10 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
     for (int rr = 0; rr < 4; ++rr) {
       const int d = 32 * i + 8 * rr + 4 * h;
       if (d < p.D)
-        store4<E, kPrefix>(p, it.s0 + tok, head, d, acc[i][4 * rr] * inv, acc[i][4 * rr + 1] * inv, acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv);
+        store4<E>(p, it.s0 + tok, head, d, acc[i][4 * rr] * inv, acc[i][4 * rr + 1] * inv, acc[i][4 * rr + 2] * inv, acc[i][4 * rr + 3] * inv);
     }
   if constexpr (kLse) {
-    if (h == 0) store_lse<E, kPrefix>(p, it.s0 + tok, head, top, full);
+    if (h == 0) store_lse<E>(p, it.s0 + tok, head, top, full);
   }
 }
 
@@ -387,9 +387,9 @@ int launch8(const latent_attn_prompt_args& a, int32_t code, const Plan& pl, cons
     auto with_lse = [&](auto lse) {
       constexpr bool kLse = decltype(lse)::value;
       hipLaunchKernelGGL((prompt8_kernel<E, decltype(q), kDP, kDP == 256 ? 32 : 64, kLse, kPrefix>),
-                         dim3(static_cast<unsigned>(units + (p.max_parts ? more : 0))), dim3(kThreads), 0, s, p);
-      if (p.max_parts)
-        hipLaunchKernelGGL((join_kernel<E, kDP, true, kLse, kPrefix>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32), dim3(kThreads), 0, s, p);
+                         dim3(static_cast<unsigned>(kPrefix ? p.max_parts : units + (p.max_parts ? more : 0))), dim3(kThreads), 0, s, p);
+      if (!kPrefix && p.max_parts)
+        hipLaunchKernelGGL((join_kernel<E, kDP, true, kLse>), dim3(static_cast<unsigned>(std::min(units, more)), kDP / 32), dim3(kThreads), 0, s, p);
     };
     if constexpr (kPrefix)
       with_lse(std::true_type{});
@@ -407,17 +407,13 @@ int launch8(const latent_attn_prompt_args& a, int32_t code, const Plan& pl, cons
 
 }  // namespace
 
-int launch_prefix8(const latent_attn_decode_args& a, const latent_kv_scales& scales, const int32_t* prefix, int64_t n_prefix, const Prior& prior,
-                   void* workspace, hipStream_t s) {
-  latent_attn_prompt_args r = prefix_args(a, prefix, n_prefix);
-  r.workspace = workspace;
-  r.workspace_bytes = SIZE_MAX;
-  const Plan pl = plan_for(r);
+int launch_prefix8(const latent_attn_decode_args& a, const latent_kv_scales& scales, const int32_t* prefix, int64_t n_prefix, const Prior& prior, hipStream_t s) {
+  const latent_attn_prompt_args r = prefix_args(a, prefix, n_prefix);
   PromptParams p{};
-  const int st = prefix_params(r, 1, pl, prior, &p);
+  const int st = prefix_params(r, 1, prior, &p);
   if (st != LATENT_OK) return st;
   p.scales = device_scales(scales);
-  return launch8<true>(r, scales.code, pl, p, s);
+  return launch8<true>(r, scales.code, Plan{}, p, s);
 }
 
 }  // namespace attend

@@ -3,22 +3,21 @@
 //   out[b][h] = sum_j p_j v[j] / sum_j p_j over the prefix's keys and the sequence's own
 //
 // The rows of all sequences against the prefix's keys are the products of a prompt without a mask (B G rows of a key/value head
-// over one sequence of keys: each key is read once for 128 rows, split over the chip), and leave an fp32 row and the log2 of its
-// sum.  The sequences' own keys are a decode that begins behind the prefix and joins its rows with those, where it finishes them.
+// over one sequence of keys: each key is read once for 128 rows, split over the chip); the sequences' own keys are a decode that
+// begins behind the prefix.  Both leave parts in fp32, and a third launch joins a row's.  (Rows joined where the decode finishes
+// them, without that launch, took longer: few lanes read all of the prior's parts one after the other, 64 sequences behind 16000 126 us.)
 #include "shared.hpp"
-
-#include <algorithm>
 
 using namespace latent;
 using namespace latent::attend;
 
 namespace {
 
-size_t up(size_t n) { return (n + 255) & ~size_t{255}; }
-
 struct Layout {
-  size_t out, lse, prefix, after;  // bytes
-  size_t all() const { return out + lse + std::max(prefix, after); }
+  Prior prior;
+  PriorBytes bytes;
+  size_t after;
+  size_t all() const { return bytes.acc + bytes.ml + after; }
 };
 
 int layout_of(const latent_attn_shared_args& a, Layout* l) {
@@ -32,10 +31,8 @@ int layout_of(const latent_attn_shared_args& a, Layout* l) {
   const int64_t rows = d.cache.n_seq * d.n_head;
   // Row tiles of the prefix's launch are counted in 32 bits, rows with their elements in 31.
   if (rows * d.head_dim > INT32_MAX || (rows / 128 + d.n_kv_head) > 1 << 20) return LATENT_E_UNSUPPORTED;
-  l->out = up(static_cast<size_t>(rows * d.head_dim) * sizeof(float));
-  l->lse = up(static_cast<size_t>(rows) * sizeof(float));
-  l->prefix = prefix_workspace(d, a.n_prefix);
-  l->after = after_workspace(d, a.n_prefix, a.scales != nullptr);
+  if (a.n_prefix) l->bytes = plan_prior(d, a.n_prefix, &l->prior);
+  l->after = a.n_prefix ? after_workspace(d, a.n_prefix, a.scales != nullptr) : n;
   return LATENT_OK;
 }
 
@@ -65,11 +62,13 @@ extern "C" int latent_attn_decode_shared(const latent_attn_shared_args* args, la
   if ((a.n_head > 1 && !a.out_head_stride) || (a.cache.n_seq > 1 && !a.out_token_stride)) return LATENT_E_INVALID;
   if (!a.workspace || a.workspace_bytes < l.all()) return LATENT_E_WORKSPACE;
   char* ws = static_cast<char*>(a.workspace);
-  const Prior prior{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + l.out)};
-  void* scratch = ws + l.out + l.lse;  // one half's, then the other's
+  Prior& prior = l.prior;
+  prior.acc = reinterpret_cast<float*>(ws);
+  prior.ml = reinterpret_cast<float*>(ws + l.bytes.acc);
+  void* scratch = ws + l.bytes.acc + l.bytes.ml;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  st = args->scales ? launch_prefix8(a, *args->scales, args->prefix, args->n_prefix, prior, scratch, s)
-                    : launch_prefix16(a, args->prefix, args->n_prefix, prior, scratch, s);
+  st = args->scales ? launch_prefix8(a, *args->scales, args->prefix, args->n_prefix, prior, s)
+                    : launch_prefix16(a, args->prefix, args->n_prefix, prior, s);
   if (st != LATENT_OK) return st;
   return args->scales ? launch_after8(a, *args->scales, args->n_prefix, prior, scratch, s) : launch_after16(a, args->n_prefix, prior, scratch, s);
 }
