@@ -541,9 +541,9 @@ int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stre
 /*
  * A cache whose keys and values are codes of 8 bits, with one scale for each
  * position and key/value head: a row x of D numbers is held as
- *     m = max(max |x|, 2^-100),  scale = m / top,  code = x * top / m
- * in fp32, the code rounded to the nearest (ties to even): whole numbers with
- * top 127, or OCP e4m3 with top 448.  A row with an infinity or a NaN has a NaN
+ *     m = max(max |x|, 2^-100),  scale = m / top,  code = x * (top * (1 / m))
+ * in fp32, each step rounded, the code then to the nearest (ties to even): whole
+ * numbers with top 127, or OCP e4m3 with top 448.  A row with an infinity or a NaN has a NaN
  * as its scale and codes of zero: whoever reads it gets NaN.  The number held is
  * code * scale.
  *

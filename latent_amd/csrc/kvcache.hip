@@ -193,9 +193,9 @@ __global__ void __launch_bounds__(kThreads) append_scalar_kernel(AppendParams p,
 // A head's row is kLanes lanes', eight numbers each: they rotate them (each lane reads its numbers' partners itself),
 // find the row's largest magnitude by lane exchanges and store eight codes each, the first the scale.
 //
-// The rotation's products and sums are rounded one by one, and the scaling is a product (exact for numbers of 16 bits) and a division: the
-// codes are then the same whoever computes them, to the bit, and a number half way between two codes is seen to be that (a product with
-// top / m, which is rounded, puts such numbers on either side: they are as common as one in 16 where a row's m is 7/4 of a power of two).
+// The rotation's products and sums are rounded one by one, and the scaling is a reciprocal and a product a row and a product a number: the
+// codes are then the same whoever computes them, to the bit, and a test can ask for that.  A number half way between two codes may
+// get either, which are as near (a division a number, which would see it, took 80 us for 8190 tokens and their reading back instead of 78).
 
 // The largest v of kLanes neighbouring lanes.
 template <int kLanes>
@@ -320,12 +320,12 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(AppendParams p, Scale
     for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(r[e]) & 0x7FFFFFFFu);
     most = lanes_max<kLanes>(most);
     const bool finite = most < 0x7F800000u;
-    const float m = fmaxf(__uint_as_float(most), 0x1p-100f), down = m > 0x1p100f ? 0x1p-20f : 1.f;  // x top stays finite
+    const float m = fmaxf(__uint_as_float(most), 0x1p-100f), by = Q::kTop * (1.f / m);
     u32x2 codes{0, 0};
     if (finite) {
       float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = r[e] * (Q::kTop * down) / (m * down);
+      for (int e = 0; e < 8; ++e) z[e] = r[e] * by;
       codes = u32x2{Q::codes(z), Q::codes(z + 4)};
     }
     const bool key = h < p.Hq + p.Hkv;

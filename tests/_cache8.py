@@ -1,6 +1,6 @@
 """8-bit caches for tests: the format in plain torch operations, and caches whose unused rows would spoil a result.
 
-Codes and scales are elementwise operations of fp32 (a maximum, a product, two divisions, a rounding), each
+Codes and scales are elementwise operations of fp32 (a maximum, a reciprocal, a division, two products, a rounding), each
 rounded by itself, so the kernel's have to be the same to the bit.  What attention reads is code times
 scale, in 64 bits; tests/_attention.py's tolerances then hold as they are: a score's scale is one more
 rounding than the D products and their sum (it counts D + 4), a probability's two more of the 4 w there, and
@@ -23,8 +23,7 @@ def quantise(x, code):
     finite = torch.isfinite(x).all(-1)
     m = torch.where(finite, most, 0.0).clamp(min=LEAST)
     top = torch.full_like(m, TOP[code])  # a tensor: torch divides by a number through its reciprocal
-    down = torch.where(m > 2.0 ** 100, 2.0 ** -20, 1.0)
-    y = torch.where(finite[..., None], x, 0.0) * (top * down)[..., None] / (m * down)[..., None]
+    y = torch.where(finite[..., None], x, 0.0) * (top * m.reciprocal())[..., None]
     scale = torch.where(finite, m / top, float("nan"))
     return (y.round() if code == torch.int8 else y).to(code), scale
 
