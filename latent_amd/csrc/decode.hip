@@ -35,12 +35,12 @@ namespace latent {
 namespace attend {
 namespace {
 
-template <bool kAfter>
+template <bool kAfter, bool kTable = false>
 int launch16(const latent_attn_decode_args& a, const Plan& pl, const DecodeParams& p, hipStream_t s) {
   (void)hipGetLastError();
   auto launch = [&](auto e, auto dp, auto exact, auto mt, auto page8) {
     auto go = [&](auto once) {
-      typedef Stream<decltype(e), decltype(dp)::value, decltype(exact)::value, decltype(mt)::value, decltype(page8)::value, decltype(once)::value> S;
+      typedef Stream<decltype(e), decltype(dp)::value, decltype(exact)::value, decltype(mt)::value, decltype(page8)::value, decltype(once)::value, kTable> S;
       hipLaunchKernelGGL((decode_kernel<S, kAfter>), dim3(pl.groups), dim3(kThreads), 0, s, p);
     };
     if constexpr (decltype(exact)::value && decltype(page8)::value)
@@ -87,6 +87,16 @@ int launch_after16(const latent_attn_decode_args& a, int64_t n_prefix, const Pri
   DecodeParams p{};
   const int st = after_params(a, n_prefix, 2, w, prior, workspace, &p);
   return st == LATENT_OK ? launch16<true>(a, w.plan, p, s) : st;
+}
+
+int launch_together16(const latent_attn_decode_args& a, const int32_t* prefix, int64_t n_prefix, hipStream_t s) {
+  const Plan pl = plan_for(a);
+  DecodeParams p{};
+  const int st = decode_params(a, 2, pl, &p);
+  if (st != LATENT_OK) return st;
+  p.prefix = prefix;
+  p.prefix_pages = static_cast<uint32_t>(n_prefix);
+  return launch16<false, true>(a, pl, p, s);
 }
 
 }  // namespace attend

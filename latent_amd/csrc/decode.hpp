@@ -42,6 +42,9 @@ struct DecodeParams {
   // kAfter: keys here begin at position `ahead`, which cache.pages and cache.max_len leave out; what rows have seen before it is `prior`.  Every
   // unit leaves its rows, those that one workgroup has whole by themselves: sums [units][rows][2] and rows [units][rows][D].
   Prior prior;
+  // kTable streams: the first pages of every sequence, which its row of cache.pages need not name.
+  const int32_t* prefix;
+  uint32_t prefix_pages;
   float* unit_ml;
   float* unit_acc;
   uint32_t ahead;
@@ -129,7 +132,7 @@ __device__ __forceinline__ T load_row(const char* at) {
   return *reinterpret_cast<const T*>(at);
 }
 
-template <typename E_, int kDP_, bool kExact_, int kMT_, bool kPage8, bool kOnce>
+template <typename E_, int kDP_, bool kExact_, int kMT_, bool kPage8, bool kOnce, bool kTable>
 struct Stream {
   typedef E_ E;
   static constexpr int kDP = kDP_, kMT = kMT_, kVec = kDP / 16, kK = kDP / 32;
@@ -160,7 +163,7 @@ struct Stream {
   };
   __device__ __forceinline__ Place place_of(uint32_t key) const {
     const uint32_t slot = p.cache.by_page.of(key);
-    return {key < len ? pages[slot] : -1, key - slot * p.cache.page_size};
+    return {key < len ? (kTable && slot < p.prefix_pages ? p.prefix : pages)[slot] : -1, key - slot * p.cache.page_size};
   }
   // Row m of score block blk is key 8 (m / 4) + 4 blk + m % 4 of the step: lane (query, kq) then holds keys 8 kq .. + 7.
   __device__ __forceinline__ uint32_t k_key(uint32_t kb, int blk) const { return kb + 8 * ((lane & 15) >> 2) + 4 * blk + (lane & 3); }

@@ -6,10 +6,10 @@ namespace latent {
 namespace attend {
 namespace {
 
-template <bool kAfter>
+template <bool kAfter, bool kTable = false>
 int launch8(const latent_attn_decode_args& a, int32_t code, const Plan& pl, const DecodeParams& p, hipStream_t s) {
   (void)hipGetLastError();
-  with_stream8(a, code, pl, [&](auto t) {
+  with_stream8<kTable>(a, code, pl, [&](auto t) {
     hipLaunchKernelGGL((decode_kernel<typename decltype(t)::type, kAfter>), dim3(pl.groups), dim3(kThreads), 0, s, p);
   });
   if (hipGetLastError() != hipSuccess) return LATENT_E_HIP;
@@ -26,6 +26,17 @@ int launch_after8(const latent_attn_decode_args& a, const latent_kv_scales& scal
   if (st != LATENT_OK) return st;
   p.scales = device_scales(scales);
   return launch8<true>(a, scales.code, w.plan, p, s);
+}
+
+int launch_together8(const latent_attn_decode_args& a, const latent_kv_scales& scales, const int32_t* prefix, int64_t n_prefix, hipStream_t s) {
+  const Plan pl = plan_for(a, 1, kMaxGroups8);
+  DecodeParams p{};
+  const int st = decode_params(a, 1, pl, &p);
+  if (st != LATENT_OK) return st;
+  p.scales = device_scales(scales);
+  p.prefix = prefix;
+  p.prefix_pages = static_cast<uint32_t>(n_prefix);
+  return launch8<false, true>(a, scales.code, pl, p, s);
 }
 
 }  // namespace attend

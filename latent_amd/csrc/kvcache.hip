@@ -196,6 +196,8 @@ __global__ void __launch_bounds__(kThreads) append_scalar_kernel(AppendParams p,
 // The rotation's products and sums are rounded one by one, and the scaling is a reciprocal and a product a row and a product a number: the
 // codes are then the same whoever computes them, to the bit, and a test can ask for that.  A number half way between two codes may
 // get either, which are as near (a division a number, which would see it, took 80 us for 8190 tokens and their reading back instead of 78).
+//
+// Bound by memory: 8190 tokens of 64 + 2x8 heads of 128 64 us, 14 to read them back (78 both, 4.8 TB/s); one token 3.4 and 2.5 us of GPU.
 
 // The largest v of kLanes neighbouring lanes.
 template <int kLanes>

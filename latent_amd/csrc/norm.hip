@@ -28,8 +28,8 @@ struct NormParams {
   float post_eps, pre_eps, scale;
 };
 
-// Elements i .. i + 7 of an array of any of the three types, those below d; kVec: all of them, 16 bytes at a time.
-template <bool kVec>
+// Elements i, i + kStep, .. i + 7 kStep of an array of any of the three types, those below d; kVec: neighbours, 16 bytes at a time.
+template <bool kVec, int kStep>
 __device__ __forceinline__ void load8(const void* p, int dtype, int64_t base, uint32_t i, uint32_t d, float fill, float (&v)[8]) {
   if constexpr (kVec) {
     if (i < d) {
@@ -40,7 +40,7 @@ __device__ __forceinline__ void load8(const void* p, int dtype, int64_t base, ui
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = i + e < d ? load_act(p, dtype, base + i + e) : fill;
+    for (int e = 0; e < 8; ++e) v[e] = i + e * kStep < d ? load_act(p, dtype, base + i + e * kStep) : fill;
   }
 }
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ uint16_t to_half_bits(float v, int dtype) {
   return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
 }
 
-template <bool kVec>
+template <bool kVec, int kStep>
 __device__ __forceinline__ void store8(void* p, int dtype, int64_t base, uint32_t i, uint32_t d, const float (&v)[8]) {
   if constexpr (kVec) {
     if (i >= d) return;
@@ -66,11 +66,11 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t base, uint32_
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (i + e >= d) return;
+      if (i + e * kStep >= d) return;
       if (dtype == LATENT_F32)
-        static_cast<float*>(p)[base + i + e] = v[e];
+        static_cast<float*>(p)[base + i + e * kStep] = v[e];
       else
-        static_cast<uint16_t*>(p)[base + i + e] = to_half_bits(v[e], dtype);
+        static_cast<uint16_t*>(p)[base + i + e * kStep] = to_half_bits(v[e], dtype);
     }
   }
 }
@@ -80,6 +80,7 @@ template <int kRowWaves, int kV, bool kVec>
 __global__ void __launch_bounds__(kRowWaves > 4 ? kRowWaves * kWave : 4 * kWave) residual_norm_kernel(NormParams p) {
   constexpr int kRows = kRowWaves > 4 ? 1 : 4 / kRowWaves;  // of a workgroup
   constexpr int kLanes = kRowWaves * kWave;
+  constexpr int kStep = kVec ? 1 : kLanes;  // rows that no 16 bytes divide go by elements, neighbouring lanes' neighbours
   __shared__ float sums[4][kRowWaves];
   const int tid = threadIdx.x, wave = tid / kWave % kRowWaves;
   const uint32_t t = blockIdx.x * kRows + tid / kLanes, lane = tid % kLanes;
@@ -100,14 +101,14 @@ __global__ void __launch_bounds__(kRowWaves > 4 ? kRowWaves * kWave : 4 * kWave)
   };
   const uint32_t d = p.d;
   const float count = static_cast<float>(d);
-  auto at = [&](int j) { return 8 * (lane + j * kLanes); };
+  auto at = [&](int j) { return kVec ? 8 * (lane + j * kLanes) : lane + 8 * j * kLanes; };
   float x[kV][8];
 #pragma unroll
-  for (int j = 0; j < kV; ++j) load8<kVec>(p.x, p.x_dtype, t * p.x_stride, at(j), d, 0.f, x[j]);
+  for (int j = 0; j < kV; ++j) load8<kVec, kStep>(p.x, p.x_dtype, t * p.x_stride, at(j), d, 0.f, x[j]);
   float y[kV][8];
   if (p.y) {
 #pragma unroll
-    for (int j = 0; j < kV; ++j) load8<kVec>(p.y, p.y_dtype, t * p.y_stride, at(j), d, 0.f, y[j]);
+    for (int j = 0; j < kV; ++j) load8<kVec, kStep>(p.y, p.y_dtype, t * p.y_stride, at(j), d, 0.f, y[j]);
   }
   // Where a lane has one piece, weights, biases and the gate are fetched with the row: their latency would follow each sum's.
   constexpr bool kAhead = kV == 1;
@@ -115,18 +116,18 @@ __global__ void __launch_bounds__(kRowWaves > 4 ? kRowWaves * kWave : 4 * kWave)
     float v[kAhead ? 5 : 1][8];
   } ahead;
   if constexpr (kAhead) {
-    if (p.post_w) load8<kVec>(p.post_w, p.post_dtype, 0, at(0), p.d, 0.f, ahead.v[0]);
-    if (p.post_b) load8<kVec>(p.post_b, p.post_dtype, 0, at(0), p.d, 0.f, ahead.v[1]);
-    if (p.gate) load8<kVec>(p.gate, p.gate_dtype, t * p.gate_stride, at(0), p.d, 0.f, ahead.v[2]);
-    if (p.pre_w) load8<kVec>(p.pre_w, p.pre_dtype, 0, at(0), p.d, 0.f, ahead.v[3]);
-    if (p.pre_b) load8<kVec>(p.pre_b, p.pre_dtype, 0, at(0), p.d, 0.f, ahead.v[4]);
+    if (p.post_w) load8<kVec, kStep>(p.post_w, p.post_dtype, 0, at(0), p.d, 0.f, ahead.v[0]);
+    if (p.post_b) load8<kVec, kStep>(p.post_b, p.post_dtype, 0, at(0), p.d, 0.f, ahead.v[1]);
+    if (p.gate) load8<kVec, kStep>(p.gate, p.gate_dtype, t * p.gate_stride, at(0), p.d, 0.f, ahead.v[2]);
+    if (p.pre_w) load8<kVec, kStep>(p.pre_w, p.pre_dtype, 0, at(0), p.d, 0.f, ahead.v[3]);
+    if (p.pre_b) load8<kVec, kStep>(p.pre_b, p.pre_dtype, 0, at(0), p.d, 0.f, ahead.v[4]);
   }
   auto operand = [&](const void* from, int dtype, int64_t base, int j, int which, float (&f)[8]) {
     if constexpr (kAhead) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = ahead.v[which][e];
     } else {
-      load8<kVec>(from, dtype, base, at(j), p.d, 0.f, f);
+      load8<kVec, kStep>(from, dtype, base, at(j), p.d, 0.f, f);
     }
   };
   auto norm = [&](float (&v)[kV][8], int kind, float eps, const void* w, const void* b, int dtype, int which) {
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kRowWaves > 4 ? kRowWaves * kWave : 4 * kWave)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         // What is behind the row's end stays zero.
-        if (kind == LATENT_NORM_LAYER) v[j][e] = at(j) + e < d ? v[j][e] - mean : 0.f;
+        if (kind == LATENT_NORM_LAYER) v[j][e] = at(j) + e * kStep < d ? v[j][e] - mean : 0.f;
         s += v[j][e] * v[j][e];
       }
     const float r = 1.f / sqrtf(total(s) / count + eps);
@@ -178,12 +179,12 @@ __global__ void __launch_bounds__(kRowWaves > 4 ? kRowWaves * kWave : 4 * kWave)
   }
   if (p.x_out) {
 #pragma unroll
-    for (int j = 0; j < kV; ++j) store8<kVec>(p.x_out, p.x_dtype, t * p.xo_stride, at(j), d, x[j]);
+    for (int j = 0; j < kV; ++j) store8<kVec, kStep>(p.x_out, p.x_dtype, t * p.xo_stride, at(j), d, x[j]);
   }
   if (!p.n_out) return;
   if (p.pre != LATENT_NORM_NONE) norm(x, p.pre, p.pre_eps, p.pre_w, p.pre_b, p.pre_dtype, 3);
 #pragma unroll
-  for (int j = 0; j < kV; ++j) store8<kVec>(p.n_out, p.n_dtype, t * p.no_stride, at(j), d, x[j]);
+  for (int j = 0; j < kV; ++j) store8<kVec, kStep>(p.n_out, p.n_dtype, t * p.no_stride, at(j), d, x[j]);
 }
 
 constexpr int64_t kMaxNormDim = 32768;

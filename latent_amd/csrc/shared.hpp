@@ -28,5 +28,9 @@ size_t after_workspace(const latent_attn_decode_args& a, int64_t n_prefix, bool 
 int launch_after16(const latent_attn_decode_args& a, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s);
 int launch_after8(const latent_attn_decode_args& a, const latent_kv_scales& scales, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s);
 
+// Both at once, as a decode that looks the first pages up in `prefix`.
+int launch_together16(const latent_attn_decode_args& a, const int32_t* prefix, int64_t n_prefix, hipStream_t s);
+int launch_together8(const latent_attn_decode_args& a, const latent_kv_scales& scales, const int32_t* prefix, int64_t n_prefix, hipStream_t s);
+
 }  // namespace attend
 }  // namespace latent

@@ -124,10 +124,12 @@ def test_shared_prefix_sizes(L):
     size = la.attend_decode_shared_workspace_size
     n = ctypes.c_size_t()
     for codes in (False, True):
-        # The rows over the prefix, their sums, and the halves' scratch, one after the other in the same place.
+        # Few sequences: a decode.  Many: the prefix's parts and those of the sequences' own keys.
         assert size(4, 8, 2, 64, 20, 16, 0, codes) >= la.attend_decode_workspace_size(4, 8, 2, 64, 20, 16, codes)
         assert size(64, 64, 8, 128, 300, 64, 250, codes) < 128 << 20
-        assert 0 < size(1, 1, 1, 16, 1, 8, 1, codes) < 1 << 20
+        assert size(1, 1, 1, 16, 1, 8, 1, codes) == 0
+        assert size(5, 32, 8, 128, 300, 16, 256, codes) == la.attend_decode_workspace_size(5, 32, 8, 128, 300, 16, codes)
+        assert size(60, 6, 2, 128, 40, 128, 32, codes) > la.attend_decode_workspace_size(60, 6, 2, 128, 40, 128, codes)
     with pytest.raises(la.LatentError):
         size(4, 8, 2, 64, 20, 16, 21)
     a = _shared(L, cache=_cache(L, n_seq=1 << 20, max_pages=1, pages_stride=1), n_head=1024, n_kv_head=1024, head_dim=256, n_prefix=1)

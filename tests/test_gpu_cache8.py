@@ -181,7 +181,10 @@ def test_prompt(la, code, dt, new, ahead, Hkv, G, D, page, width, causal, order)
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("shared,lengths,Hkv,G,D,page,width", [
     (1, [9, 8, 20], 1, 1, 16, 8, None), (2, [40, 0, 33, 32, 31, 5], 2, 4, 64, 16, None), (8, [130, 128, 300, 129], 2, 3, 128, 16, None), (5, [80] * 9, 1, 16, 96, 16, 5),
-    (40, [700, 641, 640, 1200, 0, 12], 2, 8, 128, 16, 100), (70, [1200, 1121, 4], 1, 5, 256, 16, None), (130, [2100] * 40, 1, 4, 128, 16, None), (4, [70], 2, 2, 192, 16, None)])
+    (40, [700, 641, 640, 1200, 0, 12], 2, 8, 128, 16, 100), (70, [1200, 1121, 4], 1, 5, 256, 16, None), (130, [2100] * 40, 1, 4, 128, 16, None), (4, [70], 2, 2, 192, 16, None),
+    # So many numbers that the prefix goes by itself: rows of several tiles, of one, splits that end inside a chunk, lengths inside the prefix.
+    (32, [4097, 4096, 0, 4095, 700, 5000] * 10, 2, 3, 128, 128, None), (257, [4112 + 7 * i for i in range(130)], 1, 5, 64, 16, None),
+    (64, [4096, 4100, 30, 4400] * 10, 1, 2, 256, 64, 80), (256, [4096] * 80, 1, 1, 96, 16, None), (130, [2080 + i % 40 for i in range(150)], 1, 18, 128, 16, None)])
 def test_decode_over_a_shared_prefix(la, code, dt, shared, lengths, Hkv, G, D, page, width):
     g, dt = gen(sum(lengths) + D), DT[dt]
     c = torch.int8 if code == "16" else CODES[code]

@@ -67,8 +67,7 @@ def test_refusals(la, name):
     if name == "attend_decode_shared":
         pages = base["pages"]
         for change, error in ((dict(prefix=pages[0, :1].long()), ValueError), (dict(prefix=pages[:, :1]), ValueError), (dict(prefix=None), TypeError),
-                              (dict(prefix=pages[0, :1].cpu()), ValueError), (dict(prefix=ints([0] * (pages.shape[1] + 1))), ValueError),
-                              (dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda")), la.LatentError)):
+                              (dict(prefix=pages[0, :1].cpu()), ValueError), (dict(prefix=ints([0] * (pages.shape[1] + 1))), ValueError)):
             with pytest.raises(error):
                 f(**change)
     if name == "kv_read":
@@ -266,3 +265,43 @@ def test_no_sequences_no_tokens(la):
     assert [t.shape[0] for t in f["kv_read"](positions=ints([]))] == [0, 0]
     want = f["attend_decode"]()
     assert torch.equal(f["attend_decode_shared"](prefix=ints([])), want)  # nothing shared: the plain call
+
+
+@pytest.mark.parametrize("code", ["16", *CODES])
+def test_a_prefix_by_itself_with_rows_and_pages_that_are_not_there(la, code):
+    """A NaN among the prefix's rows reaches the sequences that are long enough, pages that do not exist are masked; in a graph too."""
+    g, B, P, H, D = gen(14), 70, 2048, 2, 128
+    lengths = [2100 if b % 2 else 1000 for b in range(B)]
+    kc, vc, ks, vs, pages, seqs = paged8(g, lengths, 16, H, D, torch.bfloat16, torch.int8 if code == "16" else CODES[code], shared=P // 16)
+    scales = dict(k_scale=ks, v_scale=vs)
+    if code == "16":
+        kc, vc = ((x.float() * s.transpose(1, 2)[..., None]).bfloat16() for x, s in ((kc, ks), (vc, vs)))
+        seqs = [tuple(x.bfloat16() for x in kv) for kv in seqs]
+        scales = {}
+    q = torch.randn((B, 4, D), generator=g, device="cuda").bfloat16()
+    prefix, n = pages[0, :P // 16].clone(), ints(lengths)
+    assert la.attend_decode_shared_workspace_size(B, 4, H, D, pages.shape[1], 16, P // 16) > la.attend_decode_workspace_size(B, 4, H, D, pages.shape[1], 16)
+    f = lambda: la.attend_decode_shared(q, kc, vc, prefix, pages, n, **scales)  # noqa: E731
+    want = f()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = f()
+    prefix[3], prefix[90] = -1, 1 << 30
+    for _ in range(3):
+        graph.replay()
+        out = f()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out) and not torch.equal(got, want)
+    for b in (0, 1, 69):
+        k, v = seqs[b]
+        at = torch.arange(lengths[b], device="cuda")[None]
+        seen = ~(((at >= 48) & (at < 64)) | ((at >= 1440) & (at < 1456)))
+        assert_attention(out[b:b + 1], None, q[b:b + 1], k, v, seen, D ** -0.5)
+    row = prefix[100].long()  # positions 1600 ..: past the short ones
+    if code == "16":
+        vc[row, 4, 1] = math.nan
+    else:
+        vs[row, 1, 4] = math.nan
+    out = f()
+    assert bool(torch.isfinite(out[::2]).all()) and bool(torch.isfinite(out[1::2, :2]).all()) and bool(torch.isnan(out[1::2, 2:]).all())
+    assert bool((la.attend_decode_shared(q, kc, vc, prefix, pages, n * 0, **scales) == 0).all())

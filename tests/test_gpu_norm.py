@@ -95,15 +95,16 @@ def test_in_place_strides_and_given_outputs(la):
     big, y = r(7, 3, 200), r(200, 7).t()  # rows apart; columns apart (copied)
     x = big[:, 1]
     want, n = la.residual_norm(x.clone(), y.contiguous(), post=post, pre=pre, dtype=torch.float16)
-    others, n_big = big[:, ::2].clone(), torch.full((9, 260), 5.0, dtype=torch.float16, device="cuda")
+    others, n_big = big[:, ::2].clone(), torch.full((9, 264), 5.0, dtype=torch.float16, device="cuda")
     xo, no = la.residual_norm(x, y, post=post, pre=pre, dtype=torch.float16, x_out=x, n_out=n_big[1:8, 8:208])
     assert xo is x and torch.equal(x, want) and torch.equal(big[:, ::2], others) and torch.equal(no, n)
     n_big[1:8, 8:208] = 5.0
     assert bool((n_big == 5.0).all())
-    odd = r(3, 211)[:, 3:203]  # 16 bytes do not divide the base
-    a, b = la.residual_norm(odd, y[:3], post=post, pre=pre), la.residual_norm(odd.contiguous(), y[:3].contiguous(), post=post, pre=pre)
-    for s, t in zip(a, b):
-        near(s, t.double(), 8 * W * t.double().abs() + 8 * W * 3)
+    odd = r(3, 211)[:, 3:203]  # 16 bytes do not divide the base: other sums, each as far from the exact one as reference() has it
+    xo, no = la.residual_norm(odd, y[:3], post=post, pre=pre)
+    (wx, ex), (wn, en) = reference(odd, y[:3], post, None, 1.0, pre)
+    near(xo, wx, ex)
+    near(no, wn, en)
 
 
 def test_rows_of_zeros_and_rows_that_are_not_finite(la):
