@@ -17,7 +17,7 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kStep = 32;               // keys of a wave's step
 constexpr int kTile = kStep * kWaves;   // keys of a work item
 constexpr int kMaxGroups = 512;         // workgroups of a launch: two on every CU
-// Over 8-bit caches twice as many, whose waves have half the bytes under way (35 sequences of 16 to 16000: 66 us, 75 with 512; 64 of
+// Over 8-bit caches twice as many, whose waves have half the bytes under way (35 sequences of 16 to 16000: 66 us, 70 with 512; 64 of
 // 8000: 216 and 236; but 32 of 3400 61 and 57, which are even spans either way).
 constexpr uint32_t kMaxGroups8 = 1024;
 

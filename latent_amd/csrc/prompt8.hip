@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
 
   // Loading: load i of a thread is piece tid % kPieces of row tid / kPieces + i kRowsLoad.  Eight rows from a multiple of eight share a page, so
   // a wave's rows of a load lie behind one wave-uniform address (two at D = 64), and what a lane adds to it never changes; every lane's
-  // address worked out by itself was half of the vector instructions that this kernel has beyond the 16-bit one's.  Lane g holds the
+  // address worked out by itself was a third of the vector instructions that this kernel had beyond the 16-bit one's.  Lane g holds the
   // page of rows 8 g .. and where in it they are, looked up a tile before; lane l of the first wave takes the scales of row l.
   constexpr int kRowsHere = kWave / kPieces, kGroups = kRowsHere > 8 ? 2 : 1;
   const int piece = tid % kPieces, lrow = tid / kPieces, in_group = lrow & 7;

@@ -305,3 +305,70 @@ def test_a_prefix_by_itself_with_rows_and_pages_that_are_not_there(la, code):
     out = f()
     assert bool(torch.isfinite(out[::2]).all()) and bool(torch.isfinite(out[1::2, :2]).all()) and bool(torch.isnan(out[1::2, 2:]).all())
     assert bool((la.attend_decode_shared(q, kc, vc, prefix, pages, n * 0, **scales) == 0).all())
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_more_sequences_than_lanes(la, code):
+    """70 prompts, of none to 40 tokens behind up to 50 cached ones, one of them long; the same as single tokens."""
+    g = gen(15)
+    new = [(7 * i) % 41 for i in range(70)]
+    new[33] = 300
+    lengths = [n + (11 * i) % 51 for i, n in enumerate(new)]
+    kc, vc, ks, vs, pages, seqs = paged8(g, lengths, 8, 2, 64, torch.float16, CODES[code])
+    starts = [sum(new[:i]) for i in range(71)]
+    q = torch.randn((starts[-1], 4, 64), generator=g, device="cuda").half()
+    out = la.attend_prompt_paged(q, kc, vc, pages, ints(lengths), ints(starts), k_scale=ks, v_scale=vs)
+    one = la.attend_decode(q[:70], kc, vc, pages, ints(lengths), k_scale=ks, v_scale=vs)
+    for b, (k, v) in enumerate(seqs):
+        s = slice(starts[b], starts[b + 1])
+        assert_attention(out[s], None, q[s], k, v, visible(new[b], lengths[b], True, "cuda"), 64 ** -0.5)
+        assert_attention(one[b:b + 1], None, q[b:b + 1], k, v, visible(1, lengths[b], True, "cuda"), 64 ** -0.5)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("G", [3, 20])
+def test_tables_of_more_than_the_last_level_cache(la, code, G):
+    """A page table wide enough that rows are read past that cache, of which most names nothing."""
+    g, H, D = gen(16), 4, 128
+    lengths = [1500, 0, 40, 333]
+    kc, vc, ks, vs, pages, seqs = paged8(g, lengths, 16, H, D, torch.bfloat16, CODES[code], spare=20000)  # 20000 pages of 16 KB
+    wide = torch.full((4, 20000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :pages.shape[1]] = pages
+    q = torch.randn((4, H * G, D), generator=g, device="cuda").bfloat16()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    for f in (lambda: la.attend_decode(q, kc, vc, wide, ints(lengths), lse=lse, k_scale=ks, v_scale=vs),
+              lambda: la.attend_decode_shared(q, kc, vc, pages[0, :0], wide, ints(lengths), lse=lse, k_scale=ks, v_scale=vs),
+              lambda: la.attend_prompt_paged(q, kc, vc, wide, ints(lengths), ints([0, 1, 2, 3, 4]), lse=lse, k_scale=ks, v_scale=vs)):
+        out = f()
+        for b, (k, v) in enumerate(seqs):
+            assert_attention(out[b:b + 1], lse[b:b + 1], q[b:b + 1], k, v, visible(1, lengths[b], True, "cuda"), D ** -0.5)
+
+
+def test_two_calls_at_once(la):
+    """Calls on two streams, without workspaces: each has its own."""
+    f, base, _, q = calls(la, seed=17, lengths=(3000, 100, 2900), shared=2)
+    want = [f[n]() for n in ("attend_decode", "attend_prompt_paged", "attend_decode_shared")]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        got = [[f[n](stream=s) for n in ("attend_decode", "attend_prompt_paged", "attend_decode_shared")] for s in streams]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_norm_operands_of_other_strides(la):
+    """Broadcast rows, rows apart, a stream that the call writes through; a row stride of zero is no output."""
+    g = gen(18)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    row, y = r(1, 96), r(5, 96)
+    x, n = la.residual_norm(row.expand(5, 96), y[:1].expand(5, 96), post=la.Norm(bias=r(96)), gate=r(5, 1).bfloat16(), pre=la.Norm(kind="layer"), dtype=torch.float16)
+    for b in range(5):
+        assert x.shape == (5, 96) and x.is_contiguous() and n.shape == (5, 96)
+    one = la.residual_norm(row.repeat(5, 1), y[:1].repeat(5, 1), pre=la.Norm(kind="layer"), dtype=torch.float16)
+    two = la.residual_norm(row.expand(5, 96), y[:1].expand(5, 96), pre=la.Norm(kind="layer"), dtype=torch.float16)
+    assert all(torch.equal(a, b) for a, b in zip(one, two)) and bool((two[0] == two[0][0]).all())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    three = la.residual_norm(row.expand(5, 96), y[:1].expand(5, 96), pre=la.Norm(kind="layer"), dtype=torch.float16, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(three, two))
