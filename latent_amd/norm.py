@@ -76,9 +76,8 @@ def residual_norm(
     x's); x_out may be x.  Sums are fp32, and n is taken from x' before x' is
     rounded to its type.  There is no backward pass.
     """
-    for name, n in (("post", post), ("pre", pre)):
-        if n is not None and not isinstance(n, Norm):
-            raise TypeError(f"{name} must be a Norm")
+    if not (post is None or isinstance(post, Norm)) or not (pre is None or isinstance(pre, Norm)):
+        raise TypeError("post and pre must be Norm")
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a tensor")
     want = _DTYPES.get(x.dtype if dtype is None else dtype)
