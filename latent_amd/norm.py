@@ -22,18 +22,38 @@ _DTYPES = {torch.float32: _lib.LATENT_F32, torch.float16: _lib.LATENT_F16, torch
 class Norm:
     """A norm of rows of d numbers: kind "rms", v / sqrt(mean(v^2) + eps) weight + bias, or "layer", the same of v - mean(v).
 
-    weight and bias: [d], f32, f16 or bf16 (both of one type), either None for ones and zeros.
+    weight and bias: [d], f32, f16 or bf16 (both of one type), either None for ones and zeros.  All four may be set later on: a
+    call takes them as they are then (a captured one has those of its capture).
     """
 
-    __slots__ = ("weight", "bias", "kind", "eps", "_args")
+    __slots__ = ("weight", "bias", "_kind", "_eps")
 
     def __init__(self, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, kind: str = "rms", eps: float = 1e-6):
+        self.weight, self.bias, self.kind, self.eps = weight, bias, kind, eps
+
+    @property
+    def kind(self) -> str:
+        return self._kind
+
+    @kind.setter
+    def kind(self, kind: str) -> None:
         if kind not in _KINDS:
             raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+        self._kind = kind
+
+    @property
+    def eps(self) -> float:
+        return self._eps
+
+    @eps.setter
+    def eps(self, eps: float) -> None:
         if not 0.0 <= eps < float("inf"):
             raise ValueError("eps must be finite and not negative")
-        self.weight, self.bias, self.kind, self.eps = weight, bias, kind, float(eps)
-        self._args = (_KINDS[kind], self.eps, weight, bias)
+        self._eps = float(eps)
+
+    @property
+    def _args(self):
+        return _KINDS[self._kind], self._eps, self.weight, self.bias
 
 
 class BlockNorm:
