@@ -107,29 +107,35 @@ class DecodeStack:
         self.lengths = torch.zeros((self.T,), dtype=torch.int32, device=dev)
         self.h = [torch.empty((self.T, self.d), dtype=torch.float32, device=dev) for _ in blocks]
         self.prefix: Optional[torch.Tensor] = None
-        self._attention_scratch()
+        self.attention_workspace = self._attention_scratch(None)
 
-    def _attention_scratch(self) -> None:
-        prefix = 0 if self.prefix is None else self.prefix.numel()
-        need = max(a.workspace_size(self.T, self.pages.shape[1], prefix) for a in self.attention)
-        self.attention_workspace = torch.empty((max(need, 16),), dtype=torch.uint8, device=self.pages.device)
+    def _attention_scratch(self, prefix: Optional[torch.Tensor]) -> torch.Tensor:
+        pages = 0 if prefix is None else prefix.numel()
+        need = max(a.workspace_size(self.T, self.pages.shape[1], pages) for a in self.attention)
+        return torch.empty((max(need, 16),), dtype=torch.uint8, device=self.pages.device)
 
     def share(self, prefix: Optional[torch.Tensor]) -> None:
         """From now on the first P pages of every slot are those that prefix (int32 [P], P <= max_pages) names, of every
         layer's cache alike: pages[:, :P] is set to them, and steps read them once for all slots.  Whoever fills them does so
         through a slot, by `prompt`; a slot that goes on behind them has positions >= P times the page size.  None:
-        slots have pages of their own again.  A captured graph is dropped."""
+        slots have pages of their own again.  The call waits for the device, whose steps under way, on whatever stream, read
+        what it replaces, so it cannot be part of a capture.  A captured graph is dropped; who has it by its handle may still replay
+        it, over the prefix that it was captured with."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")
         if prefix is not None:
             if prefix.dtype != torch.int32 or prefix.dim() != 1 or prefix.device != self.pages.device or prefix.numel() > self.pages.shape[1]:
                 raise ValueError(f"prefix must be int32 [pages] on {self.pages.device}, at most {self.pages.shape[1]} of them")
             prefix = prefix.clone() if prefix.numel() else None
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("share cannot be captured")
+        workspace = self._attention_scratch(prefix)
+        if self.pages.is_cuda:
+            torch.cuda.synchronize(self.pages.device)
         self.graph = None
-        self.prefix = prefix
+        self.prefix, self.attention_workspace = prefix, workspace
         if prefix is not None:
             self.pages[:, :prefix.numel()] = prefix
-        self._attention_scratch()
 
     @property
     def output(self) -> torch.Tensor:
@@ -243,8 +249,16 @@ class DecodeStack:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self._body()
+        g.held = self._captured_operands()
         self.graph = g
         return g
+
+    def _captured_operands(self) -> List[Optional[torch.Tensor]]:
+        """What a graph reads and writes that the stack may replace while somebody still has the graph: it lives as long as its handle."""
+        kept = [] if self.attention is None else [self.prefix, self.attention_workspace]
+        for b in self.norms or ():
+            kept += [b.gate, *(t for n in (b.pre, b.post) if n is not None for t in (n.weight, n.bias))]
+        return kept
 
     def replay(self) -> torch.Tensor:
         if self.graph is None:
