@@ -42,7 +42,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from .attention import Attention
+from .attention import _CODES, Attention
 from .moe import StackedLayer, moe_forward, workspace_size
 from .norm import BlockNorm, residual_norm
 from .router import Router, route
@@ -117,8 +117,10 @@ class DecodeStack:
     def share(self, prefix: Optional[torch.Tensor]) -> None:
         """From now on the first P pages of every slot are those that prefix (int32 [P], P <= max_pages) names, of every
         layer's cache alike: pages[:, :P] is set to them, and steps read them once for all slots.  Whoever fills them does so
-        through a slot, by `prompt`; a slot that goes on behind them has positions >= P times the page size.  None:
-        slots have pages of their own again.  The call waits for the device, whose steps under way, on whatever stream, read
+        through a slot, by `prompt`; a slot that goes on behind them has positions >= P times the page size.
+        None, or another prefix: first the slots' columns name again what they did before, and a slot
+        under way takes a copy of the prefix there; where its page is another slot's by now, or there was none, it keeps the prefix's,
+        and an idle slot names none.  The call waits for the device, whose steps under way, on whatever stream, read
         what it replaces, so it cannot be part of a capture.  A captured graph is dropped; who has it by its handle may still replay
         it, over the prefix that it was captured with."""
         if self.attention is None:
@@ -132,10 +134,31 @@ class DecodeStack:
         workspace = self._attention_scratch(prefix)
         if self.pages.is_cuda:
             torch.cuda.synchronize(self.pages.device)
+        if self.prefix is not None:
+            self._unshare()
         self.graph = None
         self.prefix, self.attention_workspace = prefix, workspace
         if prefix is not None:
+            self._own = self.pages[:, :prefix.numel()].clone()
             self.pages[:, :prefix.numel()] = prefix
+
+    def _unshare(self) -> None:
+        own, P = self._own, self.prefix.numel()
+        shared = self.prefix.expand(self.T, P)
+        n_pages = self.attention[0].k_cache.shape[0]
+        busy = (self.positions >= 0)[:, None]
+        given = torch.isin(own, self.pages[:, P:].contiguous())
+        # A page that the prefix has at another place is still to be read from.
+        free = (own >= 0) & (own < n_pages) & ~given & (~torch.isin(own, self.prefix) | (own == shared))
+        move = free & busy & (shared >= 0) & (shared < n_pages)
+        for b in move.any(1).nonzero().flatten().tolist():  # a slot at a time: the copies may be as large as the cache
+            to, of = own[b][move[b]].long(), self.prefix[move[b]].long()
+            for a in self.attention:
+                for t in (a.k_cache, a.v_cache, a.k_scale, a.v_scale):
+                    if t is not None:
+                        rows = t.view(torch.uint8) if t.dtype in _CODES else t
+                        rows[to] = rows[of]
+        self.pages[:, :P] = torch.where(busy & ~free, shared, torch.where(given, -1, own))
 
     @property
     def output(self) -> torch.Tensor:
