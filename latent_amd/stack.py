@@ -19,7 +19,8 @@ is cached and stores nothing more; behind its pages it attends to what is there,
 behind the table its attention is zeros.
 `prompt` runs whole prompts, or chunks of them, through the same layers and
 leaves the slots ready to decode.  After `share` the slots' first pages are the
-same ones, which a step reads once for all slots (latent_attn_decode_shared).
+same ones, which a step reads once for all slots (latent_attn_decode_shared);
+`start_behind` puts slots behind them.
 
 With norms each block, attention and experts alike, reads pre(x) and adds
 scale gate post(y) to the stream, in one launch with the next block's pre
@@ -117,7 +118,8 @@ class DecodeStack:
     def share(self, prefix: Optional[torch.Tensor]) -> None:
         """From now on the first P pages of every slot are those that prefix (int32 [P], P <= max_pages) names, of every
         layer's cache alike: pages[:, :P] is set to them, and steps read them once for all slots.  Whoever fills them does so
-        through a slot, by `prompt`; a slot that goes on behind them has positions >= P times the page size.
+        through a slot, by `prompt`: an idle slot's prompt starts at position 0, in the shared pages.  A slot that is to go on behind
+        them, with a prompt or a step, is put there by `start_behind`.
         None, or another prefix: first the slots' columns name again what they did before, and a slot
         under way takes a copy of the prefix there; where its page is another slot's by now, or there was none, it keeps the prefix's,
         and an idle slot names none.  The call waits for the device, whose steps under way, on whatever stream, read
@@ -141,6 +143,15 @@ class DecodeStack:
         if prefix is not None:
             self._own = self.pages[:, :prefix.numel()].clone()
             self.pages[:, :prefix.numel()] = prefix
+
+    def start_behind(self, slots: torch.Tensor) -> None:
+        """Puts these slots (int32 [B]; others than 0 .. n_tokens - 1 are left out), idle or not, at the first position behind the shared prefix."""
+        if self.attention is None or self.prefix is None:
+            raise RuntimeError("this stack shares no prefix")
+        if slots.dtype != torch.int32 or slots.dim() != 1 or slots.device != self.positions.device:
+            raise ValueError(f"slots must be int32 [slots] on {self.positions.device}")
+        rows = torch.arange(self.T, dtype=torch.int32, device=slots.device)
+        self.positions.masked_fill_((rows[:, None] == slots).any(1), self.prefix.numel() * self.attention[0].k_cache.shape[1])
 
     def _unshare(self) -> None:
         own, P = self._own, self.prefix.numel()
@@ -221,7 +232,7 @@ class DecodeStack:
         """New tokens of several sequences through every layer: x [N, d], packed; sequence b is rows starts[b] ..
         starts[b + 1] - 1 (int32 [B + 1], ascending, up to N) and goes on in slot slots[b] (int32 [B], different
         ones of 0 .. n_tokens - 1) at that slot's position, or from 0 where the slot is idle (also
-        with no tokens: a slot that is to stay idle is left out).  The slots' pages have to have
+        with no tokens: a slot that is to stay idle is left out; behind a shared prefix: start_behind).  The slots' pages have to have
         room.  Returns the output rows f32 [N, d]; the slots then decode what follows.  Rows of no sequence
         (padding) reach no cache, their attention is zeros, and they pass the experts."""
         if self.attention is None:

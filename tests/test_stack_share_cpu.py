@@ -109,6 +109,21 @@ def test_a_prefix_of_slots_pages_in_another_order():
     assert s.pages[2].tolist() == TABLE[2]
 
 
+def test_slots_start_behind_the_prefix():
+    s = stack(TABLE, [3, -1, -1], [block(1)])
+    with pytest.raises(RuntimeError):
+        s.start_behind(ints([1]))
+    s.share(ints([20, 21]))
+    s.start_behind(ints([2, 1]))
+    assert s.positions.tolist() == [3, 8, 8]
+    s.start_behind(ints([-1, 3]))
+    s.start_behind(ints([]))
+    assert s.positions.tolist() == [3, 8, 8]
+    for bad in (torch.tensor([1]), ints([[1]]), torch.zeros(1)):
+        with pytest.raises(ValueError):
+            s.start_behind(bad)
+
+
 def test_a_graph_keeps_what_it_reads():
     """share replaces scratch and prefix; a graph that was captured with the old ones may still be replayed by whoever has it."""
     s = stack(TABLE, [-1, -1, -1], [block(1)])
