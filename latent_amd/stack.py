@@ -127,12 +127,12 @@ class DecodeStack:
         it, over the prefix that it was captured with."""
         if self.attention is None:
             raise RuntimeError("this stack has no attention")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("share cannot be captured")
         if prefix is not None:
             if prefix.dtype != torch.int32 or prefix.dim() != 1 or prefix.device != self.pages.device or prefix.numel() > self.pages.shape[1]:
                 raise ValueError(f"prefix must be int32 [pages] on {self.pages.device}, at most {self.pages.shape[1]} of them")
             prefix = prefix.clone() if prefix.numel() else None
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("share cannot be captured")
         workspace = self._attention_scratch(prefix)
         if self.pages.is_cuda:
             torch.cuda.synchronize(self.pages.device)
