@@ -262,8 +262,17 @@ __device__ __forceinline__ void rotated8(const uint16_t* row, const u32x4& own, 
   }
 }
 
+// Queries may be rotated where they stand, and a lane reads numbers that its row's other lanes write: all of them belong to one wave, in which
+// nothing that is written behind this fence is written before what stands in front of it is read.
+__device__ __forceinline__ void row_is_read() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 template <typename E, typename Q, int kKind, int kLanes, int kHeads>
 __global__ void __launch_bounds__(kThreads) append8_kernel(AppendParams p, Scales scales, bool inter) {
+  static_assert(kWave % kLanes == 0, "a row's lanes are of one wave");
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t u = i % kLanes, t = i / kLanes / p.groups, g = i / kLanes % p.groups;
   if (t >= p.T) return;
@@ -298,6 +307,7 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(AppendParams p, Scale
     x[j] = live ? *reinterpret_cast<const u32x4*>(src[j] + 2 * d0) : u32x4{0, 0, 0, 0};
     if (kKind == kHalf) y[j] = live && turned && h < p.Hq + p.Hkv ? *reinterpret_cast<const u32x4*>(src[j] + 2 * other) : u32x4{0, 0, 0, 0};
   }
+  row_is_read();
 #pragma unroll
   for (int j = 0; j < kHeads; ++j) {
     const uint32_t h = h0 + j;
@@ -307,6 +317,7 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(AppendParams p, Scale
       rotated8<E, kKind>(reinterpret_cast<const uint16_t*>(src[j]), x[j], y[j], d0, p, inter, table, c, s, r);
     else
       widen<E>(x[j], r);
+    if (kKind == kScalar) row_is_read();
     if (h < p.Hq) {
       if (in) {
         u32x4 o;
