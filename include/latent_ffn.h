@@ -545,8 +545,9 @@ int latent_attn_prompt(const latent_attn_prompt_args* args, latent_stream_t stre
  * in fp32, each step rounded, the code then to the nearest (ties to even): whole
  * numbers with top 127, or OCP e4m3 with top 448.  A row with an infinity or a NaN has a NaN
  * as its scale and codes of zero: whoever reads it gets NaN, in its output where the row
- * is a value's, whose key counts in the log-sum-exp as any other.  The number held is
- * code * scale.
+ * is a value's, whose key counts in the log-sum-exp as any other.  A value's row whose
+ * largest number LATENT_F16 cannot hold (appended as LATENT_BF16) is one of these to
+ * queries of that type.  The number held is code * scale.
  *
  * In the calls below, latent_kv_cache holds codes: strides count them and are
  * multiples of 16; page_size is a multiple of 8, head_dim of 16.  Scales of a

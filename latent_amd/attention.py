@@ -31,7 +31,8 @@ as codes and one scale, f32 in k_scale and v_scale [pages, kv heads, page rows],
 
 computed in fp32 step by step, the code rounded to nearest; top is 127 for int8, 448 for
 float8_e4m3fn.  A row with an infinity or a NaN is a NaN wherever it is read (values' in the
-output alone: lse is the keys').
+output alone: lse is the keys'), and to f16 queries a row of values appended as
+bf16 that f16 cannot hold.
 There D and the strides are multiples of 16 (bytes; of the scales 4 elements, and
 a page's rows adjacent) and page rows of 8; kv_scales makes the scales.
 """

@@ -213,6 +213,13 @@ struct E4M3 {
   }
 };
 
+// Whether a value row of scale s is one to queries of the type: not a NaN, nor, to f16, one whose largest rounds to an infinity there (appended as bf16),
+// whose codes times their scale f16 has no elements and no weights for.
+template <typename E, typename Q>
+__device__ __forceinline__ bool held(float s) {
+  return __is_same(E, F16) ? s <= 65520.f / Q::kTop : s == s;
+}
+
 // ---- host ---------------------------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s <= int64_t{1} << 40; }

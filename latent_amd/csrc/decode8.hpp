@@ -190,10 +190,17 @@ struct Stream8 {
       float most = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = fmaxf(most, vs[j]);
+      if (__any(!held<E, Q>(most))) {
+        most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          vs[j] = held<E, Q>(vs[j]) ? vs[j] : __uint_as_float(0x7FC00000u);
+          most = fmaxf(most, vs[j]);
+        }
+      }
       const uint32_t up = max(base, __float_as_uint(op_over(most, 16, 64, OpMax{})) & 0x7F800000u);
       const float inv = __uint_as_float(0x7E800000u - up);  // half over the power: 2^k has the exponent bits 127 + k, 253 less those are 2^(-1 - k)'s
-      const uint32_t grown = up - base;  // as exponent bits
-      rebase = grown < 0x3F800000u ? __uint_as_float(0x3F800000u - grown) : 0.f;  // scales appended as bf16 may be further apart than exponents go
+      rebase = __uint_as_float(0x3F800000u + base - up);
       base = up;
 #pragma unroll
       for (int j = 0; j < 8; ++j) vs[j] *= inv;

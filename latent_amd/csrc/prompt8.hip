@@ -22,14 +22,14 @@ namespace {
 // is from 1 to 2, so that a weight has the bits of its probability, whatever the values' size; the elements are exact but for those
 // below the type's normal numbers, which are as near as it has them.  bf16 has fp32's range: the weight takes all of a scale that is
 // not tiny.
-template <typename E>
+template <typename E, typename Q>
 struct Split {
   static __device__ __forceinline__ float power(float s) {
     const uint32_t e = __float_as_uint(s) & 0x7F800000u;
-    if (e >= 0x7F000000u || (E::kLift == 0.f && e >= 0x21800000u)) return 1.f;  // a NaN's; 2^-60
+    if (!held<E, Q>(s) || (E::kLift == 0.f && e >= 0x21800000u)) return 1.f;  // 2^-60
     return __uint_as_float(e);  // 0 for 0
   }
-  static __device__ __forceinline__ float rest(float s) {  // of a finite one
+  static __device__ __forceinline__ float rest(float s) {  // of one that is held
     const float p = power(s);
     return p == 0.f ? 1.f : s * __uint_as_float(0x7F000000u - __float_as_uint(p));
   }
@@ -65,7 +65,7 @@ struct Shared8 {
   float ks[2][kKeys], add[2][kKeys];  // a score's factor, base 2, and what is added: the log2 of its value's rest
   float whole[2][kKeys];              // one over the rest; the log-sum-exp takes it unrounded
   u32x4 over[2][kKeys / 4];           // one over the rests of four keys as two summands of the element type: (0, 1), (2, 3), then the smaller
-  int bad[2];                         // the first key whose value row is a NaN, INT32_MAX: none
+  int bad[2];                         // the first key whose value row is not held, INT32_MAX: none
   static __device__ __forceinline__ int k_turn(int key) { return kC >= 16 ? key & 15 : (key >> 1) & 7; }
   static __device__ __forceinline__ int v_turn(int key) { return kC >= 16 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 };
@@ -188,15 +188,15 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
       lds_st(lds_k + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::k_turn(row)), convert8<E, Q>(raw_k[i][2 * j], raw_k[i][2 * j + 1]));
     else
       lds_st(lds_v + buf * S::kTile + row * kRow + 16 * ((2 * piece + j) ^ S::v_turn(row)),
-             convert_value8<E, Q>(raw_v[i][2 * j], raw_v[i][2 * j + 1], Split<E>::power(scale_v[i])));
+             convert_value8<E, Q>(raw_v[i][2 * j], raw_v[i][2 * j + 1], Split<E, Q>::power(scale_v[i])));
   };
   auto store_scales = [&](int buf) {
     if (wave == 0 && lane < kKeys) {
-      // The key of a value row that is a NaN counts in the sums as any other; the rows that see it, and no others, are divided by a NaN.
-      const bool is = raw_vs == raw_vs;
+      // The key of a value row that is not held counts in the sums as any other; the rows that see it, and no others, are divided by a NaN.
+      const bool is = held<E, Q>(raw_vs);
       const int bad = __ffsll(__ballot(!is)) - 1;
       if (lane == 0) sm.bad[buf] = bad < 0 ? INT32_MAX : bad;
-      const float f = is ? Split<E>::rest(raw_vs) : 1.f, over = 1.f / f;
+      const float f = is ? Split<E, Q>::rest(raw_vs) : 1.f, over = 1.f / f;
       sm.ks[buf][lane] = raw_ks * p.scale_log2;
       sm.add[buf][lane] = __log2f(f);
       if constexpr (kLse) sm.whole[buf][lane] = over;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 256 ? 1 : 2) prompt8_kernel(P
       }
       return;
     }
-    if (uniform(sm.bad[buf]) < vis - kt) sum = __uint_as_float(0x7FC00000u);  // for the rows that see a value row that is a NaN
+    if (uniform(sm.bad[buf]) < vis - kt) sum = __uint_as_float(0x7FC00000u);  // for the rows that see a value row that is not held
     // Scores; the next tile's codes are converted in the products' shadow (two prompts of 4099 behind 8 and 5701: 1005 us, 1031 before them).
     f32x16 s[kKeyBlocks] = {};
     auto scores = [&](auto converting) {
