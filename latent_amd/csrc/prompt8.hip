@@ -21,12 +21,12 @@ namespace {
 // A value row of scale s: its codes times `power`, of two, are the elements; the probability takes `rest`.  s = power rest.  f16: rest
 // is from 1 to 2, so that a weight has the bits of its probability, whatever the values' size; the elements are exact but for those
 // below the type's normal numbers, which are as near as it has them.  bf16 has fp32's range: the weight takes all of a scale that is
-// not tiny.
+// neither tiny nor huge, beside which the others' weights would be nothing.
 template <typename E, typename Q>
 struct Split {
   static __device__ __forceinline__ float power(float s) {
     const uint32_t e = __float_as_uint(s) & 0x7F800000u;
-    if (!held<E, Q>(s) || (E::kLift == 0.f && e >= 0x21800000u)) return 1.f;  // 2^-60
+    if (!held<E, Q>(s) || (E::kLift == 0.f && e - 0x21800000u < 0x32000000u)) return 1.f;  // from 2^-60 to 2^40
     return __uint_as_float(e);  // 0 for 0
   }
   static __device__ __forceinline__ float rest(float s) {  // of one that is held

@@ -17,7 +17,7 @@ H, D, N = 2, 128, 300
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("tiny", [40, 128])  # what is held against small values when the large ones come
-@pytest.mark.parametrize("large", [65280.0, 65536.0, 2.0 ** 20, 1e9, 1e15])  # 65280: bf16's last that f16 can hold
+@pytest.mark.parametrize("large", [65280.0, 65536.0, 2.0 ** 20, 1e9, 1e15, 2.0 ** 120])  # 65280: bf16's last that f16 can hold
 def test_values_of_all_sizes(gpu, code, dt, large, tiny):
     g = gen(7)
     kc, ks = empty_cache(24, 16, H, D, CODES[code])
