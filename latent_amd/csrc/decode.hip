@@ -36,7 +36,7 @@ namespace attend {
 namespace {
 
 template <bool kAfter, bool kTable = false>
-int launch16(const latent_attn_decode_args& a, const Plan& pl, const DecodeParams& p, hipStream_t s) {
+int launch16(const latent_attn_decode_args& a, const Plan& pl, const Params<kAfter || kTable>& p, hipStream_t s) {
   (void)hipGetLastError();
   auto launch = [&](auto e, auto dp, auto exact, auto mt, auto page8) {
     auto go = [&](auto once) {
@@ -84,14 +84,14 @@ size_t after_workspace(const latent_attn_decode_args& a, int64_t n_prefix, bool 
 
 int launch_after16(const latent_attn_decode_args& a, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s) {
   const After w = plan_after(behind(a, n_prefix), 2, kMaxGroups);
-  DecodeParams p{};
+  MoreParams p{};
   const int st = after_params(a, n_prefix, 2, w, prior, workspace, &p);
   return st == LATENT_OK ? launch16<true>(a, w.plan, p, s) : st;
 }
 
 int launch_together16(const latent_attn_decode_args& a, const int32_t* prefix, int64_t n_prefix, hipStream_t s) {
   const Plan pl = plan_for(a);
-  DecodeParams p{};
+  MoreParams p{};
   const int st = decode_params(a, 2, pl, &p);
   if (st != LATENT_OK) return st;
   p.prefix = prefix;

@@ -38,6 +38,10 @@ struct DecodeParams {
   float* part_ml;
   float* part_acc;
   int2* unit_parts;
+};
+// What only 8-bit caches and shared prefixes take, apart from what every launch has to fetch (96 sequences of up to 2500 tokens, 20 heads of 64 over
+// one: 17.0 us the whole call, 17.1 with all of it in one structure).
+struct MoreParams : DecodeParams {
   Scales scales;  // of an 8-bit cache
   // kAfter: keys here begin at position `ahead`, which cache.pages and cache.max_len leave out; what rows have seen before it is `prior`.  Every
   // unit leaves its rows, those that one workgroup has whole by themselves: sums [units][rows][2] and rows [units][rows][D].
@@ -49,9 +53,11 @@ struct DecodeParams {
   float* unit_acc;
   uint32_t ahead;
 };
+template <bool kMore>
+using Params = std::conditional_t<kMore, MoreParams, DecodeParams>;
 
 template <bool kAfter>
-__device__ __forceinline__ uint32_t length_of(const DecodeParams& p, uint32_t b) {
+__device__ __forceinline__ uint32_t length_of(const Params<kAfter>& p, uint32_t b) {
   const int32_t n = p.lengths[b];
   if constexpr (kAfter) return n < static_cast<int64_t>(p.ahead) ? 0u : min(static_cast<uint32_t>(n) - p.ahead, p.cache.max_len);
   return n < 0 ? 0u : min(static_cast<uint32_t>(n), p.cache.max_len);
@@ -77,7 +83,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
 
 template <bool kAfter>
-__device__ __forceinline__ Span find_span(const DecodeParams& p, int lane) {
+__device__ __forceinline__ Span find_span(const Params<kAfter>& p, int lane) {
   uint32_t total = 0;
   for (uint32_t b0 = 0; b0 < p.B; b0 += kWave) {
     const uint32_t b = b0 + lane;
@@ -139,16 +145,17 @@ struct Stream {
   static constexpr bool kExact = kExact_;
   static constexpr int kRound = kDP <= 128 ? kMT : 1;  // row blocks that the waves exchange at once
   static constexpr int kPerSimd = kDP == 256 ? 1 : 2;  // waves
+  static constexpr bool kMore = kTable;
   // The first of the eight dimensions that lane quarter kq holds of product s.
   static __device__ __forceinline__ int q_dim(int s, int kq) { return 32 * s + 8 * kq; }
 
-  const DecodeParams& p;
+  const Params<kMore>& p;
   int lane, kq;
   uint32_t len;
   const int32_t* pages;
   const char* kbase;
   const char* vbase;
-  __device__ __forceinline__ Stream(const DecodeParams& p, int lane, int kq, uint32_t len, uint32_t b, uint32_t hk)
+  __device__ __forceinline__ Stream(const Params<kMore>& p, int lane, int kq, uint32_t len, uint32_t b, uint32_t hk)
       : p(p), lane(lane), kq(kq), len(len), pages(p.cache.pages + b * p.cache.pages_stride), kbase(p.cache.k + hk * p.cache.k_head),
         vbase(p.cache.v + hk * p.cache.v_head) {}
 
@@ -163,7 +170,9 @@ struct Stream {
   };
   __device__ __forceinline__ Place place_of(uint32_t key) const {
     const uint32_t slot = p.cache.by_page.of(key);
-    return {key < len ? (kTable && slot < p.prefix_pages ? p.prefix : pages)[slot] : -1, key - slot * p.cache.page_size};
+    const int32_t* of = pages;
+    if constexpr (kTable) of = slot < p.prefix_pages ? p.prefix : pages;
+    return {key < len ? of[slot] : -1, key - slot * p.cache.page_size};
   }
   // Row m of score block blk is key 8 (m / 4) + 4 blk + m % 4 of the step: lane (query, kq) then holds keys 8 kq .. + 7.
   __device__ __forceinline__ uint32_t k_key(uint32_t kb, int blk) const { return kb + 8 * ((lane & 15) >> 2) + 4 * blk + (lane & 3); }
@@ -304,7 +313,7 @@ __device__ __forceinline__ void finish(const DecodeParams& p, uint32_t b, uint32
 }
 
 template <typename S, bool kAfter>
-__global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(Params<S::kMore || kAfter> p) {
   using E = typename S::E;
   constexpr int kDP = S::kDP, kMT = S::kMT, kVec = kDP / 16, kK = kDP / 32, kPad = kDP + 4, kRound = S::kRound;
   constexpr bool kExact = S::kExact;
@@ -425,8 +434,10 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
         } else {
           const bool alone = kAfter && whole;
           const int64_t at = (alone ? (static_cast<int64_t>(b) * p.U + u) * p.rows : part) + row;
-          f32x4* dst = reinterpret_cast<f32x4*>((alone ? p.unit_acc : p.part_acc) + at * p.D + 8 * c);
-          float* ml = (alone ? p.unit_ml : p.part_ml) + 2 * at;
+          float *acc = p.part_acc, *ml = p.part_ml;
+          if constexpr (kAfter) acc = alone ? p.unit_acc : acc, ml = alone ? p.unit_ml : ml;
+          f32x4* dst = reinterpret_cast<f32x4*>(acc + at * p.D + 8 * c);
+          ml += 2 * at;
           dst[0] = x[0];
           dst[1] = x[1];
           if (c == 0) {
@@ -454,12 +465,13 @@ __global__ void __launch_bounds__(kThreads, S::kPerSimd) decode_kernel(DecodePar
 // A single pass under a running maximum, four parts in flight.
 constexpr int kJoinWaves = 16;
 template <typename E, bool kAfter>
-__global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(Params<kAfter> p) {
   __shared__ float sm[kJoinWaves][10][kWave];
   const uint32_t unit = blockIdx.x, b = unit / p.U, u = unit % p.U;
   const int2 parts = p.unit_parts[unit];
   if (!kAfter && parts.y < 2) return;
-  const int count = kAfter ? parts.y + p.prior.parts : parts.y;
+  int count = parts.y;
+  if constexpr (kAfter) count += p.prior.parts;
   const uint32_t hk = u / p.chunks, r0 = (u % p.chunks) * p.rows, nr = min(p.rows, p.G - r0);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   // A part's pieces of one row are neighbours, the prior's those of neighbouring rows (kAfter).
@@ -470,37 +482,55 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) join_kernel(DecodeParams p
   const int waves = blockDim.x / kWave;
   // kAfter: the prior's parts of this row lie in the prompt kernels' layout: thread 64 wave + 32 half + row % 32 has dimensions 8 c + 4 half ..
   const uint32_t pr = b * p.G + r0 + row, tile = pr / 128, thread = pr % 128 / 32 * 64 + pr % 32, Hkv = p.Hq / p.G, width = p.D <= 64 ? 64 : p.D <= 128 ? 128 : 256;
-  const int64_t pfirst = static_cast<int64_t>(p.prior.tiles - 1 - static_cast<int>(tile)) * Hkv + hk, pstep = static_cast<int64_t>(p.prior.tiles) * Hkv;
+  int64_t pfirst = 0, pstep = 0;
+  if constexpr (kAfter) {
+    pfirst = static_cast<int64_t>(p.prior.tiles - 1 - static_cast<int>(tile)) * Hkv + hk;
+    pstep = static_cast<int64_t>(p.prior.tiles) * Hkv;
+  }
   for (int i0 = wave; i0 < count; i0 += 4 * waves) {
     float pm[4], pl[4];
     f32x4 px[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = min(i0 + j * waves, count - 1);
-      if (kAfter && i >= parts.y) {
-        const int64_t at = pfirst + (i - parts.y) * pstep;
-        const f32x4 ml = reinterpret_cast<const f32x4*>(p.prior.ml)[at * 256 + thread];
-        const f32x4* src = reinterpret_cast<const f32x4*>(p.prior.acc) + at * (width / 8 * 256) + c * 256 + thread;
-        // Its rows are to be divided by the sum of the rounded weights, the second of ml, and count with the full one.
-        const float by = ml[1] > 0.f ? ml[2] / ml[1] : ml[1] == 0.f ? 0.f : ml[1];
-        pm[j] = ml[0] - p.prior.up + E::kLift;
-        pl[j] = ml[2];
-        px[j][0] = src[0] * by;
-        px[j][1] = src[32] * by;
-      } else {
-        const bool alone = kAfter && parts.y == 1;
-        const int64_t at = (alone ? static_cast<int64_t>(unit) : static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
-        const float* ml = (alone ? p.unit_ml : p.part_ml) + 2 * at;
-        pm[j] = ml[0];
-        pl[j] = ml[1];
-        const f32x4* src = reinterpret_cast<const f32x4*>((alone ? p.unit_acc : p.part_acc) + at * p.D + 8 * c);
+      auto own = [&](const float* part_ml, const float* part_acc, int64_t part) {
+        const int64_t at = part * p.rows + row;
+        const f32x4* src = reinterpret_cast<const f32x4*>(part_acc + at * p.D + 8 * c);
+        pm[j] = part_ml[2 * at];
+        pl[j] = part_ml[2 * at + 1];
         px[j][0] = src[0];
         px[j][1] = src[1];
+      };
+      const int64_t part = static_cast<int64_t>(parts.x + i) * 2 + (i == 0 ? 1 : 0);
+      if constexpr (kAfter) {
+        if (i >= parts.y) {
+          const int64_t at = pfirst + (i - parts.y) * pstep;
+          const f32x4 ml = reinterpret_cast<const f32x4*>(p.prior.ml)[at * 256 + thread];
+          const f32x4* src = reinterpret_cast<const f32x4*>(p.prior.acc) + at * (width / 8 * 256) + c * 256 + thread;
+          // Its rows are to be divided by the sum of the rounded weights, the second of ml, and count with the full one.
+          const float by = ml[1] > 0.f ? ml[2] / ml[1] : ml[1] == 0.f ? 0.f : ml[1];
+          pm[j] = ml[0] - p.prior.up + E::kLift;
+          pl[j] = ml[2];
+          px[j][0] = src[0] * by;
+          px[j][1] = src[32] * by;
+        } else if (parts.y == 1) {
+          own(p.unit_ml, p.unit_acc, unit);
+        } else {
+          own(p.part_ml, p.part_acc, part);
+        }
+      } else {
+        own(p.part_ml, p.part_acc, part);
       }
       if (i0 + j * waves >= count) {
         pm[j] = -INFINITY;
         pl[j] = 0.f;
       }
+    }
+    // All loads are under way before the first is looked at: left alone, the first part's rows are fetched once its maximum is there, a second
+    // latency (those 96 sequences 17.3 us).
+    if constexpr (!kAfter) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(px[j][0]), "+v"(px[j][1]));
     }
     const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), mm = finite_max(top), f = exp2_fast(m - mm);
     m = top;
@@ -631,14 +661,16 @@ int decode_params(const latent_attn_decode_args& a, int64_t size, const Plan& pl
 
 // The second launch, where units were left in parts.
 template <bool kAfter>
-void launch_join(const Plan& pl, const DecodeParams& p, bool f16, hipStream_t s) {
+void launch_join(const Plan& pl, const Params<kAfter>& p, bool f16, hipStream_t s) {
   if (pl.whole && !kAfter) return;
   // A unit has about groups / units parts, four in flight a wave.  Of few parts two waves join soonest (96 units of six:
   // 16.8 us the whole call, 17.1 with one or four), of hundreds sixteen (one unit of 235: 16.6, 23.1 with four).
   const uint32_t units = p.B * p.U;
   uint32_t waves = pl.groups > 16 * units ? kJoinWaves : pl.groups > 8 * units ? 4 : 2;
   // The prior's parts are as many for each unit (5 sequences, 16 parts, 40 units: 5.1 us by eight waves, 7.2 by four; 512 units 12.0 and 10.0).
-  if (kAfter && p.prior.parts > 8) waves = std::max<uint32_t>(waves, units <= 256 ? 8 : 4);
+  if constexpr (kAfter) {
+    if (p.prior.parts > 8) waves = std::max<uint32_t>(waves, units <= 256 ? 8 : 4);
+  }
   const dim3 grid(units, (p.rows * (p.D / 8) + kWave - 1) / kWave), block(kWave * waves);
   if (f16)
     hipLaunchKernelGGL((join_kernel<F16, kAfter>), grid, block, 0, s, p);
@@ -668,7 +700,7 @@ After plan_after(const latent_attn_decode_args& own, int64_t size, uint32_t most
   r.acc_bytes = rows * own.head_dim * sizeof(float);
   return r;
 }
-int after_params(const latent_attn_decode_args& a, int64_t n_prefix, int64_t size, const After& w, const Prior& prior, void* workspace, DecodeParams* p) {
+int after_params(const latent_attn_decode_args& a, int64_t n_prefix, int64_t size, const After& w, const Prior& prior, void* workspace, MoreParams* p) {
   latent_attn_decode_args own = behind(a, n_prefix);
   own.workspace = workspace;
   own.workspace_bytes = SIZE_MAX;

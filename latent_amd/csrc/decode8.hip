@@ -7,7 +7,7 @@ namespace attend {
 namespace {
 
 template <bool kAfter, bool kTable = false>
-int launch8(const latent_attn_decode_args& a, int32_t code, const Plan& pl, const DecodeParams& p, hipStream_t s) {
+int launch8(const latent_attn_decode_args& a, int32_t code, const Plan& pl, const MoreParams& p, hipStream_t s) {
   (void)hipGetLastError();
   with_stream8<kTable>(a, code, pl, [&](auto t) {
     hipLaunchKernelGGL((decode_kernel<typename decltype(t)::type, kAfter>), dim3(pl.groups), dim3(kThreads), 0, s, p);
@@ -21,7 +21,7 @@ int launch8(const latent_attn_decode_args& a, int32_t code, const Plan& pl, cons
 
 int launch_after8(const latent_attn_decode_args& a, const latent_kv_scales& scales, int64_t n_prefix, const Prior& prior, void* workspace, hipStream_t s) {
   const After w = plan_after(behind(a, n_prefix), 1, kMaxGroups8);
-  DecodeParams p{};
+  MoreParams p{};
   const int st = after_params(a, n_prefix, 1, w, prior, workspace, &p);
   if (st != LATENT_OK) return st;
   p.scales = device_scales(scales);
@@ -30,7 +30,7 @@ int launch_after8(const latent_attn_decode_args& a, const latent_kv_scales& scal
 
 int launch_together8(const latent_attn_decode_args& a, const latent_kv_scales& scales, const int32_t* prefix, int64_t n_prefix, hipStream_t s) {
   const Plan pl = plan_for(a, 1, kMaxGroups8);
-  DecodeParams p{};
+  MoreParams p{};
   const int st = decode_params(a, 1, pl, &p);
   if (st != LATENT_OK) return st;
   p.scales = device_scales(scales);
@@ -61,7 +61,7 @@ extern "C" int latent_attn_decode_q8(const latent_attn_decode_args* args, const 
   if (st == LATENT_OK) st = check_codes(a.cache, *scales, a.head_dim);
   if (st != LATENT_OK || a.cache.n_seq == 0) return st;
   const Plan pl = plan_for(a, 1, kMaxGroups8);
-  DecodeParams p{};
+  MoreParams p{};
   st = decode_params(a, 1, pl, &p);
   if (st != LATENT_OK) return st;
   if (p.cache.max_len && (!scales->k || !scales->v)) return LATENT_E_INVALID;

@@ -40,14 +40,15 @@ struct Stream8 {
   static constexpr bool kExact = false;
   static constexpr int kRound = kDP <= 128 ? kMT : 1;
   static constexpr int kPerSimd = kDP == 256 ? 1 : 2;
+  static constexpr bool kMore = true;
   static __device__ __forceinline__ int q_dim(int s, int kq) { return kDP / 4 * kq + 8 * s; }
 
-  const DecodeParams& p;
+  const MoreParams& p;
   int lane, kq;
   uint32_t len;
   const int32_t* pages;
   uint64_t kbase, vbase, kscale, vscale;
-  __device__ __forceinline__ Stream8(const DecodeParams& p, int lane, int kq, uint32_t len, uint32_t b, uint32_t hk)
+  __device__ __forceinline__ Stream8(const MoreParams& p, int lane, int kq, uint32_t len, uint32_t b, uint32_t hk)
       : p(p), lane(lane), kq(kq), len(len), pages(p.cache.pages + b * p.cache.pages_stride),
         kbase(reinterpret_cast<uint64_t>(p.cache.k + hk * p.cache.k_head)), vbase(reinterpret_cast<uint64_t>(p.cache.v + hk * p.cache.v_head)),
         kscale(reinterpret_cast<uint64_t>(p.scales.k + hk * p.scales.k_head)), vscale(reinterpret_cast<uint64_t>(p.scales.v + hk * p.scales.v_head)) {}
