@@ -593,11 +593,12 @@ typedef struct latent_kv_read_args {
 int latent_kv_read(const latent_kv_read_args* args, const latent_kv_scales* scales, latent_stream_t stream);
 
 /* latent_attn_decode over an 8-bit cache.  Scores and probabilities take the scales in fp32; a probability times
- * its value's scale is rounded once to dtype. */
+ * its value's scale is held as two summands of dtype, the second the first one's rounding. */
 int latent_attn_decode_q8_workspace_size(const latent_attn_decode_args* args, size_t* bytes);
 int latent_attn_decode_q8(const latent_attn_decode_args* args, const latent_kv_scales* scales, latent_stream_t stream);
 
-/* latent_attn_prompt over an 8-bit cache (k NULL); its scratch is latent_attn_prompt_workspace_size(). */
+/* latent_attn_prompt over an 8-bit cache (k NULL); its scratch is latent_attn_prompt_workspace_size().  A weight is
+ * rounded once to dtype, and the row divided by the sum of the rounded ones. */
 int latent_attn_prompt_q8(const latent_attn_prompt_args* args, const latent_kv_scales* scales, latent_stream_t stream);
 
 /* ---- one new token for each of a batch that shares its first positions ---- */

@@ -13,7 +13,7 @@
 // nine tenths of the time here, take both (one key of bf16: off by 0.0029 of the row's size without, 0.0017, the output's rounding, with).
 //
 // Measured (heads of 128, 32 over 8 unless said): 301 tokens 8.0 us, 35 sequences of 16 to 16000 (228 MB) 66 us, 64 of 8000 214 us over e4m3 and
-// 217 over int8 (362 over a 16-bit cache), 64 of 10000 to 20000, 64 heads, f16 over int8, 394 us (5.0 TB/s).  Bound by HBM, behind 15 to 20 us of
+// 217 over int8 (362 over a 16-bit cache), 64 of 10000 to 20000, 64 heads, f16 over int8, 392 us (5.0 TB/s).  Bound by HBM, behind 15 to 20 us of
 // launch, prologue and join; rows of a head that are together in a page, instead of all heads' of a position, go at 5.6 TB/s.
 #pragma once
 

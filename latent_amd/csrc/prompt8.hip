@@ -9,8 +9,8 @@
 // it.  A value's scale is a power of two, which its elements take exactly, times a rest, which its weight takes: as the
 // logarithm added to the score (the product with the key's scale becomes a multiply-add), so that one exponential gives p[j] rest[j].
 //
-// Measured (heads of 128, 32 over 8): two prompts of 4099 behind 8 and 5701 921 us in bf16 over e4m3, 962 over int8, 790 over a 16-bit cache; four
-// chunks of 287 to 517 29, 32 and 25 us.  Bound by vector and matrix instructions, which the SIMDs' two waves take in turn (85 % of the
+// Measured (heads of 128, 32 over 8): two prompts of 4099 behind 8 and 5701 916 us in bf16 over e4m3, 960 over int8, 782 over a 16-bit cache; four
+// chunks of 287 to 517 29, 31 and 25 us.  Bound by vector and matrix instructions, which the SIMDs' two waves take in turn (85 % of the
 // cycles together): the products are the 16-bit kernel's, the rest is conversions, two operations more a score and the sums.
 #include "prompt.hpp"
 

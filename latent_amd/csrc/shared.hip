@@ -8,8 +8,8 @@
 // them, without that launch, took longer: few lanes read all of the prior's parts one after the other, 64 sequences behind 16000 126 us.)
 // Few sequences, or a short prefix, are a decode that looks the first pages up in the prefix instead (kTogether).
 //
-// Measured: 5 sequences behind 4096 shared positions, up to 700 of their own, 32 over 8 heads, 16-bit, 20 us, as a decode; 64 behind
-// 16000, up to 2000 of their own, 64 over 8 heads, 104 us (16-bit) to 108 (int8): the prefix 69, bound by its products as prompts are
+// Measured: 5 sequences behind 4096 shared positions, up to 700 of their own, 32 over 8 heads, 16-bit, 18.7 us, as a decode; 64 behind
+// 16000, up to 2000 of their own, 64 over 8 heads, 106 us (16-bit) to 109 (int8): the prefix 69, bound by its products as prompts are
 // (490 TFLOP/s), own keys 31, the join 10.  A decode that reads all positions of each sequence takes 460 us there (int8 306).
 #include "shared.hpp"
 
@@ -19,7 +19,9 @@ using namespace latent::attend;
 namespace {
 
 // Numbers that all sequences together would read of the prefix's keys and values up to which they do, each for itself, in the one or two
-// launches of a decode: what the last-level cache gives them costs less than the third launch and the parts.  32 over 8 heads of 128, up to 300
+// launches of a decode: what the last-level cache gives them costs less than the third launch and the parts.  One number for caches of all types and any
+// batch, near where the two cross over 16 bits; over codes, and for a sequence or two, which read little or nothing again, together would be the shorter
+// a while longer (int8 at 67M below; one sequence 27.6 us behind 28672 positions, together, and 43.8 behind 32768, split).  32 over 8 heads of 128, up to 300
 // positions of their own, together and split: 5 sequences behind 4096 (42M) 19.8 and 23.9 us (int8 23.4 and 27.5), 8 (67M) 27.8 and 23.4 (26.2
 // and 27.6), 16 (134M) 42.9 and 25.6 (40.2 and 29.6); 16 over one head of 64, 64 behind 4096 (34M) 18.7 and 22.6.
 constexpr int64_t kTogether = 56 << 20;
