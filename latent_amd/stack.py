@@ -169,7 +169,9 @@ class DecodeStack:
                     if t is not None:
                         rows = t.view(torch.uint8) if t.dtype in _CODES else t
                         rows[to] = rows[of]
-        self.pages[:, :P] = torch.where(busy & ~free, shared, torch.where(given, -1, own))
+        kept = torch.where(busy & ~free, shared, -1)
+        given = given | torch.isin(own, kept)
+        self.pages[:, :P] = torch.where(busy & ~free, shared, torch.where(given & ~busy, -1, own))
 
     @property
     def output(self) -> torch.Tensor:

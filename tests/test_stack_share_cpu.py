@@ -144,3 +144,15 @@ def test_not_while_a_graph_is_captured(monkeypatch):
     with pytest.raises(RuntimeError):
         s.share(ints([20]))
     assert s.pages.tolist() == TABLE and s.prefix is None
+
+
+def test_a_page_that_somebody_goes_on_reading_is_nobody_elses():
+    """The prefix is slot 0's own pages; slot 1, which has none, keeps them when slot 0 has ended."""
+    s = stack([[1, 2, 3, 4], [-1, -1, 7, 8], [9, 10, 11, 12]], [-1, -1, -1], [block(1)])
+    s.share(s.pages[0, :2])
+    s.positions.copy_(ints([-1, 9, 9]))
+    before = [held(s, b, 9) for b in (1, 2)]
+    s.share(None)
+    assert s.pages.tolist() == [[-1, -1, 3, 4], [1, 2, 7, 8], [9, 10, 11, 12]]
+    for b in (1, 2):
+        assert all(torch.equal(x, y) for x, y in zip(before[b - 1], held(s, b, 9)))
